@@ -2,7 +2,7 @@
 
 The library is the product: gfx950 HIP kernels behind the C-ABI launch layer
 of ``include/nn_hip.h`` (the reference's ``launch_*`` entry points, reference
-src/nn.h:348-466) plus the C host modules of ``include/nn_modules.h``.  This
+src/nn.h:348-466) and of ``include/nn_attention.h`` plus the C host modules of ``include/nn_modules.h``.  This
 module only binds that C-ABI with ctypes so that Python tests and the bench
 can drive it; device memory, copies, streams and events come from the
 library's own plumbing (``include/nn_hip_rt.h``), so no other GPU runtime is
@@ -32,6 +32,11 @@ ACT_IDENTITY, ACT_RELU, ACT_GELU, ACT_SILU, ACT_TANH, ACT_MP_SILU = range(6)
 ACT_NAMES = {"identity": 0, "relu": 1, "gelu": 2, "silu": 3, "tanh": 4, "mp_silu": 5}
 
 
+# Types and masks of the attention operators (include/nn_attention.h)
+NN_F32, NN_BF16 = range(2)
+NN_MASK_NONE, NN_MASK_CAUSAL, NN_MASK_PREFIX = range(3)
+
+
 class NnHipError(RuntimeError):
     """A launcher refused its arguments or a HIP call failed."""
 
@@ -41,6 +46,27 @@ I = C.c_int
 F = C.c_float
 SZ = C.c_size_t
 LL = C.c_longlong
+
+
+class NnQkNormRope(C.Structure):
+    """Mirror of NnQkNormRope in include/nn_attention.h (pass the structure itself)."""
+
+    _fields_ = [("dtype", I), ("tokens", I), ("heads", I), ("kv_heads", I), ("head_dim", I), ("rot_dim", I),
+                ("axes", I), ("interleaved", I), ("eps", F), ("q_stride", LL * 2), ("k_stride", LL * 2),
+                ("q_out_stride", LL * 2), ("k_out_stride", LL * 2), ("q_weight", P), ("k_weight", P), ("pos", P),
+                ("freq", P)]
+
+
+class NnAttention(C.Structure):
+    """Mirror of NnAttention in include/nn_attention.h (pass the structure itself)."""
+
+    _fields_ = [("dtype", I), ("batch", I), ("len_q", I), ("len_k", I), ("heads", I), ("kv_heads", I),
+                ("head_dim", I), ("scale", F), ("softcap", F), ("mask", I), ("buckets", I), ("max_distance", I),
+                ("q_stride", LL * 3), ("k_stride", LL * 3), ("v_stride", LL * 3), ("out_stride", LL * 3),
+                ("q_start", P), ("k_len", P), ("prefix", P), ("doc_q", P), ("doc_k", P), ("bucket", P), ("bias", P)]
+
+
+ROPE, ATTN = C.POINTER(NnQkNormRope), C.POINTER(NnAttention)
 
 # name -> (restype, argtypes, is_launcher)
 _SIGS = {
@@ -137,6 +163,14 @@ _SIGS = {
     "nnhip_multi_tensor_plan_destroy": (None, [P], False),
     "launch_adam_ema_step": (None, [P, F, F, F, F, F, F, F, F, P], True),
     "launch_ema_update": (None, [P, F, F, P], True),
+    # attention operators (nn_attention.h)
+    "launch_qk_norm_rope_forward": (None, [P, P, P, P, ROPE, P], True),
+    "nnhip_qk_norm_rope_workspace": (SZ, [ROPE], True),
+    "launch_qk_norm_rope_backward": (None, [P] * 8 + [ROPE, P, P], True),
+    "nnhip_attention_forward_workspace": (SZ, [ATTN], True),
+    "launch_attention_forward": (None, [P] * 5 + [ATTN, P, P], True),
+    "nnhip_attention_backward_workspace": (SZ, [ATTN], True),
+    "launch_attention_backward": (None, [P] * 10 + [ATTN, P, P], True),
 }
 
 

@@ -1,0 +1,153 @@
+// attention.hip -- the attention launchers: checks of the call, workspaces, order of the
+// kernels.
+#include "attn_common.h"
+
+namespace {
+using namespace attn;
+
+constexpr long long kMostGroups = (1LL << 31) - 1;
+
+// Workspaces, in floats; documents come first (16-byte records).
+size_t docs_floats(const NnAttention* a) {
+    if (!a->doc_q) return 0;
+    const size_t nk = ((size_t)a->len_k + kBlock - 1) / kBlock, nq = ((size_t)a->len_q + kBlock - 1) / kBlock;
+    return 4 * (size_t)a->batch * (nk + nq);
+}
+size_t stat_floats(const NnAttention* a) { return 2 * (size_t)a->batch * a->heads * a->len_q; }
+
+bool sizes_fit(const NnAttention* a, const char* what) {
+    NNK_REQUIRE_RET(a, false, what, "%s: null description", what);
+    NNK_REQUIRE_RET(a->dtype == NN_F32 || a->dtype == NN_BF16, false, what, "%s: unknown dtype %d", what, a->dtype);
+    NNK_REQUIRE_RET(a->batch >= 0 && a->len_q >= 0 && a->len_k >= 0 && a->len_q <= 1 << 30 && a->len_k <= 1 << 30,
+        false, what, "%s: bad shape batch=%d len_q=%d len_k=%d", what, a->batch, a->len_q, a->len_k);
+    NNK_REQUIRE_RET(a->heads > 0 && a->kv_heads > 0 && a->heads % a->kv_heads == 0, false, what,
+        "%s: heads=%d is not a multiple of kv_heads=%d", what, a->heads, a->kv_heads);
+    NNK_REQUIRE_RET(a->head_dim >= 1 && a->head_dim <= 128, false, what, "%s: head_dim=%d is not in 1..128", what,
+        a->head_dim);
+    NNK_REQUIRE_RET(a->buckets >= 0 && a->max_distance >= 0 && a->max_distance <= kMaxDistance, false, what,
+        "%s: buckets=%d max_distance=%d (at most %d)", what, a->buckets, a->max_distance, kMaxDistance);
+    const long long rows = std::max(((long long)a->len_q + kRows - 1) / kRows, ((long long)a->len_k + kBlock - 1) / kBlock);
+    NNK_REQUIRE_RET(rows * a->batch <= kMostGroups / a->heads && (long long)a->buckets * a->heads <= kMostGroups, false,
+        what, "%s: too many rows (batch=%d heads=%d len_q=%d len_k=%d)", what, a->batch, a->heads, a->len_q, a->len_k);
+    return true;
+}
+
+// Fills `p` for the call's description; false after recording an error.
+bool take(Args& p, const NnAttention* a, const char* what) {
+    if (!sizes_fit(a, what)) return false;
+    NNK_REQUIRE_RET(a->scale > 0.0f && a->scale < INFINITY, false, what, "%s: scale=%g is not positive", what, a->scale);
+    NNK_REQUIRE_RET(a->softcap >= 0.0f && a->softcap < INFINITY, false, what, "%s: softcap=%g is negative", what,
+        a->softcap);
+    NNK_REQUIRE_RET(a->mask == NN_MASK_NONE || a->mask == NN_MASK_CAUSAL || a->mask == NN_MASK_PREFIX, false, what,
+        "%s: unknown mask %d", what, a->mask);
+    NNK_REQUIRE_RET(a->mask != NN_MASK_PREFIX || a->prefix, false, what, "%s: null prefix", what);
+    NNK_REQUIRE_RET(!a->doc_q == !a->doc_k, false, what, "%s: documents of queries or keys only", what);
+    NNK_REQUIRE_RET(!a->buckets || (a->bucket && a->bias), false, what, "%s: null bucket or bias", what);
+    p = Args{};
+    for (int i = 0; i < 3; ++i) {
+        p.qs[i] = a->q_stride[i];
+        p.ks[i] = a->k_stride[i];
+        p.vs[i] = a->v_stride[i];
+        p.os[i] = a->out_stride[i];
+    }
+    p.batch = a->batch;
+    p.len_q = a->len_q;
+    p.len_k = a->len_k;
+    p.heads = a->heads;
+    p.kv_heads = a->kv_heads;
+    p.group = a->heads / a->kv_heads;
+    p.dim = a->head_dim;
+    p.mask = a->mask;
+    p.buckets = a->buckets;
+    p.max_distance = a->max_distance;
+    p.scale = a->scale;
+    p.c1 = a->softcap > 0.0f ? a->scale / a->softcap : a->scale * kLog2e;
+    p.c2 = a->softcap * kLog2e;
+    p.q_start = a->q_start;
+    p.k_len = a->k_len;
+    p.prefix = a->prefix;
+    p.doc_q = a->doc_q;
+    p.doc_k = a->doc_k;
+    p.bucket = a->bucket;
+    p.bias = a->bias;
+    return true;
+}
+
+// Whether rows of 16-byte chunks can be read and written: strides here, pointers by the
+// callers.
+bool strides_by_16(const NnAttention* a) {
+    const long long e = a->dtype == NN_BF16 ? 8 : 4;
+    bool ok = a->head_dim % e == 0;
+    for (int i = 0; i < 3; ++i)
+        ok = ok && a->q_stride[i] % e == 0 && a->k_stride[i] % e == 0 && a->v_stride[i] % e == 0 &&
+            a->out_stride[i] % e == 0;
+    return ok;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t nnhip_attention_forward_workspace(const NnAttention* a) {
+    if (!sizes_fit(a, "nnhip_attention_forward_workspace")) return 0;
+    return docs_floats(a);
+}
+
+void launch_attention_forward(void* out, float* lse, const void* q, const void* k, const void* v,
+    const NnAttention* a, float* workspace, hipStream_t s) {
+    const char* what = "launch_attention_forward";
+    Args p;
+    if (!take(p, a, what)) return;
+    if (!a->batch || !a->len_q) return;
+    NNK_REQUIRE(out && lse && q && (!a->len_k || (k && v)), what, "%s: null pointer", what);
+    NNK_REQUIRE(!nnhip_attention_forward_workspace(a) || workspace, what, "%s: null workspace", what);
+    NNK_REQUIRE(nnk::aligned16(workspace), what, "%s: workspace is not aligned to 16 bytes", what);
+    p.q = q;
+    p.k = k;
+    p.v = v;
+    p.out = out;
+    p.lse = lse;
+    p.vec = strides_by_16(a) && nnk::aligned16(q) && nnk::aligned16(k) && nnk::aligned16(v) && nnk::aligned16(out);
+    nnk_attention_docs(p, workspace, s, what);
+    nnk_attention_forward(p, a->dtype == NN_BF16, s, what);
+}
+
+size_t nnhip_attention_backward_workspace(const NnAttention* a) {
+    if (!sizes_fit(a, "nnhip_attention_backward_workspace")) return 0;
+    return docs_floats(a) + stat_floats(a) + (a->buckets ? nnk_attention_dist_floats(a) : 0);
+}
+
+void launch_attention_backward(void* dq, void* dk, void* dv, float* dbias, const void* dout,
+    const void* q, const void* k, const void* v, const void* out, const float* lse,
+    const NnAttention* a, float* workspace, hipStream_t s) {
+    const char* what = "launch_attention_backward";
+    Args p;
+    if (!take(p, a, what)) return;
+    NNK_REQUIRE(!dbias || a->buckets, what, "%s: a bias gradient without a bias", what);
+    const bool has_q = a->batch && a->len_q, has_k = a->batch && a->len_k;
+    NNK_REQUIRE(!has_q || (dq && dout && q && out && lse), what, "%s: null pointer of the queries", what);
+    NNK_REQUIRE(!has_k || (dk && dv && k && v), what, "%s: null pointer of the keys", what);
+    NNK_REQUIRE(!nnhip_attention_backward_workspace(a) || workspace, what, "%s: null workspace", what);
+    NNK_REQUIRE(nnk::aligned16(workspace), what, "%s: workspace is not aligned to 16 bytes", what);
+    p.q = q;
+    p.k = k;
+    p.v = v;
+    p.out = const_cast<void*>(out);
+    p.lse = const_cast<float*>(lse);
+    p.dout = dout;
+    p.dq = dq;
+    p.dk = dk;
+    p.dv = dv;
+    p.vec = strides_by_16(a);
+    for (const void* x : {q, k, v, out, dout, (const void*)dq, (const void*)dk, (const void*)dv})
+        p.vec = p.vec && nnk::aligned16(x);
+    p.stat = reinterpret_cast<float2*>(workspace + docs_floats(a));
+    if (dbias) p.dist_sums = workspace + docs_floats(a) + stat_floats(a);
+    const bool half = a->dtype == NN_BF16;
+    if (has_q && has_k) nnk_attention_docs(p, workspace, s, what);
+    if (has_q && !nnk_attention_backward_q(p, half, s, what)) return;
+    if (has_k && !nnk_attention_backward_kv(p, half, s, what)) return;
+    if (dbias) nnk_attention_bias_grad(p, dbias, s, what);
+}
+
+}  // extern "C"

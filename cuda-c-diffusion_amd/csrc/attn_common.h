@@ -1,0 +1,410 @@
+// attn_common.h -- what the attention kernels share: fragments of the matrix
+// cores, tiles in LDS, score functions, masks.
+//
+// Layout.  All products are 32 x 32 tiles of the matrix cores (bf16: 32x32x16,
+// fp32: 32x32x2, four of them where bf16 has one).  In such a tile the lane
+// l = (l & 31) + 32 h holds column l & 31 and the rows 8 g + 4 h + j (g, j in
+// 0..3) in its 16 registers.  A product whose result is the next one's operand is
+// therefore formed with the next one's free index in the columns: scores as keys x
+// queries where they go on to values or query gradients, as queries x keys where
+// they go on to key and value gradients.  A lane's registers are then already the
+// operand, with the contracted index in the order 8 g + 4 h + j, and the other
+// operand is read from LDS in that order: rows by 16-byte reads, columns by the
+// transposing read (bf16) or by one read a row (fp32).
+//
+// Rows in LDS are DP values and 32 bytes long: 8 lanes' 16-byte reads of
+// successive rows, and the 4 x 32 bytes of a transposing read, meet different
+// banks.
+#pragma once
+
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+#include <type_traits>
+
+#include "nn_attention.h"
+#include "nnk_common.h"
+
+namespace attn {
+
+typedef __bf16 bf16;
+typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kBlock = 64;     // keys (or queries) of a tile in LDS
+constexpr int kTpb = 256;
+constexpr int kWaves = kTpb / 64;
+constexpr int kRows = 32 * kWaves;  // columns of a workgroup: queries, or keys in the key gradients
+constexpr int kMaxDistance = 1023;
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+
+template <typename T>
+struct Type;
+template <>
+struct Type<bf16> {
+    typedef bf16x8 Frag;
+    static constexpr int CE = 8;  // values of 16 bytes, and of a lane's operand
+};
+template <>
+struct Type<float> {
+    typedef f32x4 Frag;
+    static constexpr int CE = 4;
+};
+template <typename T>
+using Frag = typename Type<T>::Frag;
+
+__device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma(f32x4 a, f32x4 b, f32x16 c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+}
+
+__device__ __forceinline__ f32x16 zero16() {
+    f32x16 z;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) z[r] = 0.0f;
+    return z;
+}
+
+// Row of register r in half h of a 32 x 32 tile.
+__device__ __forceinline__ int row_of(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
+
+// The values of both halves' lanes l and l + 32, in both.
+struct Halves {
+    float lower, upper;
+};
+__device__ __forceinline__ Halves halves(float v) {
+    const unsigned u = __builtin_bit_cast(unsigned, v);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const unsigned lower = r[0], upper = r[1];  // a bit cast of r[1] itself gives r[0]
+    return {__builtin_bit_cast(float, lower), __builtin_bit_cast(float, upper)};
+}
+__device__ __forceinline__ float sum_halves(float v) {
+    const Halves x = halves(v);
+    return x.lower + x.upper;
+}
+__device__ __forceinline__ float max_halves(float v) {
+    const Halves x = halves(v);
+    return fmaxf(x.lower, x.upper);
+}
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// ---------------------------------------------------------------------------
+// Tiles in LDS
+// ---------------------------------------------------------------------------
+template <typename T, int DP>
+struct Lds {
+    static constexpr int kRowBytes = DP * (int)sizeof(T) + 32;
+    static constexpr int kBytes = kBlock * kRowBytes;
+    static constexpr int kSteps = DP / (2 * Type<T>::CE);  // fragments of a row
+    static constexpr int kKeySteps = 32 / (2 * Type<T>::CE);  // fragments of 32 rows
+
+    // Operand whose free index is the tile's row: 16 bytes of row `row`.
+    static __device__ __forceinline__ Frag<T> rows(const char* t, int row, int u, int h) {
+        return *reinterpret_cast<const Frag<T>*>(t + row * kRowBytes + (2 * u + h) * 16);
+    }
+    // Operand whose free index is the column d0 + (lane & 31) and whose contracted
+    // index is the 32 rows from `row` on, fragment f of kKeySteps.
+    static __device__ __forceinline__ Frag<T> cols(const char* t, int row, int f, int d0, int lane) {
+        const int h = lane >> 5;
+        if constexpr (sizeof(T) == 2) {
+            const char* p = t + (row + 16 * f + 4 * h + (lane >> 2 & 3)) * kRowBytes +
+                (d0 + (lane & 16) + (lane & 3) * 4) * 2;
+            typedef __attribute__((address_space(3))) i16x4* LdsPtr;
+            const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(p));
+            const i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(p + 8 * kRowBytes));
+            const bf16x4 x = __builtin_bit_cast(bf16x4, a), y = __builtin_bit_cast(bf16x4, b);
+            return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+        } else {
+            const char* p = t + (row + 8 * f + 4 * h) * kRowBytes + (d0 + (lane & 31)) * 4;
+            f32x4 v;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const float*>(p + j * kRowBytes);
+            return v;
+        }
+    }
+};
+
+// Registers of a tile's fragment f as the operand of the next product.  bf16: the
+// probabilities (or score gradients) are rounded to bf16 here, each by at most 2^-8 of
+// itself and independently of the others, so that the sum over them is off by about what
+// its own rounding to bf16 adds; softmax sums and the bias gradient are taken before.
+__device__ __forceinline__ bf16x8 operand(const f32x16& s, int f, bf16) {
+    bf16x8 v;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = (bf16)s[8 * f + j];
+    return v;
+}
+__device__ __forceinline__ f32x4 operand(const f32x16& s, int f, float) {
+    f32x4 v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = s[4 * f + j];
+    return v;
+}
+
+// 16 bytes of a row from feature d0 on, zeros from `dim` on.
+template <typename T>
+__device__ __forceinline__ u32x4 load_chunk(const T* row, int d0, int dim, bool vec) {
+    u32x4 v = {0, 0, 0, 0};
+    if (vec) {
+        if (d0 < dim) v = *reinterpret_cast<const u32x4*>(row + d0);
+    } else {
+        T e[Type<T>::CE];
+#pragma unroll
+        for (int j = 0; j < Type<T>::CE; ++j) e[j] = d0 + j < dim ? row[d0 + j] : (T)0.0f;
+        __builtin_memcpy(&v, e, 16);
+    }
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ Frag<T> load_frag(const T* row, int d0, int dim, bool vec) {
+    return __builtin_bit_cast(Frag<T>, load_chunk<T>(row, d0, dim, vec));
+}
+
+// Four consecutive features d..d+3 of an output row.
+template <typename T>
+__device__ __forceinline__ void store4(T* row, int d, int dim, bool vec, float a, float b, float c, float e) {
+    const float v[4] = {a, b, c, e};
+    if (vec) {
+        if (d >= dim) return;
+        if constexpr (sizeof(T) == 2) {
+            bf16x4 o;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] = (bf16)v[j];
+            *reinterpret_cast<bf16x4*>(row + d) = o;
+        } else {
+            f32x4 o = {a, b, c, e};
+            *reinterpret_cast<f32x4*>(row + d) = o;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (d + j < dim) row[d + j] = (T)v[j];
+    }
+}
+
+// A 64-row tile on its way from memory to LDS: loaded into registers while the tile
+// before it is used, stored when that is done.
+template <typename T, int DP>
+struct Staged {
+    static constexpr int kPerRow = DP / Type<T>::CE;
+    static constexpr int N = kBlock * kPerRow / kTpb;
+    u32x4 v[N];
+
+    // Row r of the tile is base + r * stride if live(r), zeros otherwise.
+    template <typename Live>
+    __device__ __forceinline__ void load(const T* base, long long stride, int dim, bool vec, const Live& live) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int at = n * kTpb + (int)threadIdx.x, r = at / kPerRow, c = at % kPerRow;
+            v[n] = u32x4{0, 0, 0, 0};
+            if (live(r)) v[n] = load_chunk<T>(base + r * stride, c * Type<T>::CE, dim, vec);
+        }
+    }
+    __device__ __forceinline__ void store(char* lds) const {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int at = n * kTpb + (int)threadIdx.x, r = at / kPerRow, c = at % kPerRow;
+            *reinterpret_cast<u32x4*>(lds + r * Lds<T, DP>::kRowBytes + c * 16) = v[n];
+        }
+    }
+};
+
+// ---------------------------------------------------------------------------
+// The call, as the kernels take it
+// ---------------------------------------------------------------------------
+struct Args {
+    const void *q, *k, *v;
+    void* out;
+    float* lse;
+    const void* dout;
+    void *dq, *dk, *dv;
+    float2* stat;      // backward: per query, log2 of its sum and its <p, dp>
+    float* dist_sums;  // backward: sums of score gradients by distance, per key tile
+    const int4* key_docs;    // per block of 64 keys: least and largest document, whether any is negative
+    const int4* query_docs;  // per block of 64 queries
+    long long qs[3], ks[3], vs[3], os[3];
+    int batch, len_q, len_k, heads, kv_heads, group, dim;
+    int mask, buckets, max_distance;
+    float scale, c1, c2;  // score in units of log2: c1 * s, or c2 * tanh(c1 * s)
+    const int *q_start, *k_len, *prefix, *doc_q, *doc_k, *bucket;
+    const float* bias;
+    bool vec;
+};
+
+// Keys of request b, and the position of its query 0.
+__device__ __forceinline__ int keys_of(const Args& a, int b) {
+    return a.k_len ? min(max(a.k_len[b], 0), a.len_k) : a.len_k;
+}
+__device__ __forceinline__ int start_of(const Args& a, int b) {
+    // far enough from the ends of the type that positions and distances stay in it
+    return a.q_start ? min(max(a.q_start[b], -(1 << 30)), 1 << 29) : a.len_k - a.len_q;
+}
+// The query at position pos sees keys 0 .. limit - 1, of which its document's.
+__device__ __forceinline__ int limit_of(const Args& a, int b, int keys, int pos) {
+    if (a.mask == NN_MASK_NONE) return keys;
+    int n = pos + 1;
+    if (a.mask == NN_MASK_PREFIX) n = max(n, a.prefix[b]);
+    return min(keys, max(n, 0));
+}
+
+// ---------------------------------------------------------------------------
+// Scores
+// ---------------------------------------------------------------------------
+// t = tanh(y) and its slope 1 - t^2.  With r = 1 / (e^2|y| + 1): |t| = 1 - 2 r and
+// slope = 4 r (1 - r), which keeps its digits where the cap is reached (1 - t t would
+// not).  t is off by about 2^-23 of 1, so for small y it is the odd series to y^11
+// instead (relative error below 2^-24 for |y| < 3/8).  A cap is chosen so that most
+// scores are far below it; a wave that has them all there forms only the series, half
+// the other's cycles.
+__device__ __forceinline__ float tanh_series(float y) {
+    const float w = y * y;
+    float c = fmaf(w, -0.00886323553f, 0.0218694885f);
+    c = fmaf(w, c, -0.0539682540f);
+    c = fmaf(w, c, 0.133333333f);
+    c = fmaf(w, c, -0.333333333f);
+    return fmaf(y * w, c, y);
+}
+// s[r] = tanh(c1 s[r]) and, if wanted, its slope
+template <bool SLOPE>
+__device__ __forceinline__ void cap_scores(f32x16& s, f32x16& slope, float c1) {
+    float top = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        s[r] *= c1;
+        top = fmaxf(top, fabsf(s[r]));
+    }
+    if (__all(top < 0.375f)) {  // fmaxf passes over NaN; the series keeps it
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s[r] = tanh_series(s[r]);
+            if constexpr (SLOPE) slope[r] = fmaf(-s[r], s[r], 1.0f);
+        }
+    } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float y = s[r], q = __builtin_amdgcn_rcpf(exp2_fast(fabsf(y) * (2.0f * kLog2e)) + 1.0f);
+            const bool small = fabsf(y) < 0.375f;
+            s[r] = small ? tanh_series(y) : copysignf(fmaf(-2.0f, q, 1.0f), y);
+            if constexpr (SLOPE) slope[r] = small ? fmaf(-s[r], s[r], 1.0f) : 4.0f * q * (1.0f - q);
+        }
+    }
+}
+
+// Bias of head `head` by distance -m..m, in units of log2, into LDS.
+__device__ __forceinline__ void load_bias(const Args& a, float* table, int head) {
+    for (int i = threadIdx.x; i < 2 * a.max_distance + 1; i += kTpb) {
+        const int n = min(max(a.bucket[i], 0), a.buckets - 1);
+        table[i] = a.bias[(size_t)n * a.heads + head] * kLog2e;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Blocks of 64 that can meet
+// ---------------------------------------------------------------------------
+// Two ranges of documents with one in common (an empty range has none).
+__device__ __forceinline__ bool docs_meet(const int4& x, const int4& y) { return x.x <= y.y && y.x <= x.y; }
+__device__ __forceinline__ int4 join_docs(const int4* docs, int first, int last) {
+    int4 all = {INT32_MAX, INT32_MIN, 0, 0};
+    for (int i = first; i < last; ++i) {
+        all.x = min(all.x, docs[i].x);
+        all.y = max(all.y, docs[i].y);
+    }
+    return all;
+}
+// Documents of the blocks first .. first + count - 1 of queries, or of keys.
+__device__ __forceinline__ int4 query_docs_of(const Args& a, int b, int first, int count) {
+    const int n = (a.len_q + kBlock - 1) / kBlock;
+    return a.query_docs ? join_docs(a.query_docs + (size_t)b * n, first, min(first + count, n)) : int4{0, 0, 0, 0};
+}
+__device__ __forceinline__ int4 key_docs_of(const Args& a, int b, int first, int count) {
+    const int n = (a.len_k + kBlock - 1) / kBlock;
+    return a.key_docs ? join_docs(a.key_docs + (size_t)b * n, first, min(first + count, n)) : int4{0, 0, 0, 0};
+}
+
+// The blocks first..last-1 that `meets`, in order, 64 of them looked at a time (one a
+// lane).  Uniform over the wave, and over the workgroup if `meets` is.
+template <typename Meets>
+struct Blocks {
+    const Meets& meets;
+    int base, last;
+    unsigned long long m;
+    __device__ __forceinline__ Blocks(int first, int last_, const Meets& meets_) : meets(meets_), base(first), last(last_) {
+        look();
+    }
+    __device__ __forceinline__ void look() {
+        const int b = base + (int)(threadIdx.x & 63);
+        m = __ballot(b < last && meets(b));
+    }
+    // The next block, or -1.
+    __device__ __forceinline__ int next() {
+        while (!m) {
+            base += 64;
+            if (base >= last) return -1;
+            look();
+        }
+        const int b = base + __builtin_ctzll(m);
+        m &= m - 1;
+        return b;
+    }
+};
+
+// Raises kernel fn's limit of dynamic LDS to `bytes` on the current device, once a
+// device (`done` has a bit for each).  False after recording an error.
+inline bool raise_lds(const void* fn, size_t bytes, std::atomic<unsigned long long>& done, const char* what) {
+    int dev = -1;
+    hipError_t e = hipGetDevice(&dev);
+    if (e == hipSuccess && dev >= 64) e = hipErrorInvalidDevice;
+    if (e == hipSuccess && !(done.load(std::memory_order_relaxed) >> dev & 1)) {
+        e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        if (e == hipSuccess) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+    }
+    if (e == hipSuccess) return true;
+    (void)hipGetLastError();
+    nnk_set_error((int)e, "%s: LDS of %zu bytes on device %d: %s", what, bytes, dev, hipGetErrorString(e));
+    return false;
+}
+
+}  // namespace attn
+
+// Documents of each block of 64 into `ws`, for args.key_docs and query_docs (no documents:
+// nothing).
+void nnk_attention_docs(attn::Args& args, float* ws, hipStream_t s, const char* what);
+// One launch each; `half`: bf16.  False after recording an error.
+bool nnk_attention_forward(const attn::Args& args, bool half, hipStream_t s, const char* what);
+bool nnk_attention_backward_q(const attn::Args& args, bool half, hipStream_t s, const char* what);
+bool nnk_attention_backward_kv(const attn::Args& args, bool half, hipStream_t s, const char* what);
+// Bias gradient from args.dist_sums, and the floats that those take.
+void nnk_attention_bias_grad(const attn::Args& args, float* dbias, hipStream_t s, const char* what);
+size_t nnk_attention_dist_floats(const NnAttention* a);
+
+// FN<T, DP, CAP, BIAS> for the call's type, feature count and score terms.
+#define NNK_ATTN_DISPATCH(args, bf, FN, ...)                                                       \
+    [&]() {                                                                                        \
+        const bool cap_ = (args).c2 != 0.0f, bias_ = (args).buckets > 0;                           \
+        const int dp_ = ((args).dim + 31) / 32;                                                    \
+        auto by_dim = [&](auto type, auto cap, auto bias) {                                        \
+            using T_ = decltype(type);                                                             \
+            switch (dp_) {                                                                         \
+            case 1: return FN<T_, 32, decltype(cap)::value, decltype(bias)::value>(__VA_ARGS__);   \
+            case 2: return FN<T_, 64, decltype(cap)::value, decltype(bias)::value>(__VA_ARGS__);   \
+            case 3: return FN<T_, 96, decltype(cap)::value, decltype(bias)::value>(__VA_ARGS__);   \
+            default: return FN<T_, 128, decltype(cap)::value, decltype(bias)::value>(__VA_ARGS__); \
+            }                                                                                      \
+        };                                                                                         \
+        auto by_terms = [&](auto type) {                                                           \
+            if (cap_) return bias_ ? by_dim(type, std::true_type{}, std::true_type{})              \
+                                   : by_dim(type, std::true_type{}, std::false_type{});            \
+            return bias_ ? by_dim(type, std::false_type{}, std::true_type{})                       \
+                         : by_dim(type, std::false_type{}, std::false_type{});                     \
+        };                                                                                         \
+        return (bf) ? by_terms(attn::bf16{}) : by_terms(0.0f);                                     \
+    }()

@@ -1,0 +1,292 @@
+// k_attn_bwd_kv.hip -- attention, gradients of keys, values and the bias.
+//
+// With p_ij = 2^(x_ij - M_i) and dx_ij = p_ij (dp_ij - D_i) from the statistics that the
+// query gradient left:
+//     dv_j = sum_i p_ij dout_i,   dk_j = scale * sum_i dx_ij (1 - t_ij^2) q_i
+// over the queries of all heads that share the key.  A workgroup has 128 keys of a key
+// head, 32 a wave, with k and v in registers, and goes over the blocks of 64 queries of
+// its heads; q and dout of a block are in LDS.  Scores are formed as queries x keys, so
+// that their registers are the operand of both gradients.  No atomics: a key's sums are
+// one wave's, in a fixed order.
+//
+// Bias: sums of dx by distance j - P.  A 32 x 32 tile has its distances on diagonals;
+// row m's values go m lanes along, after which a lane holds two distances (one for what
+// went past the end), and the tile is 32 shuffles and adds and one addition to the
+// wave's table in LDS.  Tiles wholly past max_distance are added up whole.
+#include "attn_common.h"
+
+namespace {
+using namespace attn;
+
+constexpr int kSlack = 64;  // distances of a tile that reaches past max_distance
+
+template <typename T, int DP, bool CAP, bool BIAS>
+__global__ __launch_bounds__(kTpb, 1) void attn_bwd_kv_kernel(Args a, int tiles) {
+    using L = Lds<T, DP>;
+    __shared__ __attribute__((aligned(16))) char q_lds[L::kBytes];
+    __shared__ __attribute__((aligned(16))) char g_lds[L::kBytes];
+    __shared__ __attribute__((aligned(16))) float M_lds[kBlock];
+    __shared__ __attribute__((aligned(16))) float D_lds[kBlock];
+    __shared__ __attribute__((aligned(16))) int limit_lds[kBlock];
+    __shared__ __attribute__((aligned(16))) int doc_lds[kBlock];
+    __shared__ float table[BIAS ? 2 * kMaxDistance + 1 : 1];
+    extern __shared__ float dist[];  // BIAS: a table of 2 (max_distance + kSlack) + 1 a wave
+
+    const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
+    const int w = nnk::xcd_swizzle(blockIdx.x, gridDim.x);
+    const int tile = w % tiles, kv = w / tiles % a.kv_heads, b = w / tiles / a.kv_heads;
+    const int k0 = tile * kRows, key = k0 + wave * 32 + (lane & 31);
+    const int keys = keys_of(a, b), start = start_of(a, b);
+    const int* docs = a.doc_k ? a.doc_k + (size_t)b * a.len_k : nullptr;
+    const bool in = key < a.len_k;
+    const int doc = docs && in ? docs[key] : -1;
+    const bool live = key < keys && (!docs || doc >= 0);
+    const int wave_doc = __builtin_amdgcn_readfirstlane(doc);
+    const bool whole_keys = __all(live && (!docs || doc == wave_doc));
+    const int last_key = k0 + wave * 32 + 31;
+
+    const int q_blocks = (a.len_q + kBlock - 1) / kBlock;
+    const int4 mine = key_docs_of(a, b, k0 / kBlock, kRows / kBlock);
+    const int4* query_docs = a.query_docs ? a.query_docs + (size_t)b * q_blocks : nullptr;
+    const auto meets = [&](int i) {
+        return limit_of(a, b, keys, start + min((i + 1) * kBlock, a.len_q) - 1) > k0 &&
+            (!query_docs || docs_meet(query_docs[i], mine));
+    };
+
+    Frag<T> kf[L::kSteps], vf[L::kSteps];
+    {
+        const long long r = min(key, a.len_k - 1);
+        const T* k = (const T*)a.k + b * a.ks[0] + r * a.ks[1] + kv * a.ks[2];
+        const T* v = (const T*)a.v + b * a.vs[0] + r * a.vs[1] + kv * a.vs[2];
+#pragma unroll
+        for (int u = 0; u < L::kSteps; ++u) {
+            const int d0 = (2 * u + h) * Type<T>::CE, dim = live ? a.dim : 0;
+            kf[u] = load_frag<T>(k, d0, dim, a.vec);
+            vf[u] = load_frag<T>(v, d0, dim, a.vec);
+        }
+    }
+    f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) {
+        dk[d] = zero16();
+        dv[d] = zero16();
+    }
+    const int span = 2 * (a.max_distance + kSlack) + 1;
+    float* my_dist = dist + wave * span;
+
+    for (int head = kv * a.group; head < (kv + 1) * a.group; ++head) {
+        float far_lo = 0.0f, far_hi = 0.0f;
+        if constexpr (BIAS) {
+            __syncthreads();
+            load_bias(a, table, head);
+            for (int i = threadIdx.x; i < kWaves * span; i += kTpb) dist[i] = 0.0f;
+        }
+        const T* qp = (const T*)a.q + b * a.qs[0] + head * a.qs[2];
+        const T* gp = (const T*)a.dout + b * a.os[0] + head * a.os[2];
+        const float2* stats = a.stat + ((size_t)b * a.heads + head) * a.len_q;
+
+        Staged<T, DP> qs, gs;
+        float2 st = {INFINITY, 0.0f};
+        int lim = 0, qdoc = -1;
+        const auto load = [&](int block) {
+            const int q0 = block * kBlock;
+            // queries that see nothing are zeros, whatever they hold
+            const auto alive = [&](int r) { return q0 + r < a.len_q && stats[q0 + r].x != INFINITY; };
+            qs.load(qp + q0 * a.qs[1], a.qs[1], a.dim, a.vec, alive);
+            gs.load(gp + q0 * a.os[1], a.os[1], a.dim, a.vec, alive);
+            if (threadIdx.x < kBlock) {
+                const int i = q0 + (int)threadIdx.x;
+                st = i < a.len_q ? stats[i] : float2{INFINITY, 0.0f};
+                lim = i < a.len_q ? limit_of(a, b, keys, start + i) : 0;
+                qdoc = a.doc_q && i < a.len_q ? a.doc_q[(size_t)b * a.len_q + i] : -2;
+            }
+        };
+
+        Blocks<decltype(meets)> at(0, q_blocks, meets);
+        int block = at.next();
+        if (block >= 0) load(block);
+        while (block >= 0) {
+            __syncthreads();
+            qs.store(q_lds);
+            gs.store(g_lds);
+            if (threadIdx.x < kBlock) {
+                M_lds[threadIdx.x] = st.x;
+                D_lds[threadIdx.x] = st.y;
+                limit_lds[threadIdx.x] = lim;
+                doc_lds[threadIdx.x] = qdoc;
+            }
+            __syncthreads();
+            const int q0 = block * kBlock;
+            block = at.next();
+            if (block >= 0) load(block);
+
+            bool whole = whole_keys && limit_lds[0] > last_key;
+            if (docs) {
+                const int4 d = query_docs[q0 / kBlock];
+                whole = whole && d.x == wave_doc && d.y == wave_doc && !d.z;
+            }
+#pragma unroll 1
+            for (int i = 0; i < 2; ++i) {
+                f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+                for (int u = 0; u < L::kSteps; ++u) {
+                    s = mma(L::rows(q_lds, 32 * i + (lane & 31), u, h), kf[u], s);
+                    dp = mma(L::rows(g_lds, 32 * i + (lane & 31), u, h), vf[u], dp);
+                }
+                f32x16 slope;
+                if constexpr (CAP) cap_scores<true>(s, slope, a.c1);
+                const float c = CAP ? a.c2 : a.c1;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] *= c;
+                if constexpr (BIAS) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int rel = key - (start + q0 + 32 * i + row_of(r, h));
+                        s[r] += table[min(max(rel, -a.max_distance), a.max_distance) + a.max_distance];
+                    }
+                }
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const f32x4 M = *reinterpret_cast<const f32x4*>(M_lds + 32 * i + 8 * g + 4 * h);
+                    const f32x4 D = *reinterpret_cast<const f32x4*>(D_lds + 32 * i + 8 * g + 4 * h);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int r = 4 * g + j, row = 32 * i + 8 * g + 4 * h + j;
+                        float p = exp2_fast(s[r] - M[j]);
+                        if (!whole) {
+                            const bool sees = live && key < limit_lds[row] && (!docs || doc_lds[row] == doc);
+                            p = sees ? p : 0.0f;
+                        }
+                        s[r] = p;
+                        dp[r] = p == 0.0f ? 0.0f : p * (dp[r] - D[j]);
+                    }
+                }
+                if constexpr (BIAS) {
+                    const int base = k0 + wave * 32 - (start + q0 + 32 * i);  // distance of row 0, column 0
+                    const int m = a.max_distance;
+                    if (base + 31 <= -m || base - 31 >= m) {
+                        float sum = 0.0f;
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) sum += dp[r];
+                        if (base + 31 <= -m) far_lo += sum;
+                        else far_hi += sum;
+                    } else {
+                        float up = 0.0f, down = 0.0f;  // distances base + n and base + n - 32
+                        const int n = lane & 31;
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const int row = row_of(r, h), from = (n + row) & 31;
+                            const float v = __shfl(dp[r], from + 32 * h);
+                            up += n + row < 32 ? v : 0.0f;
+                            down += n + row < 32 ? 0.0f : v;
+                        }
+                        up = sum_halves(up);
+                        down = sum_halves(down);
+                        const int where = base + n - 32 * h + m + kSlack;
+                        my_dist[where] += h ? down : up;
+                    }
+                }
+                if constexpr (CAP) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) dp[r] *= slope[r];
+                }
+#pragma unroll
+                for (int f = 0; f < L::kKeySteps; ++f) {
+                    const Frag<T> p = operand(s, f, T{}), x = operand(dp, f, T{});
+#pragma unroll
+                    for (int d = 0; d < DP / 32; ++d) {
+                        dv[d] = mma(L::cols(g_lds, 32 * i, f, 32 * d, lane), p, dv[d]);
+                        dk[d] = mma(L::cols(q_lds, 32 * i, f, 32 * d, lane), x, dk[d]);
+                    }
+                }
+            }
+        }
+        if constexpr (BIAS) {
+            // the far tiles join the ends of the table; then one sum a distance
+            far_lo = nnk::wave_sum(far_lo);
+            far_hi = nnk::wave_sum(far_hi);
+            __syncthreads();
+            if (lane == 0) {
+                my_dist[0] += far_lo;
+                my_dist[span - 1] += far_hi;
+            }
+            __syncthreads();
+            if (a.dist_sums) {
+                const int n = 2 * a.max_distance + 1;
+                float* to = a.dist_sums + (((size_t)b * a.heads + head) * tiles + tile) * n;
+                for (int i = threadIdx.x; i < n; i += kTpb) {
+                    float sum = 0.0f;
+                    const int first = i == 0 ? 0 : i + kSlack, last = i == n - 1 ? span : i + kSlack + 1;
+                    for (int wv = 0; wv < kWaves; ++wv)
+                        for (int j = first; j < last; ++j) sum += dist[wv * span + j];
+                    to[i] = sum;
+                }
+            }
+        }
+    }
+
+    if (!in) return;
+    T* kout = (T*)a.dk + b * a.ks[0] + (long long)key * a.ks[1] + kv * a.ks[2];
+    T* vout = (T*)a.dv + b * a.vs[0] + (long long)key * a.vs[1] + kv * a.vs[2];
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int at = 32 * d + 8 * g + 4 * h;
+            store4<T>(kout, at, a.dim, a.vec, dk[d][4 * g] * a.scale, dk[d][4 * g + 1] * a.scale,
+                dk[d][4 * g + 2] * a.scale, dk[d][4 * g + 3] * a.scale);
+            store4<T>(vout, at, a.dim, a.vec, dv[d][4 * g], dv[d][4 * g + 1], dv[d][4 * g + 2], dv[d][4 * g + 3]);
+        }
+}
+
+// dbias[bucket, head]: the sums of its distances over batch and key tiles, in 64 bits,
+// a thread's rows in order and the threads' sums as a tree.
+__global__ __launch_bounds__(kTpb) void attn_bias_grad_kernel(float* dbias, const float* dist_sums, const int* bucket,
+    int batch, int heads, int buckets, int tiles, int n) {
+    __shared__ double part[kTpb];
+    const int head = blockIdx.x % heads, mine = blockIdx.x / heads;
+    double sum = 0.0;
+    for (int i = 0; i < n; ++i) {
+        if (min(max(bucket[i], 0), buckets - 1) != mine) continue;
+        for (int r = threadIdx.x; r < batch * tiles; r += kTpb)
+            sum += dist_sums[(((size_t)(r / tiles) * heads + head) * tiles + r % tiles) * n + i];
+    }
+    part[threadIdx.x] = sum;
+    for (int m = kTpb / 2; m > 0; m >>= 1) {
+        __syncthreads();
+        if ((int)threadIdx.x < m) part[threadIdx.x] += part[threadIdx.x + m];
+    }
+    if (threadIdx.x == 0) dbias[(size_t)mine * heads + head] = (float)part[0];
+}
+
+template <typename T, int DP, bool CAP, bool BIAS>
+bool launch(const Args& a, hipStream_t s, const char* what) {
+    const int tiles = (a.len_k + kRows - 1) / kRows;
+    const size_t lds = BIAS ? kWaves * (2 * (a.max_distance + kSlack) + 1) * sizeof(float) : 0;
+    if constexpr (BIAS) {
+        static std::atomic<unsigned long long> done{0};
+        if (!raise_lds((const void*)attn_bwd_kv_kernel<T, DP, CAP, BIAS>,
+                kWaves * (2 * (kMaxDistance + kSlack) + 1) * sizeof(float), done, what))
+            return false;
+    }
+    attn_bwd_kv_kernel<T, DP, CAP, BIAS>
+        <<<(unsigned)((long long)tiles * a.kv_heads * a.batch), kTpb, lds, s>>>(a, tiles);
+    nnk_after_launch(what, s);
+    return true;
+}
+
+}  // namespace
+
+bool nnk_attention_backward_kv(const Args& a, bool half, hipStream_t s, const char* what) {
+    return NNK_ATTN_DISPATCH(a, half, launch, a, s, what);
+}
+
+size_t nnk_attention_dist_floats(const NnAttention* a) {
+    return (size_t)a->batch * a->heads * ((a->len_k + kRows - 1) / kRows) * (2 * a->max_distance + 1);
+}
+
+void nnk_attention_bias_grad(const Args& a, float* dbias, hipStream_t s, const char* what) {
+    attn_bias_grad_kernel<<<(unsigned)(a.buckets * a.heads), kTpb, 0, s>>>(dbias, a.dist_sums, a.bucket, a.batch,
+        a.heads, a.buckets, (a.len_k + kRows - 1) / kRows, 2 * a.max_distance + 1);
+    nnk_after_launch(what, s);
+}

@@ -1,0 +1,214 @@
+// k_attn_bwd_q.hip -- attention, gradient of the queries.
+//
+// With p_ij = 2^(x_ij - M_i), dp_ij = <dout_i, v_j> and D_i = sum_j p_ij dp_ij:
+//     dx_ij = p_ij (dp_ij - D_i),   dq_i = scale * sum_j dx_ij (1 - t_ij^2) k_j
+// (t the capped score's tanh).  A workgroup has 128 queries of a head, 32 a wave, with
+// q and dout in registers, and goes over the blocks of keys as the forward kernel does.
+//
+// M comes from the forward pass's lse and D from <dout, out>, both of which that pass
+// rounded.  The sums of p and of p dp are taken along, and their exact results are what
+// the key gradients and the bias gradient use (stat).  Where all keys of the workgroup
+// lie in one block they are there before it is used, and the query gradient takes them
+// too: a query that sees a single key then gets a gradient of exactly zero.
+#include "attn_common.h"
+
+namespace {
+using namespace attn;
+
+template <typename T, int DP, bool CAP, bool BIAS>
+__global__ __launch_bounds__(kTpb, 1) void attn_bwd_q_kernel(Args a, int tiles) {
+    using L = Lds<T, DP>;
+    __shared__ __attribute__((aligned(16))) char k_lds[L::kBytes];
+    __shared__ __attribute__((aligned(16))) char v_lds[L::kBytes];
+    __shared__ int doc_lds[kBlock];
+    __shared__ float table[BIAS ? 2 * kMaxDistance + 1 : 1];
+
+    const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
+    const int w = nnk::xcd_swizzle(blockIdx.x, gridDim.x);
+    const int tile = tiles - 1 - w % tiles;
+    const int head = w / tiles % a.heads, b = w / tiles / a.heads;
+    const int row0 = tile * kRows, row = row0 + wave * 32 + (lane & 31);
+    const bool in = row < a.len_q;
+    const int keys = keys_of(a, b), start = start_of(a, b);
+    const int pos = start + row;
+    const int limit = in ? limit_of(a, b, keys, pos) : 0;
+    const int doc = in && a.doc_q ? a.doc_q[(size_t)b * a.len_q + row] : -1;
+    int least = in ? limit : INT32_MAX;
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) least = min(least, __shfl_xor(least, m));
+    const int wave_doc = __builtin_amdgcn_readfirstlane(doc);
+    const bool one_doc = __all(doc == wave_doc || !in) && wave_doc >= 0;
+
+    const int most = limit_of(a, b, keys, start + min(row0 + kRows, a.len_q) - 1);
+    const int4 mine = query_docs_of(a, b, row0 / kBlock, kRows / kBlock);
+    const int blocks = (a.len_k + kBlock - 1) / kBlock;
+    const int4* key_docs = a.key_docs ? a.key_docs + (size_t)b * blocks : nullptr;
+    const auto meets = [&](int i) { return !key_docs || docs_meet(key_docs[i], mine); };
+    Blocks<decltype(meets)> at(0, (most + kBlock - 1) / kBlock, meets);
+
+    const size_t stat_at = ((size_t)b * a.heads + head) * a.len_q + row;
+    const float lse = in ? a.lse[stat_at] : -INFINITY;
+    const bool sees_any = lse != -INFINITY;  // a query that sees nothing may hold anything
+    float M = sees_any ? lse * kLog2e : INFINITY;
+    Frag<T> qf[L::kSteps], gf[L::kSteps];
+    float D = 0.0f;
+    {
+        const long long r = min(row, a.len_q - 1);
+        const T* q = (const T*)a.q + b * a.qs[0] + r * a.qs[1] + head * a.qs[2];
+        const long long o = b * a.os[0] + r * a.os[1] + head * a.os[2];
+        const T *g = (const T*)a.dout + o, *out = (const T*)a.out + o;
+#pragma unroll
+        for (int u = 0; u < L::kSteps; ++u) {
+            const int d0 = (2 * u + h) * Type<T>::CE, dim = sees_any ? a.dim : 0;
+            qf[u] = load_frag<T>(q, d0, dim, a.vec);
+            gf[u] = load_frag<T>(g, d0, dim, a.vec);
+            const Frag<T> of = load_frag<T>(out, d0, dim, a.vec);
+#pragma unroll
+            for (int j = 0; j < Type<T>::CE; ++j) D = fmaf((float)gf[u][j], (float)of[j], D);
+        }
+        D = sum_halves(D);
+    }
+    const int kv = head / a.group;
+    const T* kp = (const T*)a.k + b * a.ks[0] + kv * a.ks[2];
+    const T* vp = (const T*)a.v + b * a.vs[0] + kv * a.vs[2];
+    const int* docs = a.doc_k ? a.doc_k + (size_t)b * a.len_k : nullptr;
+    if constexpr (BIAS) load_bias(a, table, head);
+
+    Staged<T, DP> ks, vs;
+    int next_doc = 0;
+    const auto load = [&](int block) {
+        const int k0 = block * kBlock;
+        const auto live = [&](int r) { return k0 + r < keys && (!docs || docs[k0 + r] >= 0); };
+        ks.load(kp + k0 * a.ks[1], a.ks[1], a.dim, a.vec, live);
+        vs.load(vp + k0 * a.vs[1], a.vs[1], a.dim, a.vec, live);
+        if (docs && threadIdx.x < kBlock) next_doc = k0 + (int)threadIdx.x < keys ? docs[k0 + threadIdx.x] : -1;
+    };
+
+    f32x16 dq[DP / 32];
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) dq[d] = zero16();
+    float l = 0.0f, pd = 0.0f;  // sums of p and of p dp
+
+    int block = at.next();
+    if (block >= 0) load(block);
+    for (bool first = true; block >= 0; first = false) {
+        __syncthreads();
+        ks.store(k_lds);
+        vs.store(v_lds);
+        if (docs && threadIdx.x < kBlock) doc_lds[threadIdx.x] = next_doc;
+        __syncthreads();
+        const int k0 = block * kBlock;
+        block = at.next();
+        if (block >= 0) load(block);
+
+        bool whole = k0 + kBlock <= least;
+        if (docs) {
+            const int4 d = key_docs[k0 / kBlock];
+            whole = whole && one_doc && d.x == wave_doc && d.y == wave_doc && !d.z;
+        }
+        // scores (in units of log2) and dp of keys 32 i .. 32 i + 31; slope: 1 - tanh^2
+        const auto products = [&](int i, f32x16& s, f32x16& dp, f32x16& slope) {
+            s = zero16();
+            dp = zero16();
+#pragma unroll
+            for (int u = 0; u < L::kSteps; ++u) {
+                s = mma(L::rows(k_lds, 32 * i + (lane & 31), u, h), qf[u], s);
+                dp = mma(L::rows(v_lds, 32 * i + (lane & 31), u, h), gf[u], dp);
+            }
+            if constexpr (CAP) cap_scores<true>(s, slope, a.c1);
+            const float c = CAP ? a.c2 : a.c1;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] *= c;
+            if constexpr (BIAS) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int rel = k0 + 32 * i + row_of(r, h) - pos;
+                    s[r] += table[min(max(rel, -a.max_distance), a.max_distance) + a.max_distance];
+                }
+            }
+            if (!whole) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int j = 32 * i + row_of(r, h);
+                    const bool sees = k0 + j < limit && (!docs || (doc_lds[j] == doc && doc >= 0));
+                    s[r] = sees ? s[r] : -INFINITY;
+                }
+            }
+        };
+        if (first && block < 0) {  // the only block
+            float m = -INFINITY, sum = 0.0f, dot = 0.0f;
+#pragma unroll 1
+            for (int i = 0; i < 2; ++i) {
+                f32x16 s, dp, slope;
+                products(i, s, dp, slope);
+                float top = m;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
+                top = max_halves(top);
+                const float base = top == -INFINITY ? 0.0f : top, f = exp2_fast(m - base);
+                sum *= f;
+                dot *= f;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const float p = exp2_fast(s[r] - base);
+                    sum += p;
+                    dot = p == 0.0f ? dot : fmaf(p, dp[r], dot);
+                }
+                m = top;
+            }
+            sum = sum_halves(sum);
+            dot = sum_halves(dot);
+            if (sees_any) {
+                M = m + log2f(sum);
+                D = dot / sum;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            f32x16 s, dp, slope;
+            products(i, s, dp, slope);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float p = exp2_fast(s[r] - M);
+                l += p;
+                const float w = p * dp[r];
+                pd += p == 0.0f ? 0.0f : w;
+                float dx = p == 0.0f ? 0.0f : p * (dp[r] - D);
+                if constexpr (CAP) dx *= slope[r];
+                s[r] = dx;
+            }
+#pragma unroll
+            for (int f = 0; f < L::kKeySteps; ++f) {
+                const Frag<T> x = operand(s, f, T{});
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d) dq[d] = mma(L::cols(k_lds, 32 * i, f, 32 * d, lane), x, dq[d]);
+            }
+        }
+    }
+
+    if (!in) return;
+    l = sum_halves(l);
+    pd = sum_halves(pd);
+    T* out = (T*)a.dq + b * a.qs[0] + (long long)row * a.qs[1] + head * a.qs[2];
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            store4<T>(out, 32 * d + 8 * g + 4 * h, a.dim, a.vec, dq[d][4 * g] * a.scale, dq[d][4 * g + 1] * a.scale,
+                dq[d][4 * g + 2] * a.scale, dq[d][4 * g + 3] * a.scale);
+    if (h == 0) a.stat[stat_at] = sees_any ? float2{M + log2f(l), pd / l} : float2{INFINITY, 0.0f};
+}
+
+template <typename T, int DP, bool CAP, bool BIAS>
+bool launch(const Args& a, hipStream_t s, const char* what) {
+    const int tiles = (a.len_q + kRows - 1) / kRows;
+    attn_bwd_q_kernel<T, DP, CAP, BIAS><<<(unsigned)((long long)tiles * a.heads * a.batch), kTpb, 0, s>>>(a, tiles);
+    nnk_after_launch(what, s);
+    return true;
+}
+
+}  // namespace
+
+bool nnk_attention_backward_q(const Args& a, bool half, hipStream_t s, const char* what) {
+    return NNK_ATTN_DISPATCH(a, half, launch, a, s, what);
+}

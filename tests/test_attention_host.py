@@ -1,0 +1,186 @@
+"""The attention operators' host side: refusals, sizes of workspaces, calls with nothing
+to do, and the tests' own gradient formulas against differences."""
+from __future__ import annotations
+
+import ctypes
+import re
+
+import numpy as np
+import pytest
+
+from attention_ref import attention, norm_rope
+
+DUMMY = 16  # never dereferenced: every check of the host comes before a launch
+
+
+def _attn(nn, **more):
+    a = dict(dtype=nn.NN_F32, batch=1, len_q=4, len_k=4, heads=2, kv_heads=1, head_dim=8, scale=0.3, softcap=0.0,
+             mask=nn.NN_MASK_NONE, q_stride=(64, 16, 8), k_stride=(32, 8, 8), v_stride=(32, 8, 8),
+             out_stride=(64, 16, 8))
+    a.update(more)
+    return nn.NnAttention(**a)
+
+
+def _rope(nn, **more):
+    a = dict(dtype=nn.NN_F32, tokens=4, heads=2, kv_heads=1, head_dim=8, rot_dim=8, axes=1, interleaved=0, eps=1e-6,
+             q_stride=(16, 8), k_stride=(8, 8), q_out_stride=(16, 8), k_out_stride=(8, 8), pos=DUMMY, freq=DUMMY)
+    a.update(more)
+    return nn.NnQkNormRope(**a)
+
+
+BAD_ATTN = [
+    (dict(dtype=7), "unknown dtype 7"),
+    (dict(batch=-1), "bad shape"),
+    (dict(len_q=-2), "bad shape"),
+    (dict(heads=3, kv_heads=2), "not a multiple of kv_heads"),
+    (dict(heads=0), "not a multiple of kv_heads|heads=0"),
+    (dict(kv_heads=0), "kv_heads=0"),
+    (dict(head_dim=0), "head_dim=0"),
+    (dict(head_dim=129), "head_dim=129"),
+    (dict(scale=0.0), "scale=0"),
+    (dict(scale=float("nan")), "scale=nan"),
+    (dict(softcap=-1.0), "softcap=-1"),
+    (dict(mask=9), "unknown mask 9"),
+    (dict(mask=2), "null prefix"),
+    (dict(doc_q=DUMMY), "documents of queries or keys only"),
+    (dict(buckets=4, max_distance=4), "null bucket or bias"),
+    (dict(buckets=4, max_distance=1024, bucket=DUMMY, bias=DUMMY), "max_distance=1024"),
+    (dict(buckets=-1), "buckets=-1"),
+    (dict(batch=1 << 20, len_q=1 << 20), "too many rows"),
+]
+
+
+@pytest.mark.parametrize("more, text", BAD_ATTN, ids=[t for _, t in BAD_ATTN])
+def test_attention_refusals(nn, more, text):
+    L = nn.lib()
+    L.last_error()
+    a = _attn(nn, **more)
+    with pytest.raises(nn.NnHipError, match=f"launch_attention_forward: error 1: .*({text})"):
+        L.launch_attention_forward(DUMMY, DUMMY, DUMMY, DUMMY, DUMMY, a, DUMMY, None)
+    with pytest.raises(nn.NnHipError, match=f"launch_attention_backward: error 1: .*({text})"):
+        L.launch_attention_backward(*[DUMMY] * 3, None, *[DUMMY] * 6, a, DUMMY, None)
+    assert L.last_error()[0] == 0
+
+
+def test_attention_null_pointers(nn):
+    L = nn.lib()
+    L.last_error()
+    a = _attn(nn)
+    for hole in range(5):
+        args = [None if i == hole else DUMMY for i in range(5)]
+        with pytest.raises(nn.NnHipError, match="null pointer"):
+            L.launch_attention_forward(*args, a, None, None)
+    for hole in (0, 1, 2, 4, 5, 6, 7, 8, 9):
+        args = [None if i in (hole, 3) else DUMMY for i in range(10)]
+        with pytest.raises(nn.NnHipError, match="null pointer"):
+            L.launch_attention_backward(*args, a, DUMMY, None)
+    with pytest.raises(nn.NnHipError, match="null description"):
+        L.launch_attention_forward(*[DUMMY] * 5, None, None, None)
+    with pytest.raises(nn.NnHipError, match="null workspace"):
+        L.launch_attention_backward(*[DUMMY] * 3, None, *[DUMMY] * 6, a, None, None)
+    with pytest.raises(nn.NnHipError, match="not aligned"):
+        L.launch_attention_backward(*[DUMMY] * 3, None, *[DUMMY] * 6, a, 20, None)
+    with pytest.raises(nn.NnHipError, match="bias gradient without a bias"):
+        L.launch_attention_backward(*[DUMMY] * 10, a, DUMMY, None)
+
+
+BAD_ROPE = [
+    (dict(dtype=-1), "unknown dtype"),
+    (dict(tokens=-1), "bad shape"),
+    (dict(heads=-1), "bad shape"),
+    (dict(head_dim=0, rot_dim=0), "head_dim=0"),
+    (dict(head_dim=257), "head_dim=257"),
+    (dict(rot_dim=10), "rot_dim=10"),
+    (dict(rot_dim=3), "rot_dim=3"),
+    (dict(axes=0), "axes=0"),
+    (dict(axes=3), "axes=3"),
+    (dict(eps=-1.0), "eps=-1"),
+    (dict(pos=None), "null pos or freq"),
+    (dict(freq=None), "null pos or freq"),
+    (dict(tokens=1 << 30), "too many rows"),
+]
+
+
+@pytest.mark.parametrize("more, text", BAD_ROPE, ids=[t for _, t in BAD_ROPE])
+def test_rope_refusals(nn, more, text):
+    L = nn.lib()
+    L.last_error()
+    a = _rope(nn, **more)
+    with pytest.raises(nn.NnHipError, match=f"launch_qk_norm_rope_forward: error 1: .*{text}"):
+        L.launch_qk_norm_rope_forward(*[DUMMY] * 4, a, None)
+    with pytest.raises(nn.NnHipError, match=f"launch_qk_norm_rope_backward: error 1: .*{text}"):
+        L.launch_qk_norm_rope_backward(*[DUMMY] * 8, a, DUMMY, None)
+
+
+def test_rope_null_pointers(nn):
+    L = nn.lib()
+    L.last_error()
+    a = _rope(nn)
+    for hole in range(4):
+        with pytest.raises(nn.NnHipError, match="null pointer"):
+            L.launch_qk_norm_rope_forward(*[None if i == hole else DUMMY for i in range(4)], a, None)
+    with pytest.raises(nn.NnHipError, match="null workspace"):
+        L.launch_qk_norm_rope_backward(*[DUMMY] * 8, a, None, None)
+
+
+def test_nothing_to_do(nn):
+    L = nn.lib()
+    L.last_error()
+    L.launch_attention_forward(*[None] * 5, _attn(nn, batch=0), None, None)
+    L.launch_attention_forward(*[None] * 5, _attn(nn, len_q=0), None, None)
+    L.launch_attention_backward(*[None] * 10, _attn(nn, batch=0), None, None)
+    L.launch_qk_norm_rope_forward(*[None] * 4, _rope(nn, tokens=0), None)
+    L.launch_qk_norm_rope_backward(*[None] * 8, _rope(nn, heads=0, kv_heads=0), None, None)
+    assert L.last_error()[0] == 0
+
+
+def test_structures_match_the_header(nn):
+    """Field names and kinds of the ctypes mirrors, in the header's order."""
+    text = (nn.INCLUDE_DIR / "nn_attention.h").read_text()
+    text = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
+    for name in ("NnQkNormRope", "NnAttention"):
+        body = re.search(r"typedef struct \{([^}]*)\} " + name, text).group(1)
+        want = []
+        for line in filter(None, (s.strip() for s in body.split(";"))):
+            kind, names = re.match(r"((?:const )?(?:long long|\w+)\*?)\s*(.*)", line, flags=re.S).groups()
+            for field in names.split(","):
+                n = re.match(r"\s*(\w+)(?:\[(\d)\])?", field)
+                base = {"int": ctypes.c_int, "float": ctypes.c_float, "long long": ctypes.c_longlong}.get(kind, ctypes.c_void_p)
+                want.append((n.group(1), base * int(n.group(2)) if n.group(2) else base))
+        assert getattr(nn, name)._fields_ == want
+
+
+def test_reference_gradients_by_differences():
+    """The formulas that the GPU tests compare with, against central differences in 64 bits."""
+    rng = np.random.default_rng(3)
+    c = dict(batch=2, len_q=5, len_k=6, heads=4, kv_heads=2, dim=3, scale=0.7, cap=2.0, mask="prefix", prefix=[3, 0],
+             buckets=3, max_distance=2, doc_q=[[0, 0, 1, 1, -1], [0, 0, 0, 2, 2]],
+             doc_k=[[0, 0, 0, 1, 1, -1], [0, 0, 0, 0, 2, 2]])
+    x = {"q": rng.standard_normal((2, 5, 4, 3)), "k": rng.standard_normal((2, 6, 2, 3)),
+         "v": rng.standard_normal((2, 6, 2, 3)), "bias": rng.standard_normal((3, 4))}
+    bucket = np.array([0, 1, 1, 2, 2])
+    dout = rng.standard_normal((2, 5, 4, 3))
+    got, _ = attention(c, **x, bucket=bucket, dout=dout)
+    for n in x:
+        for _ in range(12):
+            at = tuple(rng.integers(0, s) for s in x[n].shape)
+            side = []
+            for step in (1e-5, -1e-5):
+                y = {m: z.copy() for m, z in x.items()}
+                y[n][at] += step
+                side.append((attention(c, **y, bucket=bucket)[0]["out"] * dout).sum())
+            # truncation 1e-10 of the third derivative, cancellation 1e-16 / 1e-5
+            assert abs((side[0] - side[1]) / 2e-5 - got["d" + n][at]) < 1e-7
+    for interleaved in (False, True):
+        x, w = rng.standard_normal((4, 2, 8)), rng.standard_normal(8)
+        grad, pos, freq = rng.standard_normal((4, 2, 8)), rng.integers(0, 50, (4, 2)), rng.random(2)
+        call = lambda x, w: (norm_rope(x, w, 1e-6, pos, freq, 4, 2, interleaved) * grad).sum()  # noqa: E731
+        _, dx, dw, _ = norm_rope(x, w, 1e-6, pos, freq, 4, 2, interleaved, grad)
+        for _ in range(12):
+            at, d = tuple(rng.integers(0, s) for s in x.shape), rng.integers(0, 8)
+            e = np.zeros_like(x)
+            e[at] = 1e-5
+            assert abs((call(x + e, w) - call(x - e, w)) / 2e-5 - dx[at]) < 1e-7
+            f = np.zeros(8)
+            f[d] = 1e-5
+            assert abs((call(x, w + f) - call(x, w - f)) / 2e-5 - dw[d]) < 1e-7
