@@ -150,23 +150,23 @@ __device__ __forceinline__ f32x4 operand(const f32x16& s, int f, float) {
     return v;
 }
 
-// 16 bytes of a row from feature d0 on, zeros from `dim` on.
+// 16 bytes of a row from feature d0 on.  Features from `dim` on are zeros, or (vec) a
+// chunk wholly past them is the row's first one, for the caller to leave out: a choice
+// here would wait for the load.
 template <typename T>
 __device__ __forceinline__ u32x4 load_chunk(const T* row, int d0, int dim, bool vec) {
-    u32x4 v = {0, 0, 0, 0};
-    if (vec) {
-        if (d0 < dim) v = *reinterpret_cast<const u32x4*>(row + d0);
-    } else {
-        T e[Type<T>::CE];
+    if (vec) return *reinterpret_cast<const u32x4*>(row + (d0 < dim ? d0 : 0));
+    T e[Type<T>::CE];
 #pragma unroll
-        for (int j = 0; j < Type<T>::CE; ++j) e[j] = d0 + j < dim ? row[d0 + j] : (T)0.0f;
-        __builtin_memcpy(&v, e, 16);
-    }
+    for (int j = 0; j < Type<T>::CE; ++j) e[j] = d0 + j < dim ? row[d0 + j] : (T)0.0f;
+    u32x4 v;
+    __builtin_memcpy(&v, e, 16);
     return v;
 }
 template <typename T>
 __device__ __forceinline__ Frag<T> load_frag(const T* row, int d0, int dim, bool vec) {
-    return __builtin_bit_cast(Frag<T>, load_chunk<T>(row, d0, dim, vec));
+    const u32x4 v = load_chunk<T>(row, d0, dim, vec);
+    return __builtin_bit_cast(Frag<T>, d0 < dim ? v : u32x4{0, 0, 0, 0});
 }
 
 // Four consecutive features d..d+3 of an output row.
@@ -199,21 +199,24 @@ struct Staged {
     static constexpr int N = kBlock * kPerRow / kTpb;
     u32x4 v[N];
 
-    // Row r of the tile is base + r * stride if live(r), zeros otherwise.
-    template <typename Live>
-    __device__ __forceinline__ void load(const T* base, long long stride, int dim, bool vec, const Live& live) {
+    static __device__ __forceinline__ int row(int n) { return (n * kTpb + (int)threadIdx.x) / kPerRow; }
+    // Row r of the tile is base + min(r, last) * stride.
+    __device__ __forceinline__ void load(const T* base, long long stride, int last, int dim, bool vec) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int at = n * kTpb + (int)threadIdx.x, r = at / kPerRow, c = at % kPerRow;
-            v[n] = u32x4{0, 0, 0, 0};
-            if (live(r)) v[n] = load_chunk<T>(base + r * stride, c * Type<T>::CE, dim, vec);
+            const int c = (n * kTpb + (int)threadIdx.x) % kPerRow;
+            v[n] = load_chunk<T>(base + min(row(n), last) * stride, c * Type<T>::CE, dim, vec);
         }
     }
-    __device__ __forceinline__ void store(char* lds) const {
+    // Zeros in place of the rows that are not kept, whatever they hold, and of features
+    // from `dim` on; keep(n): this lane's n-th row.
+    template <typename Keep>
+    __device__ __forceinline__ void store(char* lds, int dim, const Keep& keep) const {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int at = n * kTpb + (int)threadIdx.x, r = at / kPerRow, c = at % kPerRow;
-            *reinterpret_cast<u32x4*>(lds + r * Lds<T, DP>::kRowBytes + c * 16) = v[n];
+            const int c = (n * kTpb + (int)threadIdx.x) % kPerRow;
+            *reinterpret_cast<u32x4*>(lds + row(n) * Lds<T, DP>::kRowBytes + c * 16) =
+                keep(n) && c * Type<T>::CE < dim ? v[n] : u32x4{0, 0, 0, 0};
         }
     }
 };
@@ -330,19 +333,23 @@ __device__ __forceinline__ int4 key_docs_of(const Args& a, int b, int first, int
     return a.key_docs ? join_docs(a.key_docs + (size_t)b * n, first, min(first + count, n)) : int4{0, 0, 0, 0};
 }
 
-// The blocks first..last-1 that `meets`, in order, 64 of them looked at a time (one a
-// lane).  Uniform over the wave, and over the workgroup if `meets` is.
-template <typename Meets>
+// The blocks first..last-1 that have documents of `mine` among theirs (`docs` null: all),
+// in order, 64 of them looked at a time, one a lane.
 struct Blocks {
-    const Meets& meets;
+    const int4* docs;
+    int4 mine, own;  // own: documents of this lane's block
     int base, last;
     unsigned long long m;
-    __device__ __forceinline__ Blocks(int first, int last_, const Meets& meets_) : meets(meets_), base(first), last(last_) {
+    int doc;  // of the block that next() gave: the one document of all its positions, or -1
+
+    __device__ __forceinline__ Blocks(int first, int last_, const int4* docs_, const int4& mine_)
+        : docs(docs_), mine(mine_), own{0, 0, 0, 0}, base(first), last(last_), doc(-1) {
         look();
     }
     __device__ __forceinline__ void look() {
         const int b = base + (int)(threadIdx.x & 63);
-        m = __ballot(b < last && meets(b));
+        if (docs && b < last) own = docs[b];
+        m = __ballot(b < last && (!docs || docs_meet(own, mine)));
     }
     // The next block, or -1.
     __device__ __forceinline__ int next() {
@@ -351,9 +358,13 @@ struct Blocks {
             if (base >= last) return -1;
             look();
         }
-        const int b = base + __builtin_ctzll(m);
+        const int i = __builtin_ctzll(m);
         m &= m - 1;
-        return b;
+        if (docs) {
+            const int lo = __builtin_amdgcn_readlane(own.x, i), hi = __builtin_amdgcn_readlane(own.y, i);
+            doc = lo == hi && !__builtin_amdgcn_readlane(own.z, i) ? lo : -1;
+        }
+        return base + i;
     }
 };
 

@@ -48,10 +48,10 @@ __global__ __launch_bounds__(kTpb, 1) void attn_bwd_kv_kernel(Args a, int tiles)
     const int q_blocks = (a.len_q + kBlock - 1) / kBlock;
     const int4 mine = key_docs_of(a, b, k0 / kBlock, kRows / kBlock);
     const int4* query_docs = a.query_docs ? a.query_docs + (size_t)b * q_blocks : nullptr;
-    const auto meets = [&](int i) {
-        return limit_of(a, b, keys, start + min((i + 1) * kBlock, a.len_q) - 1) > k0 &&
-            (!query_docs || docs_meet(query_docs[i], mine));
-    };
+    // the first block of queries that can see the tile: their limits rise with their positions
+    int first_block = keys > k0 ? 0 : q_blocks;
+    if (a.mask == NN_MASK_CAUSAL || (a.mask == NN_MASK_PREFIX && a.prefix[b] <= k0))
+        first_block = max(first_block, (k0 - start) >> 6);
 
     Frag<T> kf[L::kSteps], vf[L::kSteps];
     {
@@ -86,45 +86,47 @@ __global__ __launch_bounds__(kTpb, 1) void attn_bwd_kv_kernel(Args a, int tiles)
         const float2* stats = a.stat + ((size_t)b * a.heads + head) * a.len_q;
 
         Staged<T, DP> qs, gs;
+        float row_M[Staged<T, DP>::N];
         float2 st = {INFINITY, 0.0f};
-        int lim = 0, qdoc = -1;
+        int lim = 0, qdoc = -2;
         const auto load = [&](int block) {
-            const int q0 = block * kBlock;
-            // queries that see nothing are zeros, whatever they hold
-            const auto alive = [&](int r) { return q0 + r < a.len_q && stats[q0 + r].x != INFINITY; };
-            qs.load(qp + q0 * a.qs[1], a.qs[1], a.dim, a.vec, alive);
-            gs.load(gp + q0 * a.os[1], a.os[1], a.dim, a.vec, alive);
-            if (threadIdx.x < kBlock) {
-                const int i = q0 + (int)threadIdx.x;
-                st = i < a.len_q ? stats[i] : float2{INFINITY, 0.0f};
-                lim = i < a.len_q ? limit_of(a, b, keys, start + i) : 0;
-                qdoc = a.doc_q && i < a.len_q ? a.doc_q[(size_t)b * a.len_q + i] : -2;
+            const int q0 = block * kBlock, last = a.len_q - 1 - q0;
+#pragma unroll
+            for (int n = 0; n < Staged<T, DP>::N; ++n) row_M[n] = stats[q0 + min(Staged<T, DP>::row(n), last)].x;
+            if (wave == 0) {
+                const int i = q0 + min(lane, last);
+                st = stats[i];
+                if (a.doc_q) qdoc = a.doc_q[(size_t)b * a.len_q + i];
+                lim = limit_of(a, b, keys, start + i);
             }
+            qs.load(qp + q0 * a.qs[1], a.qs[1], last, a.dim, a.vec);
+            gs.load(gp + q0 * a.os[1], a.os[1], last, a.dim, a.vec);
         };
 
-        Blocks<decltype(meets)> at(0, q_blocks, meets);
+        Blocks at(first_block, q_blocks, query_docs, mine);
         int block = at.next();
         if (block >= 0) load(block);
         while (block >= 0) {
             __syncthreads();
-            qs.store(q_lds);
-            gs.store(g_lds);
-            if (threadIdx.x < kBlock) {
-                M_lds[threadIdx.x] = st.x;
-                D_lds[threadIdx.x] = st.y;
-                limit_lds[threadIdx.x] = lim;
-                doc_lds[threadIdx.x] = qdoc;
+            const int q0 = block * kBlock, block_doc = at.doc;
+            // queries that see nothing are zeros
+            const auto keep = [&](int n) {
+                return q0 + Staged<T, DP>::row(n) < a.len_q && row_M[n] != INFINITY;
+            };
+            qs.store(q_lds, a.dim, keep);
+            gs.store(g_lds, a.dim, keep);
+            if (wave == 0) {
+                const bool there = q0 + lane < a.len_q;
+                M_lds[lane] = there ? st.x : INFINITY;
+                D_lds[lane] = st.y;
+                limit_lds[lane] = there ? lim : 0;
+                doc_lds[lane] = there ? qdoc : -2;
             }
             __syncthreads();
-            const int q0 = block * kBlock;
             block = at.next();
             if (block >= 0) load(block);
 
-            bool whole = whole_keys && limit_lds[0] > last_key;
-            if (docs) {
-                const int4 d = query_docs[q0 / kBlock];
-                whole = whole && d.x == wave_doc && d.y == wave_doc && !d.z;
-            }
+            const bool whole = whole_keys && limit_lds[0] > last_key && (!docs || block_doc == wave_doc);
 #pragma unroll 1
             for (int i = 0; i < 2; ++i) {
                 f32x16 s = zero16(), dp = zero16();

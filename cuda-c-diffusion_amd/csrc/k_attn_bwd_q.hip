@@ -43,8 +43,7 @@ __global__ __launch_bounds__(kTpb, 1) void attn_bwd_q_kernel(Args a, int tiles) 
     const int4 mine = query_docs_of(a, b, row0 / kBlock, kRows / kBlock);
     const int blocks = (a.len_k + kBlock - 1) / kBlock;
     const int4* key_docs = a.key_docs ? a.key_docs + (size_t)b * blocks : nullptr;
-    const auto meets = [&](int i) { return !key_docs || docs_meet(key_docs[i], mine); };
-    Blocks<decltype(meets)> at(0, (most + kBlock - 1) / kBlock, meets);
+    Blocks at(0, (most + kBlock - 1) / kBlock, key_docs, mine);
 
     const size_t stat_at = ((size_t)b * a.heads + head) * a.len_q + row;
     const float lse = in ? a.lse[stat_at] : -INFINITY;
@@ -75,13 +74,16 @@ __global__ __launch_bounds__(kTpb, 1) void attn_bwd_q_kernel(Args a, int tiles) 
     if constexpr (BIAS) load_bias(a, table, head);
 
     Staged<T, DP> ks, vs;
-    int next_doc = 0;
+    int row_doc[Staged<T, DP>::N], next_doc = 0;
     const auto load = [&](int block) {
-        const int k0 = block * kBlock;
-        const auto live = [&](int r) { return k0 + r < keys && (!docs || docs[k0 + r] >= 0); };
-        ks.load(kp + k0 * a.ks[1], a.ks[1], a.dim, a.vec, live);
-        vs.load(vp + k0 * a.vs[1], a.vs[1], a.dim, a.vec, live);
-        if (docs && threadIdx.x < kBlock) next_doc = k0 + (int)threadIdx.x < keys ? docs[k0 + threadIdx.x] : -1;
+        const int k0 = block * kBlock, last = keys - 1 - k0;
+        if (docs) {
+#pragma unroll
+            for (int n = 0; n < Staged<T, DP>::N; ++n) row_doc[n] = docs[k0 + min(Staged<T, DP>::row(n), last)];
+            next_doc = docs[k0 + min(lane, last)];
+        }
+        ks.load(kp + k0 * a.ks[1], a.ks[1], last, a.dim, a.vec);
+        vs.load(vp + k0 * a.vs[1], a.vs[1], last, a.dim, a.vec);
     };
 
     f32x16 dq[DP / 32];
@@ -93,19 +95,19 @@ __global__ __launch_bounds__(kTpb, 1) void attn_bwd_q_kernel(Args a, int tiles) 
     if (block >= 0) load(block);
     for (bool first = true; block >= 0; first = false) {
         __syncthreads();
-        ks.store(k_lds);
-        vs.store(v_lds);
-        if (docs && threadIdx.x < kBlock) doc_lds[threadIdx.x] = next_doc;
+        const int k0 = block * kBlock, block_doc = at.doc;
+        // keys that nothing sees are zeros
+        const auto keep = [&](int n) {
+            return k0 + Staged<T, DP>::row(n) < keys && (!docs || row_doc[n] >= 0);
+        };
+        ks.store(k_lds, a.dim, keep);
+        vs.store(v_lds, a.dim, keep);
+        if (docs && wave == 0) doc_lds[lane] = k0 + lane < keys ? next_doc : -1;
         __syncthreads();
-        const int k0 = block * kBlock;
         block = at.next();
         if (block >= 0) load(block);
 
-        bool whole = k0 + kBlock <= least;
-        if (docs) {
-            const int4 d = key_docs[k0 / kBlock];
-            whole = whole && one_doc && d.x == wave_doc && d.y == wave_doc && !d.z;
-        }
+        const bool whole = k0 + kBlock <= least && (!docs || (one_doc && block_doc == wave_doc));
         // scores (in units of log2) and dp of keys 32 i .. 32 i + 31; slope: 1 - tanh^2
         const auto products = [&](int i, f32x16& s, f32x16& dp, f32x16& slope) {
             s = zero16();

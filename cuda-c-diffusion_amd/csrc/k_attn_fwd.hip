@@ -39,8 +39,7 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kernel(
     const int4 mine = query_docs_of(a, b, row0 / kBlock, kRows / kBlock);
     const int blocks = (a.len_k + kBlock - 1) / kBlock;
     const int4* key_docs = a.key_docs ? a.key_docs + (size_t)b * blocks : nullptr;
-    const auto meets = [&](int i) { return !key_docs || docs_meet(key_docs[i], mine); };
-    Blocks<decltype(meets)> at(0, (most + kBlock - 1) / kBlock, meets);
+    Blocks at(0, (most + kBlock - 1) / kBlock, key_docs, mine);
 
     Frag<T> qf[L::kSteps];
     {
@@ -55,14 +54,16 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kernel(
     if constexpr (BIAS) load_bias(a, table, head);
 
     Staged<T, DP> ks, vs;
-    int next_doc = 0;
+    int row_doc[Staged<T, DP>::N], next_doc = 0;
     const auto load = [&](int block) {
-        const int k0 = block * kBlock;
-        // keys that nothing sees are zeros, whatever they hold
-        const auto live = [&](int r) { return k0 + r < keys && (!docs || docs[k0 + r] >= 0); };
-        ks.load(kp + k0 * a.ks[1], a.ks[1], a.dim, a.vec, live);
-        vs.load(vp + k0 * a.vs[1], a.vs[1], a.dim, a.vec, live);
-        if (docs && threadIdx.x < kBlock) next_doc = k0 + (int)threadIdx.x < keys ? docs[k0 + threadIdx.x] : -1;
+        const int k0 = block * kBlock, last = keys - 1 - k0;
+        if (docs) {
+#pragma unroll
+            for (int n = 0; n < Staged<T, DP>::N; ++n) row_doc[n] = docs[k0 + min(Staged<T, DP>::row(n), last)];
+            next_doc = docs[k0 + min(lane, last)];
+        }
+        ks.load(kp + k0 * a.ks[1], a.ks[1], last, a.dim, a.vec);
+        vs.load(vp + k0 * a.vs[1], a.vs[1], last, a.dim, a.vec);
     };
 
     f32x16 o[DP / 32];
@@ -74,11 +75,15 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kernel(
     if (block >= 0) load(block);
     while (block >= 0) {
         __syncthreads();
-        ks.store(k_lds);
-        vs.store(v_lds);
-        if (docs && threadIdx.x < kBlock) doc_lds[threadIdx.x] = next_doc;
+        const int k0 = block * kBlock, block_doc = at.doc;
+        // keys that nothing sees are zeros
+        const auto keep = [&](int n) {
+            return k0 + Staged<T, DP>::row(n) < keys && (!docs || row_doc[n] >= 0);
+        };
+        ks.store(k_lds, a.dim, keep);
+        vs.store(v_lds, a.dim, keep);
+        if (docs && wave == 0) doc_lds[lane] = k0 + lane < keys ? next_doc : -1;
         __syncthreads();
-        const int k0 = block * kBlock;
         block = at.next();
         if (block >= 0) load(block);
 
@@ -103,11 +108,7 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kernel(
                 }
             }
         }
-        bool whole = k0 + kBlock <= least;
-        if (docs) {
-            const int4 d = key_docs[k0 / kBlock];
-            whole = whole && one_doc && d.x == wave_doc && d.y == wave_doc && !d.z;
-        }
+        const bool whole = k0 + kBlock <= least && (!docs || (one_doc && block_doc == wave_doc));
         if (!whole) {
 #pragma unroll
             for (int i = 0; i < 2; ++i)
