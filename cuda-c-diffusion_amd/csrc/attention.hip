@@ -63,6 +63,12 @@ bool take(Args& p, const NnAttention* a, const char* what) {
     p.scale = a->scale;
     p.c1 = a->softcap > 0.0f ? a->scale / a->softcap : a->scale * kLog2e;
     p.c2 = a->softcap * kLog2e;
+    if (a->softcap > 0.0f) {
+        const double tanh_of[6] = {1.0, -1.0 / 3, 2.0 / 15, -17.0 / 315, 62.0 / 2835, -1382.0 / 155925};
+        double power = (double)p.c2 * p.c1;
+        for (int i = 0; i < 6; ++i, power *= (double)p.c1 * p.c1) p.series[i] = (float)(tanh_of[i] * power);
+        p.small = kSeriesEnd / p.c1;
+    }
     p.q_start = a->q_start;
     p.k_len = a->k_len;
     p.prefix = a->prefix;

@@ -12,9 +12,10 @@
 // operand is read from LDS in that order: rows by 16-byte reads, columns by the
 // transposing read (bf16) or by one read a row (fp32).
 //
-// Rows in LDS are DP values and 32 bytes long: 8 lanes' 16-byte reads of
-// successive rows, and the 4 x 32 bytes of a transposing read, meet different
-// banks.
+// Rows in LDS are a power of two long and hold their 16-byte chunks in an order of
+// their own, chunk c at c ^ F(row), so that 16 lanes' reads of successive rows, and the
+// 4 rows x 64 bytes of two transposing reads, meet different banks.  (Rows 32 bytes
+// apart from a power of two had 40 % of the LDS cycles in conflicts.)
 #pragma once
 
 #include <algorithm>
@@ -102,32 +103,49 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 // ---------------------------------------------------------------------------
 template <typename T, int DP>
 struct Lds {
-    static constexpr int kRowBytes = DP * (int)sizeof(T) + 32;
+    static constexpr int kUsed = DP * (int)sizeof(T);
+    static constexpr int kRowBytes = kUsed <= 64 ? 64 : kUsed <= 128 ? 128 : kUsed <= 256 ? 256 : 512;
     static constexpr int kBytes = kBlock * kRowBytes;
-    static constexpr int kSteps = DP / (2 * Type<T>::CE);  // fragments of a row
+    static constexpr int kSteps = DP / (2 * Type<T>::CE);     // fragments of a row
     static constexpr int kKeySteps = 32 / (2 * Type<T>::CE);  // fragments of 32 rows
 
-    // Operand whose free index is the tile's row: 16 bytes of row `row`.
-    static __device__ __forceinline__ Frag<T> rows(const char* t, int row, int u, int h) {
-        return *reinterpret_cast<const Frag<T>*>(t + row * kRowBytes + (2 * u + h) * 16);
+    // Bits of the row in other places, so F(a ^ b) = F(a) ^ F(b).
+    static __host__ __device__ constexpr int F(int row) {
+        if (sizeof(T) == 2)
+            return kRowBytes == 256 ? (row & 3) << 2 | (row >> 2 & 3)
+                : kRowBytes == 128 ? (row >> 1 & 1) << 2 | (row >> 2 & 3) : row >> 2 & 3;
+        return kRowBytes == 128 ? row >> 1 & 7 : (row >> 2 & 1) << 3 | (row >> 3 & 1) << 2 | (row & 3);
     }
-    // Operand whose free index is the column d0 + (lane & 31) and whose contracted
-    // index is the 32 rows from `row` on, fragment f of kKeySteps.
-    static __device__ __forceinline__ Frag<T> cols(const char* t, int row, int f, int d0, int lane) {
+    static __device__ __forceinline__ int at(int row, int chunk) { return row * kRowBytes + ((chunk ^ F(row)) << 4); }
+
+    // This lane's place in the operands below.
+    static __device__ __forceinline__ int row_base(int lane) { return at(lane & 31, lane >> 5); }
+    static __device__ __forceinline__ int col_base(int lane) {
         const int h = lane >> 5;
+        if (sizeof(T) == 2)
+            return at(4 * h + (lane >> 2 & 3), (lane & 16) >> 3 | (lane & 2) >> 1) + (lane & 1) * 8;
+        return at(4 * h, lane >> 2 & 7) + (lane & 3) * 4;
+    }
+    // Operand whose free index is the tile's row: fragment u of rows 32 i ...
+    static __device__ __forceinline__ Frag<T> rows(const char* t, int i, int u, int base) {
+        return *reinterpret_cast<const Frag<T>*>(t + 32 * i * kRowBytes + (base ^ (u << 5)));
+    }
+    // Operand whose free index is the column 32 d + (lane & 31) and whose contracted
+    // index is the rows 32 i ..., fragment f of kKeySteps.
+    static __device__ __forceinline__ Frag<T> cols(const char* t, int i, int f, int d, int base) {
         if constexpr (sizeof(T) == 2) {
-            const char* p = t + (row + 16 * f + 4 * h + (lane >> 2 & 3)) * kRowBytes +
-                (d0 + (lane & 16) + (lane & 3) * 4) * 2;
             typedef __attribute__((address_space(3))) i16x4* LdsPtr;
-            const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(p));
-            const i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(p + 8 * kRowBytes));
+            const char* p = t + (32 * i + 16 * f) * kRowBytes;
+            const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(p + (base ^ (d << 6))));
+            const i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(p + 8 * kRowBytes + (base ^ (d << 6) ^ (F(8) << 4))));
             const bf16x4 x = __builtin_bit_cast(bf16x4, a), y = __builtin_bit_cast(bf16x4, b);
             return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
         } else {
-            const char* p = t + (row + 8 * f + 4 * h) * kRowBytes + (d0 + (lane & 31)) * 4;
             f32x4 v;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const float*>(p + j * kRowBytes);
+            for (int j = 0; j < 4; ++j)
+                v[j] = *reinterpret_cast<const float*>(t + (32 * i + 8 * f + j) * kRowBytes +
+                    (base ^ ((8 * d ^ F(8 * f & 31) ^ F(j)) << 4)));
             return v;
         }
     }
@@ -153,9 +171,9 @@ __device__ __forceinline__ f32x4 operand(const f32x16& s, int f, float) {
 // 16 bytes of a row from feature d0 on.  Features from `dim` on are zeros, or (vec) a
 // chunk wholly past them is the row's first one, for the caller to leave out: a choice
 // here would wait for the load.
-template <typename T>
-__device__ __forceinline__ u32x4 load_chunk(const T* row, int d0, int dim, bool vec) {
-    if (vec) return *reinterpret_cast<const u32x4*>(row + (d0 < dim ? d0 : 0));
+template <typename T, bool VEC>
+__device__ __forceinline__ u32x4 load_chunk(const T* row, int d0, int dim) {
+    if constexpr (VEC) return *reinterpret_cast<const u32x4*>(row + (d0 < dim ? d0 : 0));
     T e[Type<T>::CE];
 #pragma unroll
     for (int j = 0; j < Type<T>::CE; ++j) e[j] = d0 + j < dim ? row[d0 + j] : (T)0.0f;
@@ -163,17 +181,17 @@ __device__ __forceinline__ u32x4 load_chunk(const T* row, int d0, int dim, bool 
     __builtin_memcpy(&v, e, 16);
     return v;
 }
-template <typename T>
-__device__ __forceinline__ Frag<T> load_frag(const T* row, int d0, int dim, bool vec) {
-    const u32x4 v = load_chunk<T>(row, d0, dim, vec);
+template <typename T, bool VEC>
+__device__ __forceinline__ Frag<T> load_frag(const T* row, int d0, int dim) {
+    const u32x4 v = load_chunk<T, VEC>(row, d0, dim);
     return __builtin_bit_cast(Frag<T>, d0 < dim ? v : u32x4{0, 0, 0, 0});
 }
 
 // Four consecutive features d..d+3 of an output row.
-template <typename T>
-__device__ __forceinline__ void store4(T* row, int d, int dim, bool vec, float a, float b, float c, float e) {
+template <typename T, bool VEC>
+__device__ __forceinline__ void store4(T* row, int d, int dim, float a, float b, float c, float e) {
     const float v[4] = {a, b, c, e};
-    if (vec) {
+    if constexpr (VEC) {
         if (d >= dim) return;
         if constexpr (sizeof(T) == 2) {
             bf16x4 o;
@@ -193,7 +211,7 @@ __device__ __forceinline__ void store4(T* row, int d, int dim, bool vec, float a
 
 // A 64-row tile on its way from memory to LDS: loaded into registers while the tile
 // before it is used, stored when that is done.
-template <typename T, int DP>
+template <typename T, int DP, bool VEC>
 struct Staged {
     static constexpr int kPerRow = DP / Type<T>::CE;
     static constexpr int N = kBlock * kPerRow / kTpb;
@@ -201,11 +219,11 @@ struct Staged {
 
     static __device__ __forceinline__ int row(int n) { return (n * kTpb + (int)threadIdx.x) / kPerRow; }
     // Row r of the tile is base + min(r, last) * stride.
-    __device__ __forceinline__ void load(const T* base, long long stride, int last, int dim, bool vec) {
+    __device__ __forceinline__ void load(const T* base, long long stride, int last, int dim) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int c = (n * kTpb + (int)threadIdx.x) % kPerRow;
-            v[n] = load_chunk<T>(base + min(row(n), last) * stride, c * Type<T>::CE, dim, vec);
+            v[n] = load_chunk<T, VEC>(base + min(row(n), last) * stride, c * Type<T>::CE, dim);
         }
     }
     // Zeros in place of the rows that are not kept, whatever they hold, and of features
@@ -215,8 +233,8 @@ struct Staged {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int c = (n * kTpb + (int)threadIdx.x) % kPerRow;
-            *reinterpret_cast<u32x4*>(lds + row(n) * Lds<T, DP>::kRowBytes + c * 16) =
-                keep(n) && c * Type<T>::CE < dim ? v[n] : u32x4{0, 0, 0, 0};
+            *reinterpret_cast<u32x4*>(lds + Lds<T, DP>::at(row(n), c)) =
+                (keep(n) & (c * Type<T>::CE < dim)) ? v[n] : u32x4{0, 0, 0, 0};
         }
     }
 };
@@ -238,6 +256,8 @@ struct Args {
     int batch, len_q, len_k, heads, kv_heads, group, dim;
     int mask, buckets, max_distance;
     float scale, c1, c2;  // score in units of log2: c1 * s, or c2 * tanh(c1 * s)
+    float series[6];      // c2 tanh(c1 s) = s (series[0] + w (series[1] + ...)), w = s^2, for small c1 s
+    float small;          // how small: |s| below this
     const int *q_start, *k_len, *prefix, *doc_q, *doc_k, *bucket;
     const float* bias;
     bool vec;
@@ -276,6 +296,7 @@ __device__ __forceinline__ float tanh_series(float y) {
     c = fmaf(w, c, -0.333333333f);
     return fmaf(y * w, c, y);
 }
+constexpr float kSeriesEnd = 0.375f;
 // s[r] = tanh(c1 s[r]) and, if wanted, its slope
 template <bool SLOPE>
 __device__ __forceinline__ void cap_scores(f32x16& s, f32x16& slope, float c1) {
@@ -285,7 +306,7 @@ __device__ __forceinline__ void cap_scores(f32x16& s, f32x16& slope, float c1) {
         s[r] *= c1;
         top = fmaxf(top, fabsf(s[r]));
     }
-    if (__all(top < 0.375f)) {  // fmaxf passes over NaN; the series keeps it
+    if (__all(top < kSeriesEnd)) {  // fmaxf passes over NaN; the series keeps it
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             s[r] = tanh_series(s[r]);
@@ -295,9 +316,28 @@ __device__ __forceinline__ void cap_scores(f32x16& s, f32x16& slope, float c1) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const float y = s[r], q = __builtin_amdgcn_rcpf(exp2_fast(fabsf(y) * (2.0f * kLog2e)) + 1.0f);
-            const bool small = fabsf(y) < 0.375f;
+            const bool small = fabsf(y) < kSeriesEnd;
             s[r] = small ? tanh_series(y) : copysignf(fmaf(-2.0f, q, 1.0f), y);
             if constexpr (SLOPE) slope[r] = small ? fmaf(-s[r], s[r], 1.0f) : 4.0f * q * (1.0f - q);
+        }
+    }
+}
+
+// Entries of a keys x queries tile that this lane's query does not see become -inf: keys
+// from `limit` on and, with documents (`docs`: the tile's 32 keys', in LDS), of others than
+// `doc`.  No branches: a tile's border is a few of these, not a path of its own.
+__device__ __forceinline__ void hide(f32x16& s, int k0, int limit, const int* docs, int doc, int h) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = k0 + row_of(r, h) < limit ? s[r] : -INFINITY;
+    if (docs) {
+        const int own = doc >= 0 ? doc : -2;  // -1 is a key of no document
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int4 d = *reinterpret_cast<const int4*>(docs + 8 * g + 4 * h);
+            s[4 * g] = d.x == own ? s[4 * g] : -INFINITY;
+            s[4 * g + 1] = d.y == own ? s[4 * g + 1] : -INFINITY;
+            s[4 * g + 2] = d.z == own ? s[4 * g + 2] : -INFINITY;
+            s[4 * g + 3] = d.w == own ? s[4 * g + 3] : -INFINITY;
         }
     }
 }
@@ -307,6 +347,15 @@ __device__ __forceinline__ void load_bias(const Args& a, float* table, int head)
     for (int i = threadIdx.x; i < 2 * a.max_distance + 1; i += kTpb) {
         const int n = min(max(a.bucket[i], 0), a.buckets - 1);
         table[i] = a.bias[(size_t)n * a.heads + head] * kLog2e;
+    }
+}
+
+// s = c s + bias of the tile's entries; rel: distance of register 0.
+__device__ __forceinline__ void add_bias(f32x16& s, float c, const float* table, int m, int rel) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const int d = rel + 8 * (r >> 2) + (r & 3);
+        s[r] = s[r] * c + table[min(max(d, -m), m) + m];
     }
 }
 
@@ -397,25 +446,26 @@ bool nnk_attention_backward_kv(const attn::Args& args, bool half, hipStream_t s,
 void nnk_attention_bias_grad(const attn::Args& args, float* dbias, hipStream_t s, const char* what);
 size_t nnk_attention_dist_floats(const NnAttention* a);
 
-// FN<T, DP, CAP, BIAS> for the call's type, feature count and score terms.
-#define NNK_ATTN_DISPATCH(args, bf, FN, ...)                                                       \
-    [&]() {                                                                                        \
-        const bool cap_ = (args).c2 != 0.0f, bias_ = (args).buckets > 0;                           \
-        const int dp_ = ((args).dim + 31) / 32;                                                    \
-        auto by_dim = [&](auto type, auto cap, auto bias) {                                        \
-            using T_ = decltype(type);                                                             \
-            switch (dp_) {                                                                         \
-            case 1: return FN<T_, 32, decltype(cap)::value, decltype(bias)::value>(__VA_ARGS__);   \
-            case 2: return FN<T_, 64, decltype(cap)::value, decltype(bias)::value>(__VA_ARGS__);   \
-            case 3: return FN<T_, 96, decltype(cap)::value, decltype(bias)::value>(__VA_ARGS__);   \
-            default: return FN<T_, 128, decltype(cap)::value, decltype(bias)::value>(__VA_ARGS__); \
-            }                                                                                      \
-        };                                                                                         \
-        auto by_terms = [&](auto type) {                                                           \
-            if (cap_) return bias_ ? by_dim(type, std::true_type{}, std::true_type{})              \
-                                   : by_dim(type, std::true_type{}, std::false_type{});            \
-            return bias_ ? by_dim(type, std::false_type{}, std::true_type{})                       \
-                         : by_dim(type, std::false_type{}, std::false_type{});                     \
-        };                                                                                         \
-        return (bf) ? by_terms(attn::bf16{}) : by_terms(0.0f);                                     \
+// FN<T, DP, CAP, BIAS, VEC> for the call's type, feature count, score terms and alignment.
+// Rows that are not on 16 bytes are taken element by element, in one size.
+#define NNK_ATTN_DISPATCH(args, bf, FN, ...)                                                              \
+    [&]() {                                                                                               \
+        auto by_dim = [&](auto type, auto cap, auto bias) {                                               \
+            using T_ = decltype(type);                                                                    \
+            constexpr bool C_ = decltype(cap)::value, B_ = decltype(bias)::value;                         \
+            if (!(args).vec) return FN<T_, 128, C_, B_, false>(__VA_ARGS__);                              \
+            switch (((args).dim + 31) / 32) {                                                             \
+            case 1: return FN<T_, 32, C_, B_, true>(__VA_ARGS__);                                         \
+            case 2: return FN<T_, 64, C_, B_, true>(__VA_ARGS__);                                         \
+            case 3: return FN<T_, 96, C_, B_, true>(__VA_ARGS__);                                         \
+            default: return FN<T_, 128, C_, B_, true>(__VA_ARGS__);                                       \
+            }                                                                                             \
+        };                                                                                                \
+        auto by_terms = [&](auto type) {                                                                  \
+            using Yes = std::true_type;                                                                   \
+            using No = std::false_type;                                                                   \
+            if ((args).c2 != 0.0f) return (args).buckets > 0 ? by_dim(type, Yes{}, Yes{}) : by_dim(type, Yes{}, No{}); \
+            return (args).buckets > 0 ? by_dim(type, No{}, Yes{}) : by_dim(type, No{}, No{});             \
+        };                                                                                                \
+        return (bf) ? by_terms(attn::bf16{}) : by_terms(0.0f);                                            \
     }()

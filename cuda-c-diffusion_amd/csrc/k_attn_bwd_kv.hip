@@ -20,15 +20,17 @@ using namespace attn;
 
 constexpr int kSlack = 64;  // distances of a tile that reaches past max_distance
 
-template <typename T, int DP, bool CAP, bool BIAS>
+template <typename T, int DP, bool CAP, bool BIAS, bool VEC>
 __global__ __launch_bounds__(kTpb, 1) void attn_bwd_kv_kernel(Args a, int tiles) {
     using L = Lds<T, DP>;
-    __shared__ __attribute__((aligned(16))) char q_lds[L::kBytes];
-    __shared__ __attribute__((aligned(16))) char g_lds[L::kBytes];
-    __shared__ __attribute__((aligned(16))) float M_lds[kBlock];
-    __shared__ __attribute__((aligned(16))) float D_lds[kBlock];
-    __shared__ __attribute__((aligned(16))) int limit_lds[kBlock];
-    __shared__ __attribute__((aligned(16))) int doc_lds[kBlock];
+    // two blocks in LDS; one where they and the distances would not fit (fp32, over 64 features)
+    constexpr int kBufs = L::kRowBytes > 256 ? 1 : 2;
+    __shared__ __attribute__((aligned(16))) char q_lds[kBufs][L::kBytes];
+    __shared__ __attribute__((aligned(16))) char g_lds[kBufs][L::kBytes];
+    __shared__ __attribute__((aligned(16))) float M_lds[kBufs][kBlock];
+    __shared__ __attribute__((aligned(16))) float D_lds[kBufs][kBlock];
+    __shared__ __attribute__((aligned(16))) int limit_lds[kBufs][kBlock];
+    __shared__ __attribute__((aligned(16))) int doc_lds[kBufs][kBlock];
     __shared__ float table[BIAS ? 2 * kMaxDistance + 1 : 1];
     extern __shared__ float dist[];  // BIAS: a table of 2 (max_distance + kSlack) + 1 a wave
 
@@ -61,8 +63,8 @@ __global__ __launch_bounds__(kTpb, 1) void attn_bwd_kv_kernel(Args a, int tiles)
 #pragma unroll
         for (int u = 0; u < L::kSteps; ++u) {
             const int d0 = (2 * u + h) * Type<T>::CE, dim = live ? a.dim : 0;
-            kf[u] = load_frag<T>(k, d0, dim, a.vec);
-            vf[u] = load_frag<T>(v, d0, dim, a.vec);
+            kf[u] = load_frag<T, VEC>(k, d0, dim);
+            vf[u] = load_frag<T, VEC>(v, d0, dim);
         }
     }
     f32x16 dk[DP / 32], dv[DP / 32];
@@ -71,13 +73,14 @@ __global__ __launch_bounds__(kTpb, 1) void attn_bwd_kv_kernel(Args a, int tiles)
         dk[d] = zero16();
         dv[d] = zero16();
     }
+    const int rbase = L::row_base(lane), cbase = L::col_base(lane);
     const int span = 2 * (a.max_distance + kSlack) + 1;
     float* my_dist = dist + wave * span;
 
     for (int head = kv * a.group; head < (kv + 1) * a.group; ++head) {
         float far_lo = 0.0f, far_hi = 0.0f;
+        __syncthreads();  // the head before is done with
         if constexpr (BIAS) {
-            __syncthreads();
             load_bias(a, table, head);
             for (int i = threadIdx.x; i < kWaves * span; i += kTpb) dist[i] = 0.0f;
         }
@@ -85,82 +88,99 @@ __global__ __launch_bounds__(kTpb, 1) void attn_bwd_kv_kernel(Args a, int tiles)
         const T* gp = (const T*)a.dout + b * a.os[0] + head * a.os[2];
         const float2* stats = a.stat + ((size_t)b * a.heads + head) * a.len_q;
 
-        Staged<T, DP> qs, gs;
-        float row_M[Staged<T, DP>::N];
+        Staged<T, DP, VEC> qs, gs;
+        float row_M[Staged<T, DP, VEC>::N];
         float2 st = {INFINITY, 0.0f};
         int lim = 0, qdoc = -2;
         const auto load = [&](int block) {
             const int q0 = block * kBlock, last = a.len_q - 1 - q0;
 #pragma unroll
-            for (int n = 0; n < Staged<T, DP>::N; ++n) row_M[n] = stats[q0 + min(Staged<T, DP>::row(n), last)].x;
+            for (int n = 0; n < Staged<T, DP, VEC>::N; ++n) row_M[n] = stats[q0 + min(Staged<T, DP, VEC>::row(n), last)].x;
             if (wave == 0) {
                 const int i = q0 + min(lane, last);
                 st = stats[i];
                 if (a.doc_q) qdoc = a.doc_q[(size_t)b * a.len_q + i];
                 lim = limit_of(a, b, keys, start + i);
             }
-            qs.load(qp + q0 * a.qs[1], a.qs[1], last, a.dim, a.vec);
-            gs.load(gp + q0 * a.os[1], a.os[1], last, a.dim, a.vec);
+            qs.load(qp + q0 * a.qs[1], a.qs[1], last, a.dim);
+            gs.load(gp + q0 * a.os[1], a.os[1], last, a.dim);
+        };
+
+        const auto store = [&](int block, int to) {
+            const int q0 = block * kBlock;
+            // queries that see nothing are zeros
+            const auto keep = [&](int n) {
+                return (q0 + Staged<T, DP, VEC>::row(n) < a.len_q) & (row_M[n] != INFINITY);
+            };
+            qs.store(q_lds[to], a.dim, keep);
+            gs.store(g_lds[to], a.dim, keep);
+            if (wave == 0) {
+                const bool there = q0 + lane < a.len_q;
+                M_lds[to][lane] = there ? st.x : INFINITY;
+                D_lds[to][lane] = st.y;
+                limit_lds[to][lane] = there ? lim : 0;
+                doc_lds[to][lane] = there ? qdoc : -2;
+            }
         };
 
         Blocks at(first_block, q_blocks, query_docs, mine);
-        int block = at.next();
-        if (block >= 0) load(block);
-        while (block >= 0) {
-            __syncthreads();
-            const int q0 = block * kBlock, block_doc = at.doc;
-            // queries that see nothing are zeros
-            const auto keep = [&](int n) {
-                return q0 + Staged<T, DP>::row(n) < a.len_q && row_M[n] != INFINITY;
-            };
-            qs.store(q_lds, a.dim, keep);
-            gs.store(g_lds, a.dim, keep);
-            if (wave == 0) {
-                const bool there = q0 + lane < a.len_q;
-                M_lds[lane] = there ? st.x : INFINITY;
-                D_lds[lane] = st.y;
-                limit_lds[lane] = there ? lim : 0;
-                doc_lds[lane] = there ? qdoc : -2;
-            }
-            __syncthreads();
-            block = at.next();
-            if (block >= 0) load(block);
+        int next = at.next();
+        if (next >= 0) {
+            load(next);
+            store(next, 0);
+        }
+        for (int buf = 0; next >= 0; buf ^= kBufs - 1) {
+            const int q0 = next * kBlock, block_doc = at.doc;
+            next = at.next();
+            __syncthreads();  // this block is stored; the one before it is done with
+            if (next >= 0) load(next);
 
-            const bool whole = whole_keys && limit_lds[0] > last_key && (!docs || block_doc == wave_doc);
+            const bool whole = whole_keys && limit_lds[buf][0] > last_key && (!docs || block_doc == wave_doc);
 #pragma unroll 1
             for (int i = 0; i < 2; ++i) {
                 f32x16 s = zero16(), dp = zero16();
 #pragma unroll
                 for (int u = 0; u < L::kSteps; ++u) {
-                    s = mma(L::rows(q_lds, 32 * i + (lane & 31), u, h), kf[u], s);
-                    dp = mma(L::rows(g_lds, 32 * i + (lane & 31), u, h), vf[u], dp);
+                    s = mma(L::rows(q_lds[buf], i, u, rbase), kf[u], s);
+                    dp = mma(L::rows(g_lds[buf], i, u, rbase), vf[u], dp);
                 }
                 f32x16 slope;
                 if constexpr (CAP) cap_scores<true>(s, slope, a.c1);
                 const float c = CAP ? a.c2 : a.c1;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] *= c;
                 if constexpr (BIAS) {
+                    const int rel = key - (start + q0 + 32 * i + 4 * h);
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        const int rel = key - (start + q0 + 32 * i + row_of(r, h));
-                        s[r] += table[min(max(rel, -a.max_distance), a.max_distance) + a.max_distance];
+                        const int d = rel - 8 * (r >> 2) - (r & 3), m = a.max_distance;
+                        s[r] = s[r] * c + table[min(max(d, -m), m) + m];
+                    }
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[r] *= c;
+                }
+                if (!whole) {
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const int at4 = 32 * i + 8 * g + 4 * h;
+                        const int4 lm = *reinterpret_cast<const int4*>(limit_lds[buf] + at4);
+                        int4 dc = {doc, doc, doc, doc};
+                        if (docs) dc = *reinterpret_cast<const int4*>(doc_lds[buf] + at4);
+                        const auto sees = [&](int lm1, int dc1) { return live & (key < lm1) & (dc1 == doc); };
+                        s[4 * g] = sees(lm.x, dc.x) ? s[4 * g] : -INFINITY;
+                        s[4 * g + 1] = sees(lm.y, dc.y) ? s[4 * g + 1] : -INFINITY;
+                        s[4 * g + 2] = sees(lm.z, dc.z) ? s[4 * g + 2] : -INFINITY;
+                        s[4 * g + 3] = sees(lm.w, dc.w) ? s[4 * g + 3] : -INFINITY;
                     }
                 }
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    const f32x4 M = *reinterpret_cast<const f32x4*>(M_lds + 32 * i + 8 * g + 4 * h);
-                    const f32x4 D = *reinterpret_cast<const f32x4*>(D_lds + 32 * i + 8 * g + 4 * h);
+                    const f32x4 M = *reinterpret_cast<const f32x4*>(M_lds[buf] + 32 * i + 8 * g + 4 * h);
+                    const f32x4 D = *reinterpret_cast<const f32x4*>(D_lds[buf] + 32 * i + 8 * g + 4 * h);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const int r = 4 * g + j, row = 32 * i + 8 * g + 4 * h + j;
-                        float p = exp2_fast(s[r] - M[j]);
-                        if (!whole) {
-                            const bool sees = live && key < limit_lds[row] && (!docs || doc_lds[row] == doc);
-                            p = sees ? p : 0.0f;
-                        }
-                        s[r] = p;
-                        dp[r] = p == 0.0f ? 0.0f : p * (dp[r] - D[j]);
+                        const int r = 4 * g + j;
+                        s[r] = exp2_fast(s[r] - M[j]);
+                        dp[r] = s[r] * (dp[r] - D[j]);
                     }
                 }
                 if constexpr (BIAS) {
@@ -197,11 +217,13 @@ __global__ __launch_bounds__(kTpb, 1) void attn_bwd_kv_kernel(Args a, int tiles)
                     const Frag<T> p = operand(s, f, T{}), x = operand(dp, f, T{});
 #pragma unroll
                     for (int d = 0; d < DP / 32; ++d) {
-                        dv[d] = mma(L::cols(g_lds, 32 * i, f, 32 * d, lane), p, dv[d]);
-                        dk[d] = mma(L::cols(q_lds, 32 * i, f, 32 * d, lane), x, dk[d]);
+                        dv[d] = mma(L::cols(g_lds[buf], i, f, d, cbase), p, dv[d]);
+                        dk[d] = mma(L::cols(q_lds[buf], i, f, d, cbase), x, dk[d]);
                     }
                 }
             }
+            if (kBufs == 1) __syncthreads();
+            if (next >= 0) store(next, buf ^ (kBufs - 1));
         }
         if constexpr (BIAS) {
             // the far tiles join the ends of the table; then one sum a distance
@@ -235,9 +257,9 @@ __global__ __launch_bounds__(kTpb, 1) void attn_bwd_kv_kernel(Args a, int tiles)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int at = 32 * d + 8 * g + 4 * h;
-            store4<T>(kout, at, a.dim, a.vec, dk[d][4 * g] * a.scale, dk[d][4 * g + 1] * a.scale,
+            store4<T, VEC>(kout, at, a.dim, dk[d][4 * g] * a.scale, dk[d][4 * g + 1] * a.scale,
                 dk[d][4 * g + 2] * a.scale, dk[d][4 * g + 3] * a.scale);
-            store4<T>(vout, at, a.dim, a.vec, dv[d][4 * g], dv[d][4 * g + 1], dv[d][4 * g + 2], dv[d][4 * g + 3]);
+            store4<T, VEC>(vout, at, a.dim, dv[d][4 * g], dv[d][4 * g + 1], dv[d][4 * g + 2], dv[d][4 * g + 3]);
         }
 }
 
@@ -261,17 +283,17 @@ __global__ __launch_bounds__(kTpb) void attn_bias_grad_kernel(float* dbias, cons
     if (threadIdx.x == 0) dbias[(size_t)mine * heads + head] = (float)part[0];
 }
 
-template <typename T, int DP, bool CAP, bool BIAS>
+template <typename T, int DP, bool CAP, bool BIAS, bool VEC>
 bool launch(const Args& a, hipStream_t s, const char* what) {
     const int tiles = (a.len_k + kRows - 1) / kRows;
     const size_t lds = BIAS ? kWaves * (2 * (a.max_distance + kSlack) + 1) * sizeof(float) : 0;
     if constexpr (BIAS) {
         static std::atomic<unsigned long long> done{0};
-        if (!raise_lds((const void*)attn_bwd_kv_kernel<T, DP, CAP, BIAS>,
+        if (!raise_lds((const void*)attn_bwd_kv_kernel<T, DP, CAP, BIAS, VEC>,
                 kWaves * (2 * (kMaxDistance + kSlack) + 1) * sizeof(float), done, what))
             return false;
     }
-    attn_bwd_kv_kernel<T, DP, CAP, BIAS>
+    attn_bwd_kv_kernel<T, DP, CAP, BIAS, VEC>
         <<<(unsigned)((long long)tiles * a.kv_heads * a.batch), kTpb, lds, s>>>(a, tiles);
     nnk_after_launch(what, s);
     return true;

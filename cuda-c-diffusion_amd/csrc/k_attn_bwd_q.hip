@@ -15,12 +15,12 @@
 namespace {
 using namespace attn;
 
-template <typename T, int DP, bool CAP, bool BIAS>
+template <typename T, int DP, bool CAP, bool BIAS, bool VEC>
 __global__ __launch_bounds__(kTpb, 1) void attn_bwd_q_kernel(Args a, int tiles) {
     using L = Lds<T, DP>;
-    __shared__ __attribute__((aligned(16))) char k_lds[L::kBytes];
-    __shared__ __attribute__((aligned(16))) char v_lds[L::kBytes];
-    __shared__ int doc_lds[kBlock];
+    __shared__ __attribute__((aligned(16))) char k_lds[2][L::kBytes];
+    __shared__ __attribute__((aligned(16))) char v_lds[2][L::kBytes];
+    __shared__ __attribute__((aligned(16))) int doc_lds[2][kBlock];
     __shared__ float table[BIAS ? 2 * kMaxDistance + 1 : 1];
 
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
@@ -59,9 +59,9 @@ __global__ __launch_bounds__(kTpb, 1) void attn_bwd_q_kernel(Args a, int tiles) 
 #pragma unroll
         for (int u = 0; u < L::kSteps; ++u) {
             const int d0 = (2 * u + h) * Type<T>::CE, dim = sees_any ? a.dim : 0;
-            qf[u] = load_frag<T>(q, d0, dim, a.vec);
-            gf[u] = load_frag<T>(g, d0, dim, a.vec);
-            const Frag<T> of = load_frag<T>(out, d0, dim, a.vec);
+            qf[u] = load_frag<T, VEC>(q, d0, dim);
+            gf[u] = load_frag<T, VEC>(g, d0, dim);
+            const Frag<T> of = load_frag<T, VEC>(out, d0, dim);
 #pragma unroll
             for (int j = 0; j < Type<T>::CE; ++j) D = fmaf((float)gf[u][j], (float)of[j], D);
         }
@@ -73,17 +73,30 @@ __global__ __launch_bounds__(kTpb, 1) void attn_bwd_q_kernel(Args a, int tiles) 
     const int* docs = a.doc_k ? a.doc_k + (size_t)b * a.len_k : nullptr;
     if constexpr (BIAS) load_bias(a, table, head);
 
-    Staged<T, DP> ks, vs;
-    int row_doc[Staged<T, DP>::N], next_doc = 0;
+    Staged<T, DP, VEC> ks, vs;
+    int row_doc[Staged<T, DP, VEC>::N], next_doc = 0;
+#pragma unroll
+    for (int n = 0; n < Staged<T, DP, VEC>::N; ++n) row_doc[n] = 0;
     const auto load = [&](int block) {
         const int k0 = block * kBlock, last = keys - 1 - k0;
         if (docs) {
 #pragma unroll
-            for (int n = 0; n < Staged<T, DP>::N; ++n) row_doc[n] = docs[k0 + min(Staged<T, DP>::row(n), last)];
+            for (int n = 0; n < Staged<T, DP, VEC>::N; ++n)
+                row_doc[n] = docs[k0 + min(Staged<T, DP, VEC>::row(n), last)];
             next_doc = docs[k0 + min(lane, last)];
         }
-        ks.load(kp + k0 * a.ks[1], a.ks[1], last, a.dim, a.vec);
-        vs.load(vp + k0 * a.vs[1], a.vs[1], last, a.dim, a.vec);
+        ks.load(kp + k0 * a.ks[1], a.ks[1], last, a.dim);
+        vs.load(vp + k0 * a.vs[1], a.vs[1], last, a.dim);
+    };
+    const auto store = [&](int block, int to) {
+        const int k0 = block * kBlock;
+        // keys that nothing sees are zeros
+        const auto keep = [&](int n) {
+            return (k0 + Staged<T, DP, VEC>::row(n) < keys) & (row_doc[n] >= 0);
+        };
+        ks.store(k_lds[to], a.dim, keep);
+        vs.store(v_lds[to], a.dim, keep);
+        if (docs && wave == 0) doc_lds[to][lane] = k0 + lane < keys ? next_doc : -1;
     };
 
     f32x16 dq[DP / 32];
@@ -91,21 +104,18 @@ __global__ __launch_bounds__(kTpb, 1) void attn_bwd_q_kernel(Args a, int tiles) 
     for (int d = 0; d < DP / 32; ++d) dq[d] = zero16();
     float l = 0.0f, pd = 0.0f;  // sums of p and of p dp
 
-    int block = at.next();
-    if (block >= 0) load(block);
-    for (bool first = true; block >= 0; first = false) {
-        __syncthreads();
-        const int k0 = block * kBlock, block_doc = at.doc;
-        // keys that nothing sees are zeros
-        const auto keep = [&](int n) {
-            return k0 + Staged<T, DP>::row(n) < keys && (!docs || row_doc[n] >= 0);
-        };
-        ks.store(k_lds, a.dim, keep);
-        vs.store(v_lds, a.dim, keep);
-        if (docs && wave == 0) doc_lds[lane] = k0 + lane < keys ? next_doc : -1;
-        __syncthreads();
-        block = at.next();
-        if (block >= 0) load(block);
+    const int rbase = L::row_base(lane), cbase = L::col_base(lane);
+    int next = at.next();
+    if (next >= 0) {
+        load(next);
+        store(next, 0);
+    }
+    bool first = true;
+    for (int buf = 0; next >= 0; buf ^= 1, first = false) {
+        const int k0 = next * kBlock, block_doc = at.doc;
+        next = at.next();
+        __syncthreads();  // this block is stored; the one before it is done with
+        if (next >= 0) load(next);
 
         const bool whole = k0 + kBlock <= least && (!docs || (one_doc && block_doc == wave_doc));
         // scores (in units of log2) and dp of keys 32 i .. 32 i + 31; slope: 1 - tanh^2
@@ -114,30 +124,20 @@ __global__ __launch_bounds__(kTpb, 1) void attn_bwd_q_kernel(Args a, int tiles) 
             dp = zero16();
 #pragma unroll
             for (int u = 0; u < L::kSteps; ++u) {
-                s = mma(L::rows(k_lds, 32 * i + (lane & 31), u, h), qf[u], s);
-                dp = mma(L::rows(v_lds, 32 * i + (lane & 31), u, h), gf[u], dp);
+                s = mma(L::rows(k_lds[buf], i, u, rbase), qf[u], s);
+                dp = mma(L::rows(v_lds[buf], i, u, rbase), gf[u], dp);
             }
             if constexpr (CAP) cap_scores<true>(s, slope, a.c1);
             const float c = CAP ? a.c2 : a.c1;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] *= c;
             if constexpr (BIAS) {
+                add_bias(s, c, table, a.max_distance, k0 + 32 * i + 4 * h - pos);
+            } else {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int rel = k0 + 32 * i + row_of(r, h) - pos;
-                    s[r] += table[min(max(rel, -a.max_distance), a.max_distance) + a.max_distance];
-                }
+                for (int r = 0; r < 16; ++r) s[r] *= c;
             }
-            if (!whole) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int j = 32 * i + row_of(r, h);
-                    const bool sees = k0 + j < limit && (!docs || (doc_lds[j] == doc && doc >= 0));
-                    s[r] = sees ? s[r] : -INFINITY;
-                }
-            }
+            if (!whole) hide(s, k0 + 32 * i, limit, docs ? doc_lds[buf] + 32 * i : nullptr, doc, h);
         };
-        if (first && block < 0) {  // the only block
+        if (first && next < 0) {  // the only block
             float m = -INFINITY, sum = 0.0f, dot = 0.0f;
 #pragma unroll 1
             for (int i = 0; i < 2; ++i) {
@@ -154,7 +154,7 @@ __global__ __launch_bounds__(kTpb, 1) void attn_bwd_q_kernel(Args a, int tiles) 
                 for (int r = 0; r < 16; ++r) {
                     const float p = exp2_fast(s[r] - base);
                     sum += p;
-                    dot = p == 0.0f ? dot : fmaf(p, dp[r], dot);
+                    dot = fmaf(p, dp[r], dot);
                 }
                 m = top;
             }
@@ -173,9 +173,8 @@ __global__ __launch_bounds__(kTpb, 1) void attn_bwd_q_kernel(Args a, int tiles) 
             for (int r = 0; r < 16; ++r) {
                 const float p = exp2_fast(s[r] - M);
                 l += p;
-                const float w = p * dp[r];
-                pd += p == 0.0f ? 0.0f : w;
-                float dx = p == 0.0f ? 0.0f : p * (dp[r] - D);
+                pd = fmaf(p, dp[r], pd);
+                float dx = p * (dp[r] - D);
                 if constexpr (CAP) dx *= slope[r];
                 s[r] = dx;
             }
@@ -183,9 +182,10 @@ __global__ __launch_bounds__(kTpb, 1) void attn_bwd_q_kernel(Args a, int tiles) 
             for (int f = 0; f < L::kKeySteps; ++f) {
                 const Frag<T> x = operand(s, f, T{});
 #pragma unroll
-                for (int d = 0; d < DP / 32; ++d) dq[d] = mma(L::cols(k_lds, 32 * i, f, 32 * d, lane), x, dq[d]);
+                for (int d = 0; d < DP / 32; ++d) dq[d] = mma(L::cols(k_lds[buf], i, f, d, cbase), x, dq[d]);
             }
         }
+        if (next >= 0) store(next, buf ^ 1);
     }
 
     if (!in) return;
@@ -196,15 +196,15 @@ __global__ __launch_bounds__(kTpb, 1) void attn_bwd_q_kernel(Args a, int tiles) 
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
-            store4<T>(out, 32 * d + 8 * g + 4 * h, a.dim, a.vec, dq[d][4 * g] * a.scale, dq[d][4 * g + 1] * a.scale,
+            store4<T, VEC>(out, 32 * d + 8 * g + 4 * h, a.dim, dq[d][4 * g] * a.scale, dq[d][4 * g + 1] * a.scale,
                 dq[d][4 * g + 2] * a.scale, dq[d][4 * g + 3] * a.scale);
     if (h == 0) a.stat[stat_at] = sees_any ? float2{M + log2f(l), pd / l} : float2{INFINITY, 0.0f};
 }
 
-template <typename T, int DP, bool CAP, bool BIAS>
+template <typename T, int DP, bool CAP, bool BIAS, bool VEC>
 bool launch(const Args& a, hipStream_t s, const char* what) {
     const int tiles = (a.len_q + kRows - 1) / kRows;
-    attn_bwd_q_kernel<T, DP, CAP, BIAS><<<(unsigned)((long long)tiles * a.heads * a.batch), kTpb, 0, s>>>(a, tiles);
+    attn_bwd_q_kernel<T, DP, CAP, BIAS, VEC><<<(unsigned)((long long)tiles * a.heads * a.batch), kTpb, 0, s>>>(a, tiles);
     nnk_after_launch(what, s);
     return true;
 }

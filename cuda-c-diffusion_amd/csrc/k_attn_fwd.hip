@@ -1,21 +1,35 @@
 // k_attn_fwd.hip -- attention, many queries a head.
 //
-// One pass over the keys with the running maximum m and sum l of each query's softmax:
+// One pass over the keys with a reference m and the running sum l of each query's softmax:
 // per block of 64 keys  S = K Q^T,  p = 2^(x - m),  O = O 2^(m_old - m) + V^T p.
 // A workgroup of 4 waves has 128 queries of a head, 32 a wave, whose operand stays in
-// registers; keys and values of a block are in LDS for all four, the next block's
-// loads under way meanwhile.  Blocks that no query of the workgroup sees are left out.
+// registers; keys and values of a block are in LDS for all four, two blocks at a time, the
+// next one's loads under way meanwhile.  Blocks that no query of the workgroup sees are
+// left out.
+//
+// What bounds it is the softmax's arithmetic, a vector instruction of 4 cycles for 64
+// scores against 32 cycles of matrix products (128 features), so each score term has the
+// form with the fewest:
+//   plain:  m is kept in units of s, p = 2^(c s - c m): one multiply-add, one power;
+//   cap:    scores within +-c2 (units of log2) need no running maximum.  m is that of the
+//           first block that a query sees, or c2 - 80 if that is more: then p <= 2^80 and,
+//           for c2 up to 80, l >= 2^-80, both far from the ends of fp32.  For scores below
+//           3/8 of the cap, tanh, its factors and the reference are one polynomial;
+//   else:   running maximum of x.
 #include "attn_common.h"
 
 namespace {
 using namespace attn;
 
-template <typename T, int DP, bool CAP, bool BIAS>
-__global__ __launch_bounds__(kTpb, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kernel(Args a, int tiles) {
+// CAP: 0 none, 1 any, 2 at most kFixedCap and no bias
+constexpr float kFixedCap = 80.0f;
+
+template <typename T, int DP, int CAP, bool BIAS, bool VEC>
+__global__ __launch_bounds__(kTpb, sizeof(T) == 2 && VEC ? 2 : 1) void attn_fwd_kernel(Args a, int tiles) {
     using L = Lds<T, DP>;
-    __shared__ __attribute__((aligned(16))) char k_lds[L::kBytes];
-    __shared__ __attribute__((aligned(16))) char v_lds[L::kBytes];
-    __shared__ int doc_lds[kBlock];
+    __shared__ __attribute__((aligned(16))) char k_lds[2][L::kBytes];
+    __shared__ __attribute__((aligned(16))) char v_lds[2][L::kBytes];
+    __shared__ __attribute__((aligned(16))) int doc_lds[2][kBlock];
     __shared__ float table[BIAS ? 2 * kMaxDistance + 1 : 1];
 
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
@@ -45,7 +59,7 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kernel(
     {
         const T* q = (const T*)a.q + b * a.qs[0] + (long long)min(row, a.len_q - 1) * a.qs[1] + head * a.qs[2];
 #pragma unroll
-        for (int u = 0; u < L::kSteps; ++u) qf[u] = load_frag<T>(q, (2 * u + h) * Type<T>::CE, a.dim, a.vec);
+        for (int u = 0; u < L::kSteps; ++u) qf[u] = load_frag<T, VEC>(q, (2 * u + h) * Type<T>::CE, a.dim);
     }
     const int kv = head / a.group;
     const T* kp = (const T*)a.k + b * a.ks[0] + kv * a.ks[2];
@@ -53,102 +67,162 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kernel(
     const int* docs = a.doc_k ? a.doc_k + (size_t)b * a.len_k : nullptr;
     if constexpr (BIAS) load_bias(a, table, head);
 
-    Staged<T, DP> ks, vs;
-    int row_doc[Staged<T, DP>::N], next_doc = 0;
+    Staged<T, DP, VEC> ks, vs;
+    int row_doc[Staged<T, DP, VEC>::N], next_doc = 0;
+#pragma unroll
+    for (int n = 0; n < Staged<T, DP, VEC>::N; ++n) row_doc[n] = 0;
     const auto load = [&](int block) {
         const int k0 = block * kBlock, last = keys - 1 - k0;
         if (docs) {
 #pragma unroll
-            for (int n = 0; n < Staged<T, DP>::N; ++n) row_doc[n] = docs[k0 + min(Staged<T, DP>::row(n), last)];
+            for (int n = 0; n < Staged<T, DP, VEC>::N; ++n)
+                row_doc[n] = docs[k0 + min(Staged<T, DP, VEC>::row(n), last)];
             next_doc = docs[k0 + min(lane, last)];
         }
-        ks.load(kp + k0 * a.ks[1], a.ks[1], last, a.dim, a.vec);
-        vs.load(vp + k0 * a.vs[1], a.vs[1], last, a.dim, a.vec);
+        ks.load(kp + k0 * a.ks[1], a.ks[1], last, a.dim);
+        vs.load(vp + k0 * a.vs[1], a.vs[1], last, a.dim);
+    };
+    const auto store = [&](int block, int to) {
+        const int k0 = block * kBlock;
+        // keys that nothing sees are zeros
+        const auto keep = [&](int n) {
+            return (k0 + Staged<T, DP, VEC>::row(n) < keys) & (row_doc[n] >= 0);
+        };
+        ks.store(k_lds[to], a.dim, keep);
+        vs.store(v_lds[to], a.dim, keep);
+        if (docs && wave == 0) doc_lds[to][lane] = k0 + lane < keys ? next_doc : -1;
     };
 
     f32x16 o[DP / 32];
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d) o[d] = zero16();
-    float m = -INFINITY, l = 0.0f;
+    float m = -INFINITY, l = 0.0f;  // m in units of the score: of s if there is neither cap nor bias
+    const int rbase = L::row_base(lane), cbase = L::col_base(lane);
 
-    int block = at.next();
-    if (block >= 0) load(block);
-    while (block >= 0) {
-        __syncthreads();
-        const int k0 = block * kBlock, block_doc = at.doc;
-        // keys that nothing sees are zeros
-        const auto keep = [&](int n) {
-            return k0 + Staged<T, DP>::row(n) < keys && (!docs || row_doc[n] >= 0);
-        };
-        ks.store(k_lds, a.dim, keep);
-        vs.store(v_lds, a.dim, keep);
-        if (docs && wave == 0) doc_lds[lane] = k0 + lane < keys ? next_doc : -1;
-        __syncthreads();
-        block = at.next();
-        if (block >= 0) load(block);
+    int next = at.next();
+    if (next >= 0) {
+        load(next);
+        store(next, 0);
+    }
+    for (int buf = 0; next >= 0; buf ^= 1) {
+        const int k0 = next * kBlock, block_doc = at.doc;
+        next = at.next();
+        __syncthreads();  // this block is stored; the one before it is done with
+        if (next >= 0) load(next);
 
         f32x16 s[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             s[i] = zero16();
 #pragma unroll
-            for (int u = 0; u < L::kSteps; ++u) s[i] = mma(L::rows(k_lds, 32 * i + (lane & 31), u, h), qf[u], s[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            if constexpr (CAP) cap_scores<false>(s[i], s[i], a.c1);
-            const float c = CAP ? a.c2 : a.c1;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[i][r] *= c;
-            if constexpr (BIAS) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int rel = k0 + 32 * i + row_of(r, h) - pos;
-                    s[i][r] += table[min(max(rel, -a.max_distance), a.max_distance) + a.max_distance];
-                }
-            }
+            for (int u = 0; u < L::kSteps; ++u) s[i] = mma(L::rows(k_lds[buf], i, u, rbase), qf[u], s[i]);
         }
         const bool whole = k0 + kBlock <= least && (!docs || (one_doc && block_doc == wave_doc));
-        if (!whole) {
+        const auto hide_both = [&]() {
+            if (whole) return;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                hide(s[i], k0 + 32 * i, limit, docs ? doc_lds[buf] + 32 * i : nullptr, doc, h);
+        };
+        // the largest score so far, and sums and outputs in its terms
+        const auto raise = [&](float unit) {
+            float top = m;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int j = 32 * i + row_of(r, h);
-                    const bool sees = k0 + j < limit && (!docs || (doc_lds[j] == doc && doc >= 0));
-                    s[i][r] = sees ? s[i][r] : -INFINITY;
+                for (int r = 0; r < 16; ++r) top = fmaxf(top, s[i][r]);
+            top = max_halves(top);
+            const float base = top == -INFINITY ? 0.0f : top * unit;
+            if (__any(top > m)) {
+                const float f = exp2_fast(m * unit - base);
+                l *= f;
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[d][r] *= f;
+                m = top;
+            }
+            return base;
+        };
+        if constexpr (CAP == 2) {
+            float top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(s[i][r]));
+            const bool series = __all(top < a.small);
+            if (whole && series && __all(m != -INFINITY)) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const float w = s[i][r] * s[i][r];
+                        float c = fmaf(w, a.series[5], a.series[4]);
+                        c = fmaf(w, c, a.series[3]);
+                        c = fmaf(w, c, a.series[2]);
+                        c = fmaf(w, c, a.series[1]);
+                        c = fmaf(w, c, a.series[0]);
+                        s[i][r] = exp2_fast(fmaf(s[i][r], c, -m));
+                    }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    cap_scores<false>(s[i], s[i], a.c1);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[i][r] *= a.c2;
                 }
-        }
-        float top = m;
+                hide_both();
+                float first = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+                for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) top = fmaxf(top, s[i][r]);
-        top = max_halves(top);
-        const float base = top == -INFINITY ? 0.0f : top;
-        if (__any(top > m)) {
-            const float f = exp2_fast(m - base);
-            l *= f;
+                    for (int r = 0; r < 16; ++r) first = fmaxf(first, s[i][r]);
+                first = max_halves(first);
+                if (m == -INFINITY && first > -INFINITY) m = fmaxf(first, a.c2 - kFixedCap);
+                const float base = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-            for (int d = 0; d < DP / 32; ++d)
+                for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) o[d][r] *= f;
-            m = top;
+                    for (int r = 0; r < 16; ++r) s[i][r] = exp2_fast(s[i][r] - base);
+            }
+        } else if constexpr (CAP == 0 && !BIAS) {
+            hide_both();
+            const float base = raise(a.c1);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[i][r] = exp2_fast(fmaf(s[i][r], a.c1, -base));
+        } else {
+            const float c = CAP ? a.c2 : a.c1;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if constexpr (CAP) cap_scores<false>(s[i], s[i], a.c1);
+                if constexpr (BIAS) {
+                    add_bias(s[i], c, table, a.max_distance, k0 + 32 * i + 4 * h - pos);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[i][r] *= c;
+                }
+            }
+            hide_both();
+            const float base = raise(1.0f);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[i][r] = exp2_fast(s[i][r] - base);
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s[i][r] = exp2_fast(s[i][r] - base);
-                l += s[i][r];
-            }
+            for (int r = 0; r < 16; ++r) l += s[i][r];
 #pragma unroll
             for (int f = 0; f < L::kKeySteps; ++f) {
                 const Frag<T> p = operand(s[i], f, T{});
 #pragma unroll
-                for (int d = 0; d < DP / 32; ++d) o[d] = mma(L::cols(v_lds, 32 * i, f, 32 * d, lane), p, o[d]);
+                for (int d = 0; d < DP / 32; ++d) o[d] = mma(L::cols(v_lds[buf], i, f, d, cbase), p, o[d]);
             }
         }
+        if (next >= 0) store(next, buf ^ 1);
     }
 
     if (!in) return;
@@ -159,16 +233,25 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kernel(
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
-            store4<T>(out, 32 * d + 8 * g + 4 * h, a.dim, a.vec, o[d][4 * g] * inv, o[d][4 * g + 1] * inv,
+            store4<T, VEC>(out, 32 * d + 8 * g + 4 * h, a.dim, o[d][4 * g] * inv, o[d][4 * g + 1] * inv,
                 o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv);
     if (h == 0)
-        a.lse[((size_t)b * a.heads + head) * a.len_q + row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+        a.lse[((size_t)b * a.heads + head) * a.len_q + row] =
+            l == 0.0f ? -INFINITY : (m * (CAP || BIAS ? 1.0f : a.c1) + log2f(l)) * kLn2;
 }
 
-template <typename T, int DP, bool CAP, bool BIAS>
+template <typename T, int DP, bool CAP, bool BIAS, bool VEC>
 bool launch(const Args& a, hipStream_t s, const char* what) {
     const int tiles = (a.len_q + kRows - 1) / kRows;
-    attn_fwd_kernel<T, DP, CAP, BIAS><<<(unsigned)((long long)tiles * a.heads * a.batch), kTpb, 0, s>>>(a, tiles);
+    const unsigned blocks = (unsigned)((long long)tiles * a.heads * a.batch);
+    bool done = false;
+    if constexpr (CAP && !BIAS) {
+        if (a.c2 <= kFixedCap) {
+            attn_fwd_kernel<T, DP, 2, false, VEC><<<blocks, kTpb, 0, s>>>(a, tiles);
+            done = true;
+        }
+    }
+    if (!done) attn_fwd_kernel<T, DP, CAP, BIAS, VEC><<<blocks, kTpb, 0, s>>>(a, tiles);
     nnk_after_launch(what, s);
     return true;
 }
