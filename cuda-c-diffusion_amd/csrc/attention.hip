@@ -68,6 +68,7 @@ bool take(Args& p, const NnAttention* a, const char* what) {
         double power = (double)p.c2 * p.c1;
         for (int i = 0; i < 6; ++i, power *= (double)p.c1 * p.c1) p.series[i] = (float)(tanh_of[i] * power);
         p.small = kSeriesEnd / p.c1;
+        p.tiny = kShortSeriesEnd / p.c1;
     }
     p.q_start = a->q_start;
     p.k_len = a->k_len;
@@ -80,13 +81,13 @@ bool take(Args& p, const NnAttention* a, const char* what) {
 }
 
 // Whether rows of 16-byte chunks can be read and written: strides here, pointers by the
-// callers.
+// callers.  The offsets of 64 rows have to fit in 32 bits.
 bool strides_by_16(const NnAttention* a) {
-    const long long e = a->dtype == NN_BF16 ? 8 : 4;
+    const long long e = a->dtype == NN_BF16 ? 8 : 4, far = (1LL << 32) / (16 / e) / 64 - 128;
     bool ok = a->head_dim % e == 0;
     for (int i = 0; i < 3; ++i)
-        ok = ok && a->q_stride[i] % e == 0 && a->k_stride[i] % e == 0 && a->v_stride[i] % e == 0 &&
-            a->out_stride[i] % e == 0;
+        for (const long long* s : {a->q_stride, a->k_stride, a->v_stride, a->out_stride})
+            ok = ok && s[i] % e == 0 && (i != 1 || (s[i] >= 0 && s[i] <= far));
     return ok;
 }
 

@@ -168,7 +168,7 @@ __device__ __forceinline__ f32x4 operand(const f32x16& s, int f, float) {
     return v;
 }
 
-// 16 bytes of a row from feature d0 on.  Features from `dim` on are zeros, or (vec) a
+// 16 bytes of a row from feature d0 on.  Features from `dim` on are zeros, or (VEC) a
 // chunk wholly past them is the row's first one, for the caller to leave out: a choice
 // here would wait for the load.
 template <typename T, bool VEC>
@@ -210,31 +210,57 @@ __device__ __forceinline__ void store4(T* row, int d, int dim, float a, float b,
 }
 
 // A 64-row tile on its way from memory to LDS: loaded into registers while the tile
-// before it is used, stored when that is done.
+// before it is used, stored when that is done.  A lane's offsets in a tile are formed
+// once, in 32 bits (the host sees to it), and added to the tile's uniform address.
 template <typename T, int DP, bool VEC>
 struct Staged {
     static constexpr int kPerRow = DP / Type<T>::CE;
     static constexpr int N = kBlock * kPerRow / kTpb;
     u32x4 v[N];
+    unsigned off[VEC ? N : 1];
 
     static __device__ __forceinline__ int row(int n) { return (n * kTpb + (int)threadIdx.x) / kPerRow; }
-    // Row r of the tile is base + min(r, last) * stride.
-    __device__ __forceinline__ void load(const T* base, long long stride, int last, int dim) {
+    static __device__ __forceinline__ int chunk(int n) { return (n * kTpb + (int)threadIdx.x) % kPerRow; }
+    // A chunk past the features is the row's first one: whatever it meets has zeros there,
+    // or is not stored.
+    static __device__ __forceinline__ unsigned offset(int n, int r, long long stride, int dim) {
+        return (unsigned)r * (unsigned)(stride * (int)sizeof(T)) + (chunk(n) * Type<T>::CE < dim ? chunk(n) * 16 : 0);
+    }
+    __device__ __forceinline__ void init(long long stride, int dim) {
+        if constexpr (VEC) {
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int c = (n * kTpb + (int)threadIdx.x) % kPerRow;
-            v[n] = load_chunk<T, VEC>(base + min(row(n), last) * stride, c * Type<T>::CE, dim);
+            for (int n = 0; n < N; ++n) off[n] = offset(n, row(n), stride, dim);
         }
     }
-    // Zeros in place of the rows that are not kept, whatever they hold, and of features
-    // from `dim` on; keep(n): this lane's n-th row.
-    template <typename Keep>
-    __device__ __forceinline__ void store(char* lds, int dim, const Keep& keep) const {
+    // Row r of the tile is base + min(r, last) * stride.
+    __device__ __forceinline__ void load(const T* base, long long stride, int last, int dim) {
+        if constexpr (VEC) {
+            const char* p = reinterpret_cast<const char*>(base);
+            if (last >= kBlock - 1) {
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int c = (n * kTpb + (int)threadIdx.x) % kPerRow;
-            *reinterpret_cast<u32x4*>(lds + Lds<T, DP>::at(row(n), c)) =
-                (keep(n) & (c * Type<T>::CE < dim)) ? v[n] : u32x4{0, 0, 0, 0};
+                for (int n = 0; n < N; ++n) v[n] = *reinterpret_cast<const u32x4*>(p + off[n]);
+            } else {
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+                    v[n] = *reinterpret_cast<const u32x4*>(p + offset(n, min(row(n), last), stride, dim));
+            }
+        } else {
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+                v[n] = load_chunk<T, false>(base + min(row(n), last) * stride, chunk(n) * Type<T>::CE, dim);
+        }
+    }
+    // All of the rows, or (!all) zeros in place of those that are not kept, whatever they
+    // hold; keep(n): this lane's n-th row.
+    template <typename Keep>
+    __device__ __forceinline__ void store(char* lds, bool all, const Keep& keep) const {
+        if (all) {
+#pragma unroll
+            for (int n = 0; n < N; ++n) *reinterpret_cast<u32x4*>(lds + Lds<T, DP>::at(row(n), chunk(n))) = v[n];
+        } else {
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+                *reinterpret_cast<u32x4*>(lds + Lds<T, DP>::at(row(n), chunk(n))) = keep(n) ? v[n] : u32x4{0, 0, 0, 0};
         }
     }
 };
@@ -257,7 +283,7 @@ struct Args {
     int mask, buckets, max_distance;
     float scale, c1, c2;  // score in units of log2: c1 * s, or c2 * tanh(c1 * s)
     float series[6];      // c2 tanh(c1 s) = s (series[0] + w (series[1] + ...)), w = s^2, for small c1 s
-    float small;          // how small: |s| below this
+    float small, tiny;    // how small: |s| below this; and for its first 4 terms alone
     const int *q_start, *k_len, *prefix, *doc_q, *doc_k, *bucket;
     const float* bias;
     bool vec;
@@ -296,7 +322,8 @@ __device__ __forceinline__ float tanh_series(float y) {
     c = fmaf(w, c, -0.333333333f);
     return fmaf(y * w, c, y);
 }
-constexpr float kSeriesEnd = 0.375f;
+// ends of the series of 6 and of 4 terms: the next term is below 2^-24 of the first
+constexpr float kSeriesEnd = 0.375f, kShortSeriesEnd = 0.14f;
 // s[r] = tanh(c1 s[r]) and, if wanted, its slope
 template <bool SLOPE>
 __device__ __forceinline__ void cap_scores(f32x16& s, f32x16& slope, float c1) {
@@ -389,10 +416,12 @@ struct Blocks {
     int4 mine, own;  // own: documents of this lane's block
     int base, last;
     unsigned long long m;
-    int doc;  // of the block that next() gave: the one document of all its positions, or -1
+    int doc;        // of the block that next() gave: the one document of all its positions, or -1
+    bool negative;  // whether any of its positions has none
 
     __device__ __forceinline__ Blocks(int first, int last_, const int4* docs_, const int4& mine_)
-        : docs(docs_), mine(mine_), own{0, 0, 0, 0}, base(first), last(last_), doc(-1) {
+        : docs(docs_), mine(mine_), own{0, 0, 0, 0}, base(first), last(last_), doc(-1),
+          negative(false) {
         look();
     }
     __device__ __forceinline__ void look() {
@@ -411,7 +440,8 @@ struct Blocks {
         m &= m - 1;
         if (docs) {
             const int lo = __builtin_amdgcn_readlane(own.x, i), hi = __builtin_amdgcn_readlane(own.y, i);
-            doc = lo == hi && !__builtin_amdgcn_readlane(own.z, i) ? lo : -1;
+            negative = __builtin_amdgcn_readlane(own.z, i) != 0;
+            doc = lo == hi && !negative ? lo : -1;
         }
         return base + i;
     }

@@ -89,16 +89,15 @@ __global__ __launch_bounds__(kTpb, 1) void attn_bwd_kv_kernel(Args a, int tiles)
         const float2* stats = a.stat + ((size_t)b * a.heads + head) * a.len_q;
 
         Staged<T, DP, VEC> qs, gs;
-        float row_M[Staged<T, DP, VEC>::N];
+        qs.init(a.qs[1], a.dim);
+        gs.init(a.os[1], a.dim);
         float2 st = {INFINITY, 0.0f};
         int lim = 0, qdoc = -2;
         const auto load = [&](int block) {
             const int q0 = block * kBlock, last = a.len_q - 1 - q0;
-#pragma unroll
-            for (int n = 0; n < Staged<T, DP, VEC>::N; ++n) row_M[n] = stats[q0 + min(Staged<T, DP, VEC>::row(n), last)].x;
+            st = stats[q0 + min(lane, last)];
             if (wave == 0) {
                 const int i = q0 + min(lane, last);
-                st = stats[i];
                 if (a.doc_q) qdoc = a.doc_q[(size_t)b * a.len_q + i];
                 lim = limit_of(a, b, keys, start + i);
             }
@@ -110,10 +109,12 @@ __global__ __launch_bounds__(kTpb, 1) void attn_bwd_kv_kernel(Args a, int tiles)
             const int q0 = block * kBlock;
             // queries that see nothing are zeros
             const auto keep = [&](int n) {
-                return (q0 + Staged<T, DP, VEC>::row(n) < a.len_q) & (row_M[n] != INFINITY);
+                const int i = q0 + Staged<T, DP, VEC>::row(n);
+                return i < a.len_q && stats[i].x != INFINITY;
             };
-            qs.store(q_lds[to], a.dim, keep);
-            gs.store(g_lds[to], a.dim, keep);
+            const bool all = __all(q0 + lane < a.len_q && st.x != INFINITY);
+            qs.store(q_lds[to], all, keep);
+            gs.store(g_lds[to], all, keep);
             if (wave == 0) {
                 const bool there = q0 + lane < a.len_q;
                 M_lds[to][lane] = there ? st.x : INFINITY;

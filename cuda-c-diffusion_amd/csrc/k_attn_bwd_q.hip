@@ -74,28 +74,25 @@ __global__ __launch_bounds__(kTpb, 1) void attn_bwd_q_kernel(Args a, int tiles) 
     if constexpr (BIAS) load_bias(a, table, head);
 
     Staged<T, DP, VEC> ks, vs;
-    int row_doc[Staged<T, DP, VEC>::N], next_doc = 0;
-#pragma unroll
-    for (int n = 0; n < Staged<T, DP, VEC>::N; ++n) row_doc[n] = 0;
+    ks.init(a.ks[1], a.dim);
+    vs.init(a.vs[1], a.dim);
+    int next_doc = 0;
     const auto load = [&](int block) {
         const int k0 = block * kBlock, last = keys - 1 - k0;
-        if (docs) {
-#pragma unroll
-            for (int n = 0; n < Staged<T, DP, VEC>::N; ++n)
-                row_doc[n] = docs[k0 + min(Staged<T, DP, VEC>::row(n), last)];
-            next_doc = docs[k0 + min(lane, last)];
-        }
+        if (docs) next_doc = docs[k0 + min(lane, last)];
         ks.load(kp + k0 * a.ks[1], a.ks[1], last, a.dim);
         vs.load(vp + k0 * a.vs[1], a.vs[1], last, a.dim);
     };
-    const auto store = [&](int block, int to) {
+    const auto store = [&](int block, bool negative, int to) {
         const int k0 = block * kBlock;
         // keys that nothing sees are zeros
         const auto keep = [&](int n) {
-            return (k0 + Staged<T, DP, VEC>::row(n) < keys) & (row_doc[n] >= 0);
+            const int r = Staged<T, DP, VEC>::row(n);
+            return k0 + r < keys && (!docs || docs[k0 + r] >= 0);
         };
-        ks.store(k_lds[to], a.dim, keep);
-        vs.store(v_lds[to], a.dim, keep);
+        const bool all = k0 + kBlock <= keys && !negative;
+        ks.store(k_lds[to], all, keep);
+        vs.store(v_lds[to], all, keep);
         if (docs && wave == 0) doc_lds[to][lane] = k0 + lane < keys ? next_doc : -1;
     };
 
@@ -108,7 +105,7 @@ __global__ __launch_bounds__(kTpb, 1) void attn_bwd_q_kernel(Args a, int tiles) 
     int next = at.next();
     if (next >= 0) {
         load(next);
-        store(next, 0);
+        store(next, at.negative, 0);
     }
     bool first = true;
     for (int buf = 0; next >= 0; buf ^= 1, first = false) {
@@ -185,7 +182,7 @@ __global__ __launch_bounds__(kTpb, 1) void attn_bwd_q_kernel(Args a, int tiles) 
                 for (int d = 0; d < DP / 32; ++d) dq[d] = mma(L::cols(k_lds[buf], i, f, d, cbase), x, dq[d]);
             }
         }
-        if (next >= 0) store(next, buf ^ 1);
+        if (next >= 0) store(next, at.negative, buf ^ 1);
     }
 
     if (!in) return;

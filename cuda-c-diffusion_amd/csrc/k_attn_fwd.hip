@@ -14,7 +14,8 @@
 //   cap:    scores within +-c2 (units of log2) need no running maximum.  m is that of the
 //           first block that a query sees, or c2 - 80 if that is more: then p <= 2^80 and,
 //           for c2 up to 80, l >= 2^-80, both far from the ends of fp32.  For scores below
-//           3/8 of the cap, tanh, its factors and the reference are one polynomial;
+//           3/8 of the cap, tanh, its factors and the reference are one polynomial, of 4
+//           terms instead of 6 below 0.14 of it;
 //   else:   running maximum of x.
 #include "attn_common.h"
 
@@ -68,28 +69,25 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && VEC ? 2 : 1) void attn_fwd_
     if constexpr (BIAS) load_bias(a, table, head);
 
     Staged<T, DP, VEC> ks, vs;
-    int row_doc[Staged<T, DP, VEC>::N], next_doc = 0;
-#pragma unroll
-    for (int n = 0; n < Staged<T, DP, VEC>::N; ++n) row_doc[n] = 0;
+    ks.init(a.ks[1], a.dim);
+    vs.init(a.vs[1], a.dim);
+    int next_doc = 0;
     const auto load = [&](int block) {
         const int k0 = block * kBlock, last = keys - 1 - k0;
-        if (docs) {
-#pragma unroll
-            for (int n = 0; n < Staged<T, DP, VEC>::N; ++n)
-                row_doc[n] = docs[k0 + min(Staged<T, DP, VEC>::row(n), last)];
-            next_doc = docs[k0 + min(lane, last)];
-        }
+        if (docs) next_doc = docs[k0 + min(lane, last)];
         ks.load(kp + k0 * a.ks[1], a.ks[1], last, a.dim);
         vs.load(vp + k0 * a.vs[1], a.vs[1], last, a.dim);
     };
-    const auto store = [&](int block, int to) {
+    const auto store = [&](int block, bool negative, int to) {
         const int k0 = block * kBlock;
         // keys that nothing sees are zeros
         const auto keep = [&](int n) {
-            return (k0 + Staged<T, DP, VEC>::row(n) < keys) & (row_doc[n] >= 0);
+            const int r = Staged<T, DP, VEC>::row(n);
+            return k0 + r < keys && (!docs || docs[k0 + r] >= 0);
         };
-        ks.store(k_lds[to], a.dim, keep);
-        vs.store(v_lds[to], a.dim, keep);
+        const bool all = k0 + kBlock <= keys && !negative;
+        ks.store(k_lds[to], all, keep);
+        vs.store(v_lds[to], all, keep);
         if (docs && wave == 0) doc_lds[to][lane] = k0 + lane < keys ? next_doc : -1;
     };
 
@@ -102,7 +100,7 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && VEC ? 2 : 1) void attn_fwd_
     int next = at.next();
     if (next >= 0) {
         load(next);
-        store(next, 0);
+        store(next, at.negative, 0);
     }
     for (int buf = 0; next >= 0; buf ^= 1) {
         const int k0 = next * kBlock, block_doc = at.doc;
@@ -150,20 +148,23 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && VEC ? 2 : 1) void attn_fwd_
             for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(s[i][r]));
-            const bool series = __all(top < a.small);
-            if (whole && series && __all(m != -INFINITY)) {
+            const auto by_series = [&](auto terms) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
                         const float w = s[i][r] * s[i][r];
-                        float c = fmaf(w, a.series[5], a.series[4]);
-                        c = fmaf(w, c, a.series[3]);
-                        c = fmaf(w, c, a.series[2]);
-                        c = fmaf(w, c, a.series[1]);
-                        c = fmaf(w, c, a.series[0]);
+                        float c = a.series[decltype(terms)::value - 1];
+#pragma unroll
+                        for (int t = decltype(terms)::value - 2; t >= 0; --t) c = fmaf(w, c, a.series[t]);
                         s[i][r] = exp2_fast(fmaf(s[i][r], c, -m));
                     }
+            };
+            const bool plain = whole && __all(m != -INFINITY);
+            if (plain && __all(top < a.tiny)) {
+                by_series(std::integral_constant<int, 4>{});
+            } else if (plain && __all(top < a.small)) {
+                by_series(std::integral_constant<int, 6>{});
             } else {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
@@ -222,7 +223,7 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && VEC ? 2 : 1) void attn_fwd_
                 for (int d = 0; d < DP / 32; ++d) o[d] = mma(L::cols(v_lds[buf], i, f, d, cbase), p, o[d]);
             }
         }
-        if (next >= 0) store(next, buf ^ 1);
+        if (next >= 0) store(next, at.negative, buf ^ 1);
     }
 
     if (!in) return;
