@@ -97,7 +97,9 @@ extern "C" {
 
 size_t nnhip_attention_forward_workspace(const NnAttention* a) {
     if (!sizes_fit(a, "nnhip_attention_forward_workspace")) return 0;
-    return docs_floats(a);
+    if (!a->batch || !a->len_q) return 0;
+    const size_t n = docs_floats(a) + (nnk_attention_is_few(a) ? nnk_attention_few_floats(a) : 0);
+    return n ? kTicketWords + n : 0;
 }
 
 void launch_attention_forward(void* out, float* lse, const void* q, const void* k, const void* v,
@@ -115,8 +117,11 @@ void launch_attention_forward(void* out, float* lse, const void* q, const void* 
     p.out = out;
     p.lse = lse;
     p.vec = strides_by_16(a) && nnk::aligned16(q) && nnk::aligned16(k) && nnk::aligned16(v) && nnk::aligned16(out);
-    nnk_attention_docs(p, workspace, s, what);
-    nnk_attention_forward(p, a->dtype == NN_BF16, s, what);
+    const bool few = nnk_attention_is_few(a);
+    if (a->doc_q)
+        nnk_attention_docs(p, workspace + kTicketWords + (few ? nnk_attention_few_floats(a) : 0), s, what);
+    if (few) nnk_attention_few(p, a->dtype == NN_BF16, workspace, s, what);
+    else nnk_attention_forward(p, a->dtype == NN_BF16, s, what);
 }
 
 size_t nnhip_attention_backward_workspace(const NnAttention* a) {

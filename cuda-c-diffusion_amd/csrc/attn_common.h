@@ -41,6 +41,7 @@ constexpr int kTpb = 256;
 constexpr int kWaves = kTpb / 64;
 constexpr int kRows = 32 * kWaves;  // columns of a workgroup: queries, or keys in the key gradients
 constexpr int kMaxDistance = 1023;
+constexpr int kTicketWords = 2048;  // at the front of every forward workspace: zeros between calls
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
@@ -472,6 +473,10 @@ void nnk_attention_docs(attn::Args& args, float* ws, hipStream_t s, const char* 
 bool nnk_attention_forward(const attn::Args& args, bool half, hipStream_t s, const char* what);
 bool nnk_attention_backward_q(const attn::Args& args, bool half, hipStream_t s, const char* what);
 bool nnk_attention_backward_kv(const attn::Args& args, bool half, hipStream_t s, const char* what);
+// The form for few queries; when it is taken; the floats that it needs after the tickets.
+bool nnk_attention_is_few(const NnAttention* a);
+size_t nnk_attention_few_floats(const NnAttention* a);
+bool nnk_attention_few(const attn::Args& args, bool half, float* ws, hipStream_t s, const char* what);
 // Bias gradient from args.dist_sums, and the floats that those take.
 void nnk_attention_bias_grad(const attn::Args& args, float* dbias, hipStream_t s, const char* what);
 size_t nnk_attention_dist_floats(const NnAttention* a);
