@@ -13,6 +13,10 @@ size_t docs_floats(const NnAttention* a) {
     const size_t nk = ((size_t)a->len_k + kBlock - 1) / kBlock, nq = ((size_t)a->len_q + kBlock - 1) / kBlock;
     return 4 * (size_t)a->batch * (nk + nq);
 }
+size_t head_floats(const NnAttention* a) {
+    const size_t n = (size_t)a->batch * a->heads * a->len_k * a->head_dim;
+    return nnk_attention_splits_heads(a) ? (2 * n + 3) / 4 * 4 : 0;
+}
 size_t stat_floats(const NnAttention* a) { return 2 * (size_t)a->batch * a->heads * a->len_q; }
 
 bool sizes_fit(const NnAttention* a, const char* what) {
@@ -126,7 +130,7 @@ void launch_attention_forward(void* out, float* lse, const void* q, const void* 
 
 size_t nnhip_attention_backward_workspace(const NnAttention* a) {
     if (!sizes_fit(a, "nnhip_attention_backward_workspace")) return 0;
-    return docs_floats(a) + stat_floats(a) + (a->buckets ? nnk_attention_dist_floats(a) : 0);
+    return docs_floats(a) + head_floats(a) + stat_floats(a) + (a->buckets ? nnk_attention_dist_floats(a) : 0);
 }
 
 void launch_attention_backward(void* dq, void* dk, void* dv, float* dbias, const void* dout,
@@ -153,8 +157,12 @@ void launch_attention_backward(void* dq, void* dk, void* dv, float* dbias, const
     p.vec = strides_by_16(a);
     for (const void* x : {q, k, v, out, dout, (const void*)dq, (const void*)dk, (const void*)dv})
         p.vec = p.vec && nnk::aligned16(x);
-    p.stat = reinterpret_cast<float2*>(workspace + docs_floats(a));
-    if (dbias) p.dist_sums = workspace + docs_floats(a) + stat_floats(a);
+    float* ws = workspace + docs_floats(a);
+    if (head_floats(a)) p.head_sums = ws;
+    p.heads_each = p.head_sums ? 1 : p.group;
+    ws += head_floats(a);
+    p.stat = reinterpret_cast<float2*>(ws);
+    if (dbias) p.dist_sums = ws + stat_floats(a);
     const bool half = a->dtype == NN_BF16;
     if (has_q && has_k) nnk_attention_docs(p, workspace, s, what);
     if (has_q && !nnk_attention_backward_q(p, half, s, what)) return;

@@ -40,6 +40,7 @@ constexpr int kBlock = 64;     // keys (or queries) of a tile in LDS
 constexpr int kTpb = 256;
 constexpr int kWaves = kTpb / 64;
 constexpr int kRows = 32 * kWaves;  // columns of a workgroup: queries, or keys in the key gradients
+constexpr int kCus = 256;
 constexpr int kMaxDistance = 1023;
 constexpr int kTicketWords = 2048;  // at the front of every forward workspace: zeros between calls
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -109,6 +110,8 @@ struct Lds {
     static constexpr int kBytes = kBlock * kRowBytes;
     static constexpr int kSteps = DP / (2 * Type<T>::CE);     // fragments of a row
     static constexpr int kKeySteps = 32 / (2 * Type<T>::CE);  // fragments of 32 rows
+    // fragments of a stage of one or of two operands: enough products to hide its reads
+    static constexpr int kWide = sizeof(T) == 2 ? 4 : 2, kStage = kWide / 2;
 
     // Bits of the row in other places, so F(a ^ b) = F(a) ^ F(b).
     static __host__ __device__ constexpr int F(int row) {
@@ -151,6 +154,23 @@ struct Lds {
         }
     }
 };
+
+// Products whose operands come from LDS: stage n + 1's reads are issued before stage n's
+// products, and vector instructions may move anywhere.  The compiler by itself puts each
+// read next to its product and waits for it there, which at one or two waves a SIMD is the
+// latency of LDS for every product.  load(stage, n) reads, use(stage, n) multiplies;
+// stages[0] is read by the caller, early enough to have other work in between.
+constexpr int kMayCross = 0x6;  // vector and scalar instructions
+template <int N, typename Stage, typename Load, typename Use>
+__device__ __forceinline__ void piped(Stage (&stages)[2], const Load& load, const Use& use) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        if (n + 1 < N) load(stages[(n + 1) & 1], n + 1);
+        __builtin_amdgcn_sched_barrier(kMayCross);
+        use(stages[n & 1], n);
+        __builtin_amdgcn_sched_barrier(kMayCross);
+    }
+}
 
 // Registers of a tile's fragment f as the operand of the next product.  bf16: the
 // probabilities (or score gradients) are rounded to bf16 here, each by at most 2^-8 of
@@ -277,6 +297,8 @@ struct Args {
     void *dq, *dk, *dv;
     float2* stat;      // backward: per query, log2 of its sum and its <p, dp>
     float* dist_sums;  // backward: sums of score gradients by distance, per key tile
+    float* head_sums;  // backward: dk / scale, then dv, of each head [batch, heads, len_k, dim], or null
+    int heads_each;    // backward: heads of a workgroup, 1 or all that share a key head
     const int4* key_docs;    // per block of 64 keys: least and largest document, whether any is negative
     const int4* query_docs;  // per block of 64 queries
     long long qs[3], ks[3], vs[3], os[3];
@@ -477,6 +499,8 @@ bool nnk_attention_backward_kv(const attn::Args& args, bool half, hipStream_t s,
 bool nnk_attention_is_few(const NnAttention* a);
 size_t nnk_attention_few_floats(const NnAttention* a);
 bool nnk_attention_few(const attn::Args& args, bool half, float* ws, hipStream_t s, const char* what);
+// Whether the key gradients of heads that share a key head are summed apart first.
+bool nnk_attention_splits_heads(const NnAttention* a);
 // Bias gradient from args.dist_sums, and the floats that those take.
 void nnk_attention_bias_grad(const attn::Args& args, float* dbias, hipStream_t s, const char* what);
 size_t nnk_attention_dist_floats(const NnAttention* a);

@@ -7,7 +7,10 @@
 // head, 32 a wave, with k and v in registers, and goes over the blocks of 64 queries of
 // its heads; q and dout of a block are in LDS.  Scores are formed as queries x keys, so
 // that their registers are the operand of both gradients.  No atomics: a key's sums are
-// one wave's, in a fixed order.
+// one wave's, in a fixed order.  Where key heads are shared and key tiles are few, a
+// workgroup takes one head's queries and leaves fp32 sums, which a second kernel adds up
+// in the heads' order: documents and causal masks give tiles very uneven work, which only
+// more workgroups even out.
 //
 // Bias: sums of dx by distance j - P.  A 32 x 32 tile has its distances on diagonals;
 // row m's values go m lanes along, after which a lane holds two distances (one for what
@@ -21,7 +24,7 @@ using namespace attn;
 constexpr int kSlack = 64;  // distances of a tile that reaches past max_distance
 
 template <typename T, int DP, bool CAP, bool BIAS, bool VEC>
-__global__ __launch_bounds__(kTpb, 1) void attn_bwd_kv_kernel(Args a, int tiles) {
+__global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn_bwd_kv_kernel(Args a, int tiles) {
     using L = Lds<T, DP>;
     // two blocks in LDS; one where they and the distances would not fit (fp32, over 64 features)
     constexpr int kBufs = L::kRowBytes > 256 ? 1 : 2;
@@ -36,7 +39,8 @@ __global__ __launch_bounds__(kTpb, 1) void attn_bwd_kv_kernel(Args a, int tiles)
 
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
     const int w = nnk::xcd_swizzle(blockIdx.x, gridDim.x);
-    const int tile = w % tiles, kv = w / tiles % a.kv_heads, b = w / tiles / a.kv_heads;
+    const int tile = w % tiles, part = w / tiles % (a.heads / a.heads_each), b = w / tiles / (a.heads / a.heads_each);
+    const int head0 = part * a.heads_each, kv = head0 / a.group;
     const int k0 = tile * kRows, key = k0 + wave * 32 + (lane & 31);
     const int keys = keys_of(a, b), start = start_of(a, b);
     const int* docs = a.doc_k ? a.doc_k + (size_t)b * a.len_k : nullptr;
@@ -77,7 +81,7 @@ __global__ __launch_bounds__(kTpb, 1) void attn_bwd_kv_kernel(Args a, int tiles)
     const int span = 2 * (a.max_distance + kSlack) + 1;
     float* my_dist = dist + wave * span;
 
-    for (int head = kv * a.group; head < (kv + 1) * a.group; ++head) {
+    for (int head = head0; head < head0 + a.heads_each; ++head) {
         float far_lo = 0.0f, far_hi = 0.0f;
         __syncthreads();  // the head before is done with
         if constexpr (BIAS) {
@@ -140,11 +144,36 @@ __global__ __launch_bounds__(kTpb, 1) void attn_bwd_kv_kernel(Args a, int tiles)
 #pragma unroll 1
             for (int i = 0; i < 2; ++i) {
                 f32x16 s = zero16(), dp = zero16();
+                struct Pair {
+                    Frag<T> q[L::kStage], g[L::kStage];
+                };
+                Pair two[2];
+                const auto read_rows = [&](Pair& x, int n) {
 #pragma unroll
-                for (int u = 0; u < L::kSteps; ++u) {
-                    s = mma(L::rows(q_lds[buf], i, u, rbase), kf[u], s);
-                    dp = mma(L::rows(g_lds[buf], i, u, rbase), vf[u], dp);
-                }
+                    for (int j = 0; j < L::kStage; ++j) {
+                        x.q[j] = L::rows(q_lds[buf], i, n * L::kStage + j, rbase);
+                        x.g[j] = L::rows(g_lds[buf], i, n * L::kStage + j, rbase);
+                    }
+                };
+                read_rows(two[0], 0);
+                piped<L::kSteps / L::kStage>(two, read_rows, [&](const Pair& x, int n) {
+#pragma unroll
+                    for (int j = 0; j < L::kStage; ++j) {
+                        s = mma(x.q[j], kf[n * L::kStage + j], s);
+                        dp = mma(x.g[j], vf[n * L::kStage + j], dp);
+                    }
+                });
+                // columns of fragment n / kCols, features 32 (n % kCols) ...
+                constexpr int kCols = DP / 32 / (DP / 32 % L::kStage ? 1 : L::kStage), kWide = DP / 32 / kCols;
+                const auto read_cols = [&](Pair& x, int n) {
+#pragma unroll
+                    for (int j = 0; j < kWide; ++j) {
+                        x.g[j] = L::cols(g_lds[buf], i, n / kCols, n % kCols * kWide + j, cbase);
+                        x.q[j] = L::cols(q_lds[buf], i, n / kCols, n % kCols * kWide + j, cbase);
+                    }
+                };
+                read_cols(two[0], 0);
+                __builtin_amdgcn_sched_barrier(kMayCross);
                 f32x16 slope;
                 if constexpr (CAP) cap_scores<true>(s, slope, a.c1);
                 const float c = CAP ? a.c2 : a.c1;
@@ -213,15 +242,20 @@ __global__ __launch_bounds__(kTpb, 1) void attn_bwd_kv_kernel(Args a, int tiles)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) dp[r] *= slope[r];
                 }
+                Frag<T> p[L::kKeySteps], x[L::kKeySteps];
 #pragma unroll
                 for (int f = 0; f < L::kKeySteps; ++f) {
-                    const Frag<T> p = operand(s, f, T{}), x = operand(dp, f, T{});
-#pragma unroll
-                    for (int d = 0; d < DP / 32; ++d) {
-                        dv[d] = mma(L::cols(g_lds[buf], i, f, d, cbase), p, dv[d]);
-                        dk[d] = mma(L::cols(q_lds[buf], i, f, d, cbase), x, dk[d]);
-                    }
+                    p[f] = operand(s, f, T{});
+                    x[f] = operand(dp, f, T{});
                 }
+                piped<L::kKeySteps * kCols>(two, read_cols, [&](const Pair& y, int n) {
+#pragma unroll
+                    for (int j = 0; j < kWide; ++j) {
+                        const int d = n % kCols * kWide + j;
+                        dv[d] = mma(y.g[j], p[n / kCols], dv[d]);
+                        dk[d] = mma(y.q[j], x[n / kCols], dk[d]);
+                    }
+                });
             }
             if (kBufs == 1) __syncthreads();
             if (next >= 0) store(next, buf ^ (kBufs - 1));
@@ -251,6 +285,19 @@ __global__ __launch_bounds__(kTpb, 1) void attn_bwd_kv_kernel(Args a, int tiles)
     }
 
     if (!in) return;
+    if (a.head_sums) {
+        const size_t at = (((size_t)b * a.heads + head0) * a.len_k + key) * a.dim;
+        float *kout = a.head_sums + at, *vout = kout + (size_t)a.batch * a.heads * a.len_k * a.dim;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int at = 32 * d + 8 * g + 4 * h;
+                store4<float, VEC>(kout, at, a.dim, dk[d][4 * g], dk[d][4 * g + 1], dk[d][4 * g + 2], dk[d][4 * g + 3]);
+                store4<float, VEC>(vout, at, a.dim, dv[d][4 * g], dv[d][4 * g + 1], dv[d][4 * g + 2], dv[d][4 * g + 3]);
+            }
+        return;
+    }
     T* kout = (T*)a.dk + b * a.ks[0] + (long long)key * a.ks[1] + kv * a.ks[2];
     T* vout = (T*)a.dv + b * a.vs[0] + (long long)key * a.vs[1] + kv * a.vs[2];
 #pragma unroll
@@ -262,6 +309,34 @@ __global__ __launch_bounds__(kTpb, 1) void attn_bwd_kv_kernel(Args a, int tiles)
                 dk[d][4 * g + 2] * a.scale, dk[d][4 * g + 3] * a.scale);
             store4<T, VEC>(vout, at, a.dim, dv[d][4 * g], dv[d][4 * g + 1], dv[d][4 * g + 2], dv[d][4 * g + 3]);
         }
+}
+
+// dk and dv from the sums of the heads that share a key head, in their order; 4 features a
+// thread.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(kTpb) void attn_head_sum_kernel(Args a, int quads, long long total) {
+    const long long n = (long long)blockIdx.x * kTpb + threadIdx.x;
+    if (n >= total) return;
+    const int d = (int)(n % quads) * 4;
+    const long long row = n / quads;
+    const int key = (int)(row % a.len_k), kv = (int)(row / a.len_k % a.kv_heads), b = (int)(row / a.len_k / a.kv_heads);
+    const float* from = a.head_sums + (((size_t)b * a.heads + kv * a.group) * a.len_k + key) * a.dim + d;
+    const size_t step = (size_t)a.len_k * a.dim, v_at = (size_t)a.batch * a.heads * a.len_k * a.dim;
+    float k[4] = {0.0f, 0.0f, 0.0f, 0.0f}, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int g = 0; g < a.group; ++g) {
+        if constexpr (VEC) {
+            const float4 x = nnk::ld4(from + g * step), y = nnk::ld4(from + g * step + v_at);
+            k[0] += x.x, k[1] += x.y, k[2] += x.z, k[3] += x.w;
+            v[0] += y.x, v[1] += y.y, v[2] += y.z, v[3] += y.w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (d + j < a.dim) k[j] += from[g * step + j], v[j] += from[g * step + v_at + j];
+        }
+    }
+    store4<T, VEC>((T*)a.dk + b * a.ks[0] + key * a.ks[1] + kv * a.ks[2], d, a.dim, k[0] * a.scale, k[1] * a.scale,
+        k[2] * a.scale, k[3] * a.scale);
+    store4<T, VEC>((T*)a.dv + b * a.vs[0] + key * a.vs[1] + kv * a.vs[2], d, a.dim, v[0], v[1], v[2], v[3]);
 }
 
 // dbias[bucket, head]: the sums of its distances over batch and key tiles, in 64 bits,
@@ -295,8 +370,14 @@ bool launch(const Args& a, hipStream_t s, const char* what) {
             return false;
     }
     attn_bwd_kv_kernel<T, DP, CAP, BIAS, VEC>
-        <<<(unsigned)((long long)tiles * a.kv_heads * a.batch), kTpb, lds, s>>>(a, tiles);
+        <<<(unsigned)((long long)tiles * (a.heads / a.heads_each) * a.batch), kTpb, lds, s>>>(a, tiles);
     nnk_after_launch(what, s);
+    if (a.head_sums) {
+        const int quads = (a.dim + 3) / 4;
+        const long long total = (long long)a.batch * a.kv_heads * a.len_k * quads;
+        attn_head_sum_kernel<T, VEC><<<(unsigned)((total + kTpb - 1) / kTpb), kTpb, 0, s>>>(a, quads, total);
+        nnk_after_launch(what, s);
+    }
     return true;
 }
 
@@ -304,6 +385,11 @@ bool launch(const Args& a, hipStream_t s, const char* what) {
 
 bool nnk_attention_backward_kv(const Args& a, bool half, hipStream_t s, const char* what) {
     return NNK_ATTN_DISPATCH(a, half, launch, a, s, what);
+}
+
+bool nnk_attention_splits_heads(const NnAttention* a) {
+    const long long tiles = ((long long)a->len_k + kRows - 1) / kRows * a->kv_heads * a->batch;
+    return a->heads > a->kv_heads && tiles < 4 * kCus;
 }
 
 size_t nnk_attention_dist_floats(const NnAttention* a) {

@@ -16,7 +16,7 @@ namespace {
 using namespace attn;
 
 template <typename T, int DP, bool CAP, bool BIAS, bool VEC>
-__global__ __launch_bounds__(kTpb, 1) void attn_bwd_q_kernel(Args a, int tiles) {
+__global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn_bwd_q_kernel(Args a, int tiles) {
     using L = Lds<T, DP>;
     __shared__ __attribute__((aligned(16))) char k_lds[2][L::kBytes];
     __shared__ __attribute__((aligned(16))) char v_lds[2][L::kBytes];
@@ -115,15 +115,32 @@ __global__ __launch_bounds__(kTpb, 1) void attn_bwd_q_kernel(Args a, int tiles) 
         if (next >= 0) load(next);
 
         const bool whole = k0 + kBlock <= least && (!docs || (one_doc && block_doc == wave_doc));
+        struct Pair {
+            Frag<T> k[L::kStage], v[L::kStage];
+        };
+        struct Columns {
+            Frag<T> x[DP / 32];
+        };
         // scores (in units of log2) and dp of keys 32 i .. 32 i + 31; slope: 1 - tanh^2
         const auto products = [&](int i, f32x16& s, f32x16& dp, f32x16& slope) {
             s = zero16();
             dp = zero16();
+            Pair two[2];
+            const auto read_rows = [&](Pair& y, int n) {
 #pragma unroll
-            for (int u = 0; u < L::kSteps; ++u) {
-                s = mma(L::rows(k_lds[buf], i, u, rbase), qf[u], s);
-                dp = mma(L::rows(v_lds[buf], i, u, rbase), gf[u], dp);
-            }
+                for (int j = 0; j < L::kStage; ++j) {
+                    y.k[j] = L::rows(k_lds[buf], i, n * L::kStage + j, rbase);
+                    y.v[j] = L::rows(v_lds[buf], i, n * L::kStage + j, rbase);
+                }
+            };
+            read_rows(two[0], 0);
+            piped<L::kSteps / L::kStage>(two, read_rows, [&](const Pair& y, int n) {
+#pragma unroll
+                for (int j = 0; j < L::kStage; ++j) {
+                    s = mma(y.k[j], qf[n * L::kStage + j], s);
+                    dp = mma(y.v[j], gf[n * L::kStage + j], dp);
+                }
+            });
             if constexpr (CAP) cap_scores<true>(s, slope, a.c1);
             const float c = CAP ? a.c2 : a.c1;
             if constexpr (BIAS) {
@@ -166,6 +183,13 @@ __global__ __launch_bounds__(kTpb, 1) void attn_bwd_q_kernel(Args a, int tiles) 
         for (int i = 0; i < 2; ++i) {
             f32x16 s, dp, slope;
             products(i, s, dp, slope);
+            Columns columns[2];
+            const auto read_columns = [&](Columns& y, int n) {
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d) y.x[d] = L::cols(k_lds[buf], i, n, d, cbase);
+            };
+            read_columns(columns[0], 0);
+            __builtin_amdgcn_sched_barrier(kMayCross);
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const float p = exp2_fast(s[r] - M);
@@ -175,12 +199,11 @@ __global__ __launch_bounds__(kTpb, 1) void attn_bwd_q_kernel(Args a, int tiles) 
                 if constexpr (CAP) dx *= slope[r];
                 s[r] = dx;
             }
+            piped<L::kKeySteps>(columns, read_columns, [&](const Columns& y, int n) {
+                const Frag<T> x = operand(s, n, T{});
 #pragma unroll
-            for (int f = 0; f < L::kKeySteps; ++f) {
-                const Frag<T> x = operand(s, f, T{});
-#pragma unroll
-                for (int d = 0; d < DP / 32; ++d) dq[d] = mma(L::cols(k_lds[buf], i, f, d, cbase), x, dq[d]);
-            }
+                for (int d = 0; d < DP / 32; ++d) dq[d] = mma(y.x[d], x, dq[d]);
+            });
         }
         if (next >= 0) store(next, at.negative, buf ^ 1);
     }

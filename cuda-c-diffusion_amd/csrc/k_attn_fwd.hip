@@ -28,6 +28,9 @@ constexpr float kFixedCap = 80.0f;
 template <typename T, int DP, int CAP, bool BIAS, bool VEC>
 __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && VEC ? 2 : 1) void attn_fwd_kernel(Args a, int tiles) {
     using L = Lds<T, DP>;
+    // fp32, one wave a SIMD: reads of LDS ahead of their products.  bf16 has two waves, which
+    // hide them for each other, and no registers for it (128 features: 1.6 ms became 2.4)
+    constexpr bool kPiped = sizeof(T) == 4;
     __shared__ __attribute__((aligned(16))) char k_lds[2][L::kBytes];
     __shared__ __attribute__((aligned(16))) char v_lds[2][L::kBytes];
     __shared__ __attribute__((aligned(16))) int doc_lds[2][kBlock];
@@ -108,12 +111,47 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && VEC ? 2 : 1) void attn_fwd_
         __syncthreads();  // this block is stored; the one before it is done with
         if (next >= 0) load(next);
 
-        f32x16 s[2];
+        f32x16 s[2] = {zero16(), zero16()};
+        struct Keys {
+            Frag<T> x[L::kWide];
+        };
+        Keys rows[2];
+        const auto read_rows = [&](Keys& y, int n) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            s[i] = zero16();
+            for (int j = 0; j < L::kWide; ++j) {
+                const int u = n * L::kWide + j;
+                y.x[j] = L::rows(k_lds[buf], u / L::kSteps, u % L::kSteps, rbase);
+            }
+        };
+        const auto score = [&](const Keys& y, int n) {
 #pragma unroll
-            for (int u = 0; u < L::kSteps; ++u) s[i] = mma(L::rows(k_lds[buf], i, u, rbase), qf[u], s[i]);
+            for (int j = 0; j < L::kWide; ++j) {
+                const int u = n * L::kWide + j;
+                s[u / L::kSteps] = mma(y.x[j], qf[u % L::kSteps], s[u / L::kSteps]);
+            }
+        };
+        if constexpr (kPiped) {
+            read_rows(rows[0], 0);
+            piped<2 * L::kSteps / L::kWide>(rows, read_rows, score);
+        } else {
+#pragma unroll
+            for (int n = 0; n < 2 * L::kSteps / L::kWide; ++n) {
+                read_rows(rows[0], n);
+                score(rows[0], n);
+            }
+        }
+        struct Values {
+            Frag<T> x[DP / 32];
+        };
+        Values columns[2];
+        const auto read_columns = [&](Values& y, int n) {
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+                y.x[d] = L::cols(v_lds[buf], n / L::kKeySteps, n % L::kKeySteps, d, cbase);
+        };
+        if constexpr (kPiped) {
+            read_columns(columns[0], 0);
+            __builtin_amdgcn_sched_barrier(kMayCross);
         }
         const bool whole = k0 + kBlock <= least && (!docs || (one_doc && block_doc == wave_doc));
         const auto hide_both = [&]() {
@@ -213,14 +251,21 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && VEC ? 2 : 1) void attn_fwd_
                 for (int r = 0; r < 16; ++r) s[i][r] = exp2_fast(s[i][r] - base);
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int r = 0; r < 16; ++r) l += s[i][r];
+        const auto mix = [&](const Values& y, int n) {
+            const Frag<T> p = operand(s[n / L::kKeySteps], n % L::kKeySteps, T{});
 #pragma unroll
-            for (int f = 0; f < L::kKeySteps; ++f) {
-                const Frag<T> p = operand(s[i], f, T{});
+            for (int d = 0; d < DP / 32; ++d) o[d] = mma(y.x[d], p, o[d]);
+        };
+        if constexpr (kPiped) {
+            piped<2 * L::kKeySteps>(columns, read_columns, mix);
+        } else {
 #pragma unroll
-                for (int d = 0; d < DP / 32; ++d) o[d] = mma(L::cols(v_lds[buf], i, f, d, cbase), p, o[d]);
+            for (int n = 0; n < 2 * L::kKeySteps; ++n) {
+                read_columns(columns[0], n);
+                mix(columns[0], n);
             }
         }
         if (next >= 0) store(next, at.negative, buf ^ 1);
