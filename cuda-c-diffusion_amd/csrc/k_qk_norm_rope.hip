@@ -6,9 +6,12 @@
 //     dw = sum over rows of g x r,   dx = r (g w - x r mean(g w x r)).
 // Both read a row once and write it once; at the sizes that matter memory bounds them.  A
 // row belongs to the G lanes of one group, 16 bytes a lane, so that the two sums are
-// shuffles in the group; the pair's other member, half a rotation away, comes from the
-// group's row in LDS (interleaved pairs are one lane's).  A workgroup takes whole tokens,
-// whose sines and cosines it forms once for all their heads.
+// cross-lane adds in the group.  The pair's other member is one lane's own if pairs are
+// interleaved, else half a rotation away, and comes from the group's row in LDS: where that
+// is whole 16-byte chunks, by 16-byte accesses in an order without bank conflicts, and the
+// lane keeps its sines and cosines in registers for all heads of a token (they took a third
+// of the time as element-wise reads).  A workgroup takes whole tokens, whose sines and
+// cosines it forms once, first all their queries, then their keys.
 #include "nn_attention.h"
 #include "nnk_common.h"
 
@@ -34,8 +37,9 @@ struct Rope {
     const float *q_weight, *k_weight;
     const int* pos;
     const double* freq;
-    int tokens, heads, all_heads, dim, half, axes, per_axis, interleaved;
+    int tokens, heads, kv_heads, all_heads, dim, half, axes, per_axis, interleaved;
     int tokens_each, head_parts;        // tokens of a workgroup at a time; workgroups that share them
+    int tokens_all;                     // backward: tokens of a workgroup
     float eps, inv_dim;
     bool vec;
 };
@@ -76,9 +80,49 @@ struct Row {
         }
     }
     static __device__ __forceinline__ float group_sum(float v) {
+        v += nnk::dpp_mov<nnk::kDppQuadXor1>(v);
+        v += nnk::dpp_mov<nnk::kDppQuadXor2>(v);
+        if constexpr (G >= 8) v += nnk::dpp_mov<nnk::kDppRowHalfMirror>(v);
+        if constexpr (G >= 16) v += nnk::dpp_mov<nnk::kDppRowMirror>(v);
 #pragma unroll
-        for (int m = 1; m < G; m <<= 1) v += __shfl_xor(v, m);
+        for (int m = 16; m < G; m <<= 1) v += __shfl_xor(v, m);
         return v;
+    }
+    // This lane's part in a turn of whole chunks: cosines, signed sines and the lane of the
+    // pairs' other members.
+    struct Part {
+        float cos[CE], sin[CE];
+        int other;
+    };
+    static __device__ __forceinline__ void part_of(Part& t, int d0, const float2* cs, const Rope& a, float back) {
+        const int c = d0 / CE, hc = a.half / CE;
+        const bool first = c < hc, turns = c < 2 * hc;
+        t.other = !turns ? c : first ? c + hc : c - hc;
+#pragma unroll
+        for (int j = 0; j < CE; ++j) {
+            const float2 x = turns ? cs[(first ? c : c - hc) * CE + j] : make_float2(1.0f, 0.0f);
+            t.cos[j] = x.x;
+            t.sin[j] = first ? -back * x.y : back * x.y;
+        }
+    }
+    static __device__ __forceinline__ void turn(float* y, int d0, float* row, const Part& t) {
+        const int c = d0 / CE;
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int j = 0; j < CE; j += 4)
+            nnk::st4(row + j * G + 4 * c, make_float4(y[j], y[j + 1], y[j + 2], y[j + 3]));
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int j = 0; j < CE; j += 4) {
+            const float4 z = nnk::ld4(row + j * G + 4 * t.other);
+            y[j] = y[j] * t.cos[j] + z.x * t.sin[j];
+            y[j + 1] = y[j + 1] * t.cos[j + 1] + z.y * t.sin[j + 1];
+            y[j + 2] = y[j + 2] * t.cos[j + 2] + z.z * t.sin[j + 2];
+            y[j + 3] = y[j + 3] * t.cos[j + 3] + z.w * t.sin[j + 3];
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
     }
     // Turns the pairs of the group's row, whose features d0.. of this lane are y; `back`: by
     // the opposite angle.  `row`: the group's floats in LDS.
@@ -136,110 +180,155 @@ __device__ __forceinline__ void weights(float* w, const float* from, int d0, int
     for (int j = 0; j < Row<T, G>::CE; ++j) w[j] = d0 + j < dim ? (from ? from[d0 + j] : 1.0f) : 0.0f;
 }
 
-// A row's token, head and place in a tensor of queries or keys.
-struct Place {
-    int token, head;
-    bool key;
+// The rows of `tokens` tokens' heads head0 .. head0 + heads - 1, one after another for each
+// group: token and head of row r, and how both move on.
+struct Rows {
+    int token, head, heads, token_step, head_step;
+    __device__ __forceinline__ Rows(int r, int step, int heads_) : heads(heads_) {
+        token = r / heads;
+        head = r - token * heads;
+        token_step = step / heads;
+        head_step = step - token_step * heads;
+    }
+    __device__ __forceinline__ void next() {
+        token += token_step;
+        head += head_step;
+        if (head >= heads) {
+            head -= heads;
+            ++token;
+        }
+    }
 };
-__device__ __forceinline__ Place place(const Rope& a, int token0, int head0, int heads, int r) {
-    const int t = r / heads, h = head0 + r - t * heads;
-    return {token0 + t, h < a.heads ? h : h - a.heads, h >= a.heads};
-}
-template <typename T>
-__device__ __forceinline__ T* row_of(void* q, void* k, const long long* qs, const long long* ks, const Place& p) {
-    return p.key ? (T*)k + p.token * ks[0] + p.head * ks[1] : (T*)q + p.token * qs[0] + p.head * qs[1];
-}
-template <typename T>
-__device__ __forceinline__ const T* row_of(const void* q, const void* k, const long long* qs, const long long* ks,
-    const Place& p) {
-    return row_of<T>(const_cast<void*>(q), const_cast<void*>(k), qs, ks, p);
-}
 
-template <typename T, int G>
+// Sines and cosines of a row: the lane's own (CHUNKS) while the token stays, or the table's.
+template <typename T, int G, bool CHUNKS>
+struct Turner {
+    using R = Row<T, G>;
+    typename R::Part part;
+    int token = -1;
+    __device__ __forceinline__ void operator()(float* y, int t, int d0, float* row, const float2* cs, const Rope& a,
+        float back) {
+        if constexpr (CHUNKS) {
+            if (t != token) R::part_of(part, d0, cs + t * a.half, a, back);
+            token = t;
+            R::turn(y, d0, row, part);
+        } else {
+            R::turn(y, d0, row, cs + t * a.half, a, back);
+        }
+    }
+};
+
+template <typename T, int G, bool CHUNKS>
 __global__ __launch_bounds__(kTpb) void qk_norm_rope_kernel(Rope a) {
     using R = Row<T, G>;
     constexpr int CE = R::CE;
-    __shared__ float2 cs[kAngles];
+    __shared__ __attribute__((aligned(16))) float2 cs[kAngles];
     __shared__ __attribute__((aligned(16))) float rows[R::kGroups][G * CE];
     const int group = threadIdx.x / G, d0 = (threadIdx.x % G) * CE;
     const int part = blockIdx.x % a.head_parts, token0 = blockIdx.x / a.head_parts * a.tokens_each;
     const int tokens = min(a.tokens_each, a.tokens - token0);
-    const int each = (a.all_heads + a.head_parts - 1) / a.head_parts, head0 = part * each;
-    const int heads = min(each, a.all_heads - head0);
-    if (heads <= 0) return;
-    float wq[CE], wk[CE];
-    weights<T, G>(wq, a.q_weight, d0, a.dim);
-    weights<T, G>(wk, a.k_weight, d0, a.dim);
-    const int n = tokens * heads;
-    u32x4 next = {0, 0, 0, 0};
-    if (group < n) next = R::load(row_of<T>(a.q, a.k, a.qs, a.ks, place(a, token0, head0, heads, group)), d0, a);
-    angles(cs, a, token0, tokens);
-    __syncthreads();
-    for (int r = group; r < n; r += R::kGroups) {
-        float x[CE];
-        R::floats(next, x);
-        const Place p = place(a, token0, head0, heads, r);
-        if (r + R::kGroups < n)
-            next = R::load(row_of<T>(a.q, a.k, a.qs, a.ks, place(a, token0, head0, heads, r + R::kGroups)), d0, a);
-        float ss = 0.0f;
+    Turner<T, G, CHUNKS> turn;
+    bool ready = false;
+    const auto heads_of = [&](const void* in, void* out, const long long* is, const long long* os, const float* weight,
+                              int all) {
+        const int each = (all + a.head_parts - 1) / a.head_parts, head0 = part * each, heads = min(each, all - head0);
+        if (heads <= 0) return;
+        const int n = tokens * heads;
+        const T* from = (const T*)in + token0 * is[0] + head0 * is[1];
+        T* to = (T*)out + token0 * os[0] + head0 * os[1];
+        Rows at(group, R::kGroups, heads);
+        float w[CE];
+        weights<T, G>(w, weight, d0, a.dim);
+        u32x4 next = {0, 0, 0, 0};
+        if (group < n) next = R::load(from + at.token * is[0] + at.head * is[1], d0, a);
+        if (!ready) {
+            angles(cs, a, token0, tokens);
+            __syncthreads();
+            ready = true;
+        }
+        for (int r = group; r < n; r += R::kGroups) {
+            float x[CE];
+            R::floats(next, x);
+            const Rows now = at;
+            at.next();
+            if (r + R::kGroups < n) next = R::load(from + at.token * is[0] + at.head * is[1], d0, a);
+            float ss = 0.0f;
 #pragma unroll
-        for (int j = 0; j < CE; ++j) ss = fmaf(x[j], x[j], ss);
-        const float rstd = rsqrtf(R::group_sum(ss) * a.inv_dim + a.eps);
+            for (int j = 0; j < CE; ++j) ss = fmaf(x[j], x[j], ss);
+            const float rstd = rsqrtf(R::group_sum(ss) * a.inv_dim + a.eps);
 #pragma unroll
-        for (int j = 0; j < CE; ++j) x[j] = x[j] * rstd * (p.key ? wk[j] : wq[j]);
-        R::turn(x, d0, rows[group], cs + (p.token - token0) * a.half, a, 1.0f);
-        R::store(row_of<T>(a.q_out, a.k_out, a.qos, a.kos, p), d0, a, x);
-    }
+            for (int j = 0; j < CE; ++j) x[j] = x[j] * rstd * w[j];
+            turn(x, now.token, d0, rows[group], cs, a, 1.0f);
+            R::store(to + now.token * os[0] + now.head * os[1], d0, a, x);
+        }
+    };
+    heads_of(a.q, a.q_out, a.qs, a.qos, a.q_weight, a.heads);
+    heads_of(a.k, a.k_out, a.ks, a.kos, a.k_weight, a.kv_heads);
 }
 
-template <typename T, int G>
-__global__ __launch_bounds__(kTpb) void qk_norm_rope_grad_kernel(Rope a) {
+template <typename T, int G, bool CHUNKS>
+__global__ __launch_bounds__(kTpb, 4) void qk_norm_rope_grad_kernel(Rope a) {
     using R = Row<T, G>;
     constexpr int CE = R::CE;
-    __shared__ float2 cs[kAngles];
+    __shared__ __attribute__((aligned(16))) float2 cs[kAngles];
     __shared__ __attribute__((aligned(16))) float rows[R::kGroups][G * CE];
     const int group = threadIdx.x / G, d0 = (threadIdx.x % G) * CE;
-    float wq[CE], wk[CE], sum_q[CE], sum_k[CE];
-    weights<T, G>(wq, a.q_weight, d0, a.dim);
-    weights<T, G>(wk, a.k_weight, d0, a.dim);
+    float sum_q[CE], sum_k[CE];
 #pragma unroll
     for (int j = 0; j < CE; ++j) sum_q[j] = sum_k[j] = 0.0f;
-    for (long long at = (long long)blockIdx.x * a.tokens_each; at < a.tokens; at += (long long)gridDim.x * a.tokens_each) {
-        const int token0 = (int)at, tokens = min(a.tokens_each, a.tokens - token0), n = tokens * a.all_heads;
-        u32x4 next_x = {0, 0, 0, 0}, next_g = {0, 0, 0, 0};
-        const auto load = [&](int r) {
-            const Place p = place(a, token0, 0, a.all_heads, r);
-            next_x = R::load(row_of<T>(a.q, a.k, a.qs, a.ks, p), d0, a);
-            next_g = R::load(row_of<T>(a.dq_out, a.dk_out, a.qos, a.kos, p), d0, a);
+    const int begin = blockIdx.x * a.tokens_all, end = min(begin + a.tokens_all, a.tokens);
+    for (int token0 = begin; token0 < end; token0 += a.tokens_each) {
+        const int tokens = min(a.tokens_each, end - token0);
+        Turner<T, G, CHUNKS> turn;
+        bool ready = false;
+        const auto heads_of = [&](const void* in, const void* grad, void* out, const long long* is, const long long* os,
+                                  const float* weight, float* sum, int heads) {
+            if (!heads) return;
+            const int n = tokens * heads;
+            const T *from = (const T*)in + token0 * is[0], *gfrom = (const T*)grad + token0 * os[0];
+            T* to = (T*)out + token0 * is[0];
+            Rows at(group, R::kGroups, heads);
+            float w[CE];
+            weights<T, G>(w, weight, d0, a.dim);
+            u32x4 next_x = {0, 0, 0, 0}, next_g = {0, 0, 0, 0};
+            const auto load = [&]() {
+                next_x = R::load(from + at.token * is[0] + at.head * is[1], d0, a);
+                next_g = R::load(gfrom + at.token * os[0] + at.head * os[1], d0, a);
+            };
+            if (group < n) load();
+            if (!ready) {
+                __syncthreads();
+                angles(cs, a, token0, tokens);
+                __syncthreads();
+                ready = true;
+            }
+            for (int r = group; r < n; r += R::kGroups) {
+                float x[CE], g[CE];
+                R::floats(next_x, x);
+                R::floats(next_g, g);
+                const Rows now = at;
+                at.next();
+                if (r + R::kGroups < n) load();
+                turn(g, now.token, d0, rows[group], cs, a, -1.0f);
+                float ss = 0.0f, dot = 0.0f;
+#pragma unroll
+                for (int j = 0; j < CE; ++j) {
+                    ss = fmaf(x[j], x[j], ss);
+                    dot = fmaf(x[j], g[j] * w[j], dot);
+                }
+                const float rstd = rsqrtf(R::group_sum(ss) * a.inv_dim + a.eps);
+                const float mean = R::group_sum(dot) * rstd * a.inv_dim;
+#pragma unroll
+                for (int j = 0; j < CE; ++j) {
+                    const float xn = x[j] * rstd;
+                    sum[j] = fmaf(g[j], xn, sum[j]);
+                    x[j] = rstd * (g[j] * w[j] - xn * mean);
+                }
+                R::store(to + now.token * is[0] + now.head * is[1], d0, a, x);
+            }
         };
-        if (group < n) load(group);
-        __syncthreads();
-        angles(cs, a, token0, tokens);
-        __syncthreads();
-        for (int r = group; r < n; r += R::kGroups) {
-            float x[CE], g[CE];
-            R::floats(next_x, x);
-            R::floats(next_g, g);
-            const Place p = place(a, token0, 0, a.all_heads, r);
-            if (r + R::kGroups < n) load(r + R::kGroups);
-            R::turn(g, d0, rows[group], cs + (p.token - token0) * a.half, a, -1.0f);
-            float ss = 0.0f, dot = 0.0f;
-#pragma unroll
-            for (int j = 0; j < CE; ++j) {
-                ss = fmaf(x[j], x[j], ss);
-                dot = fmaf(x[j], g[j] * (p.key ? wk[j] : wq[j]), dot);
-            }
-            const float rstd = rsqrtf(R::group_sum(ss) * a.inv_dim + a.eps);
-            const float mean = R::group_sum(dot) * rstd * a.inv_dim;
-#pragma unroll
-            for (int j = 0; j < CE; ++j) {
-                const float xn = x[j] * rstd, dw = g[j] * xn;
-                sum_q[j] += p.key ? 0.0f : dw;
-                sum_k[j] += p.key ? dw : 0.0f;
-                x[j] = rstd * (g[j] * (p.key ? wk[j] : wq[j]) - xn * mean);
-            }
-            R::store(row_of<T>(a.dq, a.dk, a.qs, a.ks, p), d0, a, x);
-        }
+        heads_of(a.q, a.dq_out, a.dq, a.qs, a.qos, a.q_weight, sum_q, a.heads);
+        heads_of(a.k, a.dk_out, a.dk, a.ks, a.kos, a.k_weight, sum_k, a.kv_heads);
     }
     if (!a.partial) return;
     // the groups' sums, one feature a thread, in the groups' order
@@ -256,19 +345,35 @@ __global__ __launch_bounds__(kTpb) void qk_norm_rope_grad_kernel(Rope a) {
     }
 }
 
-// dw[d] = sum of the workgroups' partial sums, in 64 bits: a wave a feature, a lane's in
-// order, the lanes' as a tree.
-__global__ __launch_bounds__(kTpb) void qk_norm_weight_grad_kernel(float* dq_weight, float* dk_weight,
+// dw[d] = sum of the workgroups' partial sums, in 64 bits: 16 features and 64 slices of the
+// rows a workgroup, a thread's rows in order, a wave's 4 slices as a tree, the waves' sums
+// in order.
+constexpr int kSumCols = 16, kSumSlices = 64;
+__global__ __launch_bounds__(kSumCols* kSumSlices) void qk_norm_weight_grad_kernel(float* dq_weight, float* dk_weight,
     const float* partial, int groups, int dim) {
-    const int at = blockIdx.x * (kTpb / 64) + (int)(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (at >= 2 * dim) return;
+    __shared__ double part[kSumSlices / 4][kSumCols];
+    const int c = threadIdx.x % kSumCols, slice = threadIdx.x / kSumCols, at = blockIdx.x * kSumCols + c;
+    double sum = 0.0;
+    if (at < 2 * dim) {
+        const float* p = partial + (size_t)slice * 2 * dim + at;
+        float v[kGradGroups / kSumSlices];
+#pragma unroll
+        for (int i = 0; i < kGradGroups / kSumSlices; ++i)
+            v[i] = slice + i * kSumSlices < groups ? p[(size_t)i * kSumSlices * 2 * dim] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < kGradGroups / kSumSlices; ++i) sum += v[i];
+    }
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    if (slice % 4 == 0) part[slice / 4][c] = sum;
+    __syncthreads();
+    if (slice || at >= 2 * dim) return;
     float* to = at < dim ? dq_weight : dk_weight;
     if (!to) return;
-    double sum = 0.0;
-    for (int i = lane; i < groups; i += 64) sum += partial[(size_t)i * 2 * dim + at];
+    sum = 0.0;
 #pragma unroll
-    for (int m = 1; m < 64; m <<= 1) sum += __shfl_xor(sum, m);
-    if (lane == 0) to[at < dim ? at : at - dim] = (float)sum;
+    for (int i = 0; i < kSumSlices / 4; ++i) sum += part[i][c];
+    to[at < dim ? at : at - dim] = (float)sum;
 }
 
 bool shape_fits(const NnQkNormRope* a, const char* what) {
@@ -306,6 +411,7 @@ bool take(Rope& p, const NnQkNormRope* a, const char* what) {
     p.freq = a->freq;
     p.tokens = a->tokens;
     p.heads = a->heads;
+    p.kv_heads = a->kv_heads;
     p.all_heads = a->heads + a->kv_heads;
     p.dim = a->head_dim;
     p.half = a->rot_dim / 2;
@@ -317,11 +423,17 @@ bool take(Rope& p, const NnQkNormRope* a, const char* what) {
     return true;
 }
 
-// Tokens of a workgroup at a time: rows for 8 passes of its groups, as far as their sines
+// Tokens of a workgroup at a time: rows for 16 passes of its groups, as far as their sines
 // fit.  Few tokens: one each, and their heads shared by workgroups of one pass.
 int tokens_each(const Rope& p, int groups) {
-    const int by_rows = std::max(1, 8 * groups / p.all_heads), by_angles = kAngles / std::max(1, p.half);
+    const int by_rows = std::max(1, 16 * groups / p.all_heads), by_angles = kAngles / std::max(1, p.half);
     return std::min({by_rows, by_angles, std::max(1, p.tokens / kGradGroups)});
+}
+
+// Whether a pair's members lie whole 16-byte chunks apart.
+template <typename T>
+bool in_chunks(const Rope& p) {
+    return !p.interleaved && p.half > 0 && p.half % (16 / (int)sizeof(T)) == 0;
 }
 
 template <typename T, int G>
@@ -329,18 +441,21 @@ void forward(Rope& p, hipStream_t s) {
     constexpr int groups = Row<T, G>::kGroups;
     p.tokens_each = tokens_each(p, groups);
     p.head_parts = p.tokens < kGradGroups ? (p.all_heads + groups - 1) / groups : 1;
-    const long long blocks = ((long long)p.tokens + p.tokens_each - 1) / p.tokens_each * p.head_parts;
-    qk_norm_rope_kernel<T, G><<<(unsigned)blocks, kTpb, 0, s>>>(p);
+    const unsigned blocks = (unsigned)(((long long)p.tokens + p.tokens_each - 1) / p.tokens_each * p.head_parts);
+    if (in_chunks<T>(p)) qk_norm_rope_kernel<T, G, true><<<blocks, kTpb, 0, s>>>(p);
+    else qk_norm_rope_kernel<T, G, false><<<blocks, kTpb, 0, s>>>(p);
+}
+// Backward: as many workgroups as the card holds at once, of as many tokens each.
+int grad_groups(Rope& p, int groups) {
+    p.tokens_all = (p.tokens + kGradGroups - 1) / kGradGroups;
+    p.tokens_each = std::min(p.tokens_all, tokens_each(p, groups));
+    return (p.tokens + p.tokens_all - 1) / p.tokens_all;
 }
 template <typename T, int G>
 void backward(Rope& p, hipStream_t s) {
-    p.tokens_each = tokens_each(p, Row<T, G>::kGroups);
-    const int blocks = std::min(kGradGroups, (p.tokens + p.tokens_each - 1) / p.tokens_each);
-    qk_norm_rope_grad_kernel<T, G><<<(unsigned)blocks, kTpb, 0, s>>>(p);
-}
-int grad_groups(const Rope& p, int groups) {
-    const int each = tokens_each(p, groups);
-    return std::min(kGradGroups, (p.tokens + each - 1) / each);
+    const unsigned blocks = (unsigned)grad_groups(p, Row<T, G>::kGroups);
+    if (in_chunks<T>(p)) qk_norm_rope_grad_kernel<T, G, true><<<blocks, kTpb, 0, s>>>(p);
+    else qk_norm_rope_grad_kernel<T, G, false><<<blocks, kTpb, 0, s>>>(p);
 }
 
 // Lanes of a row: a power of two with 16 bytes each.
@@ -415,7 +530,7 @@ void launch_qk_norm_rope_backward(void* dq, void* dk, float* dq_weight, float* d
         groups = grad_groups(p, kTpb / lanes_of(a));
     }
     if (dq_weight || dk_weight) {
-        qk_norm_weight_grad_kernel<<<(unsigned)((2 * p.dim + 3) / 4), kTpb, 0, s>>>(dq_weight, dk_weight, workspace,
+        qk_norm_weight_grad_kernel<<<(unsigned)((2 * p.dim + kSumCols - 1) / kSumCols), kSumCols * kSumSlices, 0, s>>>(dq_weight, dk_weight, workspace,
             groups, p.dim);
         nnk_after_launch(what, s);
     }
