@@ -71,6 +71,7 @@ bool take(Args& p, const NnAttention* a, const char* what) {
         const double tanh_of[6] = {1.0, -1.0 / 3, 2.0 / 15, -17.0 / 315, 62.0 / 2835, -1382.0 / 155925};
         double power = (double)p.c2 * p.c1;
         for (int i = 0; i < 6; ++i, power *= (double)p.c1 * p.c1) p.series[i] = (float)(tanh_of[i] * power);
+        p.inv_c2 = 1.0f / p.c2;
         p.small = kSeriesEnd / p.c1;
         p.tiny = kShortSeriesEnd / p.c1;
     }

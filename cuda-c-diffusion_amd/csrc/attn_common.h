@@ -41,6 +41,7 @@ constexpr int kTpb = 256;
 constexpr int kWaves = kTpb / 64;
 constexpr int kRows = 32 * kWaves;  // columns of a workgroup: queries, or keys in the key gradients
 constexpr int kCus = 256;
+constexpr int kSplitBelow = 2 * kCus;  // workgroups of the gradient kernels that are split in two
 constexpr int kMaxDistance = 1023;
 constexpr int kTicketWords = 2048;  // at the front of every forward workspace: zeros between calls
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -306,6 +307,7 @@ struct Args {
     int mask, buckets, max_distance;
     float scale, c1, c2;  // score in units of log2: c1 * s, or c2 * tanh(c1 * s)
     float series[6];      // c2 tanh(c1 s) = s (series[0] + w (series[1] + ...)), w = s^2, for small c1 s
+    float inv_c2;
     float small, tiny;    // how small: |s| below this; and for its first 4 terms alone
     const int *q_start, *k_len, *prefix, *doc_q, *doc_k, *bucket;
     const float* bias;
@@ -347,9 +349,8 @@ __device__ __forceinline__ float tanh_series(float y) {
 }
 // ends of the series of 6 and of 4 terms: the next term is below 2^-24 of the first
 constexpr float kSeriesEnd = 0.375f, kShortSeriesEnd = 0.14f;
-// s[r] = tanh(c1 s[r]) and, if wanted, its slope
-template <bool SLOPE>
-__device__ __forceinline__ void cap_scores(f32x16& s, f32x16& slope, float c1) {
+// s[r] = c2 tanh(c1 s[r])
+__device__ __forceinline__ void cap_scores(f32x16& s, float c1, float c2) {
     float top = 0.0f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
@@ -358,17 +359,46 @@ __device__ __forceinline__ void cap_scores(f32x16& s, f32x16& slope, float c1) {
     }
     if (__all(top < kSeriesEnd)) {  // fmaxf passes over NaN; the series keeps it
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            s[r] = tanh_series(s[r]);
-            if constexpr (SLOPE) slope[r] = fmaf(-s[r], s[r], 1.0f);
-        }
+        for (int r = 0; r < 16; ++r) s[r] = tanh_series(s[r]) * c2;
     } else {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const float y = s[r], q = __builtin_amdgcn_rcpf(exp2_fast(fabsf(y) * (2.0f * kLog2e)) + 1.0f);
-            const bool small = fabsf(y) < kSeriesEnd;
-            s[r] = small ? tanh_series(y) : copysignf(fmaf(-2.0f, q, 1.0f), y);
-            if constexpr (SLOPE) slope[r] = small ? fmaf(-s[r], s[r], 1.0f) : 4.0f * q * (1.0f - q);
+            s[r] = (fabsf(y) < kSeriesEnd ? tanh_series(y) : copysignf(fmaf(-2.0f, q, 1.0f), y)) * c2;
+        }
+    }
+}
+// The same with the slope 1 - tanh^2, for the gradients.  Each score takes the same form
+// whatever its neighbours are: both gradient kernels get the same value, to the bit.
+__device__ __forceinline__ void cap_scores(f32x16& s, f32x16& slope, const Args& a) {
+    const auto series = [&](float x) {
+        const float w = x * x;
+        float c = fmaf(w, a.series[5], a.series[4]);
+        c = fmaf(w, c, a.series[3]);
+        c = fmaf(w, c, a.series[2]);
+        c = fmaf(w, c, a.series[1]);
+        return x * fmaf(w, c, a.series[0]);
+    };
+    const auto slope_of = [&](float x) {
+        const float t = x * a.inv_c2;
+        return fmaf(-t, t, 1.0f);
+    };
+    float top = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(s[r]));
+    if (__all(top < a.small)) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s[r] = series(s[r]);
+            slope[r] = slope_of(s[r]);
+        }
+    } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float x = s[r], q = __builtin_amdgcn_rcpf(exp2_fast(fabsf(x) * (2.0f * kLog2e * a.c1)) + 1.0f);
+            const bool near = fabsf(x) < a.small;
+            s[r] = near ? series(x) : copysignf(fmaf(-2.0f, q, 1.0f), x) * a.c2;
+            slope[r] = near ? slope_of(s[r]) : 4.0f * q * (1.0f - q);
         }
     }
 }

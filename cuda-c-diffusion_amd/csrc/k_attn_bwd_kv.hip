@@ -12,6 +12,9 @@
 // in the heads' order: documents and causal masks give tiles very uneven work, which only
 // more workgroups even out.
 //
+// SPLIT 2, for calls of few workgroups: 64 keys, and of each block 32 queries a wave; the
+// two waves of the same keys are added up at the end, in their order.
+//
 // Bias: sums of dx by distance j - P.  A 32 x 32 tile has its distances on diagonals;
 // row m's values go m lanes along, after which a lane holds two distances (one for what
 // went past the end), and the tile is 32 shuffles and adds and one addition to the
@@ -23,7 +26,7 @@ using namespace attn;
 
 constexpr int kSlack = 64;  // distances of a tile that reaches past max_distance
 
-template <typename T, int DP, bool CAP, bool BIAS, bool VEC>
+template <typename T, int DP, bool CAP, bool BIAS, bool VEC, int SPLIT>
 __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn_bwd_kv_kernel(Args a, int tiles) {
     using L = Lds<T, DP>;
     // two blocks in LDS; one where they and the distances would not fit (fp32, over 64 features)
@@ -37,11 +40,14 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn
     __shared__ float table[BIAS ? 2 * kMaxDistance + 1 : 1];
     extern __shared__ float dist[];  // BIAS: a table of 2 (max_distance + kSlack) + 1 a wave
 
+    constexpr int kOwn = kRows / SPLIT;  // keys of the workgroup
+
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
+    const int half = SPLIT > 1 ? wave / (kWaves / SPLIT) : 0, strip = wave - half * (kWaves / SPLIT);
     const int w = nnk::xcd_swizzle(blockIdx.x, gridDim.x);
     const int tile = w % tiles, part = w / tiles % (a.heads / a.heads_each), b = w / tiles / (a.heads / a.heads_each);
     const int head0 = part * a.heads_each, kv = head0 / a.group;
-    const int k0 = tile * kRows, key = k0 + wave * 32 + (lane & 31);
+    const int k0 = tile * kOwn, first_key = k0 + strip * 32, key = first_key + (lane & 31);
     const int keys = keys_of(a, b), start = start_of(a, b);
     const int* docs = a.doc_k ? a.doc_k + (size_t)b * a.len_k : nullptr;
     const bool in = key < a.len_k;
@@ -49,10 +55,10 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn
     const bool live = key < keys && (!docs || doc >= 0);
     const int wave_doc = __builtin_amdgcn_readfirstlane(doc);
     const bool whole_keys = __all(live && (!docs || doc == wave_doc));
-    const int last_key = k0 + wave * 32 + 31;
+    const int last_key = first_key + 31;
 
     const int q_blocks = (a.len_q + kBlock - 1) / kBlock;
-    const int4 mine = key_docs_of(a, b, k0 / kBlock, kRows / kBlock);
+    const int4 mine = key_docs_of(a, b, k0 / kBlock, kOwn / kBlock);
     const int4* query_docs = a.query_docs ? a.query_docs + (size_t)b * q_blocks : nullptr;
     // the first block of queries that can see the tile: their limits rise with their positions
     int first_block = keys > k0 ? 0 : q_blocks;
@@ -77,7 +83,8 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn
         dk[d] = zero16();
         dv[d] = zero16();
     }
-    const int rbase = L::row_base(lane), cbase = L::col_base(lane);
+    // a wave of SPLIT 2 has the upper or the lower 32 rows of every block
+    const int rbase = L::row_base(lane) + half * 32 * L::kRowBytes, cbase = L::col_base(lane) + half * 32 * L::kRowBytes;
     const int span = 2 * (a.max_distance + kSlack) + 1;
     float* my_dist = dist + wave * span;
 
@@ -134,15 +141,22 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn
             load(next);
             store(next, 0);
         }
-        for (int buf = 0; next >= 0; buf ^= kBufs - 1) {
-            const int q0 = next * kBlock, block_doc = at.doc;
+        const auto step = [&](auto buf_) {
+            constexpr int buf = decltype(buf_)::value;
+            const int q0 = next * kBlock + half * 32, block_doc = at.doc, there = a.len_q - q0;
             next = at.next();
             __syncthreads();  // this block is stored; the one before it is done with
             if (next >= 0) load(next);
 
-            const bool whole = whole_keys && limit_lds[buf][0] > last_key && (!docs || block_doc == wave_doc);
-#pragma unroll 1
-            for (int i = 0; i < 2; ++i) {
+            const int *limits = limit_lds[buf] + half * 32, *row_docs = doc_lds[buf] + half * 32;
+            const float *Ms = M_lds[buf] + half * 32, *Ds = D_lds[buf] + half * 32;
+            const bool one = !docs || block_doc == wave_doc;
+            // a document of the block's queries that none of the wave's keys is in
+            const bool other = docs && whole_keys && block_doc >= 0 && block_doc != wave_doc;
+#pragma unroll
+            for (int i = 0; i < 2 / SPLIT; ++i) {
+                if (other || 32 * i >= there || limits[min(32 * i + 31, there - 1)] <= first_key) continue;
+                const bool whole = whole_keys && one && limits[32 * i] > last_key;
                 f32x16 s = zero16(), dp = zero16();
                 struct Pair {
                     Frag<T> q[L::kStage], g[L::kStage];
@@ -175,26 +189,26 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn
                 read_cols(two[0], 0);
                 __builtin_amdgcn_sched_barrier(kMayCross);
                 f32x16 slope;
-                if constexpr (CAP) cap_scores<true>(s, slope, a.c1);
-                const float c = CAP ? a.c2 : a.c1;
+                if constexpr (CAP) cap_scores(s, slope, a);
                 if constexpr (BIAS) {
                     const int rel = key - (start + q0 + 32 * i + 4 * h);
+                    const float c = CAP ? 1.0f : a.c1;
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
                         const int d = rel - 8 * (r >> 2) - (r & 3), m = a.max_distance;
                         s[r] = s[r] * c + table[min(max(d, -m), m) + m];
                     }
-                } else {
+                } else if constexpr (!CAP) {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[r] *= c;
+                    for (int r = 0; r < 16; ++r) s[r] *= a.c1;
                 }
                 if (!whole) {
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
                         const int at4 = 32 * i + 8 * g + 4 * h;
-                        const int4 lm = *reinterpret_cast<const int4*>(limit_lds[buf] + at4);
+                        const int4 lm = *reinterpret_cast<const int4*>(limits + at4);
                         int4 dc = {doc, doc, doc, doc};
-                        if (docs) dc = *reinterpret_cast<const int4*>(doc_lds[buf] + at4);
+                        if (docs) dc = *reinterpret_cast<const int4*>(row_docs + at4);
                         const auto sees = [&](int lm1, int dc1) { return live & (key < lm1) & (dc1 == doc); };
                         s[4 * g] = sees(lm.x, dc.x) ? s[4 * g] : -INFINITY;
                         s[4 * g + 1] = sees(lm.y, dc.y) ? s[4 * g + 1] : -INFINITY;
@@ -204,8 +218,8 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn
                 }
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    const f32x4 M = *reinterpret_cast<const f32x4*>(M_lds[buf] + 32 * i + 8 * g + 4 * h);
-                    const f32x4 D = *reinterpret_cast<const f32x4*>(D_lds[buf] + 32 * i + 8 * g + 4 * h);
+                    const f32x4 M = *reinterpret_cast<const f32x4*>(Ms + 32 * i + 8 * g + 4 * h);
+                    const f32x4 D = *reinterpret_cast<const f32x4*>(Ds + 32 * i + 8 * g + 4 * h);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const int r = 4 * g + j;
@@ -214,7 +228,7 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn
                     }
                 }
                 if constexpr (BIAS) {
-                    const int base = k0 + wave * 32 - (start + q0 + 32 * i);  // distance of row 0, column 0
+                    const int base = first_key - (start + q0 + 32 * i);  // distance of row 0, column 0
                     const int m = a.max_distance;
                     if (base + 31 <= -m || base - 31 >= m) {
                         float sum = 0.0f;
@@ -259,6 +273,11 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn
             }
             if (kBufs == 1) __syncthreads();
             if (next >= 0) store(next, buf ^ (kBufs - 1));
+        };
+        while (next >= 0) {
+            step(std::integral_constant<int, 0>{});
+            if (next < 0) break;
+            step(std::integral_constant<int, kBufs - 1>{});
         }
         if constexpr (BIAS) {
             // the far tiles join the ends of the table; then one sum a distance
@@ -284,6 +303,30 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn
         }
     }
 
+    if constexpr (SPLIT > 1) {
+        // the second half's sums, through the tiles' LDS: a register's 64 lanes together
+        const int at = strip * (DP / 32 * 16 * 64) + lane;
+        float *to_k = reinterpret_cast<float*>(q_lds[0]) + at, *to_v = reinterpret_cast<float*>(g_lds[0]) + at;
+        __syncthreads();
+        if (half) {
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    to_k[(d * 16 + r) * 64] = dk[d][r];
+                    to_v[(d * 16 + r) * 64] = dv[d][r];
+                }
+        }
+        __syncthreads();
+        if (half) return;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                dk[d][r] += to_k[(d * 16 + r) * 64];
+                dv[d][r] += to_v[(d * 16 + r) * 64];
+            }
+    }
     if (!in) return;
     if (a.head_sums) {
         const size_t at = (((size_t)b * a.heads + head0) * a.len_k + key) * a.dim;
@@ -359,19 +402,36 @@ __global__ __launch_bounds__(kTpb) void attn_bias_grad_kernel(float* dbias, cons
     if (threadIdx.x == 0) dbias[(size_t)mine * heads + head] = (float)part[0];
 }
 
-template <typename T, int DP, bool CAP, bool BIAS, bool VEC>
-bool launch(const Args& a, hipStream_t s, const char* what) {
-    const int tiles = (a.len_k + kRows - 1) / kRows;
+// Keys of a workgroup: the heads of a key head apart count as workgroups here.
+int keys_each(long long batch, long long len_k, long long groups) {
+    return (len_k + kRows - 1) / kRows * groups * batch < kSplitBelow ? kRows / 2 : kRows;
+}
+int tiles_of(const Args& a) {
+    const int each = keys_each(a.batch, a.len_k, a.heads / a.heads_each);
+    return (a.len_k + each - 1) / each;
+}
+
+template <typename T, int DP, bool CAP, bool BIAS, bool VEC, int SPLIT>
+bool launch_split(const Args& a, hipStream_t s, const char* what) {
+    const int tiles = tiles_of(a);
     const size_t lds = BIAS ? kWaves * (2 * (a.max_distance + kSlack) + 1) * sizeof(float) : 0;
     if constexpr (BIAS) {
         static std::atomic<unsigned long long> done{0};
-        if (!raise_lds((const void*)attn_bwd_kv_kernel<T, DP, CAP, BIAS, VEC>,
+        if (!raise_lds((const void*)attn_bwd_kv_kernel<T, DP, CAP, BIAS, VEC, SPLIT>,
                 kWaves * (2 * (kMaxDistance + kSlack) + 1) * sizeof(float), done, what))
             return false;
     }
-    attn_bwd_kv_kernel<T, DP, CAP, BIAS, VEC>
+    attn_bwd_kv_kernel<T, DP, CAP, BIAS, VEC, SPLIT>
         <<<(unsigned)((long long)tiles * (a.heads / a.heads_each) * a.batch), kTpb, lds, s>>>(a, tiles);
     nnk_after_launch(what, s);
+    return true;
+}
+
+template <typename T, int DP, bool CAP, bool BIAS, bool VEC>
+bool launch(const Args& a, hipStream_t s, const char* what) {
+    if (!(keys_each(a.batch, a.len_k, a.heads / a.heads_each) < kRows ? launch_split<T, DP, CAP, BIAS, VEC, 2>(a, s, what)
+                                                                     : launch_split<T, DP, CAP, BIAS, VEC, 1>(a, s, what)))
+        return false;
     if (a.head_sums) {
         const int quads = (a.dim + 3) / 4;
         const long long total = (long long)a.batch * a.kv_heads * a.len_k * quads;
@@ -393,11 +453,12 @@ bool nnk_attention_splits_heads(const NnAttention* a) {
 }
 
 size_t nnk_attention_dist_floats(const NnAttention* a) {
-    return (size_t)a->batch * a->heads * ((a->len_k + kRows - 1) / kRows) * (2 * a->max_distance + 1);
+    const int each = keys_each(a->batch, a->len_k, nnk_attention_splits_heads(a) ? a->heads : a->kv_heads);
+    return (size_t)a->batch * a->heads * ((a->len_k + each - 1) / each) * (2 * a->max_distance + 1);
 }
 
 void nnk_attention_bias_grad(const Args& a, float* dbias, hipStream_t s, const char* what) {
     attn_bias_grad_kernel<<<(unsigned)(a.buckets * a.heads), kTpb, 0, s>>>(dbias, a.dist_sums, a.bucket, a.batch,
-        a.heads, a.buckets, (a.len_k + kRows - 1) / kRows, 2 * a.max_distance + 1);
+        a.heads, a.buckets, tiles_of(a), 2 * a.max_distance + 1);
     nnk_after_launch(what, s);
 }

@@ -10,12 +10,15 @@
 // the key gradients and the bias gradient use (stat).  Where all keys of the workgroup
 // lie in one block they are there before it is used, and the query gradient takes them
 // too: a query that sees a single key then gets a gradient of exactly zero.
+//
+// SPLIT 2, for calls of few workgroups: 64 queries, and of each block 32 keys a wave; the
+// two waves of the same queries are added up at the end, in their order.
 #include "attn_common.h"
 
 namespace {
 using namespace attn;
 
-template <typename T, int DP, bool CAP, bool BIAS, bool VEC>
+template <typename T, int DP, bool CAP, bool BIAS, bool VEC, int SPLIT>
 __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn_bwd_q_kernel(Args a, int tiles) {
     using L = Lds<T, DP>;
     __shared__ __attribute__((aligned(16))) char k_lds[2][L::kBytes];
@@ -23,24 +26,31 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn
     __shared__ __attribute__((aligned(16))) int doc_lds[2][kBlock];
     __shared__ float table[BIAS ? 2 * kMaxDistance + 1 : 1];
 
+    __shared__ float3 parts[SPLIT > 1 ? kRows : 1];  // of the waves: maximum, sum, <p, dp>
+    constexpr int kOwn = kRows / SPLIT;               // queries of the workgroup
+
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
+    const int half = SPLIT > 1 ? wave / (kWaves / SPLIT) : 0;
     const int w = nnk::xcd_swizzle(blockIdx.x, gridDim.x);
     const int tile = tiles - 1 - w % tiles;
     const int head = w / tiles % a.heads, b = w / tiles / a.heads;
-    const int row0 = tile * kRows, row = row0 + wave * 32 + (lane & 31);
+    const int row0 = tile * kOwn, row = row0 + (wave - half * (kWaves / SPLIT)) * 32 + (lane & 31);
     const bool in = row < a.len_q;
     const int keys = keys_of(a, b), start = start_of(a, b);
     const int pos = start + row;
     const int limit = in ? limit_of(a, b, keys, pos) : 0;
     const int doc = in && a.doc_q ? a.doc_q[(size_t)b * a.len_q + row] : -1;
-    int least = in ? limit : INT32_MAX;
+    int least = in ? limit : INT32_MAX, wave_most = limit;
 #pragma unroll
-    for (int m = 1; m < 32; m <<= 1) least = min(least, __shfl_xor(least, m));
+    for (int m = 1; m < 32; m <<= 1) {
+        least = min(least, __shfl_xor(least, m));
+        wave_most = max(wave_most, __shfl_xor(wave_most, m));
+    }
     const int wave_doc = __builtin_amdgcn_readfirstlane(doc);
     const bool one_doc = __all(doc == wave_doc || !in) && wave_doc >= 0;
 
-    const int most = limit_of(a, b, keys, start + min(row0 + kRows, a.len_q) - 1);
-    const int4 mine = query_docs_of(a, b, row0 / kBlock, kRows / kBlock);
+    const int most = limit_of(a, b, keys, start + min(row0 + kOwn, a.len_q) - 1);
+    const int4 mine = query_docs_of(a, b, row0 / kBlock, kOwn / kBlock);
     const int blocks = (a.len_k + kBlock - 1) / kBlock;
     const int4* key_docs = a.key_docs ? a.key_docs + (size_t)b * blocks : nullptr;
     Blocks at(0, (most + kBlock - 1) / kBlock, key_docs, mine);
@@ -101,20 +111,26 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn
     for (int d = 0; d < DP / 32; ++d) dq[d] = zero16();
     float l = 0.0f, pd = 0.0f;  // sums of p and of p dp
 
-    const int rbase = L::row_base(lane), cbase = L::col_base(lane);
+    // a wave of SPLIT 2 has the upper or the lower 32 rows of every block
+    const int rbase = L::row_base(lane) + half * 32 * L::kRowBytes, cbase = L::col_base(lane) + half * 32 * L::kRowBytes;
+    constexpr int kSubs = 2 / SPLIT;
     int next = at.next();
     if (next >= 0) {
         load(next);
         store(next, at.negative, 0);
     }
     bool first = true;
-    for (int buf = 0; next >= 0; buf ^= 1, first = false) {
-        const int k0 = next * kBlock, block_doc = at.doc;
+    const auto step = [&](auto buf_) {
+        constexpr int buf = decltype(buf_)::value;
+        const int k0 = next * kBlock + half * 32, block_doc = at.doc;
+        const bool block_whole = next * kBlock + kBlock <= least;
         next = at.next();
         __syncthreads();  // this block is stored; the one before it is done with
         if (next >= 0) load(next);
 
-        const bool whole = k0 + kBlock <= least && (!docs || (one_doc && block_doc == wave_doc));
+        const bool whole = block_whole && (!docs || (one_doc && block_doc == wave_doc));
+        // nothing here for the wave's queries
+        const bool none = k0 >= wave_most || (docs && one_doc && block_doc >= 0 && block_doc != wave_doc);
         struct Pair {
             Frag<T> k[L::kStage], v[L::kStage];
         };
@@ -141,20 +157,19 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn
                     dp = mma(y.v[j], gf[n * L::kStage + j], dp);
                 }
             });
-            if constexpr (CAP) cap_scores<true>(s, slope, a.c1);
-            const float c = CAP ? a.c2 : a.c1;
+            if constexpr (CAP) cap_scores(s, slope, a);
             if constexpr (BIAS) {
-                add_bias(s, c, table, a.max_distance, k0 + 32 * i + 4 * h - pos);
-            } else {
+                add_bias(s, CAP ? 1.0f : a.c1, table, a.max_distance, k0 + 32 * i + 4 * h - pos);
+            } else if constexpr (!CAP) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] *= c;
+                for (int r = 0; r < 16; ++r) s[r] *= a.c1;
             }
-            if (!whole) hide(s, k0 + 32 * i, limit, docs ? doc_lds[buf] + 32 * i : nullptr, doc, h);
+            if (!whole) hide(s, k0 + 32 * i, limit, docs ? doc_lds[buf] + half * 32 + 32 * i : nullptr, doc, h);
         };
         if (first && next < 0) {  // the only block
             float m = -INFINITY, sum = 0.0f, dot = 0.0f;
 #pragma unroll 1
-            for (int i = 0; i < 2; ++i) {
+            for (int i = 0; i < kSubs; ++i) {
                 f32x16 s, dp, slope;
                 products(i, s, dp, slope);
                 float top = m;
@@ -174,43 +189,81 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn
             }
             sum = sum_halves(sum);
             dot = sum_halves(dot);
+            if constexpr (SPLIT > 1) {
+                const int mine = wave * 32 + (lane & 31), other = (wave ^ (kWaves / 2)) * 32 + (lane & 31);
+                if (h == 0) parts[mine] = float3{m, sum, dot};
+                __syncthreads();
+                const float3 x = parts[half ? other : mine], y = parts[half ? mine : other];
+                m = fmaxf(x.x, y.x);
+                const float base = m == -INFINITY ? 0.0f : m, f = exp2_fast(x.x - base), g = exp2_fast(y.x - base);
+                sum = x.y * f + y.y * g;
+                dot = x.z * f + y.z * g;
+            }
             if (sees_any) {
                 M = m + log2f(sum);
                 D = dot / sum;
             }
         }
+        first = false;
+        if (!none) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            f32x16 s, dp, slope;
-            products(i, s, dp, slope);
-            Columns columns[2];
-            const auto read_columns = [&](Columns& y, int n) {
+            for (int i = 0; i < kSubs; ++i) {
+                f32x16 s, dp, slope;
+                products(i, s, dp, slope);
+                Columns columns[2];
+                const auto read_columns = [&](Columns& y, int n) {
 #pragma unroll
-                for (int d = 0; d < DP / 32; ++d) y.x[d] = L::cols(k_lds[buf], i, n, d, cbase);
-            };
-            read_columns(columns[0], 0);
-            __builtin_amdgcn_sched_barrier(kMayCross);
+                    for (int d = 0; d < DP / 32; ++d) y.x[d] = L::cols(k_lds[buf], i, n, d, cbase);
+                };
+                read_columns(columns[0], 0);
+                __builtin_amdgcn_sched_barrier(kMayCross);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float p = exp2_fast(s[r] - M);
-                l += p;
-                pd = fmaf(p, dp[r], pd);
-                float dx = p * (dp[r] - D);
-                if constexpr (CAP) dx *= slope[r];
-                s[r] = dx;
+                for (int r = 0; r < 16; ++r) {
+                    const float p = exp2_fast(s[r] - M);
+                    l += p;
+                    pd = fmaf(p, dp[r], pd);
+                    float dx = p * (dp[r] - D);
+                    if constexpr (CAP) dx *= slope[r];
+                    s[r] = dx;
+                }
+                piped<L::kKeySteps>(columns, read_columns, [&](const Columns& y, int n) {
+                    const Frag<T> x = operand(s, n, T{});
+#pragma unroll
+                    for (int d = 0; d < DP / 32; ++d) dq[d] = mma(y.x[d], x, dq[d]);
+                });
             }
-            piped<L::kKeySteps>(columns, read_columns, [&](const Columns& y, int n) {
-                const Frag<T> x = operand(s, n, T{});
-#pragma unroll
-                for (int d = 0; d < DP / 32; ++d) dq[d] = mma(y.x[d], x, dq[d]);
-            });
         }
         if (next >= 0) store(next, at.negative, buf ^ 1);
+    };
+    while (next >= 0) {
+        step(std::integral_constant<int, 0>{});
+        if (next < 0) break;
+        step(std::integral_constant<int, 1>{});
     }
-
-    if (!in) return;
     l = sum_halves(l);
     pd = sum_halves(pd);
+    if constexpr (SPLIT > 1) {
+        // the second half's sums, through the tiles' LDS: a register's 64 lanes together
+        float* to = reinterpret_cast<float*>(k_lds[0]) + (wave & 1) * (DP / 32 * 16 * 64) + lane;
+        __syncthreads();
+        if (half) {
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) to[(d * 16 + r) * 64] = dq[d][r];
+            if (h == 0) parts[wave * 32 + (lane & 31)] = float3{0.0f, l, pd};
+        }
+        __syncthreads();
+        if (half) return;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dq[d][r] += to[(d * 16 + r) * 64];
+        const float3 y = parts[(wave + kWaves / 2) * 32 + (lane & 31)];
+        l += y.y;
+        pd += y.z;
+    }
+    if (!in) return;
     T* out = (T*)a.dq + b * a.qs[0] + (long long)row * a.qs[1] + head * a.qs[2];
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
@@ -221,12 +274,19 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn
     if (h == 0) a.stat[stat_at] = sees_any ? float2{M + log2f(l), pd / l} : float2{INFINITY, 0.0f};
 }
 
-template <typename T, int DP, bool CAP, bool BIAS, bool VEC>
-bool launch(const Args& a, hipStream_t s, const char* what) {
-    const int tiles = (a.len_q + kRows - 1) / kRows;
-    attn_bwd_q_kernel<T, DP, CAP, BIAS, VEC><<<(unsigned)((long long)tiles * a.heads * a.batch), kTpb, 0, s>>>(a, tiles);
+template <typename T, int DP, bool CAP, bool BIAS, bool VEC, int SPLIT>
+bool launch_split(const Args& a, hipStream_t s, const char* what) {
+    const int tiles = (a.len_q + kRows / SPLIT - 1) / (kRows / SPLIT);
+    attn_bwd_q_kernel<T, DP, CAP, BIAS, VEC, SPLIT>
+        <<<(unsigned)((long long)tiles * a.heads * a.batch), kTpb, 0, s>>>(a, tiles);
     nnk_after_launch(what, s);
     return true;
+}
+template <typename T, int DP, bool CAP, bool BIAS, bool VEC>
+bool launch(const Args& a, hipStream_t s, const char* what) {
+    const long long groups = ((long long)a.len_q + kRows - 1) / kRows * a.heads * a.batch;
+    return groups < kSplitBelow ? launch_split<T, DP, CAP, BIAS, VEC, 2>(a, s, what)
+                                : launch_split<T, DP, CAP, BIAS, VEC, 1>(a, s, what);
 }
 
 }  // namespace

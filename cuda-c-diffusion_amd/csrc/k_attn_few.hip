@@ -156,10 +156,12 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && VEC ? 2 : 1) void attn_few_
         f32x16 s = zero16();
 #pragma unroll
         for (int u = 0; u < L::kSteps; ++u) s = mma(L::rows(k_lds, 0, u, rbase), qf[u], s);
-        if constexpr (CAP) cap_scores<false>(s, s, a.c1);
-        const float c = CAP ? a.c2 : a.c1;
+        if constexpr (CAP) {
+            cap_scores(s, a.c1, a.c2);
+        } else {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] *= c;
+            for (int r = 0; r < 16; ++r) s[r] *= a.c1;
+        }
         if constexpr (BIAS) {
             if (__all(at + kKeys - 1 - pos <= -a.max_distance)) {
 #pragma unroll
@@ -331,8 +333,7 @@ bool launch(const Args& a, float* ws, hipStream_t s, const char* what) {
 
 // Few queries: the rows of a key head's queries fit in two tiles.
 bool nnk_attention_is_few(const NnAttention* a) {
-    const long long rows = (long long)a->len_q * (a->heads / a->kv_heads);
-    return rows <= 64 && (long long)a->batch * a->kv_heads < 1 << 20;
+    return (long long)a->len_q * (a->heads / a->kv_heads) <= 64 && (long long)a->batch * a->kv_heads < 1 << 20;
 }
 // Floats of the workspace after the tickets.
 size_t nnk_attention_few_floats(const NnAttention* a) {

@@ -7,6 +7,9 @@
 // next one's loads under way meanwhile.  Blocks that no query of the workgroup sees are
 // left out.
 //
+// SPLIT 2, for calls of few workgroups: 64 queries, and of each block 32 keys a wave; the two
+// waves of the same queries are joined at the end.
+//
 // What bounds it is the softmax's arithmetic, a vector instruction of 4 cycles for 64
 // scores against 32 cycles of matrix products (128 features), so each score term has the
 // form with the fewest:
@@ -25,36 +28,46 @@ using namespace attn;
 // CAP: 0 none, 1 any, 2 at most kFixedCap and no bias
 constexpr float kFixedCap = 80.0f;
 
-template <typename T, int DP, int CAP, bool BIAS, bool VEC>
+template <typename T, int DP, int CAP, bool BIAS, bool VEC, int SPLIT>
 __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && VEC ? 2 : 1) void attn_fwd_kernel(Args a, int tiles) {
     using L = Lds<T, DP>;
     // fp32, one wave a SIMD: reads of LDS ahead of their products.  bf16 has two waves, which
     // hide them for each other, and no registers for it (128 features: 1.6 ms became 2.4)
     constexpr bool kPiped = sizeof(T) == 4;
+    constexpr int kWide = 2 / SPLIT * L::kSteps % L::kWide ? L::kWide / 2 : L::kWide;  // fragments of a stage
+    static_assert(2 / SPLIT * L::kSteps % kWide == 0);
     __shared__ __attribute__((aligned(16))) char k_lds[2][L::kBytes];
     __shared__ __attribute__((aligned(16))) char v_lds[2][L::kBytes];
     __shared__ __attribute__((aligned(16))) int doc_lds[2][kBlock];
     __shared__ float table[BIAS ? 2 * kMaxDistance + 1 : 1];
 
+    __shared__ float2 parts[SPLIT > 1 ? kRows : 1];  // reference and sum of the second waves
+    constexpr int kOwn = kRows / SPLIT;               // queries of the workgroup
+    constexpr int kSubs = 2 / SPLIT;                  // 32 keys of a block that are a wave's
+
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
+    const int half = SPLIT > 1 ? wave / (kWaves / SPLIT) : 0, strip = wave - half * (kWaves / SPLIT);
     const int w = nnk::xcd_swizzle(blockIdx.x, gridDim.x);
     const int tile = tiles - 1 - w % tiles;  // those that see most keys first
     const int head = w / tiles % a.heads, b = w / tiles / a.heads;
-    const int row0 = tile * kRows, row = row0 + wave * 32 + (lane & 31);
+    const int row0 = tile * kOwn, row = row0 + strip * 32 + (lane & 31);
     const bool in = row < a.len_q;
     const int keys = keys_of(a, b), start = start_of(a, b);
     const int pos = start + row;
     const int limit = in ? limit_of(a, b, keys, pos) : 0;
     const int doc = in && a.doc_q ? a.doc_q[(size_t)b * a.len_q + row] : -1;
     // a wave's least limit and whether one document has all its queries, for blocks without masked entries
-    int least = in ? limit : INT32_MAX;
+    int least = in ? limit : INT32_MAX, wave_most = limit;
 #pragma unroll
-    for (int m = 1; m < 32; m <<= 1) least = min(least, __shfl_xor(least, m));
+    for (int m = 1; m < 32; m <<= 1) {
+        least = min(least, __shfl_xor(least, m));
+        wave_most = max(wave_most, __shfl_xor(wave_most, m));
+    }
     const int wave_doc = __builtin_amdgcn_readfirstlane(doc);
     const bool one_doc = __all(doc == wave_doc || !in) && wave_doc >= 0;
 
-    const int most = limit_of(a, b, keys, start + min(row0 + kRows, a.len_q) - 1);
-    const int4 mine = query_docs_of(a, b, row0 / kBlock, kRows / kBlock);
+    const int most = limit_of(a, b, keys, start + min(row0 + kOwn, a.len_q) - 1);
+    const int4 mine = query_docs_of(a, b, row0 / kBlock, kOwn / kBlock);
     const int blocks = (a.len_k + kBlock - 1) / kBlock;
     const int4* key_docs = a.key_docs ? a.key_docs + (size_t)b * blocks : nullptr;
     Blocks at(0, (most + kBlock - 1) / kBlock, key_docs, mine);
@@ -98,7 +111,8 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && VEC ? 2 : 1) void attn_fwd_
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d) o[d] = zero16();
     float m = -INFINITY, l = 0.0f;  // m in units of the score: of s if there is neither cap nor bias
-    const int rbase = L::row_base(lane), cbase = L::col_base(lane);
+    // a wave of SPLIT 2 has the upper or the lower 32 rows of every block
+    const int rbase = L::row_base(lane) + half * 32 * L::kRowBytes, cbase = L::col_base(lane) + half * 32 * L::kRowBytes;
 
     int next = at.next();
     if (next >= 0) {
@@ -106,173 +120,194 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && VEC ? 2 : 1) void attn_fwd_
         store(next, at.negative, 0);
     }
     for (int buf = 0; next >= 0; buf ^= 1) {
-        const int k0 = next * kBlock, block_doc = at.doc;
+        const int block = next, k0 = next * kBlock + half * 32, block_doc = at.doc;
         next = at.next();
         __syncthreads();  // this block is stored; the one before it is done with
         if (next >= 0) load(next);
+        // nothing here for the wave's queries
+        const bool none = k0 >= wave_most || (docs && one_doc && block_doc >= 0 && block_doc != wave_doc);
+        if (!none) {
 
-        f32x16 s[2] = {zero16(), zero16()};
-        struct Keys {
-            Frag<T> x[L::kWide];
-        };
-        Keys rows[2];
-        const auto read_rows = [&](Keys& y, int n) {
+            f32x16 s[kSubs];
 #pragma unroll
-            for (int j = 0; j < L::kWide; ++j) {
-                const int u = n * L::kWide + j;
-                y.x[j] = L::rows(k_lds[buf], u / L::kSteps, u % L::kSteps, rbase);
-            }
-        };
-        const auto score = [&](const Keys& y, int n) {
-#pragma unroll
-            for (int j = 0; j < L::kWide; ++j) {
-                const int u = n * L::kWide + j;
-                s[u / L::kSteps] = mma(y.x[j], qf[u % L::kSteps], s[u / L::kSteps]);
-            }
-        };
-        if constexpr (kPiped) {
-            read_rows(rows[0], 0);
-            piped<2 * L::kSteps / L::kWide>(rows, read_rows, score);
-        } else {
-#pragma unroll
-            for (int n = 0; n < 2 * L::kSteps / L::kWide; ++n) {
-                read_rows(rows[0], n);
-                score(rows[0], n);
-            }
-        }
-        struct Values {
-            Frag<T> x[DP / 32];
-        };
-        Values columns[2];
-        const auto read_columns = [&](Values& y, int n) {
-#pragma unroll
-            for (int d = 0; d < DP / 32; ++d)
-                y.x[d] = L::cols(v_lds[buf], n / L::kKeySteps, n % L::kKeySteps, d, cbase);
-        };
-        if constexpr (kPiped) {
-            read_columns(columns[0], 0);
-            __builtin_amdgcn_sched_barrier(kMayCross);
-        }
-        const bool whole = k0 + kBlock <= least && (!docs || (one_doc && block_doc == wave_doc));
-        const auto hide_both = [&]() {
-            if (whole) return;
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-                hide(s[i], k0 + 32 * i, limit, docs ? doc_lds[buf] + 32 * i : nullptr, doc, h);
-        };
-        // the largest score so far, and sums and outputs in its terms
-        const auto raise = [&](float unit) {
-            float top = m;
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) top = fmaxf(top, s[i][r]);
-            top = max_halves(top);
-            const float base = top == -INFINITY ? 0.0f : top * unit;
-            if (__any(top > m)) {
-                const float f = exp2_fast(m * unit - base);
-                l *= f;
-#pragma unroll
-                for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) o[d][r] *= f;
-                m = top;
-            }
-            return base;
-        };
-        if constexpr (CAP == 2) {
-            float top = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(s[i][r]));
-            const auto by_series = [&](auto terms) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const float w = s[i][r] * s[i][r];
-                        float c = a.series[decltype(terms)::value - 1];
-#pragma unroll
-                        for (int t = decltype(terms)::value - 2; t >= 0; --t) c = fmaf(w, c, a.series[t]);
-                        s[i][r] = exp2_fast(fmaf(s[i][r], c, -m));
-                    }
+            for (int i = 0; i < kSubs; ++i) s[i] = zero16();
+            struct Keys {
+                Frag<T> x[kWide];
             };
-            const bool plain = whole && __all(m != -INFINITY);
-            if (plain && __all(top < a.tiny)) {
-                by_series(std::integral_constant<int, 4>{});
-            } else if (plain && __all(top < a.small)) {
-                by_series(std::integral_constant<int, 6>{});
+            Keys rows[2];
+            const auto read_rows = [&](Keys& y, int n) {
+#pragma unroll
+                for (int j = 0; j < kWide; ++j) {
+                    const int u = n * kWide + j;
+                    y.x[j] = L::rows(k_lds[buf], u / L::kSteps, u % L::kSteps, rbase);
+                }
+            };
+            const auto score = [&](const Keys& y, int n) {
+#pragma unroll
+                for (int j = 0; j < kWide; ++j) {
+                    const int u = n * kWide + j;
+                    s[u / L::kSteps] = mma(y.x[j], qf[u % L::kSteps], s[u / L::kSteps]);
+                }
+            };
+            if constexpr (kPiped) {
+                read_rows(rows[0], 0);
+                piped<kSubs * L::kSteps / kWide>(rows, read_rows, score);
             } else {
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    cap_scores<false>(s[i], s[i], a.c1);
+                for (int n = 0; n < kSubs * L::kSteps / kWide; ++n) {
+                    read_rows(rows[0], n);
+                    score(rows[0], n);
+                }
+            }
+            struct Values {
+                Frag<T> x[DP / 32];
+            };
+            Values columns[2];
+            const auto read_columns = [&](Values& y, int n) {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[i][r] *= a.c2;
+                for (int d = 0; d < DP / 32; ++d)
+                    y.x[d] = L::cols(v_lds[buf], n / L::kKeySteps, n % L::kKeySteps, d, cbase);
+            };
+            if constexpr (kPiped) {
+                read_columns(columns[0], 0);
+                __builtin_amdgcn_sched_barrier(kMayCross);
+            }
+            const bool whole = block * kBlock + kBlock <= least && (!docs || (one_doc && block_doc == wave_doc));
+            const auto hide_both = [&]() {
+                if (whole) return;
+#pragma unroll
+                for (int i = 0; i < kSubs; ++i)
+                    hide(s[i], k0 + 32 * i, limit, docs ? doc_lds[buf] + half * 32 + 32 * i : nullptr, doc, h);
+            };
+            // the largest score so far, and sums and outputs in its terms
+            const auto raise = [&](float unit) {
+                float top = m;
+#pragma unroll
+                for (int i = 0; i < kSubs; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[i][r]);
+                top = max_halves(top);
+                const float base = top == -INFINITY ? 0.0f : top * unit;
+                if (__any(top > m)) {
+                    const float f = exp2_fast(m * unit - base);
+                    l *= f;
+#pragma unroll
+                    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) o[d][r] *= f;
+                    m = top;
+                }
+                return base;
+            };
+            if constexpr (CAP == 2) {
+                float top = 0.0f;
+#pragma unroll
+                for (int i = 0; i < kSubs; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(s[i][r]));
+                const auto by_series = [&](auto terms) {
+#pragma unroll
+                    for (int i = 0; i < kSubs; ++i)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const float w = s[i][r] * s[i][r];
+                            float c = a.series[decltype(terms)::value - 1];
+#pragma unroll
+                            for (int t = decltype(terms)::value - 2; t >= 0; --t) c = fmaf(w, c, a.series[t]);
+                            s[i][r] = exp2_fast(fmaf(s[i][r], c, -m));
+                        }
+                };
+                const bool plain = whole && __all(m != -INFINITY);
+                if (plain && __all(top < a.tiny)) {
+                    by_series(std::integral_constant<int, 4>{});
+                } else if (plain && __all(top < a.small)) {
+                    by_series(std::integral_constant<int, 6>{});
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kSubs; ++i) {
+                        cap_scores(s[i], a.c1, a.c2);
+                    }
+                    hide_both();
+                    float first = -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < kSubs; ++i)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) first = fmaxf(first, s[i][r]);
+                    first = max_halves(first);
+                    if (m == -INFINITY && first > -INFINITY) m = fmaxf(first, a.c2 - kFixedCap);
+                    const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+                    for (int i = 0; i < kSubs; ++i)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) s[i][r] = exp2_fast(s[i][r] - base);
+                }
+            } else if constexpr (CAP == 0 && !BIAS) {
+                hide_both();
+                const float base = raise(a.c1);
+#pragma unroll
+                for (int i = 0; i < kSubs; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[i][r] = exp2_fast(fmaf(s[i][r], a.c1, -base));
+            } else {
+#pragma unroll
+                for (int i = 0; i < kSubs; ++i) {
+                    if constexpr (CAP) cap_scores(s[i], a.c1, a.c2);
+                    if constexpr (BIAS) add_bias(s[i], CAP ? 1.0f : a.c1, table, a.max_distance, k0 + 32 * i + 4 * h - pos);
                 }
                 hide_both();
-                float first = -INFINITY;
+                const float base = raise(1.0f);
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) first = fmaxf(first, s[i][r]);
-                first = max_halves(first);
-                if (m == -INFINITY && first > -INFINITY) m = fmaxf(first, a.c2 - kFixedCap);
-                const float base = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
+                for (int i = 0; i < kSubs; ++i)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) s[i][r] = exp2_fast(s[i][r] - base);
             }
-        } else if constexpr (CAP == 0 && !BIAS) {
-            hide_both();
-            const float base = raise(a.c1);
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < kSubs; ++i)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[i][r] = exp2_fast(fmaf(s[i][r], a.c1, -base));
-        } else {
-            const float c = CAP ? a.c2 : a.c1;
+                for (int r = 0; r < 16; ++r) l += s[i][r];
+            const auto mix = [&](const Values& y, int n) {
+                const Frag<T> p = operand(s[n / L::kKeySteps], n % L::kKeySteps, T{});
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if constexpr (CAP) cap_scores<false>(s[i], s[i], a.c1);
-                if constexpr (BIAS) {
-                    add_bias(s[i], c, table, a.max_distance, k0 + 32 * i + 4 * h - pos);
-                } else {
+                for (int d = 0; d < DP / 32; ++d) o[d] = mma(y.x[d], p, o[d]);
+            };
+            if constexpr (kPiped) {
+                piped<kSubs * L::kKeySteps>(columns, read_columns, mix);
+            } else {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[i][r] *= c;
+                for (int n = 0; n < kSubs * L::kKeySteps; ++n) {
+                    read_columns(columns[0], n);
+                    mix(columns[0], n);
                 }
-            }
-            hide_both();
-            const float base = raise(1.0f);
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[i][r] = exp2_fast(s[i][r] - base);
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) l += s[i][r];
-        const auto mix = [&](const Values& y, int n) {
-            const Frag<T> p = operand(s[n / L::kKeySteps], n % L::kKeySteps, T{});
-#pragma unroll
-            for (int d = 0; d < DP / 32; ++d) o[d] = mma(y.x[d], p, o[d]);
-        };
-        if constexpr (kPiped) {
-            piped<2 * L::kKeySteps>(columns, read_columns, mix);
-        } else {
-#pragma unroll
-            for (int n = 0; n < 2 * L::kKeySteps; ++n) {
-                read_columns(columns[0], n);
-                mix(columns[0], n);
             }
         }
         if (next >= 0) store(next, at.negative, buf ^ 1);
     }
 
-    if (!in) return;
     l = sum_halves(l);
+    if constexpr (SPLIT > 1) {
+        // the second half's part, through the tiles' LDS: a register's 64 lanes together
+        float* to = reinterpret_cast<float*>(k_lds[0]) + strip * (DP / 32 * 16 * 64) + lane;
+        __syncthreads();
+        if (half) {
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) to[(d * 16 + r) * 64] = o[d][r];
+            if (h == 0) parts[strip * 32 + lane] = float2{m, l};
+        }
+        __syncthreads();
+        if (half) return;
+        const float2 y = parts[strip * 32 + (lane & 31)];
+        const float unit = CAP || BIAS ? 1.0f : a.c1, top = fmaxf(m, y.x), base = top == -INFINITY ? 0.0f : top;
+        const float f = exp2_fast((m - base) * unit), g = exp2_fast((y.x - base) * unit);
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[d][r] = o[d][r] * f + to[(d * 16 + r) * 64] * g;
+        l = l * f + y.y * g;
+        m = top;
+    }
+    if (!in) return;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     T* out = (T*)a.out + b * a.os[0] + (long long)row * a.os[1] + head * a.os[2];
 #pragma unroll
@@ -286,20 +321,23 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && VEC ? 2 : 1) void attn_fwd_
             l == 0.0f ? -INFINITY : (m * (CAP || BIAS ? 1.0f : a.c1) + log2f(l)) * kLn2;
 }
 
-template <typename T, int DP, bool CAP, bool BIAS, bool VEC>
-bool launch(const Args& a, hipStream_t s, const char* what) {
-    const int tiles = (a.len_q + kRows - 1) / kRows;
+template <typename T, int DP, int CAP, bool BIAS, bool VEC>
+bool launch_split(const Args& a, hipStream_t s, const char* what) {
+    const long long groups = ((long long)a.len_q + kRows - 1) / kRows * a.heads * a.batch;
+    const bool split = groups < kSplitBelow;
+    const int own = split ? kRows / 2 : kRows, tiles = (a.len_q + own - 1) / own;
     const unsigned blocks = (unsigned)((long long)tiles * a.heads * a.batch);
-    bool done = false;
-    if constexpr (CAP && !BIAS) {
-        if (a.c2 <= kFixedCap) {
-            attn_fwd_kernel<T, DP, 2, false, VEC><<<blocks, kTpb, 0, s>>>(a, tiles);
-            done = true;
-        }
-    }
-    if (!done) attn_fwd_kernel<T, DP, CAP, BIAS, VEC><<<blocks, kTpb, 0, s>>>(a, tiles);
+    if (split) attn_fwd_kernel<T, DP, CAP, BIAS, VEC, 2><<<blocks, kTpb, 0, s>>>(a, tiles);
+    else attn_fwd_kernel<T, DP, CAP, BIAS, VEC, 1><<<blocks, kTpb, 0, s>>>(a, tiles);
     nnk_after_launch(what, s);
     return true;
+}
+template <typename T, int DP, bool CAP, bool BIAS, bool VEC>
+bool launch(const Args& a, hipStream_t s, const char* what) {
+    if constexpr (CAP && !BIAS) {
+        if (a.c2 <= kFixedCap) return launch_split<T, DP, 2, BIAS, VEC>(a, s, what);
+    }
+    return launch_split<T, DP, CAP, BIAS, VEC>(a, s, what);
 }
 
 // Documents of a block of 64 positions: least and largest, whether any is negative.
