@@ -430,12 +430,21 @@ __device__ __forceinline__ void load_bias(const Args& a, float* table, int head)
     }
 }
 
-// s = c s + bias of the tile's entries; rel: distance of register 0.
-__device__ __forceinline__ void add_bias(f32x16& s, float c, const float* table, int m, int rel) {
+// s = c s + bias of the tile's entries, whose distances are the lane's rel + STEP * (8 g + j)
+// (register 4 g + j), and in the wave `least` at least and 62 more at most.  Tiles wholly
+// past max_distance, which most are, add one value.
+template <int STEP>
+__device__ __forceinline__ void add_bias(f32x16& s, float c, const float* table, int m, int rel, int least) {
+    if (least + 62 <= -m || least >= m) {
+        const float bias = table[least >= m ? 2 * m : 0];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        const int d = rel + 8 * (r >> 2) + (r & 3);
-        s[r] = s[r] * c + table[min(max(d, -m), m) + m];
+        for (int r = 0; r < 16; ++r) s[r] = s[r] * c + bias;
+    } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int d = rel + STEP * (8 * (r >> 2) + (r & 3));
+            s[r] = s[r] * c + table[min(max(d, -m), m) + m];
+        }
     }
 }
 

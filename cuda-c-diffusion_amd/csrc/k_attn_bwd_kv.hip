@@ -191,13 +191,8 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn
                 f32x16 slope;
                 if constexpr (CAP) cap_scores(s, slope, a);
                 if constexpr (BIAS) {
-                    const int rel = key - (start + q0 + 32 * i + 4 * h);
-                    const float c = CAP ? 1.0f : a.c1;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int d = rel - 8 * (r >> 2) - (r & 3), m = a.max_distance;
-                        s[r] = s[r] * c + table[min(max(d, -m), m) + m];
-                    }
+                    const int q = start + q0 + 32 * i;
+                    add_bias<-1>(s, CAP ? 1.0f : a.c1, table, a.max_distance, key - (q + 4 * h), first_key - (q + 31));
                 } else if constexpr (!CAP) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) s[r] *= a.c1;
@@ -382,24 +377,39 @@ __global__ __launch_bounds__(kTpb) void attn_head_sum_kernel(Args a, int quads, 
     store4<T, VEC>((T*)a.dv + b * a.vs[0] + key * a.vs[1] + kv * a.vs[2], d, a.dim, v[0], v[1], v[2], v[3]);
 }
 
-// dbias[bucket, head]: the sums of its distances over batch and key tiles, in 64 bits,
-// a thread's rows in order and the threads' sums as a tree.
-__global__ __launch_bounds__(kTpb) void attn_bias_grad_kernel(float* dbias, const float* dist_sums, const int* bucket,
-    int batch, int heads, int buckets, int tiles, int n) {
-    __shared__ double part[kTpb];
-    const int head = blockIdx.x % heads, mine = blockIdx.x / heads;
-    double sum = 0.0;
-    for (int i = 0; i < n; ++i) {
-        if (min(max(bucket[i], 0), buckets - 1) != mine) continue;
-        for (int r = threadIdx.x; r < batch * tiles; r += kTpb)
-            sum += dist_sums[(((size_t)(r / tiles) * heads + head) * tiles + r % tiles) * n + i];
-    }
-    part[threadIdx.x] = sum;
-    for (int m = kTpb / 2; m > 0; m >>= 1) {
+// dbias[bucket, head]: a workgroup a head.  First the sums of each distance over batch and
+// key tiles, in 64 bits, 4 threads a distance, each its quarter of the rows in order; then
+// a thread a bucket adds its distances in their order.
+constexpr int kBiasTpb = 1024, kBiasCols = kBiasTpb / 4;
+__global__ __launch_bounds__(kBiasTpb) void attn_bias_grad_kernel(float* dbias, const float* dist_sums,
+    const int* bucket, int batch, int heads, int buckets, int tiles, int n) {
+    __shared__ double part[4][kBiasCols], sums[2 * kMaxDistance + 1];
+    __shared__ int of[2 * kMaxDistance + 1];
+    const int head = blockIdx.x, col = threadIdx.x % kBiasCols, quarter = threadIdx.x / kBiasCols;
+    const int rows = batch * tiles, each = (rows + 3) / 4, first = quarter * each, last = min(rows, first + each);
+    for (int i0 = 0; i0 < n; i0 += kBiasCols) {
+        const int i = i0 + col;
+        double sum = 0.0;
+        if (i < n) {
+#pragma unroll 8
+            for (int r = first; r < last; ++r) {
+                const int b = r / tiles;
+                sum += dist_sums[(((size_t)b * heads + head) * tiles + r - b * tiles) * n + i];
+            }
+        }
+        part[quarter][col] = sum;
         __syncthreads();
-        if ((int)threadIdx.x < m) part[threadIdx.x] += part[threadIdx.x + m];
+        if (quarter == 0 && i < n) {
+            sums[i] = ((part[0][col] + part[1][col]) + part[2][col]) + part[3][col];
+            of[i] = min(max(bucket[i], 0), buckets - 1);
+        }
+        __syncthreads();
     }
-    if (threadIdx.x == 0) dbias[(size_t)mine * heads + head] = (float)part[0];
+    for (int m = threadIdx.x; m < buckets; m += kBiasTpb) {
+        double sum = 0.0;
+        for (int i = 0; i < n; ++i) sum += of[i] == m ? sums[i] : 0.0;
+        dbias[(size_t)m * heads + head] = (float)sum;
+    }
 }
 
 // Keys of a workgroup: the heads of a key head apart count as workgroups here.
@@ -458,7 +468,7 @@ size_t nnk_attention_dist_floats(const NnAttention* a) {
 }
 
 void nnk_attention_bias_grad(const Args& a, float* dbias, hipStream_t s, const char* what) {
-    attn_bias_grad_kernel<<<(unsigned)(a.buckets * a.heads), kTpb, 0, s>>>(dbias, a.dist_sums, a.bucket, a.batch,
+    attn_bias_grad_kernel<<<(unsigned)a.heads, kBiasTpb, 0, s>>>(dbias, a.dist_sums, a.bucket, a.batch,
         a.heads, a.buckets, tiles_of(a), 2 * a.max_distance + 1);
     nnk_after_launch(what, s);
 }

@@ -30,11 +30,11 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn
     constexpr int kOwn = kRows / SPLIT;               // queries of the workgroup
 
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
-    const int half = SPLIT > 1 ? wave / (kWaves / SPLIT) : 0;
+    const int half = SPLIT > 1 ? wave / (kWaves / SPLIT) : 0, strip = wave - half * (kWaves / SPLIT);
     const int w = nnk::xcd_swizzle(blockIdx.x, gridDim.x);
     const int tile = tiles - 1 - w % tiles;
     const int head = w / tiles % a.heads, b = w / tiles / a.heads;
-    const int row0 = tile * kOwn, row = row0 + (wave - half * (kWaves / SPLIT)) * 32 + (lane & 31);
+    const int row0 = tile * kOwn, row = row0 + strip * 32 + (lane & 31);
     const bool in = row < a.len_q;
     const int keys = keys_of(a, b), start = start_of(a, b);
     const int pos = start + row;
@@ -159,7 +159,8 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn
             });
             if constexpr (CAP) cap_scores(s, slope, a);
             if constexpr (BIAS) {
-                add_bias(s, CAP ? 1.0f : a.c1, table, a.max_distance, k0 + 32 * i + 4 * h - pos);
+                add_bias<1>(s, CAP ? 1.0f : a.c1, table, a.max_distance, k0 + 32 * i + 4 * h - pos,
+                    k0 + 32 * i - (start + row0 + strip * 32 + 31));
             } else if constexpr (!CAP) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] *= a.c1;

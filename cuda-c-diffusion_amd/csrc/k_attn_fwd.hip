@@ -252,7 +252,8 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && VEC ? 2 : 1) void attn_fwd_
 #pragma unroll
                 for (int i = 0; i < kSubs; ++i) {
                     if constexpr (CAP) cap_scores(s[i], a.c1, a.c2);
-                    if constexpr (BIAS) add_bias(s[i], CAP ? 1.0f : a.c1, table, a.max_distance, k0 + 32 * i + 4 * h - pos);
+                    if constexpr (BIAS) add_bias<1>(s[i], CAP ? 1.0f : a.c1, table, a.max_distance, k0 + 32 * i + 4 * h - pos,
+                        k0 + 32 * i - (start + row0 + strip * 32 + 31));
                 }
                 hide_both();
                 const float base = raise(1.0f);
