@@ -378,15 +378,15 @@ __global__ __launch_bounds__(kTpb) void attn_head_sum_kernel(Args a, int quads, 
 }
 
 // dbias[bucket, head]: a workgroup a head.  First the sums of each distance over batch and
-// key tiles, in 64 bits, 4 threads a distance, each its quarter of the rows in order; then
-// a thread a bucket adds its distances in their order.
-constexpr int kBiasTpb = 1024, kBiasCols = kBiasTpb / 4;
+// key tiles, in 64 bits, 2 threads a distance, each its half of the rows in order; then a
+// wave a bucket, a lane's distances in order, the lanes' as a tree.
+constexpr int kBiasTpb = 1024, kBiasCols = kBiasTpb / 2;
 __global__ __launch_bounds__(kBiasTpb) void attn_bias_grad_kernel(float* dbias, const float* dist_sums,
     const int* bucket, int batch, int heads, int buckets, int tiles, int n) {
-    __shared__ double part[4][kBiasCols], sums[2 * kMaxDistance + 1];
+    __shared__ double part[2][kBiasCols], sums[2 * kMaxDistance + 1];
     __shared__ int of[2 * kMaxDistance + 1];
-    const int head = blockIdx.x, col = threadIdx.x % kBiasCols, quarter = threadIdx.x / kBiasCols;
-    const int rows = batch * tiles, each = (rows + 3) / 4, first = quarter * each, last = min(rows, first + each);
+    const int head = blockIdx.x, col = threadIdx.x % kBiasCols, half = threadIdx.x / kBiasCols;
+    const int rows = batch * tiles, each = (rows + 1) / 2, first = half * each, last = min(rows, first + each);
     for (int i0 = 0; i0 < n; i0 += kBiasCols) {
         const int i = i0 + col;
         double sum = 0.0;
@@ -397,18 +397,20 @@ __global__ __launch_bounds__(kBiasTpb) void attn_bias_grad_kernel(float* dbias, 
                 sum += dist_sums[(((size_t)b * heads + head) * tiles + r - b * tiles) * n + i];
             }
         }
-        part[quarter][col] = sum;
+        part[half][col] = sum;
         __syncthreads();
-        if (quarter == 0 && i < n) {
-            sums[i] = ((part[0][col] + part[1][col]) + part[2][col]) + part[3][col];
+        if (half == 0 && i < n) {
+            sums[i] = part[0][col] + part[1][col];
             of[i] = min(max(bucket[i], 0), buckets - 1);
         }
         __syncthreads();
     }
-    for (int m = threadIdx.x; m < buckets; m += kBiasTpb) {
+    for (int m = threadIdx.x / 64; m < buckets; m += kBiasTpb / 64) {
         double sum = 0.0;
-        for (int i = 0; i < n; ++i) sum += of[i] == m ? sums[i] : 0.0;
-        dbias[(size_t)m * heads + head] = (float)sum;
+        for (int i = threadIdx.x % 64; i < n; i += 64) sum += of[i] == m ? sums[i] : 0.0;
+#pragma unroll
+        for (int x = 1; x < 64; x <<= 1) sum += __shfl_xor(sum, x);
+        if (threadIdx.x % 64 == 0) dbias[(size_t)m * heads + head] = (float)sum;
     }
 }
 
