@@ -67,6 +67,8 @@ bool take(Args& p, const NnAttention* a, const char* what) {
     p.scale = a->scale;
     p.c1 = a->softcap > 0.0f ? a->scale / a->softcap : a->scale * kLog2e;
     p.c2 = a->softcap * kLog2e;
+    NNK_REQUIRE_RET(p.c1 < INFINITY && p.c2 < INFINITY, false, what, "%s: scale=%g with softcap=%g overflows", what,
+        a->scale, a->softcap);
     if (a->softcap > 0.0f) {
         const double tanh_of[6] = {1.0, -1.0 / 3, 2.0 / 15, -17.0 / 315, 62.0 / 2835, -1382.0 / 155925};
         double power = (double)p.c2 * p.c1;

@@ -368,17 +368,17 @@ __device__ __forceinline__ void cap_scores(f32x16& s, float c1, float c2) {
         }
     }
 }
-// The same with the slope 1 - tanh^2, for the gradients.  Each score takes the same form
-// whatever its neighbours are: both gradient kernels get the same value, to the bit.
+// c2 tanh(c1 s) by the first TERMS terms of its series
+template <int TERMS>
+__device__ __forceinline__ float cap_series(float s, const Args& a) {
+    const float w = s * s;
+    float c = a.series[TERMS - 1];
+#pragma unroll
+    for (int t = TERMS - 2; t >= 0; --t) c = fmaf(w, c, a.series[t]);
+    return s * c;
+}
+// The capped scores with the slope 1 - tanh^2, for the gradients.
 __device__ __forceinline__ void cap_scores(f32x16& s, f32x16& slope, const Args& a) {
-    const auto series = [&](float x) {
-        const float w = x * x;
-        float c = fmaf(w, a.series[5], a.series[4]);
-        c = fmaf(w, c, a.series[3]);
-        c = fmaf(w, c, a.series[2]);
-        c = fmaf(w, c, a.series[1]);
-        return x * fmaf(w, c, a.series[0]);
-    };
     const auto slope_of = [&](float x) {
         const float t = x * a.inv_c2;
         return fmaf(-t, t, 1.0f);
@@ -386,10 +386,16 @@ __device__ __forceinline__ void cap_scores(f32x16& s, f32x16& slope, const Args&
     float top = 0.0f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(s[r]));
-    if (__all(top < a.small)) {
+    if (__all(top < a.tiny)) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            s[r] = series(s[r]);
+            s[r] = cap_series<4>(s[r], a);
+            slope[r] = slope_of(s[r]);
+        }
+    } else if (__all(top < a.small)) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s[r] = cap_series<6>(s[r], a);
             slope[r] = slope_of(s[r]);
         }
     } else {
@@ -397,7 +403,7 @@ __device__ __forceinline__ void cap_scores(f32x16& s, f32x16& slope, const Args&
         for (int r = 0; r < 16; ++r) {
             const float x = s[r], q = __builtin_amdgcn_rcpf(exp2_fast(fabsf(x) * (2.0f * kLog2e * a.c1)) + 1.0f);
             const bool near = fabsf(x) < a.small;
-            s[r] = near ? series(x) : copysignf(fmaf(-2.0f, q, 1.0f), x) * a.c2;
+            s[r] = near ? cap_series<6>(x, a) : copysignf(fmaf(-2.0f, q, 1.0f), x) * a.c2;
             slope[r] = near ? slope_of(s[r]) : 4.0f * q * (1.0f - q);
         }
     }

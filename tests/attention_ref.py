@@ -135,7 +135,10 @@ def attention(c, q, k, v, bias=None, bucket=None, dout=None):
     p = e / np.where(total > 0, total, 1)[..., None]
     out = np.einsum("bhij,bjhd->bihd", p, vv)
     got = {"out": out, "lse": lse}
-    mag = {"out": np.einsum("bhij,bjhd->bihd", p, abs(vv)), "lse": abs(lse)}
+    # the log-sum adds up products of scores (those of the keys that count) and a logarithm
+    dots = np.einsum("bihd,bjhd->bhij", abs(q), abs(kk)) * scale
+    with np.errstate(divide="ignore"):
+        mag = {"out": np.einsum("bhij,bjhd->bihd", p, abs(vv)), "lse": (p * dots).sum(-1) + abs(np.log(total)) + abs(lse)}
     if dout is None:
         return got, mag
 

@@ -40,6 +40,7 @@ BAD_ATTN = [
     (dict(scale=0.0), "scale=0"),
     (dict(scale=float("nan")), "scale=nan"),
     (dict(softcap=-1.0), "softcap=-1"),
+    (dict(scale=1e10, softcap=1e-35), "overflows"),
     (dict(mask=9), "unknown mask 9"),
     (dict(mask=2), "null prefix"),
     (dict(doc_q=DUMMY), "documents of queries or keys only"),

@@ -350,6 +350,39 @@ def test_offsets_past_32_bits(nn, L, rng, dtype, len_q):
         far[m].close()
 
 
+@pytest.mark.parametrize("dtype, len_q", [("bf16", 1), ("bf16", 130), ("f32", 3)])
+def test_long_cache_of_aligned_rows(nn, L, rng, dtype, len_q):
+    """Tokens 2^20 bytes apart: a block's offsets fit in 32 bits, a block's address does not."""
+    n, dim, size = 4500, 64, 2 if dtype == "bf16" else 4
+    step = (1 << 20) // size
+    c = case(dtype, 1, len_q, n, 1, 1, dim, "causal")
+    print(f"[case] long cache {c}", flush=True)
+    small = Call(nn, L, rng, c, backward=False)
+    far = {m: L.alloc(((n - 1) * step + dim) * size // 4 + 4) for m in ("k", "v")}
+    for m in far:
+        rows = small.t[m].dev.download().view(np.uint8)
+        for j in range(n):
+            row = np.ascontiguousarray(rows[j * dim * size:(j + 1) * dim * size])
+            assert L.nnhip_memcpy_htod(far[m].p + j * step * size, row.ctypes.data, row.nbytes) == 0
+    small.args.k_stride = small.args.v_stride = (n * step, step, dim)
+    t = small.t
+    L.launch_attention_forward(t["out"].p, small.lse.p, t["q"].p, far["k"].p, far["v"].p, small.args, small.ws.p, None)
+    L.sync()
+    small.compare()
+    for m in far:
+        far[m].close()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("mask, cap, buckets", [("none", 0.0, 0), ("causal", 30.0, 0), ("prefix", 0.0, 8)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_enough_workgroups_for_whole_tiles(nn, L, rng, dtype, mask, cap, buckets, dim):
+    """Sizes at which a workgroup keeps 128 rows (fewer tiles are split), with documents that end anywhere."""
+    doc = np.sort(rng.integers(-1, 4, (32, 130)), axis=1)
+    run(nn, L, rng, case(dtype, 32, 130, 130, 8, 4 if mask == "causal" else 8, dim, mask, cap, prefix=[60] * 32,
+                         buckets=buckets, max_distance=40, **({"doc_q": doc, "doc_k": doc} if mask != "none" else {})))
+
+
 def test_large_scores_and_infinite_bias(nn, L, rng):
     """Scores of hundreds (one key takes all), and a bias of -inf, which hides its bucket."""
     c = case("f32", 1, 80, 80, 2, 2, 16, scale=40.0)
