@@ -13,9 +13,36 @@ size_t docs_floats(const NnAttention* a) {
     const size_t nk = ((size_t)a->len_k + kBlock - 1) / kBlock, nq = ((size_t)a->len_q + kBlock - 1) / kBlock;
     return 4 * (size_t)a->batch * (nk + nq);
 }
-size_t head_floats(const NnAttention* a) {
-    const size_t n = (size_t)a->batch * a->heads * a->len_k * a->head_dim;
-    return nnk_attention_splits_heads(a) ? (2 * n + 3) / 4 * 4 : 0;
+// How the gradients are divided over workgroups.  Key heads that are shared and few tiles of
+// keys: the heads apart.  Few workgroups even so: tiles of 64, and the other axis in parts of
+// 4 blocks or more, up to two workgroups a CU.  (One head of 1681 tokens, 2 images, was 27
+// workgroups' work otherwise.)
+void divide(Args& p, const NnAttention* a) {
+    const auto up = [](long long n, long long d) { return (n + d - 1) / d; };
+    const auto parts = [](long long groups, long long blocks) {
+        return groups >= kCus || !groups ? 1 : (int)std::max(1LL, std::min(2 * kCus / groups, blocks / 4));
+    };
+    const long long batch = a->batch, heads = a->heads;
+    const bool apart = heads > a->kv_heads && up(a->len_k, kRows) * a->kv_heads * batch < 4 * kCus;
+    const long long owners = (apart ? heads : a->kv_heads) * batch;
+    p.heads_each = apart ? 1 : (int)(heads / a->kv_heads);
+    p.kv_keys = up(a->len_k, kRows) * owners < kSplitBelow ? kRows / 2 : kRows;
+    p.q_splits = parts(up(a->len_k, p.kv_keys) * owners, up(a->len_q, kBlock));
+    p.q_rows = up(a->len_q, kRows) * heads * batch < kSplitBelow ? kRows / 2 : kRows;
+    p.k_splits = parts(up(a->len_q, p.q_rows) * heads * batch, up(a->len_k, kBlock));
+}
+size_t by4(size_t n) { return (n + 3) / 4 * 4; }
+size_t kv_floats(const NnAttention* a, const Args& p) {
+    const size_t parts = (size_t)a->heads / p.heads_each * p.q_splits;
+    return parts > (size_t)a->kv_heads ? by4(2 * a->batch * parts * a->len_k * a->head_dim) : 0;
+}
+size_t q_floats(const NnAttention* a, const Args& p) {
+    const size_t rows = (size_t)a->batch * a->heads * p.k_splits * a->len_q;
+    return p.k_splits > 1 ? by4(2 * rows) + by4(rows * a->head_dim) : 0;
+}
+size_t dist_floats(const NnAttention* a, const Args& p) {
+    const size_t tiles = ((size_t)a->len_k + p.kv_keys - 1) / p.kv_keys;
+    return (size_t)a->batch * a->heads * p.q_splits * tiles * (2 * a->max_distance + 1);
 }
 size_t stat_floats(const NnAttention* a) { return 2 * (size_t)a->batch * a->heads * a->len_q; }
 
@@ -133,7 +160,10 @@ void launch_attention_forward(void* out, float* lse, const void* q, const void* 
 
 size_t nnhip_attention_backward_workspace(const NnAttention* a) {
     if (!sizes_fit(a, "nnhip_attention_backward_workspace")) return 0;
-    return docs_floats(a) + head_floats(a) + stat_floats(a) + (a->buckets ? nnk_attention_dist_floats(a) : 0);
+    Args p;
+    divide(p, a);
+    return docs_floats(a) + kv_floats(a, p) + q_floats(a, p) + by4(stat_floats(a)) +
+        (a->buckets ? dist_floats(a, p) : 0);
 }
 
 void launch_attention_backward(void* dq, void* dk, void* dv, float* dbias, const void* dout,
@@ -160,12 +190,17 @@ void launch_attention_backward(void* dq, void* dk, void* dv, float* dbias, const
     p.vec = strides_by_16(a);
     for (const void* x : {q, k, v, out, dout, (const void*)dq, (const void*)dk, (const void*)dv})
         p.vec = p.vec && nnk::aligned16(x);
+    divide(p, a);
     float* ws = workspace + docs_floats(a);
-    if (head_floats(a)) p.head_sums = ws;
-    p.heads_each = p.head_sums ? 1 : p.group;
-    ws += head_floats(a);
+    if (kv_floats(a, p)) p.kv_sums = ws;
+    ws += kv_floats(a, p);
+    if (q_floats(a, p)) {
+        p.stat_sums = reinterpret_cast<float2*>(ws);
+        p.q_sums = ws + by4(2 * (size_t)a->batch * a->heads * p.k_splits * a->len_q);
+    }
+    ws += q_floats(a, p);
     p.stat = reinterpret_cast<float2*>(ws);
-    if (dbias) p.dist_sums = ws + stat_floats(a);
+    if (dbias) p.dist_sums = ws + by4(stat_floats(a));
     const bool half = a->dtype == NN_BF16;
     if (has_q && has_k) nnk_attention_docs(p, workspace, s, what);
     if (has_q && !nnk_attention_backward_q(p, half, s, what)) return;

@@ -41,7 +41,7 @@ constexpr int kTpb = 256;
 constexpr int kWaves = kTpb / 64;
 constexpr int kRows = 32 * kWaves;  // columns of a workgroup: queries, or keys in the key gradients
 constexpr int kCus = 256;
-constexpr int kSplitBelow = 2 * kCus;  // workgroups of the gradient kernels that are split in two
+constexpr int kSplitBelow = 2 * kCus;  // workgroups below which blocks are shared by two waves
 constexpr int kMaxDistance = 1023;
 constexpr int kTicketWords = 2048;  // at the front of every forward workspace: zeros between calls
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -298,8 +298,12 @@ struct Args {
     void *dq, *dk, *dv;
     float2* stat;      // backward: per query, log2 of its sum and its <p, dp>
     float* dist_sums;  // backward: sums of score gradients by distance, per key tile
-    float* head_sums;  // backward: dk / scale, then dv, of each head [batch, heads, len_k, dim], or null
-    int heads_each;    // backward: heads of a workgroup, 1 or all that share a key head
+    // How the gradients are divided, and the sums of the parts that are added up afterwards:
+    int heads_each, q_splits, kv_keys;  // key gradients: heads and share of the queries of a workgroup; its keys
+    int k_splits, q_rows;               // query gradients: share of the keys; queries
+    float* kv_sums;                     // dk / scale, then dv, [batch, parts, len_k, dim], or null
+    float* q_sums;                      // dq / scale [batch, heads, k_splits, len_q, dim], or null
+    float2* stat_sums;                  // sums of p and of p dp [batch, heads, k_splits, len_q]
     const int4* key_docs;    // per block of 64 keys: least and largest document, whether any is negative
     const int4* query_docs;  // per block of 64 queries
     long long qs[3], ks[3], vs[3], os[3];
@@ -544,11 +548,8 @@ bool nnk_attention_backward_kv(const attn::Args& args, bool half, hipStream_t s,
 bool nnk_attention_is_few(const NnAttention* a);
 size_t nnk_attention_few_floats(const NnAttention* a);
 bool nnk_attention_few(const attn::Args& args, bool half, float* ws, hipStream_t s, const char* what);
-// Whether the key gradients of heads that share a key head are summed apart first.
-bool nnk_attention_splits_heads(const NnAttention* a);
-// Bias gradient from args.dist_sums, and the floats that those take.
+// Bias gradient from args.dist_sums.
 void nnk_attention_bias_grad(const attn::Args& args, float* dbias, hipStream_t s, const char* what);
-size_t nnk_attention_dist_floats(const NnAttention* a);
 
 // FN<T, DP, CAP, BIAS, VEC> for the call's type, feature count, score terms and alignment.
 // Rows that are not on 16 bytes are taken element by element, in one size.

@@ -13,7 +13,8 @@
 // more workgroups even out.
 //
 // SPLIT 2, for calls of few workgroups: 64 keys, and of each block 32 queries a wave; the
-// two waves of the same keys are added up at the end, in their order.
+// two waves of the same keys are added up at the end, in their order.  Fewer still: the
+// queries are divided too, and their parts added up as the heads' are.
 //
 // Bias: sums of dx by distance j - P.  A 32 x 32 tile has its distances on diagonals;
 // row m's values go m lanes along, after which a lane holds two distances (one for what
@@ -45,8 +46,9 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
     const int half = SPLIT > 1 ? wave / (kWaves / SPLIT) : 0, strip = wave - half * (kWaves / SPLIT);
     const int w = nnk::xcd_swizzle(blockIdx.x, gridDim.x);
-    const int tile = w % tiles, part = w / tiles % (a.heads / a.heads_each), b = w / tiles / (a.heads / a.heads_each);
-    const int head0 = part * a.heads_each, kv = head0 / a.group;
+    const int parts = a.heads / a.heads_each * a.q_splits;
+    const int tile = w % tiles, part = w / tiles % parts, b = w / tiles / parts;
+    const int share = part % a.q_splits, head0 = part / a.q_splits * a.heads_each, kv = head0 / a.group;
     const int k0 = tile * kOwn, first_key = k0 + strip * 32, key = first_key + (lane & 31);
     const int keys = keys_of(a, b), start = start_of(a, b);
     const int* docs = a.doc_k ? a.doc_k + (size_t)b * a.len_k : nullptr;
@@ -135,7 +137,8 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn
             }
         };
 
-        Blocks at(first_block, q_blocks, query_docs, mine);
+        const int each = (q_blocks + a.q_splits - 1) / a.q_splits;
+        Blocks at(max(first_block, share * each), min(q_blocks, (share + 1) * each), query_docs, mine);
         int next = at.next();
         if (next >= 0) {
             load(next);
@@ -286,7 +289,7 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn
             __syncthreads();
             if (a.dist_sums) {
                 const int n = 2 * a.max_distance + 1;
-                float* to = a.dist_sums + (((size_t)b * a.heads + head) * tiles + tile) * n;
+                float* to = a.dist_sums + ((((size_t)b * a.heads + head) * a.q_splits + share) * tiles + tile) * n;
                 for (int i = threadIdx.x; i < n; i += kTpb) {
                     float sum = 0.0f;
                     const int first = i == 0 ? 0 : i + kSlack, last = i == n - 1 ? span : i + kSlack + 1;
@@ -323,9 +326,9 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn
             }
     }
     if (!in) return;
-    if (a.head_sums) {
-        const size_t at = (((size_t)b * a.heads + head0) * a.len_k + key) * a.dim;
-        float *kout = a.head_sums + at, *vout = kout + (size_t)a.batch * a.heads * a.len_k * a.dim;
+    if (a.kv_sums) {
+        const size_t at = (((size_t)b * parts + part) * a.len_k + key) * a.dim;
+        float *kout = a.kv_sums + at, *vout = kout + (size_t)a.batch * parts * a.len_k * a.dim;
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
@@ -349,19 +352,20 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn
         }
 }
 
-// dk and dv from the sums of the heads that share a key head, in their order; 4 features a
-// thread.
+// dk and dv from the sums of a key head's parts (heads, shares of the queries), in their
+// order; 4 features a thread.
 template <typename T, bool VEC>
-__global__ __launch_bounds__(kTpb) void attn_head_sum_kernel(Args a, int quads, long long total) {
+__global__ __launch_bounds__(kTpb) void attn_kv_sum_kernel(Args a, int quads, long long total) {
     const long long n = (long long)blockIdx.x * kTpb + threadIdx.x;
     if (n >= total) return;
     const int d = (int)(n % quads) * 4;
     const long long row = n / quads;
     const int key = (int)(row % a.len_k), kv = (int)(row / a.len_k % a.kv_heads), b = (int)(row / a.len_k / a.kv_heads);
-    const float* from = a.head_sums + (((size_t)b * a.heads + kv * a.group) * a.len_k + key) * a.dim + d;
-    const size_t step = (size_t)a.len_k * a.dim, v_at = (size_t)a.batch * a.heads * a.len_k * a.dim;
+    const int parts = a.heads / a.heads_each * a.q_splits, mine = parts / a.kv_heads;
+    const float* from = a.kv_sums + (((size_t)b * parts + kv * mine) * a.len_k + key) * a.dim + d;
+    const size_t step = (size_t)a.len_k * a.dim, v_at = (size_t)a.batch * parts * a.len_k * a.dim;
     float k[4] = {0.0f, 0.0f, 0.0f, 0.0f}, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int g = 0; g < a.group; ++g) {
+    for (int g = 0; g < mine; ++g) {
         if constexpr (VEC) {
             const float4 x = nnk::ld4(from + g * step), y = nnk::ld4(from + g * step + v_at);
             k[0] += x.x, k[1] += x.y, k[2] += x.z, k[3] += x.w;
@@ -414,18 +418,8 @@ __global__ __launch_bounds__(kBiasTpb) void attn_bias_grad_kernel(float* dbias, 
     }
 }
 
-// Keys of a workgroup: the heads of a key head apart count as workgroups here.
-int keys_each(long long batch, long long len_k, long long groups) {
-    return (len_k + kRows - 1) / kRows * groups * batch < kSplitBelow ? kRows / 2 : kRows;
-}
-int tiles_of(const Args& a) {
-    const int each = keys_each(a.batch, a.len_k, a.heads / a.heads_each);
-    return (a.len_k + each - 1) / each;
-}
-
 template <typename T, int DP, bool CAP, bool BIAS, bool VEC, int SPLIT>
-bool launch_split(const Args& a, hipStream_t s, const char* what) {
-    const int tiles = tiles_of(a);
+bool launch_split(const Args& a, int tiles, hipStream_t s, const char* what) {
     const size_t lds = BIAS ? kWaves * (2 * (a.max_distance + kSlack) + 1) * sizeof(float) : 0;
     if constexpr (BIAS) {
         static std::atomic<unsigned long long> done{0};
@@ -433,21 +427,22 @@ bool launch_split(const Args& a, hipStream_t s, const char* what) {
                 kWaves * (2 * (kMaxDistance + kSlack) + 1) * sizeof(float), done, what))
             return false;
     }
-    attn_bwd_kv_kernel<T, DP, CAP, BIAS, VEC, SPLIT>
-        <<<(unsigned)((long long)tiles * (a.heads / a.heads_each) * a.batch), kTpb, lds, s>>>(a, tiles);
+    const long long groups = (long long)tiles * (a.heads / a.heads_each) * a.q_splits * a.batch;
+    attn_bwd_kv_kernel<T, DP, CAP, BIAS, VEC, SPLIT><<<(unsigned)groups, kTpb, lds, s>>>(a, tiles);
     nnk_after_launch(what, s);
     return true;
 }
 
 template <typename T, int DP, bool CAP, bool BIAS, bool VEC>
 bool launch(const Args& a, hipStream_t s, const char* what) {
-    if (!(keys_each(a.batch, a.len_k, a.heads / a.heads_each) < kRows ? launch_split<T, DP, CAP, BIAS, VEC, 2>(a, s, what)
-                                                                     : launch_split<T, DP, CAP, BIAS, VEC, 1>(a, s, what)))
+    const int tiles = (a.len_k + a.kv_keys - 1) / a.kv_keys;
+    if (!(a.kv_keys < kRows ? launch_split<T, DP, CAP, BIAS, VEC, 2>(a, tiles, s, what)
+                            : launch_split<T, DP, CAP, BIAS, VEC, 1>(a, tiles, s, what)))
         return false;
-    if (a.head_sums) {
+    if (a.kv_sums) {
         const int quads = (a.dim + 3) / 4;
         const long long total = (long long)a.batch * a.kv_heads * a.len_k * quads;
-        attn_head_sum_kernel<T, VEC><<<(unsigned)((total + kTpb - 1) / kTpb), kTpb, 0, s>>>(a, quads, total);
+        attn_kv_sum_kernel<T, VEC><<<(unsigned)((total + kTpb - 1) / kTpb), kTpb, 0, s>>>(a, quads, total);
         nnk_after_launch(what, s);
     }
     return true;
@@ -459,18 +454,9 @@ bool nnk_attention_backward_kv(const Args& a, bool half, hipStream_t s, const ch
     return NNK_ATTN_DISPATCH(a, half, launch, a, s, what);
 }
 
-bool nnk_attention_splits_heads(const NnAttention* a) {
-    const long long tiles = ((long long)a->len_k + kRows - 1) / kRows * a->kv_heads * a->batch;
-    return a->heads > a->kv_heads && tiles < 4 * kCus;
-}
-
-size_t nnk_attention_dist_floats(const NnAttention* a) {
-    const int each = keys_each(a->batch, a->len_k, nnk_attention_splits_heads(a) ? a->heads : a->kv_heads);
-    return (size_t)a->batch * a->heads * ((a->len_k + each - 1) / each) * (2 * a->max_distance + 1);
-}
-
 void nnk_attention_bias_grad(const Args& a, float* dbias, hipStream_t s, const char* what) {
-    attn_bias_grad_kernel<<<(unsigned)a.heads, kBiasTpb, 0, s>>>(dbias, a.dist_sums, a.bucket, a.batch,
-        a.heads, a.buckets, tiles_of(a), 2 * a.max_distance + 1);
+    const int rows = (a.len_k + a.kv_keys - 1) / a.kv_keys * a.q_splits;  // of a request and head
+    attn_bias_grad_kernel<<<(unsigned)a.heads, kBiasTpb, 0, s>>>(dbias, a.dist_sums, a.bucket, a.batch, a.heads,
+        a.buckets, rows, 2 * a.max_distance + 1);
     nnk_after_launch(what, s);
 }

@@ -12,7 +12,8 @@
 // too: a query that sees a single key then gets a gradient of exactly zero.
 //
 // SPLIT 2, for calls of few workgroups: 64 queries, and of each block 32 keys a wave; the
-// two waves of the same queries are added up at the end, in their order.
+// two waves of the same queries are added up at the end, in their order.  Fewer still: the
+// keys are divided too, each part leaves fp32 sums, and a second kernel adds them in order.
 #include "attn_common.h"
 
 namespace {
@@ -32,8 +33,9 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
     const int half = SPLIT > 1 ? wave / (kWaves / SPLIT) : 0, strip = wave - half * (kWaves / SPLIT);
     const int w = nnk::xcd_swizzle(blockIdx.x, gridDim.x);
-    const int tile = tiles - 1 - w % tiles;
-    const int head = w / tiles % a.heads, b = w / tiles / a.heads;
+    const int part = w % a.k_splits, group = w / a.k_splits;
+    const int tile = tiles - 1 - group % tiles;
+    const int head = group / tiles % a.heads, b = group / tiles / a.heads;
     const int row0 = tile * kOwn, row = row0 + strip * 32 + (lane & 31);
     const bool in = row < a.len_q;
     const int keys = keys_of(a, b), start = start_of(a, b);
@@ -53,7 +55,8 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn
     const int4 mine = query_docs_of(a, b, row0 / kBlock, kOwn / kBlock);
     const int blocks = (a.len_k + kBlock - 1) / kBlock;
     const int4* key_docs = a.key_docs ? a.key_docs + (size_t)b * blocks : nullptr;
-    Blocks at(0, (most + kBlock - 1) / kBlock, key_docs, mine);
+    const int each = (blocks + a.k_splits - 1) / a.k_splits;
+    Blocks at(part * each, min((most + kBlock - 1) / kBlock, (part + 1) * each), key_docs, mine);
 
     const size_t stat_at = ((size_t)b * a.heads + head) * a.len_q + row;
     const float lse = in ? a.lse[stat_at] : -INFINITY;
@@ -119,7 +122,7 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn
         load(next);
         store(next, at.negative, 0);
     }
-    bool first = true;
+    bool first = a.k_splits == 1;
     const auto step = [&](auto buf_) {
         constexpr int buf = decltype(buf_)::value;
         const int k0 = next * kBlock + half * 32, block_doc = at.doc;
@@ -265,6 +268,18 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn
         pd += y.z;
     }
     if (!in) return;
+    if (a.q_sums) {
+        const size_t at_row = ((size_t)(b * a.heads + head) * a.k_splits + part) * a.len_q + row;
+        float* sums = a.q_sums + at_row * a.dim;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                store4<float, VEC>(sums, 32 * d + 8 * g + 4 * h, a.dim, dq[d][4 * g], dq[d][4 * g + 1], dq[d][4 * g + 2],
+                    dq[d][4 * g + 3]);
+        if (h == 0) a.stat_sums[at_row] = float2{l, pd};
+        return;
+    }
     T* out = (T*)a.dq + b * a.qs[0] + (long long)row * a.qs[1] + head * a.qs[2];
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
@@ -275,19 +290,56 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn
     if (h == 0) a.stat[stat_at] = sees_any ? float2{M + log2f(l), pd / l} : float2{INFINITY, 0.0f};
 }
 
-template <typename T, int DP, bool CAP, bool BIAS, bool VEC, int SPLIT>
-bool launch_split(const Args& a, hipStream_t s, const char* what) {
-    const int tiles = (a.len_q + kRows / SPLIT - 1) / (kRows / SPLIT);
-    attn_bwd_q_kernel<T, DP, CAP, BIAS, VEC, SPLIT>
-        <<<(unsigned)((long long)tiles * a.heads * a.batch), kTpb, 0, s>>>(a, tiles);
-    nnk_after_launch(what, s);
-    return true;
+// dq and the statistics from the parts' sums, in their order; 4 features a thread.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(kTpb) void attn_q_sum_kernel(Args a, int quads, long long total) {
+    const long long n = (long long)blockIdx.x * kTpb + threadIdx.x;
+    if (n >= total) return;
+    const int d = (int)(n % quads) * 4, row = (int)(n / quads % a.len_q);
+    const long long owner = n / quads / a.len_q;
+    const int head = (int)(owner % a.heads), b = (int)(owner / a.heads);
+    const size_t first = (size_t)owner * a.k_splits * a.len_q + row;
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f}, l = 0.0f, pd = 0.0f;
+    for (int i = 0; i < a.k_splits; ++i) {
+        const size_t at = first + (size_t)i * a.len_q;
+        const float* p = a.q_sums + at * a.dim + d;
+        if constexpr (VEC) {
+            const float4 x = nnk::ld4(p);
+            v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (d + j < a.dim) v[j] += p[j];
+        }
+        if (d == 0) {
+            const float2 x = a.stat_sums[at];
+            l += x.x;
+            pd += x.y;
+        }
+    }
+    store4<T, VEC>((T*)a.dq + b * a.qs[0] + row * a.qs[1] + head * a.qs[2], d, a.dim, v[0] * a.scale, v[1] * a.scale,
+        v[2] * a.scale, v[3] * a.scale);
+    if (d == 0) {
+        const size_t at = (size_t)owner * a.len_q + row;
+        const float lse = a.lse[at];
+        a.stat[at] = lse != -INFINITY ? float2{lse * kLog2e + log2f(l), pd / l} : float2{INFINITY, 0.0f};
+    }
 }
+
 template <typename T, int DP, bool CAP, bool BIAS, bool VEC>
 bool launch(const Args& a, hipStream_t s, const char* what) {
-    const long long groups = ((long long)a.len_q + kRows - 1) / kRows * a.heads * a.batch;
-    return groups < kSplitBelow ? launch_split<T, DP, CAP, BIAS, VEC, 2>(a, s, what)
-                                : launch_split<T, DP, CAP, BIAS, VEC, 1>(a, s, what);
+    const int tiles = (a.len_q + a.q_rows - 1) / a.q_rows;
+    const unsigned groups = (unsigned)((long long)tiles * a.heads * a.batch * a.k_splits);
+    if (a.q_rows < kRows) attn_bwd_q_kernel<T, DP, CAP, BIAS, VEC, 2><<<groups, kTpb, 0, s>>>(a, tiles);
+    else attn_bwd_q_kernel<T, DP, CAP, BIAS, VEC, 1><<<groups, kTpb, 0, s>>>(a, tiles);
+    nnk_after_launch(what, s);
+    if (a.q_sums) {
+        const int quads = (a.dim + 3) / 4;
+        const long long total = (long long)a.batch * a.heads * a.len_q * quads;
+        attn_q_sum_kernel<T, VEC><<<(unsigned)((total + kTpb - 1) / kTpb), kTpb, 0, s>>>(a, quads, total);
+        nnk_after_launch(what, s);
+    }
+    return true;
 }
 
 }  // namespace

@@ -15,6 +15,7 @@ using namespace attn;
 constexpr int kKeys = 32;        // keys of a wave at a time
 constexpr int kTickets = kTicketWords;
 constexpr int kMaxSplits = 64;
+constexpr size_t kTableBytes = 16384;  // LDS for the bias by distance
 
 // 32 rows on their way from memory to a wave's LDS.
 template <typename T, int DP, bool VEC>
@@ -55,6 +56,7 @@ __device__ __forceinline__ float2 taken(const float* p) {
 struct Few {
     unsigned* tickets;
     float* partial;  // [units, splits, 32, DP + 2]: outputs, then maximum (units of log2) and sum
+    bool table;
     int tiles, splits, each;  // 32-row tiles of a key head's queries; workgroups of a unit; their keys
 };
 
@@ -70,6 +72,7 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && VEC ? 2 : 1) void attn_few_
     __shared__ float weight[32][kMaxSplits];
     __shared__ float total[32];
     __shared__ int last_one;
+    extern __shared__ float table[];  // BIAS: of each head of the tile by distance, if it fits (f.table)
 
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6, col = lane & 31;
     const int split = blockIdx.x % f.splits, unit = blockIdx.x / f.splits;
@@ -124,11 +127,22 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && VEC ? 2 : 1) void attn_few_
         ks.load(kp + k0 * a.ks[1], a.ks[1], last, a.dim);
         vs.load(vp + k0 * a.vs[1], a.vs[1], last, a.dim);
     };
-    float far = 0.0f;  // bias of keys max_distance or more before the query
-    const auto bias_at = [&](int rel) {
-        const int n = a.bucket[min(max(rel, -a.max_distance), a.max_distance) + a.max_distance];
-        return a.bias[(size_t)min(max(n, 0), a.buckets - 1) * a.heads + (in ? head : 0)] * kLog2e;
+    const int span = 2 * a.max_distance + 1;
+    const auto bias_of = [&](int i, int of_head) {
+        return a.bias[(size_t)min(max(a.bucket[i], 0), a.buckets - 1) * a.heads + of_head] * kLog2e;
     };
+    if constexpr (BIAS) {
+        if (f.table) {
+            for (int n = threadIdx.x; n < a.group * span; n += kTpb) table[n] = bias_of(n % span, kv * a.group + n / span);
+            __syncthreads();
+        }
+    }
+    const int own = in ? head - kv * a.group : 0;
+    const auto bias_at = [&](int rel) {
+        const int i = min(max(rel, -a.max_distance), a.max_distance) + a.max_distance;
+        return f.table ? table[own * span + i] : bias_of(i, kv * a.group + own);
+    };
+    float far = 0.0f;  // bias of keys max_distance or more before the query
     if constexpr (BIAS) far = bias_at(-a.max_distance);
 
     f32x16 o[DP / 32];
@@ -301,9 +315,9 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && VEC ? 2 : 1) void attn_few_
     if (threadIdx.x == 0) __hip_atomic_store(f.tickets + unit, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// How the keys are split: enough workgroups to fill the card several times over (requests'
-// lengths differ, and those without keys of theirs end at once), of 128 keys at least, a
-// block for each wave.
+// How the keys are split: where the cache's bytes count, enough workgroups to fill the card
+// several times over (requests' lengths differ, and those without keys of theirs end at
+// once); for more rows, whose products count, once.  128 keys at least, a block a wave.
 struct Plan {
     long long units;
     int tiles, splits, each;
@@ -313,7 +327,8 @@ Plan plan_of(int batch, int len_q, int len_k, int kv_heads, int group) {
     p.tiles = (int)(((long long)len_q * group + 31) / 32);
     p.units = (long long)batch * kv_heads * p.tiles;
     const int step = kWaves * kKeys, steps = std::max(1, (len_k + step - 1) / step);
-    const long long want = p.units >= kTickets ? 1 : std::min<long long>(kMaxSplits, (2 * kTickets + p.units - 1) / p.units);
+    const long long fill = p.tiles <= 2 ? 2 * kTickets : 3 * kCus;
+    const long long want = p.units >= kTickets ? 1 : std::min<long long>(kMaxSplits, (fill + p.units - 1) / p.units);
     const int n = (int)((steps + want - 1) / want);
     p.each = n * step;
     p.splits = (steps + n - 1) / n;
@@ -323,17 +338,26 @@ Plan plan_of(int batch, int len_q, int len_k, int kv_heads, int group) {
 template <typename T, int DP, bool CAP, bool BIAS, bool VEC>
 bool launch(const Args& a, float* ws, hipStream_t s, const char* what) {
     const Plan p = plan_of(a.batch, a.len_q, a.len_k, a.kv_heads, a.group);
-    const Few f = {reinterpret_cast<unsigned*>(ws), ws + kTickets, p.tiles, p.splits, p.each};
-    attn_few_kernel<T, DP, CAP, BIAS, VEC><<<(unsigned)(p.units * p.splits), kTpb, 0, s>>>(a, f);
+    const size_t table = BIAS ? (size_t)a.group * (2 * a.max_distance + 1) * sizeof(float) : 0;
+    const Few f = {reinterpret_cast<unsigned*>(ws), ws + kTickets, table && table <= kTableBytes, p.tiles, p.splits, p.each};
+    if constexpr (BIAS) {
+        static std::atomic<unsigned long long> done{0};
+        if (!raise_lds((const void*)attn_few_kernel<T, DP, CAP, BIAS, VEC>, kTableBytes, done, what)) return false;
+    }
+    attn_few_kernel<T, DP, CAP, BIAS, VEC>
+        <<<(unsigned)(p.units * p.splits), kTpb, f.table ? table : 0, s>>>(a, f);
     nnk_after_launch(what, s);
     return true;
 }
 
 }  // namespace
 
-// Few queries: the rows of a key head's queries fit in two tiles.
+// Few queries: the rows of a key head's queries fit in two tiles; or workgroups of 64 would
+// leave half of the CUs without work while each goes over many keys.
 bool nnk_attention_is_few(const NnAttention* a) {
-    return (long long)a->len_q * (a->heads / a->kv_heads) <= 64 && (long long)a->batch * a->kv_heads < 1 << 20;
+    const long long rows = (long long)a->len_q * (a->heads / a->kv_heads);
+    const long long groups = ((long long)a->len_q + 63) / 64 * a->heads * a->batch;
+    return (rows <= 64 && (long long)a->batch * a->kv_heads < 1 << 20) || (groups < kCus / 2 && a->len_k >= 512);
 }
 // Floats of the workspace after the tickets.
 size_t nnk_attention_few_floats(const NnAttention* a) {
