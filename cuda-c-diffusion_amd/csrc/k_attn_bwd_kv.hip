@@ -20,6 +20,9 @@
 // row m's values go m lanes along, after which a lane holds two distances (one for what
 // went past the end), and the tile is 32 shuffles and adds and one addition to the
 // wave's table in LDS.  Tiles wholly past max_distance are added up whole.
+//
+// Measured, as the query gradients: 281 us and 91 us (the bias's distances are a third of
+// the latter); two waves a SIMD up to 64 features (177 us without), one above.
 #include "attn_common.h"
 
 namespace {

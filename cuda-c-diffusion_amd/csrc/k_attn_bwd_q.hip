@@ -14,6 +14,10 @@
 // SPLIT 2, for calls of few workgroups: 64 queries, and of each block 32 keys a wave; the
 // two waves of the same queries are added up at the end, in their order.  Fewer still: the
 // keys are divided too, each part leaves fp32 sums, and a second kernel adds them in order.
+//
+// Measured: 8192 packed causal tokens, 16 heads of 128 (4 of keys), capped: 236 us; 4 x 1024
+// tokens, 16 heads of 64 with a bias: 53 us.  128 features take one wave a SIMD, whose
+// products (13 % of cycles) and vector instructions (35 %) do not overlap.
 #include "attn_common.h"
 
 namespace {

