@@ -383,6 +383,25 @@ def test_enough_workgroups_for_whole_tiles(nn, L, rng, dtype, mask, cap, buckets
                          buckets=buckets, max_distance=40, **({"doc_q": doc, "doc_k": doc} if mask != "none" else {})))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("len_q, len_k, heads, kv, dim, mask, cap, buckets, docs, layout", [
+    (900, 1100, 1, 1, 72, "prefix", 20.0, 0, False, "plain"),
+    (1030, 1030, 2, 1, 33, "causal", 0.0, 0, False, "odd"),
+    (777, 777, 3, 3, 128, "none", 0.0, 12, True, "packed"),
+    (70, 2500, 2, 2, 64, "causal", 3.0, 40, False, "cache"),
+    (2500, 70, 4, 2, 24, "none", 0.0, 0, False, "plain"),
+    (1200, 1200, 2, 2, 40, "causal", 0.0, 0, True, "plain"),
+])
+def test_long_axes_in_parts(nn, L, rng, dtype, len_q, len_k, heads, kv, dim, mask, cap, buckets, docs, layout):
+    """Few heads and long sequences: the other axis is divided over workgroups, some of which have nothing."""
+    more = {}
+    if docs:
+        doc = np.sort(rng.integers(-1, 5, (1, len_q)), axis=1)
+        more = {"doc_q": doc, "doc_k": doc}
+    run(nn, L, rng, case(dtype, 1, len_q, len_k, heads, kv, dim, mask, cap, prefix=[len_k // 3], buckets=buckets,
+                         max_distance=50, **more), layout)
+
+
 def test_large_scores_and_infinite_bias(nn, L, rng):
     """Scores of hundreds (one key takes all), and a bias of -inf, which hides its bucket."""
     c = case("f32", 1, 80, 80, 2, 2, 16, scale=40.0)
