@@ -11,7 +11,12 @@ constexpr long long kMostGroups = (1LL << 31) - 1;
 size_t docs_floats(const NnAttention* a) {
     if (!a->doc_q) return 0;
     const size_t nk = ((size_t)a->len_k + kBlock - 1) / kBlock, nq = ((size_t)a->len_q + kBlock - 1) / kBlock;
-    return 4 * (size_t)a->batch * (nk + nq);
+    // with the orders of tiles of 64 positions or more
+    return 4 * (size_t)a->batch * (nk + nq) + ((size_t)a->batch * (nk + nq) + 3) / 4 * 4;
+}
+float* order_of(const NnAttention* a, float* docs, bool keys) {
+    const size_t nk = ((size_t)a->len_k + kBlock - 1) / kBlock, nq = ((size_t)a->len_q + kBlock - 1) / kBlock;
+    return docs + 4 * a->batch * (nk + nq) + (keys ? a->batch * nq : 0);
 }
 // How the gradients are divided over workgroups.  Key heads that are shared and few tiles of
 // keys: the heads apart.  Few workgroups even so: tiles of 64, and the other axis in parts of
@@ -30,6 +35,13 @@ void divide(Args& p, const NnAttention* a) {
     p.q_splits = parts(up(a->len_k, p.kv_keys) * owners, up(a->len_q, kBlock));
     p.q_rows = up(a->len_q, kRows) * heads * batch < kSplitBelow ? kRows / 2 : kRows;
     p.k_splits = parts(up(a->len_q, p.q_rows) * heads * batch, up(a->len_k, kBlock));
+}
+// Whether tiles are dealt out by their work: where a launch of a few microseconds more is
+// little, and CUs take several.
+bool worth_order(const Args& p, const NnAttention* a, bool keys) {
+    const long long own = keys ? p.kv_keys : p.q_rows, len = keys ? a->len_k : a->len_q;
+    const long long owners = keys ? (long long)a->heads / p.heads_each * p.q_splits : (long long)a->heads * p.k_splits;
+    return (len + own - 1) / own * owners * a->batch >= 2 * kCus;
 }
 size_t by4(size_t n) { return (n + 3) / 4 * 4; }
 size_t kv_floats(const NnAttention* a, const Args& p) {
@@ -152,8 +164,12 @@ void launch_attention_forward(void* out, float* lse, const void* q, const void* 
     p.lse = lse;
     p.vec = strides_by_16(a) && nnk::aligned16(q) && nnk::aligned16(k) && nnk::aligned16(v) && nnk::aligned16(out);
     const bool few = nnk_attention_is_few(a);
-    if (a->doc_q)
-        nnk_attention_docs(p, workspace + kTicketWords + (few ? nnk_attention_few_floats(a) : 0), s, what);
+    divide(p, a);
+    if (a->doc_q) {
+        float* docs = workspace + kTicketWords + (few ? nnk_attention_few_floats(a) : 0);
+        nnk_attention_docs(p, docs, s, what);
+        if (!few && worth_order(p, a, false)) p.row_order = nnk_attention_order(p, false, p.q_rows, order_of(a, docs, false), s, what);
+    }
     if (few) nnk_attention_few(p, a->dtype == NN_BF16, workspace, s, what);
     else nnk_attention_forward(p, a->dtype == NN_BF16, s, what);
 }
@@ -202,7 +218,11 @@ void launch_attention_backward(void* dq, void* dk, void* dv, float* dbias, const
     p.stat = reinterpret_cast<float2*>(ws);
     if (dbias) p.dist_sums = ws + by4(stat_floats(a));
     const bool half = a->dtype == NN_BF16;
-    if (has_q && has_k) nnk_attention_docs(p, workspace, s, what);
+    if (has_q && has_k && a->doc_q) {
+        nnk_attention_docs(p, workspace, s, what);
+        if (worth_order(p, a, false)) p.row_order = nnk_attention_order(p, false, p.q_rows, order_of(a, workspace, false), s, what);
+        if (worth_order(p, a, true)) p.key_order = nnk_attention_order(p, true, p.kv_keys, order_of(a, workspace, true), s, what);
+    }
     if (has_q && !nnk_attention_backward_q(p, half, s, what)) return;
     if (has_k && !nnk_attention_backward_kv(p, half, s, what)) return;
     if (dbias) nnk_attention_bias_grad(p, dbias, s, what);

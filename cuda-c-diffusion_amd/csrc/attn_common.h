@@ -306,6 +306,7 @@ struct Args {
     float2* stat_sums;                  // sums of p and of p dp [batch, heads, k_splits, len_q]
     const int4* key_docs;    // per block of 64 keys: least and largest document, whether any is negative
     const int4* query_docs;  // per block of 64 queries
+    const int *row_order, *key_order;  // with documents: tiles of a request by falling work, or null
     long long qs[3], ks[3], vs[3], os[3];
     int batch, len_q, len_k, heads, kv_heads, group, dim;
     int mask, buckets, max_distance;
@@ -519,6 +520,33 @@ struct Blocks {
     }
 };
 
+// What a workgroup of `owners` (heads, or parts, of all requests) times `tiles` takes.
+// Without an order of the tiles each XCD has its own owners, one after another.  With one,
+// the owners of an XCD (of all, if they do not divide) take turns at the tiles of most work:
+// uneven tiles started in their own order kept the CUs busy two thirds of the time (8192
+// packed tokens: forward 101 -> 83 us, a training step 704 -> 597 us with three launches for
+// the orders).
+struct Turn {
+    int owner, tile;
+};
+__device__ __forceinline__ Turn turn_of(int block, int blocks, int owners_each, int tiles, const int* order, bool last_first) {
+    const int owners = blocks / tiles;
+    if (!order) {
+        const int w = nnk::xcd_swizzle(block, blocks), t = w % tiles;
+        return {w / tiles, last_first ? tiles - 1 - t : t};
+    }
+    int owner, rank;
+    if (owners % nnk::kNumXcd == 0) {
+        const int own = owners / nnk::kNumXcd, k = block / nnk::kNumXcd;
+        owner = block % nnk::kNumXcd * own + k % own;
+        rank = k / own;
+    } else {
+        owner = block % owners;
+        rank = block / owners;
+    }
+    return {owner, order[owner / owners_each * tiles + rank]};
+}
+
 // Raises kernel fn's limit of dynamic LDS to `bytes` on the current device, once a
 // device (`done` has a bit for each).  False after recording an error.
 inline bool raise_lds(const void* fn, size_t bytes, std::atomic<unsigned long long>& done, const char* what) {
@@ -540,6 +568,9 @@ inline bool raise_lds(const void* fn, size_t bytes, std::atomic<unsigned long lo
 // Documents of each block of 64 into `ws`, for args.key_docs and query_docs (no documents:
 // nothing).
 void nnk_attention_docs(attn::Args& args, float* ws, hipStream_t s, const char* what);
+// Tiles of `own` queries (or keys) of each request by falling work into `order`; null if
+// there are too many to be worth it.
+const int* nnk_attention_order(const attn::Args& args, bool keys, int own, float* order, hipStream_t s, const char* what);
 // One launch each; `half`: bf16.  False after recording an error.
 bool nnk_attention_forward(const attn::Args& args, bool half, hipStream_t s, const char* what);
 bool nnk_attention_backward_q(const attn::Args& args, bool half, hipStream_t s, const char* what);

@@ -21,7 +21,7 @@
 // went past the end), and the tile is 32 shuffles and adds and one addition to the
 // wave's table in LDS.  Tiles wholly past max_distance are added up whole.
 //
-// Measured, as the query gradients: 281 us and 91 us (the bias's distances are a third of
+// Measured, as the query gradients: 243 us and 91 us (the bias's distances are a third of
 // the latter); two waves a SIMD up to 64 features (177 us without), one above.
 #include "attn_common.h"
 
@@ -48,9 +48,9 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn
 
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
     const int half = SPLIT > 1 ? wave / (kWaves / SPLIT) : 0, strip = wave - half * (kWaves / SPLIT);
-    const int w = nnk::xcd_swizzle(blockIdx.x, gridDim.x);
     const int parts = a.heads / a.heads_each * a.q_splits;
-    const int tile = w % tiles, part = w / tiles % parts, b = w / tiles / parts;
+    const Turn turn = turn_of(blockIdx.x, gridDim.x, parts, tiles, a.key_order, false);
+    const int tile = turn.tile, part = turn.owner % parts, b = turn.owner / parts;
     const int share = part % a.q_splits, head0 = part / a.q_splits * a.heads_each, kv = head0 / a.group;
     const int k0 = tile * kOwn, first_key = k0 + strip * 32, key = first_key + (lane & 31);
     const int keys = keys_of(a, b), start = start_of(a, b);

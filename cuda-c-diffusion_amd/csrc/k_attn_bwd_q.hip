@@ -15,7 +15,7 @@
 // two waves of the same queries are added up at the end, in their order.  Fewer still: the
 // keys are divided too, each part leaves fp32 sums, and a second kernel adds them in order.
 //
-// Measured: 8192 packed causal tokens, 16 heads of 128 (4 of keys), capped: 236 us; 4 x 1024
+// Measured: 8192 packed causal tokens, 16 heads of 128 (4 of keys), capped: 203 us; 4 x 1024
 // tokens, 16 heads of 64 with a bias: 53 us.  128 features take one wave a SIMD, whose
 // products (13 % of cycles) and vector instructions (35 %) do not overlap.
 #include "attn_common.h"
@@ -36,10 +36,9 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn
 
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
     const int half = SPLIT > 1 ? wave / (kWaves / SPLIT) : 0, strip = wave - half * (kWaves / SPLIT);
-    const int w = nnk::xcd_swizzle(blockIdx.x, gridDim.x);
-    const int part = w % a.k_splits, group = w / a.k_splits;
-    const int tile = tiles - 1 - group % tiles;
-    const int head = group / tiles % a.heads, b = group / tiles / a.heads;
+    const int part = blockIdx.x % a.k_splits;
+    const Turn turn = turn_of(blockIdx.x / a.k_splits, gridDim.x / a.k_splits, a.heads, tiles, a.row_order, true);
+    const int tile = turn.tile, head = turn.owner % a.heads, b = turn.owner / a.heads;
     const int row0 = tile * kOwn, row = row0 + strip * 32 + (lane & 31);
     const bool in = row < a.len_q;
     const int keys = keys_of(a, b), start = start_of(a, b);

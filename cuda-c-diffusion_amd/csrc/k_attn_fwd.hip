@@ -24,7 +24,7 @@
 // Measured: 16384 tokens, 16 heads of 128 (4 of keys), a prefix, capped scores: 1500 us, 779
 // TFLOP/s of visible scores; vector instructions take 45 %, products 31 % of the SIMDs'
 // cycles, two waves a SIMD overlapping a third of the latter.  8192 packed tokens, 16 heads
-// of 72, 13 documents: 101 us, 279 TFLOP/s, uneven documents.
+// of 72, 13 documents: 83 us, 338 TFLOP/s, two launches for the documents among it.
 #include "attn_common.h"
 
 namespace {
@@ -52,9 +52,8 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && VEC ? 2 : 1) void attn_fwd_
 
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
     const int half = SPLIT > 1 ? wave / (kWaves / SPLIT) : 0, strip = wave - half * (kWaves / SPLIT);
-    const int w = nnk::xcd_swizzle(blockIdx.x, gridDim.x);
-    const int tile = tiles - 1 - w % tiles;  // those that see most keys first
-    const int head = w / tiles % a.heads, b = w / tiles / a.heads;
+    const Turn turn = turn_of(blockIdx.x, gridDim.x, a.heads, tiles, a.row_order, true);  // those that see most keys first
+    const int tile = turn.tile, head = turn.owner % a.heads, b = turn.owner / a.heads;
     const int row0 = tile * kOwn, row = row0 + strip * 32 + (lane & 31);
     const bool in = row < a.len_q;
     const int keys = keys_of(a, b), start = start_of(a, b);
@@ -329,9 +328,8 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && VEC ? 2 : 1) void attn_fwd_
 
 template <typename T, int DP, int CAP, bool BIAS, bool VEC>
 bool launch_split(const Args& a, hipStream_t s, const char* what) {
-    const long long groups = ((long long)a.len_q + kRows - 1) / kRows * a.heads * a.batch;
-    const bool split = groups < kSplitBelow;
-    const int own = split ? kRows / 2 : kRows, tiles = (a.len_q + own - 1) / own;
+    const int own = a.q_rows, tiles = (a.len_q + own - 1) / own;
+    const bool split = own < kRows;
     const unsigned blocks = (unsigned)((long long)tiles * a.heads * a.batch);
     if (split) attn_fwd_kernel<T, DP, CAP, BIAS, VEC, 2><<<blocks, kTpb, 0, s>>>(a, tiles);
     else attn_fwd_kernel<T, DP, CAP, BIAS, VEC, 1><<<blocks, kTpb, 0, s>>>(a, tiles);
@@ -360,6 +358,37 @@ __global__ __launch_bounds__(64) void block_docs_kernel(int4* out, const int* do
     if (threadIdx.x == 0) out[blockIdx.x] = int4{lo, hi, negative, 0};
 }
 
+// A request's tiles of `own` positions by falling number of blocks that they meet on the
+// other axis, ties by their number.
+constexpr int kOrderTpb = 1024, kOrderBlocks = 1024, kOrderTiles = 512;
+__global__ __launch_bounds__(kOrderTpb) void tile_order_kernel(int* order, Args a, bool keys, int own, int tiles) {
+    __shared__ int4 other[kOrderBlocks];
+    __shared__ int4 mine[kOrderTiles];
+    __shared__ int work[kOrderTiles];
+    const int b = blockIdx.x, nq = (a.len_q + kBlock - 1) / kBlock, nk = (a.len_k + kBlock - 1) / kBlock;
+    const int blocks = keys ? nq : nk, held = keys_of(a, b), start = start_of(a, b);
+    for (int i = threadIdx.x; i < blocks; i += kOrderTpb)
+        other[i] = keys ? a.query_docs[(size_t)b * nq + i] : a.key_docs[(size_t)b * nk + i];
+    for (int t = threadIdx.x; t < tiles; t += kOrderTpb) {
+        const int first = t * own / kBlock, count = own / kBlock;
+        mine[t] = keys ? key_docs_of(a, b, first, count) : query_docs_of(a, b, first, count);
+        work[t] = 0;
+    }
+    __syncthreads();
+    for (int n = threadIdx.x; n < tiles * blocks; n += kOrderTpb) {
+        const int t = n / blocks, i = n - t * blocks;
+        // the last query of the tile or block, and the first key of the block or tile
+        const int q = keys ? min((i + 1) * kBlock, a.len_q) - 1 : min((t + 1) * own, a.len_q) - 1, k = keys ? t * own : i * kBlock;
+        if (docs_meet(other[i], mine[t]) && k < limit_of(a, b, held, start + q)) atomicAdd(&work[t], 1);
+    }
+    __syncthreads();
+    for (int t = threadIdx.x; t < tiles; t += kOrderTpb) {
+        int rank = 0;
+        for (int u = 0; u < tiles; ++u) rank += work[u] > work[t] || (work[u] == work[t] && u < t);
+        order[b * tiles + rank] = t;
+    }
+}
+
 }  // namespace
 
 bool nnk_attention_forward(const Args& a, bool half, hipStream_t s, const char* what) {
@@ -380,4 +409,14 @@ void nnk_attention_docs(Args& a, float* ws, hipStream_t s, const char* what) {
     if (a.doc_q == a.doc_k && a.len_q == a.len_k) return;
     a.query_docs = out += (size_t)a.batch * nk;
     blocks_of(out, a.doc_q, a.len_q, nq);
+}
+
+const int* nnk_attention_order(const Args& a, bool keys, int own, float* order, hipStream_t s, const char* what) {
+    const int len = keys ? a.len_k : a.len_q, tiles = (len + own - 1) / own;
+    const int blocks = ((keys ? a.len_q : a.len_k) + kBlock - 1) / kBlock;
+    if (tiles < 2 || tiles > kOrderTiles || blocks > kOrderBlocks || tiles * blocks > 64 * kOrderTpb) return nullptr;
+    int* to = reinterpret_cast<int*>(order);
+    tile_order_kernel<<<(unsigned)a.batch, kOrderTpb, 0, s>>>(to, a, keys, own, tiles);
+    nnk_after_launch(what, s);
+    return to;
 }

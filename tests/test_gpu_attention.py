@@ -384,6 +384,16 @@ def test_enough_workgroups_for_whole_tiles(nn, L, rng, dtype, mask, cap, buckets
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("mask", ["none", "causal", "prefix"])
+def test_tiles_dealt_out_by_their_work(nn, L, rng, dtype, mask):
+    """Documents and as many workgroups as make an order of the tiles worth it, heads that do not divide over XCDs."""
+    doc = np.sort(rng.integers(-1, 6, (60, 130)), axis=1)
+    doc[7], doc[8] = -1, rng.integers(0, 3, 130)
+    run(nn, L, rng, case(dtype, 60, 130, 130, 3, 3, 16, mask, prefix=[40] * 60, doc_q=doc, doc_k=doc,
+                         k_len=[0] + [130] * 58 + [77]), "packed")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("len_q, len_k, heads, kv, dim, mask, cap, buckets, docs, layout", [
     (900, 1100, 1, 1, 72, "prefix", 20.0, 0, False, "plain"),
     (1030, 1030, 2, 1, 33, "causal", 0.0, 0, False, "odd"),
