@@ -58,6 +58,29 @@ size_t dist_floats(const NnAttention* a, const Args& p) {
 }
 size_t stat_floats(const NnAttention* a) { return 2 * (size_t)a->batch * a->heads * a->len_q; }
 
+// Floats of one call.
+size_t forward_floats(const NnAttention* a) {
+    if (!a->batch || !a->len_q) return 0;
+    const size_t n = docs_floats(a) + (nnk_attention_is_few(a) ? nnk_attention_few_floats(a) : 0);
+    return n ? kTicketWords + n : 0;
+}
+size_t backward_floats(const NnAttention* a) {
+    Args p;
+    divide(p, a);
+    return docs_floats(a) + kv_floats(a, p) + q_floats(a, p) + by4(stat_floats(a)) +
+        (a->buckets ? dist_floats(a, p) : 0);
+}
+// The most that the call or one of a smaller batch takes: fewer requests are divided into
+// more parts, and a program's workspace has its largest batch's size.  (Past 4096 requests
+// of a smaller batch nothing is divided.)
+template <typename Floats>
+size_t of_smaller_batches(const NnAttention* a, const Floats& floats) {
+    NnAttention x = *a;
+    size_t most = floats(a);
+    for (x.batch = 1; x.batch < std::min(a->batch, 4096); ++x.batch) most = std::max(most, floats(&x));
+    return most;
+}
+
 bool sizes_fit(const NnAttention* a, const char* what) {
     NNK_REQUIRE_RET(a, false, what, "%s: null description", what);
     NNK_REQUIRE_RET(a->dtype == NN_F32 || a->dtype == NN_BF16, false, what, "%s: unknown dtype %d", what, a->dtype);
@@ -143,9 +166,7 @@ extern "C" {
 
 size_t nnhip_attention_forward_workspace(const NnAttention* a) {
     if (!sizes_fit(a, "nnhip_attention_forward_workspace")) return 0;
-    if (!a->batch || !a->len_q) return 0;
-    const size_t n = docs_floats(a) + (nnk_attention_is_few(a) ? nnk_attention_few_floats(a) : 0);
-    return n ? kTicketWords + n : 0;
+    return of_smaller_batches(a, forward_floats);
 }
 
 void launch_attention_forward(void* out, float* lse, const void* q, const void* k, const void* v,
@@ -155,7 +176,7 @@ void launch_attention_forward(void* out, float* lse, const void* q, const void* 
     if (!take(p, a, what)) return;
     if (!a->batch || !a->len_q) return;
     NNK_REQUIRE(out && lse && q && (!a->len_k || (k && v)), what, "%s: null pointer", what);
-    NNK_REQUIRE(!nnhip_attention_forward_workspace(a) || workspace, what, "%s: null workspace", what);
+    NNK_REQUIRE(!forward_floats(a) || workspace, what, "%s: null workspace", what);
     NNK_REQUIRE(nnk::aligned16(workspace), what, "%s: workspace is not aligned to 16 bytes", what);
     p.q = q;
     p.k = k;
@@ -176,10 +197,7 @@ void launch_attention_forward(void* out, float* lse, const void* q, const void* 
 
 size_t nnhip_attention_backward_workspace(const NnAttention* a) {
     if (!sizes_fit(a, "nnhip_attention_backward_workspace")) return 0;
-    Args p;
-    divide(p, a);
-    return docs_floats(a) + kv_floats(a, p) + q_floats(a, p) + by4(stat_floats(a)) +
-        (a->buckets ? dist_floats(a, p) : 0);
+    return of_smaller_batches(a, backward_floats);
 }
 
 void launch_attention_backward(void* dq, void* dk, void* dv, float* dbias, const void* dout,
@@ -192,7 +210,7 @@ void launch_attention_backward(void* dq, void* dk, void* dv, float* dbias, const
     const bool has_q = a->batch && a->len_q, has_k = a->batch && a->len_k;
     NNK_REQUIRE(!has_q || (dq && dout && q && out && lse), what, "%s: null pointer of the queries", what);
     NNK_REQUIRE(!has_k || (dk && dv && k && v), what, "%s: null pointer of the keys", what);
-    NNK_REQUIRE(!nnhip_attention_backward_workspace(a) || workspace, what, "%s: null workspace", what);
+    NNK_REQUIRE(!(has_q || has_k) || workspace, what, "%s: null workspace", what);
     NNK_REQUIRE(nnk::aligned16(workspace), what, "%s: workspace is not aligned to 16 bytes", what);
     p.q = q;
     p.k = k;

@@ -118,15 +118,17 @@ typedef struct {
 
 /* out, lse [batch, heads, len_q].  `workspace`: nnhip_attention_forward_workspace
    floats (NULL if that is 0), zero-filled before its first use; every launch leaves
-   it fit for the next, also of another shape that it is large enough for.  Launches
-   that may run concurrently need separate workspaces. */
+   it fit for the next, also of another shape that it is large enough for; its size
+   serves every smaller batch.  Launches that may run concurrently need separate
+   workspaces. */
 size_t nnhip_attention_forward_workspace(const NnAttention* a);
 void launch_attention_forward(void* out, float* lse, const void* q, const void* k, const void* v,
     const NnAttention* a, float* workspace, hipStream_t s);
 
 /* dq, dk, dv (layouts of q, k, v) and dbias [buckets, heads] (NULL if not wanted)
    from dout, the forward pass's inputs and its out and lse.  All are overwritten.
-   `workspace`: nnhip_attention_backward_workspace floats, nothing to be filled. */
+   `workspace`: nnhip_attention_backward_workspace floats (they serve every smaller
+   batch), nothing to be filled. */
 size_t nnhip_attention_backward_workspace(const NnAttention* a);
 void launch_attention_backward(void* dq, void* dk, void* dv, float* dbias, const void* dout,
     const void* q, const void* k, const void* v, const void* out, const float* lse,

@@ -124,6 +124,17 @@ def test_rope_null_pointers(nn):
         L.launch_qk_norm_rope_backward(*[DUMMY] * 8, a, None, None)
 
 
+@pytest.mark.parametrize("len_q, len_k, heads, kv, buckets", [(1, 3000, 8, 2, 0), (1500, 1500, 1, 1, 0), (700, 700, 8, 2, 8),
+                                                              (130, 4000, 2, 2, 4), (5, 5, 1, 1, 0)])
+def test_workspaces_serve_smaller_batches(nn, len_q, len_k, heads, kv, buckets):
+    """Fewer requests are divided into more parts; the reported sizes may not fall as the batch grows."""
+    L = nn.lib()
+    for size in (L.nnhip_attention_forward_workspace, L.nnhip_attention_backward_workspace):
+        sizes = [size(_attn(nn, batch=b, len_q=len_q, len_k=len_k, heads=heads, kv_heads=kv, buckets=buckets,
+                            max_distance=buckets, bucket=DUMMY, bias=DUMMY)) for b in list(range(1, 200)) + [1000, 3000]]
+        assert sizes == sorted(sizes)
+
+
 def test_nothing_to_do(nn):
     L = nn.lib()
     L.last_error()
