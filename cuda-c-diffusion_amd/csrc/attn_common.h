@@ -415,13 +415,14 @@ __device__ __forceinline__ void cap_scores(f32x16& s, f32x16& slope, const Args&
 }
 
 // Entries of a keys x queries tile that this lane's query does not see become -inf: keys
-// from `limit` on and, with documents (`docs`: the tile's 32 keys', in LDS), of others than
-// `doc`.  No branches: a tile's border is a few of these, not a path of its own.
+// from `limit` on and, with documents (`docs`: the tile's 32 keys', in LDS, -1 for every
+// negative one), of others than `doc`.  No branches: a tile's border is a few of these, not a
+// path of its own.
 __device__ __forceinline__ void hide(f32x16& s, int k0, int limit, const int* docs, int doc, int h) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = k0 + row_of(r, h) < limit ? s[r] : -INFINITY;
     if (docs) {
-        const int own = doc >= 0 ? doc : -2;  // -1 is a key of no document
+        const int own = doc >= 0 ? doc : -2;  // no key has this
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int4 d = *reinterpret_cast<const int4*>(docs + 8 * g + 4 * h);

@@ -109,7 +109,7 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attn
         const bool all = k0 + kBlock <= keys && !negative;
         ks.store(k_lds[to], all, keep);
         vs.store(v_lds[to], all, keep);
-        if (docs && wave == 0) doc_lds[to][lane] = k0 + lane < keys ? next_doc : -1;
+        if (docs && wave == 0) doc_lds[to][lane] = k0 + lane < keys ? max(next_doc, -1) : -1;
     };
 
     f32x16 dq[DP / 32];

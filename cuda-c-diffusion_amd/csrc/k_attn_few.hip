@@ -165,7 +165,7 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && VEC ? 2 : 1) void attn_few_
         const bool all = at + kKeys <= keys && !docs;
         ks.store(k_lds, all, keep);
         vs.store(v_lds, all, keep);
-        if (docs && h == 0) doc_lds[wave][col] = at + col < keys ? next_doc : -1;
+        if (docs && h == 0) doc_lds[wave][col] = at + col < keys ? max(next_doc, -1) : -1;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
         k0 = meeting(at + kKeys);

@@ -108,7 +108,7 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && VEC ? 2 : 1) void attn_fwd_
         const bool all = k0 + kBlock <= keys && !negative;
         ks.store(k_lds[to], all, keep);
         vs.store(v_lds[to], all, keep);
-        if (docs && wave == 0) doc_lds[to][lane] = k0 + lane < keys ? next_doc : -1;
+        if (docs && wave == 0) doc_lds[to][lane] = k0 + lane < keys ? max(next_doc, -1) : -1;
     };
 
     f32x16 o[DP / 32];
