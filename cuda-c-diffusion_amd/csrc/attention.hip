@@ -52,33 +52,37 @@ size_t q_floats(const NnAttention* a, const Args& p) {
     const size_t rows = (size_t)a->batch * a->heads * p.k_splits * a->len_q;
     return p.k_splits > 1 ? by4(2 * rows) + by4(rows * a->head_dim) : 0;
 }
-size_t dist_floats(const NnAttention* a, const Args& p) {
-    const size_t tiles = ((size_t)a->len_k + p.kv_keys - 1) / p.kv_keys;
-    return (size_t)a->batch * a->heads * p.q_splits * tiles * (2 * a->max_distance + 1);
-}
 size_t stat_floats(const NnAttention* a) { return 2 * (size_t)a->batch * a->heads * a->len_q; }
 
-// Floats of one call.
+// Floats that one forward call takes.
 size_t forward_floats(const NnAttention* a) {
     if (!a->batch || !a->len_q) return 0;
     const size_t n = docs_floats(a) + (nnk_attention_is_few(a) ? nnk_attention_few_floats(a) : 0);
     return n ? kTicketWords + n : 0;
 }
-size_t backward_floats(const NnAttention* a) {
-    Args p;
-    divide(p, a);
-    return docs_floats(a) + kv_floats(a, p) + q_floats(a, p) + by4(stat_floats(a)) +
-        (a->buckets ? dist_floats(a, p) : 0);
+// What a program lends: enough for the call and for each one of a smaller batch or of shorter
+// lengths, which may take more (fewer requests or tokens are divided into more parts).  A
+// program's workspaces have the sizes of its largest call.  So bounds over all of them, each
+// of which grows with the batch and both lengths.
+size_t forward_most(const NnAttention* a) {
+    const size_t n = a->batch && a->len_q ? docs_floats(a) + nnk_attention_few_most(a) : 0;
+    return n ? kTicketWords + n : 0;
 }
-// The most that the call or one of a smaller batch takes: fewer requests are divided into
-// more parts, and a program's workspace has its largest batch's size.  (Past 4096 requests
-// of a smaller batch nothing is divided.)
-template <typename Floats>
-size_t of_smaller_batches(const NnAttention* a, const Floats& floats) {
-    NnAttention x = *a;
-    size_t most = floats(a);
-    for (x.batch = 1; x.batch < std::min(a->batch, 4096); ++x.batch) most = std::max(most, floats(&x));
-    return most;
+size_t backward_most(const NnAttention* a) {
+    const auto up = [](long long n, long long d) { return (n + d - 1) / d; };
+    const long long batch = a->batch, heads = a->heads, len_q = a->len_q, len_k = a->len_k;
+    const long long q_parts = up(len_q, kBlock) / 4, k_parts = up(len_k, kBlock) / 4;
+    // an axis in parts: up to two workgroups a CU, of half of kRows rows each (divide())
+    constexpr long long kParted = 2 * kCus * (kRows / 2);
+    const long long kv_rows = std::max(
+        heads > a->kv_heads ? heads * std::min(batch * len_k, 4LL * kCus * kRows / a->kv_heads) : 0,
+        q_parts > 1 ? std::min(kParted, batch * heads * len_k * q_parts) : 0);
+    const long long q_rows = k_parts > 1 ? std::min(kParted, batch * heads * len_q * k_parts) : 0;
+    // tables of distances: of halves of kRows keys below kSplitBelow workgroups
+    const long long tables = std::max(std::min(2LL * kSplitBelow, batch * heads * up(len_k, kRows / 2) * std::max(1LL, q_parts)),
+        batch * heads * up(len_k, kRows));
+    return docs_floats(a) + by4(2 * kv_rows * a->head_dim) + by4(2 * q_rows) + by4(q_rows * a->head_dim) +
+        by4(stat_floats(a)) + (a->buckets ? (size_t)tables * (2 * a->max_distance + 1) : 0);
 }
 
 bool sizes_fit(const NnAttention* a, const char* what) {
@@ -166,7 +170,7 @@ extern "C" {
 
 size_t nnhip_attention_forward_workspace(const NnAttention* a) {
     if (!sizes_fit(a, "nnhip_attention_forward_workspace")) return 0;
-    return of_smaller_batches(a, forward_floats);
+    return forward_most(a);
 }
 
 void launch_attention_forward(void* out, float* lse, const void* q, const void* k, const void* v,
@@ -197,7 +201,7 @@ void launch_attention_forward(void* out, float* lse, const void* q, const void* 
 
 size_t nnhip_attention_backward_workspace(const NnAttention* a) {
     if (!sizes_fit(a, "nnhip_attention_backward_workspace")) return 0;
-    return of_smaller_batches(a, backward_floats);
+    return backward_most(a);
 }
 
 void launch_attention_backward(void* dq, void* dk, void* dv, float* dbias, const void* dout,

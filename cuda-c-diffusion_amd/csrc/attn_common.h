@@ -576,9 +576,11 @@ const int* nnk_attention_order(const attn::Args& args, bool keys, int own, float
 bool nnk_attention_forward(const attn::Args& args, bool half, hipStream_t s, const char* what);
 bool nnk_attention_backward_q(const attn::Args& args, bool half, hipStream_t s, const char* what);
 bool nnk_attention_backward_kv(const attn::Args& args, bool half, hipStream_t s, const char* what);
-// The form for few queries; when it is taken; the floats that it needs after the tickets.
+// The form for few queries; when it is taken; the floats that it needs after the tickets, and
+// a bound on them for every smaller batch and shorter lengths.
 bool nnk_attention_is_few(const NnAttention* a);
 size_t nnk_attention_few_floats(const NnAttention* a);
+size_t nnk_attention_few_most(const NnAttention* a);
 bool nnk_attention_few(const attn::Args& args, bool half, float* ws, hipStream_t s, const char* what);
 // Bias gradient from args.dist_sums.
 void nnk_attention_bias_grad(const attn::Args& args, float* dbias, hipStream_t s, const char* what);

@@ -371,6 +371,19 @@ size_t nnk_attention_few_floats(const NnAttention* a) {
     // rows that are not on 16 bytes are taken as 128 features, so all are sized for that
     return p.splits == 1 ? 0 : (size_t)p.units * p.splits * 32 * (128 + 2);
 }
+// Units and workgroups more than the fill, at most.  Up to two tiles of a key head's rows: fewer
+// units than tickets; more tiles: 2 units for each of kCus / 2 workgroups of 64 queries.
+size_t nnk_attention_few_most(const NnAttention* a) {
+    const long long owners = (long long)a->batch * a->kv_heads, group = a->heads / a->kv_heads;
+    const long long tiles = (a->len_q * group + 31) / 32, steps = ((long long)a->len_k + kWaves * kKeys - 1) / (kWaves * kKeys);
+    if (steps < 2) return 0;
+    const auto groups = [&](long long units, long long fill) {
+        return std::min(units * std::min<long long>(kMaxSplits, steps), units + fill - 1);
+    };
+    const long long few = groups(std::min(kTickets - 1LL, owners * std::min(2LL, tiles)), 2 * kTickets);
+    const long long more = groups(std::min<long long>(kCus, owners * tiles), 3 * kCus);
+    return (size_t)std::max(few, more) * 32 * (128 + 2);
+}
 bool nnk_attention_few(const Args& a, bool half, float* ws, hipStream_t s, const char* what) {
     return NNK_ATTN_DISPATCH(a, half, launch, a, ws, s, what);
 }

@@ -118,9 +118,10 @@ typedef struct {
 
 /* out, lse [batch, heads, len_q].  `workspace`: nnhip_attention_forward_workspace
    floats (NULL if that is 0), zero-filled before its first use; every launch leaves
-   it fit for the next, also of another shape that it is large enough for; its size
-   serves every smaller batch.  Launches that may run concurrently need separate
-   workspaces. */
+   it fit for the next, also of another shape that it is large enough for.  Its size
+   serves every call of a smaller batch or of fewer queries or keys too, so that of a
+   program's largest call serves all of them.  Launches that may run concurrently need
+   separate workspaces. */
 size_t nnhip_attention_forward_workspace(const NnAttention* a);
 void launch_attention_forward(void* out, float* lse, const void* q, const void* k, const void* v,
     const NnAttention* a, float* workspace, hipStream_t s);
@@ -128,7 +129,7 @@ void launch_attention_forward(void* out, float* lse, const void* q, const void* 
 /* dq, dk, dv (layouts of q, k, v) and dbias [buckets, heads] (NULL if not wanted)
    from dout, the forward pass's inputs and its out and lse.  All are overwritten.
    `workspace`: nnhip_attention_backward_workspace floats (they serve every smaller
-   batch), nothing to be filled. */
+   batch and shorter lengths), nothing to be filled. */
 size_t nnhip_attention_backward_workspace(const NnAttention* a);
 void launch_attention_backward(void* dq, void* dk, void* dv, float* dbias, const void* dout,
     const void* q, const void* k, const void* v, const void* out, const float* lse,

@@ -196,3 +196,19 @@ def test_reference_gradients_by_differences():
             f = np.zeros(8)
             f[d] = 1e-5
             assert abs((call(x, w + f) - call(x, w - f)) / 2e-5 - dw[d]) < 1e-7
+
+
+@pytest.mark.parametrize("heads, kv, batch, docs", [(1, 1, 1, False), (8, 8, 1, True), (8, 2, 3, False), (32, 8, 16, False),
+                                                    (3, 1, 200, True)])
+@pytest.mark.parametrize("buckets", [0, 8])
+def test_workspaces_serve_shorter_lengths(nn, heads, kv, batch, docs, buckets):
+    """A program's workspaces have the sizes of its longest call: no shorter one may report more."""
+    L = nn.lib()
+    # where the division into parts changes: tiles of 32, 64 and 128, counts of workgroups, few queries
+    lengths = sorted({*range(1, 200, 7), *(n + d for n in (64, 128, 512, 1024, 4096, 8192, 16384) for d in (-1, 0, 1)), 2944, 3008, 4160,
+                      30000, 100000})
+    for size in (L.nnhip_attention_forward_workspace, L.nnhip_attention_backward_workspace):
+        got = np.array([[size(_attn(nn, batch=batch, len_q=q, len_k=k, heads=heads, kv_heads=kv, buckets=buckets,
+                                    max_distance=buckets, doc_q=DUMMY if docs else None, doc_k=DUMMY if docs else None))
+                         for k in lengths] for q in lengths], np.int64)
+        assert (np.diff(got, axis=0) >= 0).all() and (np.diff(got, axis=1) >= 0).all()
