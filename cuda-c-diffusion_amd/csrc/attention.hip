@@ -2,6 +2,8 @@
 // kernels.
 #include "attn_common.h"
 
+#include <cfloat>
+
 namespace {
 using namespace attn;
 
@@ -135,13 +137,32 @@ bool take(Args& p, const NnAttention* a, const char* what) {
     p.c2 = a->softcap * kLog2e;
     NNK_REQUIRE_RET(p.c1 < INFINITY && p.c2 < INFINITY, false, what, "%s: scale=%g with softcap=%g overflows", what,
         a->scale, a->softcap);
+    NNK_REQUIRE_RET(a->softcap == 0.0f || (p.c1 >= FLT_MIN && p.c2 >= FLT_MIN), false, what,
+        "%s: scale=%g with softcap=%g underflows", what, a->scale, a->softcap);
     if (a->softcap > 0.0f) {
+        // The series takes s, where its coefficients are all normal values (the last has c1 to
+        // the 11th power); else y = c1 s, and no wave goes without the other form.
         const double tanh_of[6] = {1.0, -1.0 / 3, 2.0 / 15, -17.0 / 315, 62.0 / 2835, -1382.0 / 155925};
-        double power = (double)p.c2 * p.c1;
-        for (int i = 0; i < 6; ++i, power *= (double)p.c1 * p.c1) p.series[i] = (float)(tanh_of[i] * power);
+        const auto series_of = [&](double unit) {  // of s unit
+            double power = p.c2 * (p.c1 / unit);
+            bool normal = true;
+            for (int i = 0; i < 6; ++i, power *= (p.c1 / unit) * (p.c1 / unit)) {
+                p.series[i] = (float)(tanh_of[i] * power);
+                normal = normal && std::isnormal(p.series[i]);
+            }
+            return normal;
+        };
         p.inv_c2 = 1.0f / p.c2;
-        p.small = kSeriesEnd / p.c1;
-        p.tiny = kShortSeriesEnd / p.c1;
+        p.unit = 1.0f;
+        if (series_of(1.0)) {
+            p.small = kSeriesEnd / p.c1;
+            p.tiny = kShortSeriesEnd / p.c1;
+        } else {
+            p.unit = p.c1;
+            series_of(p.c1);
+        }
+        p.near_end = kSeriesEnd * (p.unit / p.c1);
+        p.exponent = 2.0f * kLog2e * (p.c1 / p.unit);
     }
     p.q_start = a->q_start;
     p.k_len = a->k_len;

@@ -311,9 +311,11 @@ struct Args {
     int batch, len_q, len_k, heads, kv_heads, group, dim;
     int mask, buckets, max_distance;
     float scale, c1, c2;  // score in units of log2: c1 * s, or c2 * tanh(c1 * s)
-    float series[6];      // c2 tanh(c1 s) = s (series[0] + w (series[1] + ...)), w = s^2, for small c1 s
+    float series[6];      // c2 tanh(c1 s) = x (series[0] + w (series[1] + ...)), w = x^2, for small x = s unit
     float inv_c2;
-    float small, tiny;    // how small: |s| below this; and for its first 4 terms alone
+    float unit;           // 1, or c1 where coefficients for s would not be normal values
+    float near_end, exponent;  // how small: |x| below this; 2 |c1 s| in units of log2 is |x| exponent
+    float small, tiny;    // |s| below this: the series of s alone; and of its first 4 terms (0 if unit is c1)
     const int *q_start, *k_len, *prefix, *doc_q, *doc_k, *bucket;
     const float* bias;
     bool vec;
@@ -406,8 +408,8 @@ __device__ __forceinline__ void cap_scores(f32x16& s, f32x16& slope, const Args&
     } else {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            const float x = s[r], q = __builtin_amdgcn_rcpf(exp2_fast(fabsf(x) * (2.0f * kLog2e * a.c1)) + 1.0f);
-            const bool near = fabsf(x) < a.small;
+            const float x = s[r] * a.unit, q = __builtin_amdgcn_rcpf(exp2_fast(fabsf(x) * a.exponent) + 1.0f);
+            const bool near = fabsf(x) < a.near_end;
             s[r] = near ? cap_series<6>(x, a) : copysignf(fmaf(-2.0f, q, 1.0f), x) * a.c2;
             slope[r] = near ? slope_of(s[r]) : 4.0f * q * (1.0f - q);
         }

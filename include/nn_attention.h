@@ -101,7 +101,7 @@ typedef struct {
     int heads, kv_heads;    /* heads a multiple of kv_heads */
     int head_dim;           /* 1 .. 128 */
     float scale;            /* > 0 */
-    float softcap;          /* 0: none */
+    float softcap;          /* 0: none; scale / softcap and 1.45 softcap are normal fp32 values */
     int mask;               /* NnMask */
     int buckets;            /* 0: no bias */
     int max_distance;       /* 0 .. 1023 */

@@ -212,3 +212,15 @@ def test_workspaces_serve_shorter_lengths(nn, heads, kv, batch, docs, buckets):
                                     max_distance=buckets, doc_q=DUMMY if docs else None, doc_k=DUMMY if docs else None))
                          for k in lengths] for q in lengths], np.int64)
         assert (np.diff(got, axis=0) >= 0).all() and (np.diff(got, axis=1) >= 0).all()
+
+
+@pytest.mark.parametrize("scale, cap", [(0.1, 1e38), (1e-38, 1e10), (1e-30, 1e9), (0.1, 1e-39)])
+def test_caps_too_far_for_fp32_are_refused(nn, scale, cap):
+    """scale / softcap, or the cap, below the normal fp32 values has lost its digits."""
+    L = nn.lib()
+    a = _attn(nn, scale=scale, softcap=cap)
+    with pytest.raises(nn.NnHipError, match="underflows"):
+        L.launch_attention_forward(*[DUMMY] * 5, a, DUMMY, None)
+    with pytest.raises(nn.NnHipError, match="underflows"):
+        L.launch_attention_backward(*[DUMMY] * 3, None, *[DUMMY] * 6, a, DUMMY, None)
+    assert L.last_error()[0] == 0

@@ -4,6 +4,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
+from attention_ref import Tensor
 from test_gpu_attention import TYPES, Call, case, run
 
 pytestmark = pytest.mark.gpu
@@ -72,3 +73,78 @@ def test_workspaces_of_longer_calls(nn, L, rng, dtype, long, short):
     for name, n in sizes.items():
         assert (getattr(call, name).download()[n:] == 7.0).all(), name
     call.compare()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("batch, heads", [(1, 1), (64, 8)])
+@pytest.mark.parametrize("scale, cap", [(1.0, 5e-5), (1.0, 1e-3), (100.0, 0.01), (1e-3, 50.0), (1e-4, 50.0), (1e-5, 30.0),
+                                        (1e-6, 1.0), (0.125, 5e3), (0.1, 1e4), (0.125, 30.0), (1.0, 50.0)])
+def test_caps_of_any_size(nn, L, dtype, batch, heads, scale, cap):
+    """One key of 128 has a score of y caps before the tanh, the others 0, the same for all queries of a call, so
+    that each of the forms of the cap is met by itself; workgroups of 64 rows and of 128.
+
+    The capped score x is off by up to 20 u of itself (c1 2 u, the product 1, tanh 10, c2 2, its product 1, the
+    reference 2), a log-sum by that and 12 u of its own; a probability by twice that and 32 u, a gradient by two
+    of them and its slope, whose exponential's argument is up to 30."""
+    u, n, dim = 2.0**-24, 128, 8
+    scale, cap = float(np.float32(scale)), float(np.float32(cap))
+    t = nn.NN_BF16 if dtype == "bf16" else nn.NN_F32
+    for y in (0.0, 1e-6, 1e-3, 0.1, 0.139, 0.141, 0.3, 0.37, 0.374, 0.376, 0.5, 1.0, 3.0, 10.0, -1e-3, -0.1, -0.139, -0.3,
+              -0.37, -0.376, -1.0, -10.0):
+        print(f"[case] cap {dtype} {batch} {heads} {scale} {cap} {y}", flush=True)
+        shape = (batch, n, heads, dim)
+        q, k, v = np.zeros(shape, np.float32), np.zeros(shape, np.float32), np.zeros(shape, np.float32)
+        q[..., 0] = y * cap / scale
+        k[:, 100, :, 0] = 1.0
+        v[:, 100] = 1.0
+        x = {m: Tensor(L, shape, dtype, values=val) for m, val in
+             (("q", q), ("k", k), ("v", v), ("dout", np.ones(shape)), ("out", 0), ("dq", 0), ("dk", 0), ("dv", 0))}
+        lse = L.alloc(batch * heads * n)
+        strides = x["q"].strides[:3]
+        a = nn.NnAttention(dtype=t, batch=batch, len_q=n, len_k=n, heads=heads, kv_heads=heads, head_dim=dim, scale=scale,
+                           softcap=cap, q_stride=strides, k_stride=strides, v_stride=strides, out_stride=strides)
+        ws = L.to_device(np.zeros(max(1, L.nnhip_attention_forward_workspace(a)), np.float32))
+        bws = L.alloc(max(1, L.nnhip_attention_backward_workspace(a)))
+        L.launch_attention_forward(x["out"].p, lse.p, x["q"].p, x["k"].p, x["v"].p, a, ws.p, None)
+        L.launch_attention_backward(x["dq"].p, x["dk"].p, x["dv"].p, None, x["dout"].p, x["q"].p, x["k"].p, x["v"].p,
+                                    x["out"].p, lse.p, a, bws.p, None)
+        L.sync()
+        raw = x["q"].values()[0, 0, 0, 0]
+        tanh = np.tanh(raw * scale / cap)
+        score = tanh * cap
+        own = np.logaddexp(np.log(n - 1), score)
+        p = np.exp(score - own)
+        grad = scale / np.cosh(raw * scale / cap) ** 2 * p * np.exp(np.log(n - 1) - own) * dim
+        want = {"out": (p, 32 * abs(score) + 32), "dq": (grad, 64 * abs(score) + 128), "dv": (n * p, 32 * abs(score) + 64)}
+        got = lse.download().astype(np.float64)
+        assert (abs(got - own) <= 32 * u * (abs(score) + abs(own) + 1)).all(), (y, "lse", abs(got - own).max())
+        for m, (ref, bound) in want.items():
+            got = x[m].result()
+            got = got[..., 0] if m == "dq" else got[:, 100] if m == "dv" else got
+            assert np.isfinite(got).all(), (y, m)
+            if score > 0 and m == "dq":
+                continue  # 1 - p cancels: the size of dq is that of its terms, not its own
+            # bf16: the probability or score gradient, and the result
+            off = abs(got - ref)
+            limit = (bound * u + (2 * 2.0**-8 if dtype == "bf16" else 0)) * abs(ref) + 2.0**-120
+            assert (off <= limit).all(), (y, m, float((off / limit).max()))
+        assert np.isfinite(x["dk"].result()).all(), y
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scale, cap", [(1.0, 5e-5), (1e-5, 30.0), (0.125, 30.0)])
+@pytest.mark.parametrize("part", [0.1, 0.3, 1.0])
+def test_caps_of_any_size_with_a_bias(nn, L, rng, dtype, scale, cap, part):
+    """Scores of about `part` of the cap, a seventh of the queries with scores of exactly 0."""
+    c = case(dtype, 2, 130, 130, 2, 2, 16, cap=cap, scale=scale, buckets=4, max_distance=9)
+    print(f"[case] capped {part} {c}", flush=True)
+    call = Call(nn, L, rng, c, spoil=False)
+    q = call.t["q"]
+    view = q.view(q.host)
+    view *= part * cap / scale / c["dim"] ** 0.5
+    view[:, ::7] = 0
+    q.upload()
+    call.forward()
+    call.grad()
+    L.sync()
+    call.compare(scores=max(10.0, min(1.0, 4 * part) * cap))
