@@ -90,7 +90,7 @@ size_t backward_most(const NnAttention* a) {
 bool sizes_fit(const NnAttention* a, const char* what) {
     NNK_REQUIRE_RET(a, false, what, "%s: null description", what);
     NNK_REQUIRE_RET(a->dtype == NN_F32 || a->dtype == NN_BF16, false, what, "%s: unknown dtype %d", what, a->dtype);
-    NNK_REQUIRE_RET(a->batch >= 0 && a->len_q >= 0 && a->len_k >= 0 && a->len_q <= 1 << 30 && a->len_k <= 1 << 30,
+    NNK_REQUIRE_RET(a->batch >= 0 && a->len_q >= 0 && a->len_k >= 0 && a->len_q <= kMaxLen && a->len_k <= kMaxLen,
         false, what, "%s: bad shape batch=%d len_q=%d len_k=%d", what, a->batch, a->len_q, a->len_k);
     NNK_REQUIRE_RET(a->heads > 0 && a->kv_heads > 0 && a->heads % a->kv_heads == 0, false, what,
         "%s: heads=%d is not a multiple of kv_heads=%d", what, a->heads, a->kv_heads);

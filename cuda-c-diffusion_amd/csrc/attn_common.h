@@ -43,6 +43,7 @@ constexpr int kRows = 32 * kWaves;  // columns of a workgroup: queries, or keys 
 constexpr int kCus = 256;
 constexpr int kSplitBelow = 2 * kCus;  // workgroups below which blocks are shared by two waves
 constexpr int kMaxDistance = 1023;
+constexpr int kMaxLen = (1 << 30) - 4096;  // two of them, kMaxDistance and a tile fit in 32 bits
 constexpr int kTicketWords = 2048;  // at the front of every forward workspace: zeros between calls
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
@@ -326,8 +327,10 @@ __device__ __forceinline__ int keys_of(const Args& a, int b) {
     return a.k_len ? min(max(a.k_len[b], 0), a.len_k) : a.len_k;
 }
 __device__ __forceinline__ int start_of(const Args& a, int b) {
-    // far enough from the ends of the type that positions and distances stay in it
-    return a.q_start ? min(max(a.q_start[b], -(1 << 30)), 1 << 29) : a.len_k - a.len_q;
+    // where every query lies before key 0, or behind the last one, by more than max_distance, how
+    // far does not matter: so positions and distances stay in the type (lengths below kMaxLen)
+    constexpr int kFar = kMaxDistance + 1;
+    return a.q_start ? min(max(a.q_start[b], -a.len_q - kFar), a.len_k + kFar) : a.len_k - a.len_q;
 }
 // The query at position pos sees keys 0 .. limit - 1, of which its document's.
 __device__ __forceinline__ int limit_of(const Args& a, int b, int keys, int pos) {

@@ -97,7 +97,7 @@ void launch_qk_norm_rope_backward(void* dq, void* dk, float* dq_weight, float* d
  * of a tile are multiplied by zero. */
 typedef struct {
     int dtype;              /* NnDtype of q, k, v, out and their gradients */
-    int batch, len_q, len_k;
+    int batch, len_q, len_k; /* lengths up to 2^30 - 4096 */
     int heads, kv_heads;    /* heads a multiple of kv_heads */
     int head_dim;           /* 1 .. 128 */
     float scale;            /* > 0 */
@@ -107,7 +107,7 @@ typedef struct {
     int max_distance;       /* 0 .. 1023 */
     long long q_stride[3], k_stride[3], v_stride[3]; /* of (batch, token, head): tensors and their gradients */
     long long out_stride[3];                         /* out and its gradient */
-    const int* q_start;     /* [batch], or NULL for len_k - len_q */
+    const int* q_start;     /* [batch], any value, or NULL for len_k - len_q */
     const int* k_len;       /* [batch], or NULL for len_k */
     const int* prefix;      /* [batch], for NN_MASK_PREFIX */
     const int* doc_q;       /* [batch, len_q], or NULL (both or neither) */

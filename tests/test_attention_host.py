@@ -224,3 +224,12 @@ def test_caps_too_far_for_fp32_are_refused(nn, scale, cap):
     with pytest.raises(nn.NnHipError, match="underflows"):
         L.launch_attention_backward(*[DUMMY] * 3, None, *[DUMMY] * 6, a, DUMMY, None)
     assert L.last_error()[0] == 0
+
+
+@pytest.mark.parametrize("more", [dict(len_q=(1 << 30) - 4095), dict(len_k=(1 << 30) - 4095), dict(len_q=2**31 - 1)])
+def test_lengths_whose_distances_pass_32_bits_are_refused(nn, more):
+    L = nn.lib()
+    with pytest.raises(nn.NnHipError, match="bad shape"):
+        L.launch_attention_forward(*[DUMMY] * 5, _attn(nn, **more), DUMMY, None)
+    assert L.nnhip_attention_forward_workspace(_attn(nn, len_k=(1 << 30) - 4096)) > 0
+    assert L.last_error()[0] == 0

@@ -4,7 +4,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from attention_ref import Tensor
+from attention_ref import Tensor, ints
 from test_gpu_attention import TYPES, Call, case, run
 
 pytestmark = pytest.mark.gpu
@@ -148,3 +148,33 @@ def test_caps_of_any_size_with_a_bias(nn, L, rng, dtype, scale, cap, part):
     call.grad()
     L.sync()
     call.compare(scores=max(10.0, min(1.0, 4 * part) * cap))
+
+
+def test_positions_past_2_to_the_29(nn, L):
+    """A query past the end of a cache of 2^29 + 100 keys (one row, at strides of 0): every key lies more than
+    max_distance before it, none in the buckets of the near ones."""
+    n, m = (1 << 29) + 100, 300
+    print("[case] positions past 2^29", flush=True)
+    ones = L.to_device(np.ones(8, np.float32))
+    out, lse = L.alloc(8), L.alloc(2)
+    bias, bucket = L.to_device(np.array([[0.0], [60.0]], np.float32)), ints(L, np.arange(2 * m + 1) > 0)
+    start = ints(L, [(1 << 29) + 500])
+    a = nn.NnAttention(dtype=nn.NN_F32, batch=1, len_q=1, len_k=n, heads=1, kv_heads=1, head_dim=8, scale=0.125,
+                       mask=nn.NN_MASK_CAUSAL, buckets=2, max_distance=m, q_stride=(8, 8, 8), k_stride=(0, 0, 0),
+                       v_stride=(0, 0, 0), out_stride=(8, 8, 8), q_start=start.p, bucket=bucket.p, bias=bias.p)
+    ws = L.to_device(np.zeros(max(1, L.nnhip_attention_forward_workspace(a)), np.float32))
+    L.launch_attention_forward(out.p, lse.p, ones.p, ones.p, ones.p, a, ws.p, None)
+    L.sync()
+    # 2^29 equal terms in fp32 sums of up to 2^19 each: 2^-5 at worst, far from the bias of 60
+    assert abs(lse.download()[0] - (1.0 + np.log(n))) < 0.05
+    assert np.allclose(out.download(), 1.0, rtol=0.05)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("mask", ["none", "causal", "prefix"])
+@pytest.mark.parametrize("len_q", [3, 150])
+def test_starts_at_the_ends_of_the_type(nn, L, rng, dtype, mask, len_q):
+    """Queries far before the keys see none of them unless a prefix or no mask shows them; far behind, all."""
+    starts = [-(2**31), -(2**30) - 7, -len_q - 40, 2**29 + 1, 2**30, 2**31 - 1 - len_q, 233, 260]
+    run(nn, L, rng, case(dtype, len(starts), len_q, 230, 2, 2, 16, mask, buckets=7, max_distance=30, q_start=starts,
+                         prefix=[100] * len(starts)))
