@@ -16,9 +16,11 @@
 //   plain:  m is kept in units of s, p = 2^(c s - c m): one multiply-add, one power;
 //   cap:    scores within +-c2 (units of log2) need no running maximum.  m is that of the
 //           first block that a query sees, or c2 - 80 if that is more: then p <= 2^80 and,
-//           for c2 up to 80, l >= 2^-80, both far from the ends of fp32.  For scores below
-//           3/8 of the cap, tanh, its factors and the reference are one polynomial, of 4
-//           terms instead of 6 below 0.14 of it;
+//           for c2 up to 80, l >= 2^-80.  Sums that all the same left fp32's range (values past
+//           2^47), or came near its lower end (values below 2^-20 where all scores are low),
+//           show at the end, and the workgroup goes over its keys again by the next form.
+//           For scores below 3/8 of the cap, tanh, its factors and the reference are one
+//           polynomial, of 4 terms instead of 6 below 0.14 of it;
 //   else:   running maximum of x.
 //
 // Measured: 16384 tokens, 16 heads of 128 (4 of keys), a prefix, capped scores: 1500 us, 779
@@ -32,6 +34,9 @@ using namespace attn;
 
 // CAP: 0 none, 1 any, 2 at most kFixedCap and no bias
 constexpr float kFixedCap = 80.0f;
+// below this much of a sum of probabilities, sums of values are looked at: past 2^-100 they keep
+// their digits, as their terms' roundings are 2^-149
+constexpr float kLeastSum = 0x1p-16f, kLeastValue = 0x1p-100f;
 
 template <typename T, int DP, int CAP, bool BIAS, bool VEC, int SPLIT>
 __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && VEC ? 2 : 1) void attn_fwd_kernel(Args a, int tiles) {
@@ -74,7 +79,6 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && VEC ? 2 : 1) void attn_fwd_
     const int4 mine = query_docs_of(a, b, row0 / kBlock, kOwn / kBlock);
     const int blocks = (a.len_k + kBlock - 1) / kBlock;
     const int4* key_docs = a.key_docs ? a.key_docs + (size_t)b * blocks : nullptr;
-    Blocks at(0, (most + kBlock - 1) / kBlock, key_docs, mine);
 
     Frag<T> qf[L::kSteps];
     {
@@ -112,183 +116,207 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && VEC ? 2 : 1) void attn_fwd_
     };
 
     f32x16 o[DP / 32];
-#pragma unroll
-    for (int d = 0; d < DP / 32; ++d) o[d] = zero16();
-    float m = -INFINITY, l = 0.0f;  // m in units of the score: of s if there is neither cap nor bias
+    float m, l;  // m in units of the score: of s if there is neither cap nor bias
     // a wave of SPLIT 2 has the upper or the lower 32 rows of every block
     const int rbase = L::row_base(lane) + half * 32 * L::kRowBytes, cbase = L::col_base(lane) + half * 32 * L::kRowBytes;
 
-    int next = at.next();
-    if (next >= 0) {
-        load(next);
-        store(next, at.negative, 0);
-    }
-    for (int buf = 0; next >= 0; buf ^= 1) {
-        const int block = next, k0 = next * kBlock + half * 32, block_doc = at.doc;
-        next = at.next();
-        __syncthreads();  // this block is stored; the one before it is done with
-        if (next >= 0) load(next);
-        // nothing here for the wave's queries
-        const bool none = k0 >= wave_most || (docs && one_doc && block_doc >= 0 && block_doc != wave_doc);
-        if (!none) {
+    // over all blocks, by the form of CAP
+    const auto sweep = [&](auto cap_) {
+        constexpr int kCap = decltype(cap_)::value;
+        Blocks at(0, (most + kBlock - 1) / kBlock, key_docs, mine);
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) o[d] = zero16();
+        m = -INFINITY;
+        l = 0.0f;
+        int next = at.next();
+        if (next >= 0) {
+            load(next);
+            store(next, at.negative, 0);
+        }
+        for (int buf = 0; next >= 0; buf ^= 1) {
+            const int block = next, k0 = next * kBlock + half * 32, block_doc = at.doc;
+            next = at.next();
+            __syncthreads();  // this block is stored; the one before it is done with
+            if (next >= 0) load(next);
+            // nothing here for the wave's queries
+            const bool none = k0 >= wave_most || (docs && one_doc && block_doc >= 0 && block_doc != wave_doc);
+            if (!none) {
 
-            f32x16 s[kSubs];
+                f32x16 s[kSubs];
 #pragma unroll
-            for (int i = 0; i < kSubs; ++i) s[i] = zero16();
-            struct Keys {
-                Frag<T> x[kWide];
-            };
-            Keys rows[2];
-            const auto read_rows = [&](Keys& y, int n) {
+                for (int i = 0; i < kSubs; ++i) s[i] = zero16();
+                struct Keys {
+                    Frag<T> x[kWide];
+                };
+                Keys rows[2];
+                const auto read_rows = [&](Keys& y, int n) {
 #pragma unroll
-                for (int j = 0; j < kWide; ++j) {
-                    const int u = n * kWide + j;
-                    y.x[j] = L::rows(k_lds[buf], u / L::kSteps, u % L::kSteps, rbase);
+                    for (int j = 0; j < kWide; ++j) {
+                        const int u = n * kWide + j;
+                        y.x[j] = L::rows(k_lds[buf], u / L::kSteps, u % L::kSteps, rbase);
+                    }
+                };
+                const auto score = [&](const Keys& y, int n) {
+#pragma unroll
+                    for (int j = 0; j < kWide; ++j) {
+                        const int u = n * kWide + j;
+                        s[u / L::kSteps] = mma(y.x[j], qf[u % L::kSteps], s[u / L::kSteps]);
+                    }
+                };
+                if constexpr (kPiped) {
+                    read_rows(rows[0], 0);
+                    piped<kSubs * L::kSteps / kWide>(rows, read_rows, score);
+                } else {
+#pragma unroll
+                    for (int n = 0; n < kSubs * L::kSteps / kWide; ++n) {
+                        read_rows(rows[0], n);
+                        score(rows[0], n);
+                    }
                 }
-            };
-            const auto score = [&](const Keys& y, int n) {
-#pragma unroll
-                for (int j = 0; j < kWide; ++j) {
-                    const int u = n * kWide + j;
-                    s[u / L::kSteps] = mma(y.x[j], qf[u % L::kSteps], s[u / L::kSteps]);
-                }
-            };
-            if constexpr (kPiped) {
-                read_rows(rows[0], 0);
-                piped<kSubs * L::kSteps / kWide>(rows, read_rows, score);
-            } else {
-#pragma unroll
-                for (int n = 0; n < kSubs * L::kSteps / kWide; ++n) {
-                    read_rows(rows[0], n);
-                    score(rows[0], n);
-                }
-            }
-            struct Values {
-                Frag<T> x[DP / 32];
-            };
-            Values columns[2];
-            const auto read_columns = [&](Values& y, int n) {
-#pragma unroll
-                for (int d = 0; d < DP / 32; ++d)
-                    y.x[d] = L::cols(v_lds[buf], n / L::kKeySteps, n % L::kKeySteps, d, cbase);
-            };
-            if constexpr (kPiped) {
-                read_columns(columns[0], 0);
-                __builtin_amdgcn_sched_barrier(kMayCross);
-            }
-            const bool whole = block * kBlock + kBlock <= least && (!docs || (one_doc && block_doc == wave_doc));
-            const auto hide_both = [&]() {
-                if (whole) return;
-#pragma unroll
-                for (int i = 0; i < kSubs; ++i)
-                    hide(s[i], k0 + 32 * i, limit, docs ? doc_lds[buf] + half * 32 + 32 * i : nullptr, doc, h);
-            };
-            // the largest score so far, and sums and outputs in its terms
-            const auto raise = [&](float unit) {
-                float top = m;
-#pragma unroll
-                for (int i = 0; i < kSubs; ++i)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[i][r]);
-                top = max_halves(top);
-                const float base = top == -INFINITY ? 0.0f : top * unit;
-                if (__any(top > m)) {
-                    const float f = exp2_fast(m * unit - base);
-                    l *= f;
+                struct Values {
+                    Frag<T> x[DP / 32];
+                };
+                Values columns[2];
+                const auto read_columns = [&](Values& y, int n) {
 #pragma unroll
                     for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) o[d][r] *= f;
-                    m = top;
+                        y.x[d] = L::cols(v_lds[buf], n / L::kKeySteps, n % L::kKeySteps, d, cbase);
+                };
+                if constexpr (kPiped) {
+                    read_columns(columns[0], 0);
+                    __builtin_amdgcn_sched_barrier(kMayCross);
                 }
-                return base;
-            };
-            if constexpr (CAP == 2) {
-                float top = 0.0f;
+                const bool whole = block * kBlock + kBlock <= least && (!docs || (one_doc && block_doc == wave_doc));
+                const auto hide_both = [&]() {
+                    if (whole) return;
 #pragma unroll
-                for (int i = 0; i < kSubs; ++i)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(s[i][r]));
-                const auto by_series = [&](auto terms) {
+                    for (int i = 0; i < kSubs; ++i)
+                        hide(s[i], k0 + 32 * i, limit, docs ? doc_lds[buf] + half * 32 + 32 * i : nullptr, doc, h);
+                };
+                // the largest score so far, and sums and outputs in its terms
+                const auto raise = [&](float unit) {
+                    float top = m;
 #pragma unroll
                     for (int i = 0; i < kSubs; ++i)
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const float w = s[i][r] * s[i][r];
-                            float c = a.series[decltype(terms)::value - 1];
+                        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[i][r]);
+                    top = max_halves(top);
+                    const float base = top == -INFINITY ? 0.0f : top * unit;
+                    if (__any(top > m)) {
+                        const float f = exp2_fast(m * unit - base);
+                        l *= f;
 #pragma unroll
-                            for (int t = decltype(terms)::value - 2; t >= 0; --t) c = fmaf(w, c, a.series[t]);
-                            s[i][r] = exp2_fast(fmaf(s[i][r], c, -m));
-                        }
+                        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) o[d][r] *= f;
+                        m = top;
+                    }
+                    return base;
                 };
-                const bool plain = whole && __all(m != -INFINITY);
-                if (plain && __all(top < a.tiny)) {
-                    by_series(std::integral_constant<int, 4>{});
-                } else if (plain && __all(top < a.small)) {
-                    by_series(std::integral_constant<int, 6>{});
+                if constexpr (kCap == 2) {
+                    float top = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < kSubs; ++i)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(s[i][r]));
+                    const auto by_series = [&](auto terms) {
+#pragma unroll
+                        for (int i = 0; i < kSubs; ++i)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) {
+                                const float w = s[i][r] * s[i][r];
+                                float c = a.series[decltype(terms)::value - 1];
+#pragma unroll
+                                for (int t = decltype(terms)::value - 2; t >= 0; --t) c = fmaf(w, c, a.series[t]);
+                                s[i][r] = exp2_fast(fmaf(s[i][r], c, -m));
+                            }
+                    };
+                    const bool plain = whole && __all(m != -INFINITY);
+                    if (plain && __all(top < a.tiny)) {
+                        by_series(std::integral_constant<int, 4>{});
+                    } else if (plain && __all(top < a.small)) {
+                        by_series(std::integral_constant<int, 6>{});
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < kSubs; ++i) {
+                            cap_scores(s[i], a.c1, a.c2);
+                        }
+                        hide_both();
+                        float first = -INFINITY;
+#pragma unroll
+                        for (int i = 0; i < kSubs; ++i)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) first = fmaxf(first, s[i][r]);
+                        first = max_halves(first);
+                        if (m == -INFINITY && first > -INFINITY) m = fmaxf(first, a.c2 - kFixedCap);
+                        const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+                        for (int i = 0; i < kSubs; ++i)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) s[i][r] = exp2_fast(s[i][r] - base);
+                    }
+                } else if constexpr (kCap == 0 && !BIAS) {
+                    hide_both();
+                    const float base = raise(a.c1);
+#pragma unroll
+                    for (int i = 0; i < kSubs; ++i)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) s[i][r] = exp2_fast(fmaf(s[i][r], a.c1, -base));
                 } else {
 #pragma unroll
                     for (int i = 0; i < kSubs; ++i) {
-                        cap_scores(s[i], a.c1, a.c2);
+                        if constexpr (kCap) cap_scores(s[i], a.c1, a.c2);
+                        if constexpr (BIAS) add_bias<1>(s[i], kCap ? 1.0f : a.c1, table, a.max_distance, k0 + 32 * i + 4 * h - pos,
+                            k0 + 32 * i - (start + row0 + strip * 32 + 31));
                     }
                     hide_both();
-                    float first = -INFINITY;
-#pragma unroll
-                    for (int i = 0; i < kSubs; ++i)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) first = fmaxf(first, s[i][r]);
-                    first = max_halves(first);
-                    if (m == -INFINITY && first > -INFINITY) m = fmaxf(first, a.c2 - kFixedCap);
-                    const float base = m == -INFINITY ? 0.0f : m;
+                    const float base = raise(1.0f);
 #pragma unroll
                     for (int i = 0; i < kSubs; ++i)
 #pragma unroll
                         for (int r = 0; r < 16; ++r) s[i][r] = exp2_fast(s[i][r] - base);
                 }
-            } else if constexpr (CAP == 0 && !BIAS) {
-                hide_both();
-                const float base = raise(a.c1);
 #pragma unroll
                 for (int i = 0; i < kSubs; ++i)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[i][r] = exp2_fast(fmaf(s[i][r], a.c1, -base));
-            } else {
+                    for (int r = 0; r < 16; ++r) l += s[i][r];
+                const auto mix = [&](const Values& y, int n) {
+                    const Frag<T> p = operand(s[n / L::kKeySteps], n % L::kKeySteps, T{});
 #pragma unroll
-                for (int i = 0; i < kSubs; ++i) {
-                    if constexpr (CAP) cap_scores(s[i], a.c1, a.c2);
-                    if constexpr (BIAS) add_bias<1>(s[i], CAP ? 1.0f : a.c1, table, a.max_distance, k0 + 32 * i + 4 * h - pos,
-                        k0 + 32 * i - (start + row0 + strip * 32 + 31));
-                }
-                hide_both();
-                const float base = raise(1.0f);
+                    for (int d = 0; d < DP / 32; ++d) o[d] = mma(y.x[d], p, o[d]);
+                };
+                if constexpr (kPiped) {
+                    piped<kSubs * L::kKeySteps>(columns, read_columns, mix);
+                } else {
 #pragma unroll
-                for (int i = 0; i < kSubs; ++i)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[i][r] = exp2_fast(s[i][r] - base);
-            }
-#pragma unroll
-            for (int i = 0; i < kSubs; ++i)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) l += s[i][r];
-            const auto mix = [&](const Values& y, int n) {
-                const Frag<T> p = operand(s[n / L::kKeySteps], n % L::kKeySteps, T{});
-#pragma unroll
-                for (int d = 0; d < DP / 32; ++d) o[d] = mma(y.x[d], p, o[d]);
-            };
-            if constexpr (kPiped) {
-                piped<kSubs * L::kKeySteps>(columns, read_columns, mix);
-            } else {
-#pragma unroll
-                for (int n = 0; n < kSubs * L::kKeySteps; ++n) {
-                    read_columns(columns[0], n);
-                    mix(columns[0], n);
+                    for (int n = 0; n < kSubs * L::kKeySteps; ++n) {
+                        read_columns(columns[0], n);
+                        mix(columns[0], n);
+                    }
                 }
             }
+            if (next >= 0) store(next, at.negative, buf ^ 1);
         }
-        if (next >= 0) store(next, at.negative, buf ^ 1);
+        l = sum_halves(l);
+    };
+    sweep(std::integral_constant<int, CAP>{});
+    if constexpr (CAP == 2) {
+        float zero = l * 0.0f, least = INFINITY;  // NaN where a sum has left the type; the least of |o|
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) zero = fmaf(o[d][r], 0.0f, zero);
+        if (__any(l < kLeastSum)) {
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (32 * d + row_of(r, h) < a.dim) least = fminf(least, fabsf(o[d][r]));
+        }
+        const bool held = zero == 0.0f && (l >= kLeastSum || least >= kLeastValue);
+        if (__syncthreads_or(m != -INFINITY && !held)) sweep(std::integral_constant<int, 1>{});
     }
 
-    l = sum_halves(l);
     if constexpr (SPLIT > 1) {
         // the second half's part, through the tiles' LDS: a register's 64 lanes together
         float* to = reinterpret_cast<float*>(k_lds[0]) + strip * (DP / 32 * 16 * 64) + lane;

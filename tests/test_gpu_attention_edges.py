@@ -4,7 +4,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from attention_ref import Tensor, ints
+from attention_ref import Tensor, check, ints
 from test_gpu_attention import TYPES, Call, case, run
 
 pytestmark = pytest.mark.gpu
@@ -178,3 +178,32 @@ def test_starts_at_the_ends_of_the_type(nn, L, rng, dtype, mask, len_q):
     starts = [-(2**31), -(2**30) - 7, -len_q - 40, 2**29 + 1, 2**30, 2**31 - 1 - len_q, 233, 260]
     run(nn, L, rng, case(dtype, len(starts), len_q, 230, 2, 2, 16, mask, buckets=7, max_distance=30, q_start=starts,
                          prefix=[100] * len(starts)))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", [2.0**100, 2.0**-100])
+@pytest.mark.parametrize("len_q, batch, heads", [(100, 1, 2), (130, 32, 8), (3, 1, 2)])
+@pytest.mark.parametrize("low, high", [(-200.0, 200.0), (-15.0, 15.0), (-200.0, -200.0), (15.0, -15.0)])
+def test_values_of_any_size_under_a_cap(nn, L, rng, dtype, size, len_q, batch, heads, low, high):
+    """Values near the ends of the type: probabilities that are formed from a fixed reference may not
+    carry their products past them.  The first 64 keys' scores are about `low`, the later ones' `high`."""
+    c = case(dtype, batch, len_q, 200, heads, heads, 16, cap=50.0, scale=1.0)
+    print(f"[case] values of {size} {low} {high} {c}", flush=True)
+    call = Call(nn, L, rng, c, backward=False, spoil=False)
+    for n in "qkv":
+        x = call.t[n]
+        view = x.view(x.host)
+        if n == "q":
+            view[...] = 1.0
+        if n == "k":
+            view *= 0.01
+            view[:, :64] += low / 16
+            view[:, 64:] += high / 16
+        if n == "v":
+            view *= size
+        x.upload()
+    call.forward()
+    L.sync()
+    got, (ref, mag) = call.results(), call.expected()
+    check("out", got["out"] / size, ref["out"] / size, mag["out"] / size, dtype, scores=50.0)
+    check("lse", got["lse"], ref["lse"], mag["lse"], "f32", scores=50.0)
