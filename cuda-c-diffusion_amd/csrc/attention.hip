@@ -174,6 +174,14 @@ bool take(Args& p, const NnAttention* a, const char* what) {
     return true;
 }
 
+// Whether the rows of a tensor that the call writes lie apart; false after recording an error.
+bool rows_apart(const long long* stride, int batch, int len, int heads, int dim, const char* name, const char* what) {
+    const long long n[3] = {batch, len, heads};
+    NNK_REQUIRE_RET(nnk_rows_apart(3, stride, n, dim), false, what, "%s: rows of %s overlap (strides %lld, %lld, %lld)", what,
+        name, stride[0], stride[1], stride[2]);
+    return true;
+}
+
 // Whether rows of 16-byte chunks can be read and written: strides here, pointers by the
 // callers.  The offsets of 64 rows have to fit in 32 bits.
 bool strides_by_16(const NnAttention* a) {
@@ -201,6 +209,7 @@ void launch_attention_forward(void* out, float* lse, const void* q, const void* 
     if (!take(p, a, what)) return;
     if (!a->batch || !a->len_q) return;
     NNK_REQUIRE(out && lse && q && (!a->len_k || (k && v)), what, "%s: null pointer", what);
+    if (!rows_apart(a->out_stride, a->batch, a->len_q, a->heads, a->head_dim, "out", what)) return;
     NNK_REQUIRE(!forward_floats(a) || workspace, what, "%s: null workspace", what);
     NNK_REQUIRE(nnk::aligned16(workspace), what, "%s: workspace is not aligned to 16 bytes", what);
     p.q = q;
@@ -235,6 +244,10 @@ void launch_attention_backward(void* dq, void* dk, void* dv, float* dbias, const
     const bool has_q = a->batch && a->len_q, has_k = a->batch && a->len_k;
     NNK_REQUIRE(!has_q || (dq && dout && q && out && lse), what, "%s: null pointer of the queries", what);
     NNK_REQUIRE(!has_k || (dk && dv && k && v), what, "%s: null pointer of the keys", what);
+    if ((has_q && !rows_apart(a->q_stride, a->batch, a->len_q, a->heads, a->head_dim, "dq", what)) ||
+        (has_k && (!rows_apart(a->k_stride, a->batch, a->len_k, a->kv_heads, a->head_dim, "dk", what) ||
+            !rows_apart(a->v_stride, a->batch, a->len_k, a->kv_heads, a->head_dim, "dv", what))))
+        return;
     NNK_REQUIRE(!(has_q || has_k) || workspace, what, "%s: null workspace", what);
     NNK_REQUIRE(nnk::aligned16(workspace), what, "%s: workspace is not aligned to 16 bytes", what);
     p.q = q;

@@ -426,6 +426,14 @@ bool take(Rope& p, const NnQkNormRope* a, const char* what) {
     return true;
 }
 
+// Whether the rows of a tensor that the call writes lie apart; false after recording an error.
+bool rows_apart(const long long* stride, const NnQkNormRope* a, int heads, const char* name, const char* what) {
+    const long long n[2] = {a->tokens, heads};
+    NNK_REQUIRE_RET(!heads || nnk_rows_apart(2, stride, n, a->head_dim), false, what,
+        "%s: rows of %s overlap (strides %lld, %lld)", what, name, stride[0], stride[1]);
+    return true;
+}
+
 // Tokens of a workgroup at a time: rows for 16 passes of its groups, as far as their sines
 // fit.  Few tokens: one each, and their heads shared by workgroups of one pass.
 int tokens_each(const Rope& p, int groups) {
@@ -491,6 +499,8 @@ void launch_qk_norm_rope_forward(void* q_out, void* k_out, const void* q, const 
     if (!p.tokens || !p.all_heads) return;
     NNK_REQUIRE((!a->heads || (q && q_out)) && (!a->kv_heads || (k && k_out)), what, "%s: null pointer", what);
     NNK_REQUIRE((long long)p.tokens * p.all_heads < 1LL << 31, what, "%s: too many rows", what);
+    if (!rows_apart(a->q_out_stride, a, a->heads, "q_out", what) || !rows_apart(a->k_out_stride, a, a->kv_heads, "k_out", what))
+        return;
     p.q = q;
     p.k = k;
     p.q_out = q_out;
@@ -516,6 +526,8 @@ void launch_qk_norm_rope_backward(void* dq, void* dk, float* dq_weight, float* d
     NNK_REQUIRE(!rows || ((!a->heads || (q && dq && dq_out)) && (!a->kv_heads || (k && dk && dk_out))), what,
         "%s: null pointer", what);
     NNK_REQUIRE((long long)p.tokens * p.all_heads < 1LL << 31, what, "%s: too many rows", what);
+    if (rows && (!rows_apart(a->q_stride, a, a->heads, "dq", what) || !rows_apart(a->k_stride, a, a->kv_heads, "dk", what)))
+        return;
     NNK_REQUIRE(!rows || !(dq_weight || dk_weight) || workspace, what, "%s: null workspace", what);
     p.q = q;
     p.k = k;

@@ -478,6 +478,25 @@ unsigned* nnk_wait_flag();
         }                                                    \
     } while (0)
 
+// Whether rows of `dim` values, n[i] of them at stride[i], lie apart, as those that workgroups
+// write have to: each stride passes what the smaller ones span.
+inline bool nnk_rows_apart(int axes, const long long* stride, const long long* n, long long dim) {
+    bool done[4] = {};
+    for (int i = 0; i < axes; ++i) done[i] = n[i] <= 1;
+    for (unsigned __int128 span = (unsigned __int128)dim;;) {
+        int next = -1;
+        unsigned long long least = 0;
+        for (int i = 0; i < axes; ++i) {
+            const unsigned long long size = stride[i] < 0 ? 0ull - (unsigned long long)stride[i] : (unsigned long long)stride[i];
+            if (!done[i] && (next < 0 || size < least)) next = i, least = size;
+        }
+        if (next < 0) return true;
+        if (least < span) return false;
+        done[next] = true;
+        span += (unsigned __int128)least * (unsigned long long)(n[next] - 1);
+    }
+}
+
 // As NNK_REQUIRE, in a function returning `ret`.
 #define NNK_REQUIRE_RET(cond, ret, what, ...)                \
     do {                                                     \

@@ -17,6 +17,10 @@
  * that are multiples of 16 bytes (with head_dim * size too) get 16-byte
  * accesses; any others are taken element by element, slower.
  *
+ * What a call reads may repeat rows (strides of 0); what it writes, outputs and
+ * gradients at the strides of their inputs, may not, and is refused.  Gradients of
+ * inputs that repeat rows are for the caller to form from those of their copies.
+ *
  * Nothing allocates, issues a memset or synchronises: every call can be
  * captured into a graph.  Results do not depend on the order in which
  * workgroups run.

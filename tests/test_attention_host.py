@@ -233,3 +233,46 @@ def test_lengths_whose_distances_pass_32_bits_are_refused(nn, more):
         L.launch_attention_forward(*[DUMMY] * 5, _attn(nn, **more), DUMMY, None)
     assert L.nnhip_attention_forward_workspace(_attn(nn, len_k=(1 << 30) - 4096)) > 0
     assert L.last_error()[0] == 0
+
+
+OVERLAPS = [
+    (dict(batch=3, k_stride=(0, 8, 8)), "dk"),  # one request's keys for all
+    (dict(batch=3, v_stride=(0, 8, 8)), "dv"),
+    (dict(heads=4, kv_heads=2, k_stride=(64, 8, 0)), "dk"),  # one key head's keys for all
+    (dict(k_stride=(64, 0, 8)), "dk"),
+    (dict(v_stride=(64, 7, 8)), "dv"),
+    (dict(q_stride=(64, 8, 8)), "dq"),  # tokens by the stride of heads
+    (dict(batch=2, q_stride=(48, 16, 8)), "dq"),
+    (dict(q_stride=(64, -8, 8)), "dq"),
+    (dict(batch=2, q_stride=(1 << 62, 16, 0)), "dq"),
+]
+
+
+@pytest.mark.parametrize("more, name", OVERLAPS)
+def test_gradients_that_would_overlap_are_refused(nn, more, name):
+    """Rows repeated by their strides: workgroups would write one row's gradient over another's."""
+    L = nn.lib()
+    more = {"batch": 1, **more}
+    a = _attn(nn, **{"q_stride": (128, 32, 8), "k_stride": (64, 16, 8), "v_stride": (64, 16, 8), **more})
+    with pytest.raises(nn.NnHipError, match=f"rows of {name} overlap"):
+        L.launch_attention_backward(*[DUMMY] * 3, None, *[DUMMY] * 6, a, DUMMY, None)
+    assert L.last_error()[0] == 0
+
+
+@pytest.mark.parametrize("stride", [(0, 16, 8), (64, 0, 8), (64, 16, 0), (64, 15, 8), (63, 16, 8), (64, 16, -4)])
+def test_outputs_that_would_overlap_are_refused(nn, stride):
+    L = nn.lib()
+    with pytest.raises(nn.NnHipError, match="rows of out overlap"):
+        L.launch_attention_forward(*[DUMMY] * 5, _attn(nn, batch=2, out_stride=stride), DUMMY, None)
+    assert L.last_error()[0] == 0
+
+
+def test_rotated_rows_that_would_overlap_are_refused(nn):
+    L = nn.lib()
+    for more, name in ((dict(q_out_stride=(0, 8)), "q_out"), (dict(k_out_stride=(7, 8)), "k_out"), (dict(q_out_stride=(16, 0)), "q_out")):
+        with pytest.raises(nn.NnHipError, match=f"rows of {name} overlap"):
+            L.launch_qk_norm_rope_forward(*[DUMMY] * 4, _rope(nn, **more), None)
+    for more, name in ((dict(q_stride=(0, 8)), "dq"), (dict(k_stride=(0, 8)), "dk"), (dict(q_stride=(16, 4)), "dq")):
+        with pytest.raises(nn.NnHipError, match=f"rows of {name} overlap"):
+            L.launch_qk_norm_rope_backward(*[DUMMY] * 8, _rope(nn, **more), DUMMY, None)
+    assert L.last_error()[0] == 0
