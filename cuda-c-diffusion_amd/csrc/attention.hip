@@ -7,7 +7,8 @@
 namespace {
 using namespace attn;
 
-constexpr long long kMostGroups = (1LL << 31) - 1;
+constexpr long long kMostGroups = ((1LL << 32) - 1) / kTpb;  // a launch has fewer than 2^32 threads
+constexpr long long kMostRows = (1LL << 31) - 1;
 
 // Workspaces, in floats; documents come first (16-byte records).
 size_t docs_floats(const NnAttention* a) {
@@ -18,7 +19,7 @@ size_t docs_floats(const NnAttention* a) {
 }
 float* order_of(const NnAttention* a, float* docs, bool keys) {
     const size_t nk = ((size_t)a->len_k + kBlock - 1) / kBlock, nq = ((size_t)a->len_q + kBlock - 1) / kBlock;
-    return docs + 4 * a->batch * (nk + nq) + (keys ? a->batch * nq : 0);
+    return docs + 4 * (size_t)a->batch * (nk + nq) + (keys ? a->batch * nq : 0);
 }
 // How the gradients are divided over workgroups.  Key heads that are shared and few tiles of
 // keys: the heads apart.  Few workgroups even so: tiles of 64, and the other axis in parts of
@@ -87,7 +88,7 @@ size_t backward_most(const NnAttention* a) {
         by4(stat_floats(a)) + (a->buckets ? (size_t)tables * (2 * a->max_distance + 1) : 0);
 }
 
-bool sizes_fit(const NnAttention* a, const char* what) {
+bool sizes_fit(const NnAttention* a, bool backward, const char* what) {
     NNK_REQUIRE_RET(a, false, what, "%s: null description", what);
     NNK_REQUIRE_RET(a->dtype == NN_F32 || a->dtype == NN_BF16, false, what, "%s: unknown dtype %d", what, a->dtype);
     NNK_REQUIRE_RET(a->batch >= 0 && a->len_q >= 0 && a->len_k >= 0 && a->len_q <= kMaxLen && a->len_k <= kMaxLen,
@@ -98,15 +99,23 @@ bool sizes_fit(const NnAttention* a, const char* what) {
         a->head_dim);
     NNK_REQUIRE_RET(a->buckets >= 0 && a->max_distance >= 0 && a->max_distance <= kMaxDistance, false, what,
         "%s: buckets=%d max_distance=%d (at most %d)", what, a->buckets, a->max_distance, kMaxDistance);
-    const long long rows = std::max(((long long)a->len_q + kRows - 1) / kRows, ((long long)a->len_k + kBlock - 1) / kBlock);
-    NNK_REQUIRE_RET(rows * a->batch <= kMostGroups / a->heads && (long long)a->buckets * a->heads <= kMostGroups, false,
-        what, "%s: too many rows (batch=%d heads=%d len_q=%d len_k=%d)", what, a->batch, a->heads, a->len_q, a->len_k);
+    NNK_REQUIRE_RET(a->heads <= kMostHeads, false, what, "%s: heads=%d (at most %d)", what, a->heads, kMostHeads);
+    const auto up = [](long long n, long long d) { return (n + d - 1) / d; };
+    const long long rows = std::max(up(a->len_q, kRows), up(a->len_k, kBlock));
+    bool fits = rows * a->batch <= kMostRows / a->heads && (long long)a->buckets * a->heads <= kMostRows;
+    // workgroups of tiles of queries, of keys, and of documents (of 64 threads)
+    const auto launched = [&](long long n) { return n * a->batch <= kMostGroups / a->heads; };
+    fits = fits && ((!backward && nnk_attention_is_few(a)) || launched(up(a->len_q, kRows)));
+    fits = fits && (!backward || launched(up(a->len_k, kRows)));
+    fits = fits && (!a->doc_q || up(std::max(a->len_q, a->len_k), kBlock) * a->batch <= kMostGroups * (kTpb / 64));
+    NNK_REQUIRE_RET(fits, false, what, "%s: too many rows (batch=%d heads=%d len_q=%d len_k=%d)", what, a->batch, a->heads,
+        a->len_q, a->len_k);
     return true;
 }
 
 // Fills `p` for the call's description; false after recording an error.
-bool take(Args& p, const NnAttention* a, const char* what) {
-    if (!sizes_fit(a, what)) return false;
+bool take(Args& p, const NnAttention* a, bool backward, const char* what) {
+    if (!sizes_fit(a, backward, what)) return false;
     NNK_REQUIRE_RET(a->scale > 0.0f && a->scale < INFINITY, false, what, "%s: scale=%g is not positive", what, a->scale);
     NNK_REQUIRE_RET(a->softcap >= 0.0f && a->softcap < INFINITY, false, what, "%s: softcap=%g is negative", what,
         a->softcap);
@@ -198,7 +207,7 @@ bool strides_by_16(const NnAttention* a) {
 extern "C" {
 
 size_t nnhip_attention_forward_workspace(const NnAttention* a) {
-    if (!sizes_fit(a, "nnhip_attention_forward_workspace")) return 0;
+    if (!sizes_fit(a, false, "nnhip_attention_forward_workspace")) return 0;
     return forward_most(a);
 }
 
@@ -206,7 +215,7 @@ void launch_attention_forward(void* out, float* lse, const void* q, const void* 
     const NnAttention* a, float* workspace, hipStream_t s) {
     const char* what = "launch_attention_forward";
     Args p;
-    if (!take(p, a, what)) return;
+    if (!take(p, a, false, what)) return;
     if (!a->batch || !a->len_q) return;
     NNK_REQUIRE(out && lse && q && (!a->len_k || (k && v)), what, "%s: null pointer", what);
     if (!rows_apart(a->out_stride, a->batch, a->len_q, a->heads, a->head_dim, "out", what)) return;
@@ -230,7 +239,7 @@ void launch_attention_forward(void* out, float* lse, const void* q, const void* 
 }
 
 size_t nnhip_attention_backward_workspace(const NnAttention* a) {
-    if (!sizes_fit(a, "nnhip_attention_backward_workspace")) return 0;
+    if (!sizes_fit(a, true, "nnhip_attention_backward_workspace")) return 0;
     return backward_most(a);
 }
 
@@ -239,7 +248,7 @@ void launch_attention_backward(void* dq, void* dk, void* dv, float* dbias, const
     const NnAttention* a, float* workspace, hipStream_t s) {
     const char* what = "launch_attention_backward";
     Args p;
-    if (!take(p, a, what)) return;
+    if (!take(p, a, true, what)) return;
     NNK_REQUIRE(!dbias || a->buckets, what, "%s: a bias gradient without a bias", what);
     const bool has_q = a->batch && a->len_q, has_k = a->batch && a->len_k;
     NNK_REQUIRE(!has_q || (dq && dout && q && out && lse), what, "%s: null pointer of the queries", what);

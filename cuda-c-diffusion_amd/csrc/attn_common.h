@@ -44,6 +44,7 @@ constexpr int kCus = 256;
 constexpr int kSplitBelow = 2 * kCus;  // workgroups below which blocks are shared by two waves
 constexpr int kMaxDistance = 1023;
 constexpr int kMaxLen = (1 << 30) - 4096;  // two of them, kMaxDistance and a tile fit in 32 bits
+constexpr int kMostHeads = 1 << 20;  // and requests whose tiles are put in order: workgroups of 1024 threads
 constexpr int kTicketWords = 2048;  // at the front of every forward workspace: zeros between calls
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;

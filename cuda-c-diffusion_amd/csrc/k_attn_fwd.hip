@@ -442,7 +442,7 @@ void nnk_attention_docs(Args& a, float* ws, hipStream_t s, const char* what) {
 const int* nnk_attention_order(const Args& a, bool keys, int own, float* order, hipStream_t s, const char* what) {
     const int len = keys ? a.len_k : a.len_q, tiles = (len + own - 1) / own;
     const int blocks = ((keys ? a.len_q : a.len_k) + kBlock - 1) / kBlock;
-    if (tiles < 2 || tiles > kOrderTiles || blocks > kOrderBlocks || tiles * blocks > 64 * kOrderTpb) return nullptr;
+    if (a.batch > kMostHeads || tiles < 2 || tiles > kOrderTiles || blocks > kOrderBlocks || tiles * blocks > 64 * kOrderTpb) return nullptr;
     int* to = reinterpret_cast<int*>(order);
     tile_order_kernel<<<(unsigned)a.batch, kOrderTpb, 0, s>>>(to, a, keys, own, tiles);
     nnk_after_launch(what, s);

@@ -448,13 +448,14 @@ bool in_chunks(const Rope& p) {
 }
 
 template <typename T, int G>
-void forward(Rope& p, hipStream_t s) {
+void forward(Rope& p, hipStream_t s, const char* what) {
     constexpr int groups = Row<T, G>::kGroups;
     p.tokens_each = tokens_each(p, groups);
     p.head_parts = p.tokens < kGradGroups ? (p.all_heads + groups - 1) / groups : 1;
-    const unsigned blocks = (unsigned)(((long long)p.tokens + p.tokens_each - 1) / p.tokens_each * p.head_parts);
-    if (in_chunks<T>(p)) qk_norm_rope_kernel<T, G, true><<<blocks, kTpb, 0, s>>>(p);
-    else qk_norm_rope_kernel<T, G, false><<<blocks, kTpb, 0, s>>>(p);
+    const long long blocks = ((long long)p.tokens + p.tokens_each - 1) / p.tokens_each * p.head_parts;
+    NNK_REQUIRE(blocks < (1LL << 32) / kTpb, what, "%s: too many rows", what);  // threads of a launch
+    if (in_chunks<T>(p)) qk_norm_rope_kernel<T, G, true><<<(unsigned)blocks, kTpb, 0, s>>>(p);
+    else qk_norm_rope_kernel<T, G, false><<<(unsigned)blocks, kTpb, 0, s>>>(p);
 }
 // Backward: as many workgroups as the card holds at once, of as many tokens each.
 int grad_groups(Rope& p, int groups) {
@@ -463,7 +464,7 @@ int grad_groups(Rope& p, int groups) {
     return (p.tokens + p.tokens_all - 1) / p.tokens_all;
 }
 template <typename T, int G>
-void backward(Rope& p, hipStream_t s) {
+void backward(Rope& p, hipStream_t s, const char*) {
     const unsigned blocks = (unsigned)grad_groups(p, Row<T, G>::kGroups);
     if (in_chunks<T>(p)) qk_norm_rope_grad_kernel<T, G, true><<<blocks, kTpb, 0, s>>>(p);
     else qk_norm_rope_grad_kernel<T, G, false><<<blocks, kTpb, 0, s>>>(p);
@@ -475,15 +476,15 @@ int lanes_of(const NnQkNormRope* a) {
     return n <= 4 ? 4 : n <= 8 ? 8 : n <= 16 ? 16 : n <= 32 ? 32 : 64;
 }
 
-#define ROPE_DISPATCH(FN, p, a, s)                                                     \
+#define ROPE_DISPATCH(FN, p, a, s, what)                                               \
     do {                                                                               \
         const bool half_ = (a)->dtype == NN_BF16;                                      \
         switch (lanes_of(a)) {                                                         \
-        case 4: half_ ? FN<bf16, 4>(p, s) : FN<float, 4>(p, s); break;                 \
-        case 8: half_ ? FN<bf16, 8>(p, s) : FN<float, 8>(p, s); break;                 \
-        case 16: half_ ? FN<bf16, 16>(p, s) : FN<float, 16>(p, s); break;              \
-        case 32: half_ ? FN<bf16, 32>(p, s) : FN<float, 32>(p, s); break;              \
-        default: FN<float, 64>(p, s); break;                                           \
+        case 4: half_ ? FN<bf16, 4>(p, s, what) : FN<float, 4>(p, s, what); break;     \
+        case 8: half_ ? FN<bf16, 8>(p, s, what) : FN<float, 8>(p, s, what); break;     \
+        case 16: half_ ? FN<bf16, 16>(p, s, what) : FN<float, 16>(p, s, what); break;  \
+        case 32: half_ ? FN<bf16, 32>(p, s, what) : FN<float, 32>(p, s, what); break;  \
+        default: FN<float, 64>(p, s, what); break;                                     \
         }                                                                              \
     } while (0)
 
@@ -507,7 +508,7 @@ void launch_qk_norm_rope_forward(void* q_out, void* k_out, const void* q, const 
     p.k_out = k_out;
     if (a->heads) p.vec = p.vec && nnk::aligned16(q) && nnk::aligned16(q_out);
     if (a->kv_heads) p.vec = p.vec && nnk::aligned16(k) && nnk::aligned16(k_out);
-    ROPE_DISPATCH(forward, p, a, s);
+    ROPE_DISPATCH(forward, p, a, s, what);
     nnk_after_launch(what, s);
 }
 
@@ -525,7 +526,8 @@ void launch_qk_norm_rope_backward(void* dq, void* dk, float* dq_weight, float* d
     const bool rows = p.tokens && p.all_heads;
     NNK_REQUIRE(!rows || ((!a->heads || (q && dq && dq_out)) && (!a->kv_heads || (k && dk && dk_out))), what,
         "%s: null pointer", what);
-    NNK_REQUIRE((long long)p.tokens * p.all_heads < 1LL << 31, what, "%s: too many rows", what);
+    // positions of a workgroup's tokens and of the next one's fit in 32 bits
+    NNK_REQUIRE((long long)p.tokens * p.all_heads <= 1LL << 30, what, "%s: too many rows", what);
     if (rows && (!rows_apart(a->q_stride, a, a->heads, "dq", what) || !rows_apart(a->k_stride, a, a->kv_heads, "dk", what)))
         return;
     NNK_REQUIRE(!rows || !(dq_weight || dk_weight) || workspace, what, "%s: null workspace", what);
@@ -540,7 +542,7 @@ void launch_qk_norm_rope_backward(void* dq, void* dk, float* dq_weight, float* d
     if (dq_weight || dk_weight) p.partial = workspace;
     int groups = 0;
     if (rows) {
-        ROPE_DISPATCH(backward, p, a, s);
+        ROPE_DISPATCH(backward, p, a, s, what);
         nnk_after_launch(what, s);
         groups = grad_groups(p, kTpb / lanes_of(a));
     }

@@ -54,7 +54,7 @@ typedef enum { NN_MASK_NONE = 0, NN_MASK_CAUSAL, NN_MASK_PREFIX } NnMask;
  * Angles are formed and reduced in 64 bits, so far positions keep their sine. */
 typedef struct {
     int dtype;               /* NnDtype of q, k, their outputs and gradients */
-    int tokens;
+    int tokens;              /* tokens * (heads + kv_heads) below 2^31, 2^30 at most for the gradients */
     int heads, kv_heads;     /* either may be 0: its pointers are then ignored */
     int head_dim;            /* 1 .. 256 */
     int rot_dim;             /* even, 0 .. head_dim */

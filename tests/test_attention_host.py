@@ -276,3 +276,43 @@ def test_rotated_rows_that_would_overlap_are_refused(nn):
         with pytest.raises(nn.NnHipError, match=f"rows of {name} overlap"):
             L.launch_qk_norm_rope_backward(*[DUMMY] * 8, _rope(nn, **more), DUMMY, None)
     assert L.last_error()[0] == 0
+
+
+WIDE = {n: (1 << 32, 1 << 20, 8) for n in ("q_stride", "k_stride", "v_stride", "out_stride")}
+
+
+@pytest.mark.parametrize("more, forward", [
+    (dict(batch=1 << 23, heads=2, kv_heads=2, len_q=1, len_k=1), True),
+    (dict(batch=1 << 24, heads=1, len_q=1, len_k=1), True),
+    (dict(batch=1 << 19, len_k=1, len_q=2049), True),
+    (dict(batch=1 << 14, len_q=1, len_k=1 << 18, doc_q=DUMMY, doc_k=DUMMY), True),  # documents of its keys
+    (dict(batch=1 << 19, len_k=2049, len_q=1), False),  # key gradients
+    (dict(batch=1 << 19, heads=32, len_q=1, len_k=1), False),  # few queries; query gradients
+])
+def test_more_workgroups_than_a_launch_takes_are_refused(nn, more, forward):
+    """2^32 threads and more: the first kernels of a call would run and a later one not."""
+    L = nn.lib()
+    a = _attn(nn, **WIDE, **more)
+    calls = [lambda: L.launch_attention_backward(*[DUMMY] * 3, None, *[DUMMY] * 6, a, DUMMY, None),
+             lambda: L.nnhip_attention_backward_workspace(a)]
+    if forward:
+        calls += [lambda: L.launch_attention_forward(*[DUMMY] * 5, a, DUMMY, None), lambda: L.nnhip_attention_forward_workspace(a)]
+    else:
+        L.nnhip_attention_forward_workspace(a)
+    for call in calls:
+        with pytest.raises(nn.NnHipError, match="too many rows"):
+            call()
+    assert L.last_error()[0] == 0
+
+
+def test_heads_and_tokens_past_a_launch_are_refused(nn):
+    L = nn.lib()
+    with pytest.raises(nn.NnHipError, match="heads=1048577"):
+        L.launch_attention_forward(*[DUMMY] * 5, _attn(nn, heads=(1 << 20) + 1), DUMMY, None)
+    with pytest.raises(nn.NnHipError, match="too many rows"):
+        L.launch_qk_norm_rope_forward(*[DUMMY] * 4, _rope(nn, tokens=1 << 28, heads=1, kv_heads=0, head_dim=256, rot_dim=256,
+                                                          q_out_stride=(256, 256)), None)
+    assert L.last_error()[0] == 0
+    with pytest.raises(nn.NnHipError, match="too many rows"):
+        L.launch_qk_norm_rope_backward(*[DUMMY] * 8, _rope(nn, tokens=(1 << 30) + 1, heads=1, kv_heads=0, q_stride=(8, 8)), DUMMY, None)
+    assert L.last_error()[0] == 0
