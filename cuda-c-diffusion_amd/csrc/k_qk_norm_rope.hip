@@ -164,16 +164,21 @@ struct Row {
     }
 };
 
-// Cosine and sine of each pair of `count` tokens.  The angle is formed in 64 bits and
-// reduced there to a fraction of a turn, so that it is as exact at position 2^30 as at 1.
+// Cosine and sine of each pair of `count` tokens.  The angle is formed in 64 bits (off by
+// 2^-53 of itself, 2^-24 at 2^29 rad) and reduced there to an eighth of a turn either way, so
+// that fp32 rounds what is left of it and not turns: the small one of sine and cosine near a
+// quarter turn keeps its digits.
 __device__ __forceinline__ void angles(float2* cs, const Rope& a, int token0, int count) {
     for (int i = threadIdx.x; i < count * a.half; i += kTpb) {
         const int t = i / a.half, p = i - t * a.half;
         double turns = (double)a.pos[(size_t)(token0 + t) * a.axes + p / a.per_axis] * a.freq[p] * 0.15915494309189533577;
         turns -= rint(turns);
+        const double quarters = rint(4.0 * turns);
+        const int q = (int)quarters;
         float s, c;
-        sincospif(2.0f * (float)turns, &s, &c);
-        cs[i] = make_float2(c, s);
+        sincospif(0.5f * (float)(4.0 * turns - quarters), &s, &c);
+        const float x = q & 1 ? s : c, y = q & 1 ? c : s;
+        cs[i] = make_float2((q + 1) & 2 ? -x : x, q & 2 ? -y : y);
     }
 }
 
