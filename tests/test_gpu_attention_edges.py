@@ -207,3 +207,17 @@ def test_values_of_any_size_under_a_cap(nn, L, rng, dtype, size, len_q, batch, h
     got, (ref, mag) = call.results(), call.expected()
     check("out", got["out"] / size, ref["out"] / size, mag["out"] / size, dtype, scores=50.0)
     check("lse", got["lse"], ref["lse"], mag["lse"], "f32", scores=50.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads, kv, distance", [(8, 1, 500), (4, 1, 1023), (8, 2, 1023), (4, 1, 511), (4, 1, 512), (1, 1, 1023)])
+def test_bias_of_few_queries_by_any_distance(nn, L, rng, dtype, heads, kv, distance):
+    """Tables of the bias that fit in LDS (16 KB: 4 heads of 511 distances) and that do not; keys within
+    max_distance, past it, and after the query."""
+    c = case(dtype, 2, 2, 3001, heads, kv, 40, "prefix", buckets=32, max_distance=distance, prefix=[3001, 100],
+             q_start=[1500, 2999], k_len=[3001, 2990])
+    print(f"[case] few queries {c}", flush=True)
+    call = Call(nn, L, rng, c, "cache", backward=False)
+    call.forward()
+    L.sync()
+    call.compare()
