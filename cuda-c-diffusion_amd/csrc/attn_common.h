@@ -576,7 +576,7 @@ inline bool raise_lds(const void* fn, size_t bytes, std::atomic<unsigned long lo
 // nothing).
 void nnk_attention_docs(attn::Args& args, float* ws, hipStream_t s, const char* what);
 // Tiles of `own` queries (or keys) of each request by falling work into `order`; null if
-// there are too many to be worth it.
+// there are more than the counting takes.
 const int* nnk_attention_order(const attn::Args& args, bool keys, int own, float* order, hipStream_t s, const char* what);
 // One launch each; `half`: bf16.  False after recording an error.
 bool nnk_attention_forward(const attn::Args& args, bool half, hipStream_t s, const char* what);

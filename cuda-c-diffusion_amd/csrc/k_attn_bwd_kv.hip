@@ -21,7 +21,7 @@
 // went past the end), and the tile is 32 shuffles and adds and one addition to the
 // wave's table in LDS.  Tiles wholly past max_distance are added up whole.
 //
-// Measured, as the query gradients: 243 us and 91 us (the bias's distances are a third of
+// Measured, as the query gradients: 245 us and 92 us (the bias's distances are a third of
 // the latter); two waves a SIMD up to 64 features (177 us without), one above.
 #include "attn_common.h"
 

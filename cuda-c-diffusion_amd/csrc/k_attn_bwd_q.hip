@@ -6,18 +6,22 @@
 // q and dout in registers, and goes over the blocks of keys as the forward kernel does.
 //
 // M comes from the forward pass's lse and D from <dout, out>, both of which that pass
-// rounded.  The sums of p and of p dp are taken along, and their exact results are what
-// the key gradients and the bias gradient use (stat).  Where all keys of the workgroup
-// lie in one block they are there before it is used, and the query gradient takes them
-// too: a query that sees a single key then gets a gradient of exactly zero.
+// rounded (out to the tensors' type: for bf16 D is off by up to 2^-8 of <|dout|, |out|>).  The
+// sums of p and of p dp are taken along, and their exact results are what the key gradients
+// and the bias gradient use (stat).  The query gradient would need them before its pass: two
+// of its three products a second time, or sums of p k beside those of dx k (a third more
+// products, 64 more registers at 128 features).  So a query whose softmax is nearly all one
+// key's gets a dq that is off by that rounding times k, against a dq near zero.  Where all
+// keys of the workgroup lie in one block of 64 the sums are there before they are used, and
+// the query gradient takes them too: a query that sees a single key then gets exactly zero.
 //
 // SPLIT 2, for calls of few workgroups: 64 queries, and of each block 32 keys a wave; the
 // two waves of the same queries are added up at the end, in their order.  Fewer still: the
 // keys are divided too, each part leaves fp32 sums, and a second kernel adds them in order.
 //
-// Measured: 8192 packed causal tokens, 16 heads of 128 (4 of keys), capped: 203 us; 4 x 1024
-// tokens, 16 heads of 64 with a bias: 53 us.  128 features take one wave a SIMD, whose
-// products (13 % of cycles) and vector instructions (35 %) do not overlap.
+// Measured: 8192 packed causal tokens, 16 heads of 128 (4 of keys), capped: 204 us; 4 x 1024
+// tokens, 16 heads of 64 with a bias: 54 us.  128 features take one wave a SIMD, whose
+// products (16 % of cycles) and vector instructions (34 %) do not overlap.
 #include "attn_common.h"
 
 namespace {

@@ -9,8 +9,9 @@
 // order, so the sum does not depend on who is last, and leaves the ticket at zero).
 //
 // Measured: 16 requests of 12288 to 32768 keys, 32 heads of 128 (8 of keys), bf16: 294 us, 4.57
-// TB/s of the cache (a copy reaches 4.77, read and written); one request of 777 keys 8.2 us,
-// of which a launch is about 5.
+// TB/s of the cache (an elementwise stream reaches 6.2, read and written); one request of 777
+// keys 8.3 us, of which a launch is about 5.  The same in fp32, one wave a SIMD: 862 us, 3.1
+// TB/s; 11.3 us.
 #include "attn_common.h"
 
 namespace {

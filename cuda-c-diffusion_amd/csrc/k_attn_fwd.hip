@@ -23,10 +23,11 @@
 //           polynomial, of 4 terms instead of 6 below 0.14 of it;
 //   else:   running maximum of x.
 //
-// Measured: 16384 tokens, 16 heads of 128 (4 of keys), a prefix, capped scores: 1500 us, 779
-// TFLOP/s of visible scores; vector instructions take 45 %, products 31 % of the SIMDs'
-// cycles, two waves a SIMD overlapping a third of the latter.  8192 packed tokens, 16 heads
-// of 72, 13 documents: 83 us, 338 TFLOP/s, two launches for the documents among it.
+// Measured: 16384 tokens, 16 heads of 128 (4 of keys), a prefix, scores of deviation 1 under a
+// cap of 50: 1454-1481 us, 790-804 TFLOP/s of visible scores; vector instructions take 56 %,
+// products 36 % of the SIMDs' cycles.  Of deviation 12, where most blocks go without the
+// series: 2328 us.  8192 packed tokens, 16 heads of 72, 13 documents: 84 us, 335 TFLOP/s, two
+// launches for the documents among it.
 #include "attn_common.h"
 
 namespace {
@@ -387,7 +388,10 @@ __global__ __launch_bounds__(64) void block_docs_kernel(int4* out, const int* do
 }
 
 // A request's tiles of `own` positions by falling number of blocks that they meet on the
-// other axis, ties by their number.
+// other axis, ties by their number.  One workgroup counts a request's pairs of a tile and a
+// block, up to 64 of them a thread; more (from some 23000 packed tokens on) go in their own
+// order.  That limit is of the counting, not of its use: 32768 packed tokens of 16 heads of 72
+// took 399 us with an order and 411 without, a training step of 24576 causal ones 1395 and 1481.
 constexpr int kOrderTpb = 1024, kOrderBlocks = 1024, kOrderTiles = 512;
 __global__ __launch_bounds__(kOrderTpb) void tile_order_kernel(int* order, Args a, bool keys, int own, int tiles) {
     __shared__ int4 other[kOrderBlocks];

@@ -13,8 +13,9 @@
 // of the time as element-wise reads).  A workgroup takes whole tokens, whose sines and
 // cosines it forms once, first all their queries, then their keys.
 //
-// Measured: 32768 tokens, 32 + 8 heads of 128, bf16: forward 140 us (4.8 TB/s), backward 231
-// us (4.4); eight images of 64 x 64 tokens, 16 + 16 heads of 64, fp32: 102 us (5.2 TB/s).
+// Measured: 32768 tokens, 32 + 8 heads of 128, bf16: forward 140-151 us (4.4-4.8 TB/s),
+// backward 231-244 us (4.1-4.4; 68 bytes a lane of scratch); eight images of 64 x 64 tokens,
+// 16 + 16 heads of 64, fp32: 102 us (5.3 TB/s).
 #include "nn_attention.h"
 #include "nnk_common.h"
 

@@ -10,11 +10,17 @@
  * host memory and read during the call only.
  *
  * Tensors hold fp32 or bf16 values; sums, softmax statistics, norms and the
- * gradients of weights and biases are fp32 (or wider) for both.  The last
- * dimension of every tensor is contiguous; the other strides are the caller's,
- * counted in elements, so that the parts of one projection's rows, and caches
- * with a head's tokens together, are read where they lie.  Pointers and strides
- * that are multiples of 16 bytes (with head_dim * size too) get 16-byte
+ * gradients of weights and biases are fp32 (or wider) for both.  With bf16
+ * tensors two things are rounded to bf16 before a sum: the probabilities and score
+ * gradients that are multiplied with values, queries, keys and dout (each by up to
+ * 2^-8 of itself, which about adds the result's own rounding once more), and the
+ * output from which dq takes its row sum <dout, out> (dk, dv and dbias take an fp32
+ * one).
+ *
+ * The last dimension of every tensor is contiguous; the other strides are the
+ * caller's, counted in elements, so that the parts of one projection's rows, and
+ * caches with a head's tokens together, are read where they lie.  Pointers and
+ * strides that are multiples of 16 bytes (with head_dim * size too) get 16-byte
  * accesses; any others are taken element by element, slower.
  *
  * What a call reads may repeat rows (strides of 0); what it writes, outputs and
