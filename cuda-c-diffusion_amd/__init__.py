@@ -2,7 +2,7 @@
 
 The library is the product: gfx950 HIP kernels behind the C-ABI launch layer
 of ``include/nn_hip.h`` (the reference's ``launch_*`` entry points, reference
-src/nn.h:348-466) and of ``include/nn_attention.h`` plus the C host modules of ``include/nn_modules.h``.  This
+src/nn.h:348-466), ``include/nn_attention.h`` and ``include/nn_cache.h`` plus the C host modules of ``include/nn_modules.h``.  This
 module only binds that C-ABI with ctypes so that Python tests and the bench
 can drive it; device memory, copies, streams and events come from the
 library's own plumbing (``include/nn_hip_rt.h``), so no other GPU runtime is
@@ -35,6 +35,8 @@ ACT_NAMES = {"identity": 0, "relu": 1, "gelu": 2, "silu": 3, "tanh": 4, "mp_silu
 # Types and masks of the attention operators (include/nn_attention.h)
 NN_F32, NN_BF16 = range(2)
 NN_MASK_NONE, NN_MASK_CAUSAL, NN_MASK_PREFIX = range(3)
+# Kinds of a paged cache (include/nn_cache.h)
+NN_CACHE_PLAIN, NN_CACHE_MXFP4 = range(2)
 
 
 class NnHipError(RuntimeError):
@@ -66,7 +68,28 @@ class NnAttention(C.Structure):
                 ("q_start", P), ("k_len", P), ("prefix", P), ("doc_q", P), ("doc_k", P), ("bucket", P), ("bias", P)]
 
 
+class NnCache(C.Structure):
+    """Mirror of NnCache in include/nn_cache.h (pass the structure itself)."""
+
+    _fields_ = [("kind", I), ("page_tokens", I), ("pages", I), ("requests", I), ("table_pages", I), ("table", P),
+                ("k", P), ("v", P)]
+
+
+class NnCacheAppend(C.Structure):
+    """Mirror of NnCacheAppend in include/nn_cache.h (pass the structure itself)."""
+
+    _fields_ = [("rope", NnQkNormRope), ("norm", I), ("v_stride", LL * 2), ("request", P), ("place", P)]
+
+
+class NnCacheRead(C.Structure):
+    """Mirror of NnCacheRead in include/nn_cache.h (pass the structure itself)."""
+
+    _fields_ = [("dtype", I), ("tokens", I), ("kv_heads", I), ("head_dim", I), ("k_stride", LL * 2), ("v_stride", LL * 2),
+                ("request", P), ("place", P)]
+
+
 ROPE, ATTN = C.POINTER(NnQkNormRope), C.POINTER(NnAttention)
+CACHE, APPEND, READ = C.POINTER(NnCache), C.POINTER(NnCacheAppend), C.POINTER(NnCacheRead)
 
 # name -> (restype, argtypes, is_launcher)
 _SIGS = {
@@ -171,6 +194,12 @@ _SIGS = {
     "launch_attention_forward": (None, [P] * 5 + [ATTN, P, P], True),
     "nnhip_attention_backward_workspace": (SZ, [ATTN], True),
     "launch_attention_backward": (None, [P] * 10 + [ATTN, P, P], True),
+    # the paged cache (nn_cache.h)
+    "nnhip_cache_page_bytes": (SZ, [CACHE, I, I, I], True),
+    "launch_cache_append": (None, [P] * 4 + [APPEND, CACHE, P], True),
+    "launch_cache_read": (None, [P, P, READ, CACHE, P], True),
+    "nnhip_cache_attention_workspace": (SZ, [ATTN, CACHE], True),
+    "launch_cache_attention_forward": (None, [P] * 3 + [ATTN, CACHE, P, P], True),
 }
 
 

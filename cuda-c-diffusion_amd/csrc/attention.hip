@@ -113,8 +113,28 @@ bool sizes_fit(const NnAttention* a, bool backward, const char* what) {
     return true;
 }
 
-// Fills `p` for the call's description; false after recording an error.
-bool take(Args& p, const NnAttention* a, bool backward, const char* what) {
+// Whether the rows of a tensor that the call writes lie apart; false after recording an error.
+bool rows_apart(const long long* stride, int batch, int len, int heads, int dim, const char* name, const char* what) {
+    const long long n[3] = {batch, len, heads};
+    NNK_REQUIRE_RET(nnk_rows_apart(3, stride, n, dim), false, what, "%s: rows of %s overlap (strides %lld, %lld, %lld)", what,
+        name, stride[0], stride[1], stride[2]);
+    return true;
+}
+
+// Whether rows of 16-byte chunks can be read and written: strides here, pointers by the
+// callers.  The offsets of 64 rows have to fit in 32 bits.
+bool strides_by_16(const NnAttention* a) {
+    const long long e = a->dtype == NN_BF16 ? 8 : 4, far = (1LL << 32) / (16 / e) / 64 - 128;
+    bool ok = a->head_dim % e == 0;
+    for (int i = 0; i < 3; ++i)
+        for (const long long* s : {a->q_stride, a->k_stride, a->v_stride, a->out_stride})
+            ok = ok && s[i] % e == 0 && (i != 1 || (s[i] >= 0 && s[i] <= far));
+    return ok;
+}
+
+}  // namespace
+
+bool nnk_attention_take(Args& p, const NnAttention* a, bool backward, const char* what) {
     if (!sizes_fit(a, backward, what)) return false;
     NNK_REQUIRE_RET(a->scale > 0.0f && a->scale < INFINITY, false, what, "%s: scale=%g is not positive", what, a->scale);
     NNK_REQUIRE_RET(a->softcap >= 0.0f && a->softcap < INFINITY, false, what, "%s: softcap=%g is negative", what,
@@ -183,27 +203,6 @@ bool take(Args& p, const NnAttention* a, bool backward, const char* what) {
     return true;
 }
 
-// Whether the rows of a tensor that the call writes lie apart; false after recording an error.
-bool rows_apart(const long long* stride, int batch, int len, int heads, int dim, const char* name, const char* what) {
-    const long long n[3] = {batch, len, heads};
-    NNK_REQUIRE_RET(nnk_rows_apart(3, stride, n, dim), false, what, "%s: rows of %s overlap (strides %lld, %lld, %lld)", what,
-        name, stride[0], stride[1], stride[2]);
-    return true;
-}
-
-// Whether rows of 16-byte chunks can be read and written: strides here, pointers by the
-// callers.  The offsets of 64 rows have to fit in 32 bits.
-bool strides_by_16(const NnAttention* a) {
-    const long long e = a->dtype == NN_BF16 ? 8 : 4, far = (1LL << 32) / (16 / e) / 64 - 128;
-    bool ok = a->head_dim % e == 0;
-    for (int i = 0; i < 3; ++i)
-        for (const long long* s : {a->q_stride, a->k_stride, a->v_stride, a->out_stride})
-            ok = ok && s[i] % e == 0 && (i != 1 || (s[i] >= 0 && s[i] <= far));
-    return ok;
-}
-
-}  // namespace
-
 extern "C" {
 
 size_t nnhip_attention_forward_workspace(const NnAttention* a) {
@@ -215,7 +214,7 @@ void launch_attention_forward(void* out, float* lse, const void* q, const void* 
     const NnAttention* a, float* workspace, hipStream_t s) {
     const char* what = "launch_attention_forward";
     Args p;
-    if (!take(p, a, false, what)) return;
+    if (!nnk_attention_take(p, a, false, what)) return;
     if (!a->batch || !a->len_q) return;
     NNK_REQUIRE(out && lse && q && (!a->len_k || (k && v)), what, "%s: null pointer", what);
     if (!rows_apart(a->out_stride, a->batch, a->len_q, a->heads, a->head_dim, "out", what)) return;
@@ -248,7 +247,7 @@ void launch_attention_backward(void* dq, void* dk, void* dv, float* dbias, const
     const NnAttention* a, float* workspace, hipStream_t s) {
     const char* what = "launch_attention_backward";
     Args p;
-    if (!take(p, a, true, what)) return;
+    if (!nnk_attention_take(p, a, true, what)) return;
     NNK_REQUIRE(!dbias || a->buckets, what, "%s: a bias gradient without a bias", what);
     const bool has_q = a->batch && a->len_q, has_k = a->batch && a->len_k;
     NNK_REQUIRE(!has_q || (dq && dout && q && out && lse), what, "%s: null pointer of the queries", what);

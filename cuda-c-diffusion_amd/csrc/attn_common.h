@@ -572,6 +572,8 @@ inline bool raise_lds(const void* fn, size_t bytes, std::atomic<unsigned long lo
 
 }  // namespace attn
 
+// Fills `p` for the call's description; false after recording an error.
+bool nnk_attention_take(attn::Args& p, const NnAttention* a, bool backward, const char* what);
 // Documents of each block of 64 into `ws`, for args.key_docs and query_docs (no documents:
 // nothing).
 void nnk_attention_docs(attn::Args& args, float* ws, hipStream_t s, const char* what);
