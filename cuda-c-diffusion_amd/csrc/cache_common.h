@@ -60,3 +60,11 @@ __device__ __forceinline__ void values8(unsigned code, float scale, f32x2 (&v)[4
 // Fills `p` from the description; false after recording an error.  `pools`: whether the
 // pointers are looked at.
 bool nnk_cache_take(cache::Pages& p, const NnCache* c, int dtype, int kv_heads, int head_dim, bool pools, const char* what);
+// Attention of few queries: one launch; the floats that a call takes, its tickets among them,
+// and a bound on them for every smaller batch and fewer queries or keys.
+namespace attn {
+struct Args;
+}
+size_t nnk_cache_few_floats(const NnAttention* a);
+size_t nnk_cache_few_most(const NnAttention* a);
+void nnk_cache_few(const attn::Args& a, const cache::Pages& p, const NnAttention* d, float* ws, hipStream_t s, const char* what);
