@@ -22,6 +22,7 @@ bool nnk_cache_take(cache::Pages& p, const NnCache* c, int dtype, int kv_heads, 
     p.scales = n * p.row_bytes;
     p.block_bytes = p.scales + n * p.groups;
     p.page_bytes = (long long)p.block_bytes * kv_heads;
+    NNK_REQUIRE_RET(p.page_bytes < 1LL << 32, false, what, "%s: a page of %lld bytes is too large", what, p.page_bytes);
     while (1 << p.shift < n) ++p.shift;
     p.pages = c->pages;
     p.requests = c->requests;

@@ -24,7 +24,6 @@ using cache::Pages;
 constexpr int kKeys = 32;       // keys of a wave at a time
 constexpr int kTile = 16;       // queries, or keys, of a tile
 constexpr int kHalves = kKeys / kTile;
-constexpr int kMaxSplits = 64;
 constexpr float kSlack = 8.0f;  // units of log2 that a score may be above the reference
 
 typedef cache::bf16x2 bf16x2;
@@ -35,33 +34,81 @@ __device__ __forceinline__ f32x4 mma16(bf16x8 a, bf16x8 b, f32x4 c) {
 __device__ __forceinline__ f32x4 mma16(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
 // Over the four lanes of a column.
+__device__ __forceinline__ Halves rows16(float v) {
+    const unsigned u = __builtin_bit_cast(unsigned, v);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const unsigned lower = r[0], upper = r[1];
+    return {__builtin_bit_cast(float, lower), __builtin_bit_cast(float, upper)};
+}
 __device__ __forceinline__ float max_column(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16));
-    return max_halves(v);
+    const Halves x = rows16(v);
+    return max_halves(fmaxf(x.lower, x.upper));
 }
 __device__ __forceinline__ float sum_column(float v) {
-    v += __shfl_xor(v, 16);
-    return sum_halves(v);
+    const Halves x = rows16(v);
+    return sum_halves(x.lower + x.upper);
 }
 
 // Where 16 keys lie: uniform.
 struct Place {
-    long long row, scale;  // byte of the first one's row and scales, either pool
+    unsigned long long byte;  // of the head's block in the page, either pool
+    unsigned row, scale;      // of the first one's row and scales in that
     bool held;
 };
-// Block of 32 keys from k0 on.  The table is read through the scalar cache.
-typedef const __attribute__((address_space(4))) int* Table;
-__device__ __forceinline__ void find(Place (&at)[kHalves], const Pages& p, int b, int kv, int k0) {
-#pragma unroll
-    for (int x = 0; x < kHalves; ++x) {
-        const int key = k0 + x * kTile, i = min(key >> p.shift, p.table_pages - 1);
-        const int page = ((Table)p.table)[(size_t)b * p.table_pages + i];
-        at[x].held = (unsigned)page < (unsigned)p.pages;
-        const long long block = p.block_at(at[x].held ? page : 0, kv);
-        at[x].row = block + (long long)p.slot_of(key) * p.row_bytes;
-        at[x].scale = block + p.scales + p.slot_of(key) * p.groups;
+// The blocks of 32 keys of a wave, kStep apart: the entries of 64 of them are read at a time, a
+// lane each, and handed out lane by lane (a scalar load for each made its wave wait, LDS reads
+// among it).
+constexpr int kStep = kWaves * kKeys;
+struct Blocks32 {
+    const int* table;
+    unsigned long long block;  // the head's byte in a page
+    int entry[kHalves], n;
+    __device__ __forceinline__ void look(const Pages& p, int k0, int lane) {
+        const int last = p.table_pages - 1, key = k0 + lane * kStep;
+        entry[0] = table[min(key >> p.shift, last)];
+        entry[1] = p.shift > 4 ? entry[0] : table[min((key + kTile) >> p.shift, last)];
     }
+    __device__ __forceinline__ Blocks32(const Pages& p, int b, int kv, int k0, int lane)
+        : table(p.table + (size_t)b * p.table_pages), block((unsigned long long)kv * (unsigned)p.block_bytes), n(0) {
+        look(p, k0, lane);
+    }
+    // The next block, which begins at k0.
+    __device__ __forceinline__ void next(Place (&at)[kHalves], const Pages& p, int k0, int lane) {
+        if (n == 64) {
+            look(p, k0, lane);
+            n = 0;
+        }
+        const auto place = [&](Place& x, int entry, int key) {
+            const unsigned page = __builtin_amdgcn_readlane(entry, n);
+            x.held = page < (unsigned)p.pages;
+            x.byte = (unsigned long long)(x.held ? page : 0u) * (unsigned)p.page_bytes + block;
+            x.row = p.slot_of(key) * p.row_bytes;
+            x.scale = p.scales + p.slot_of(key) * p.groups;
+        };
+        place(at[0], entry[0], k0);
+        if (p.shift > 4) {  // one page has both halves
+            at[1] = at[0];
+            at[1].row += kTile * p.row_bytes;
+            at[1].scale += kTile * p.groups;
+        } else {
+            place(at[1], entry[1], k0 + kTile);
+        }
+        ++n;
+    }
+};
+// A uniform address, for the loads' scalar operand: by itself the compiler adds the lane's offset
+// to the pool once and the place to that, 64 bits a lane, for every load.
+typedef const __attribute__((address_space(1))) char* Bytes;
+__device__ __forceinline__ Bytes at_place(const char* pool, unsigned long long byte, unsigned offset) {
+    Bytes q = (Bytes)pool + byte + offset;
+    asm("" : "+s"(q));
+    return q;
 }
+template <typename V>
+__device__ __forceinline__ V read(Bytes q, unsigned offset) {
+    return *reinterpret_cast<const __attribute__((address_space(1))) V*>(q + offset);
+}
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
 // Three bf16 parts of 8 fp32 values.
 template <int PARTS>
@@ -93,21 +140,24 @@ struct Values {
         return (r & 1) * 5 | (r & 2) | (r & 4) << 1;
     }
     static __device__ __forceinline__ int at(int row, int chunk) { return row * kRowBytes + ((chunk ^ S(row)) << 4); }
-    // This lane's part of the transposing reads of features 16 d ..: keys 4 h .. 4 h + 3 and 16 more
-    static __device__ __forceinline__ bf16x8 columns(const char* t, int d, int lane) {
-        typedef __attribute__((address_space(3))) i16x4* LdsPtr;
-        const int row = lane >> 2, chunk = 2 * d + (lane >> 1 & 1), byte = (lane & 1) * 8;
-        const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(t + at(row, chunk) + byte));
-        const i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(t + at(row + kTile, chunk) + byte));
+    // A tile begins at a multiple of kAlign bytes, so that chunk c ^ x is at the address of c with x
+    // in its bits: one register and an instruction instead of a register for each.
+    static constexpr int kAlign = 512;
+    // This lane's part of the transposing reads: keys 4 h .. 4 h + 3 and 16 more of features 16 d ..
+    static __device__ __forceinline__ unsigned column_base(int lane) { return at(lane >> 2, lane >> 1 & 1) + (lane & 1) * 8; }
+    static __device__ __forceinline__ bf16x8 columns(unsigned base, int d) {
+        const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(uintptr_t)(base ^ d << 5));
+        const i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(uintptr_t)((base ^ d << 5) + kTile * kRowBytes));
         const bf16x4 x = __builtin_bit_cast(bf16x4, a), y = __builtin_bit_cast(bf16x4, b);
         return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
     }
 };
+__device__ __forceinline__ void lds_write(unsigned at, u32x4 v) { *(__attribute__((address_space(3))) u32x4*)(uintptr_t)at = v; }
 
 template <int DP>
 struct Mxfp4 {
     typedef bf16x8 Frag;
-    static constexpr int kWaves = 2;  // a SIMD, at least
+    static constexpr bool kFourBits = true;
     static constexpr int kSteps = DP / 32;       // products of a tile of scores
     static constexpr int kGroups = DP / 32;      // scales of a row
     static constexpr int kWords = DP / 32;       // of 8 features: a lane's of a key
@@ -126,17 +176,37 @@ struct Mxfp4 {
         const unsigned row = lane & 15, h = lane >> 4;
 #pragma unroll
         for (int x = 0; x < kHalves; ++x) {
-            __builtin_memcpy(k[x], __builtin_assume_aligned(p.k + at[x].row + (row * (DP / 2) + h * (DP / 8)), DP == 128 ? 16 : DP == 64 ? 8 : 4), DP / 8);
+            const Bytes rows = at_place(p.k, at[x].byte, at[x].row), scales = at_place(p.k, at[x].byte, at[x].scale);
+            const unsigned from = row * (DP / 2) + h * (DP / 8);
+            if constexpr (DP == 128) {
+                const u32x4 y = read<u32x4>(rows, from);
 #pragma unroll
-            for (int u = 0; u < kScales; ++u)
-                ks[x][u] = *reinterpret_cast<const unsigned char*>(p.k + at[x].scale + (row * kGroups + feature(h, u) / 32));
+                for (int u = 0; u < kWords; ++u) k[x][u] = y[u];
+            } else if constexpr (DP == 64) {
+                const u32x2 y = read<u32x2>(rows, from);
+                k[x][0] = y[0];
+                k[x][1] = y[1];
+            } else {
+#pragma unroll
+                for (int u = 0; u < kWords; ++u) k[x][u] = read<unsigned>(rows, from + 4 * u);
+            }
+#pragma unroll
+            for (int u = 0; u < kScales; ++u) ks[x][u] = read<unsigned char>(scales, row * kGroups + feature(h, u) / 32);
         }
 #pragma unroll
         for (int n = 0; n < kChunks; ++n) {
             const int c = min(chunk(n, lane), kKeys * kGroups - 1), key = c / kGroups, g = c % kGroups;
-            const bool upper = key >= kTile;
-            v[n] = *reinterpret_cast<const u32x4*>(p.v + (upper ? at[1].row : at[0].row) + (unsigned)((key & 15) * (DP / 2) + g * 16));
-            vs[n] = *reinterpret_cast<const unsigned char*>(p.v + (upper ? at[1].scale : at[0].scale) + (unsigned)((key & 15) * kGroups + g));
+            const unsigned r = (key & 15) * (DP / 2) + g * 16, sc = (key & 15) * kGroups + g;
+            if constexpr (kTile * kGroups % 64 == 0) {  // 16 keys are whole chunks of a wave
+                constexpr int kEach = kTile * kGroups / 64;
+                v[n] = read<u32x4>(at_place(p.v, at[n / kEach].byte, at[n / kEach].row), r);
+                vs[n] = read<unsigned char>(at_place(p.v, at[n / kEach].byte, at[n / kEach].scale), sc);
+            } else {
+                const Bytes rows0 = at_place(p.v, at[0].byte, at[0].row), rows1 = at_place(p.v, at[1].byte, at[1].row);
+                const Bytes scales0 = at_place(p.v, at[0].byte, at[0].scale), scales1 = at_place(p.v, at[1].byte, at[1].scale);
+                v[n] = read<u32x4>(key < kTile ? rows0 : rows1, r);
+                vs[n] = read<unsigned char>(key < kTile ? scales0 : scales1, sc);
+            }
         }
     }
     __device__ __forceinline__ Frag key(int x, int u) const {
@@ -144,20 +214,26 @@ struct Mxfp4 {
         cache::values8(k[x][u], cache::scale_of(ks[x][kScales > 1 ? u : 0]), y);
         return __builtin_bit_cast(Frag, y);
     }
+    // The lane's first chunk of a tile at `lds`.
+    static __device__ __forceinline__ unsigned store_base(unsigned lds, int lane) {
+        return lds + Values<DP>::at(lane / kGroups, 4 * (lane % kGroups));
+    }
     // keep(key): whether it is one that a query sees
     template <typename Keep>
-    __device__ __forceinline__ void store(char* lds, int lane, bool all, const Keep& keep) const {
+    __device__ __forceinline__ void store(unsigned lds, unsigned base, int lane, const Keep& keep) const {
 #pragma unroll
         for (int n = 0; n < kChunks; ++n) {
             const int c = chunk(n, lane), key = c / kGroups, g = c % kGroups;
             if (kKeys * kGroups % 64 && c >= kKeys * kGroups) continue;
-            const bool some = all || keep(key);
+            // 16 keys on, the order of chunks is the same
+            const unsigned to = 64 / kGroups % kTile ? lds + Values<DP>::at(key, 4 * g) : base + n * (64 / kGroups) * Values<DP>::kRowBytes;
+            const bool some = keep(key);
             const float scale = some ? cache::scale_of(vs[n]) : 1.0f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 bf16x2 y[4];
                 cache::values8(some ? v[n][i] : 0u, scale, y);
-                *reinterpret_cast<u32x4*>(lds + Values<DP>::at(key, 4 * g + i)) = __builtin_bit_cast(u32x4, y);
+                lds_write(to ^ i << 4, __builtin_bit_cast(u32x4, y));
             }
         }
     }
@@ -166,7 +242,7 @@ struct Mxfp4 {
 template <int DP>
 struct Bf16 {
     typedef bf16x8 Frag;
-    static constexpr int kWaves = 2;
+    static constexpr bool kFourBits = false;
     static constexpr int kSteps = DP / 32;
     static constexpr int kPerRow = DP / 8;
     static constexpr int kChunks = kKeys * kPerRow / 64;
@@ -181,21 +257,34 @@ struct Bf16 {
         for (int x = 0; x < kHalves; ++x)
 #pragma unroll
             for (int u = 0; u < kSteps; ++u)  // past the features: some of the row's, which meet zeros
-                k[x][u] = *reinterpret_cast<const u32x4*>(p.k + at[x].row + (row * p.row_bytes + min((unsigned)feature(h, u) * 2, last)));
+                k[x][u] = read<u32x4>(at_place(p.k, at[x].byte, at[x].row), row * p.row_bytes + min((unsigned)feature(h, u) * 2, last));
 #pragma unroll
         for (int n = 0; n < kChunks; ++n) {
             const int c = n * 64 + lane, key = c / kPerRow;
-            v[n] = *reinterpret_cast<const u32x4*>(p.v + (key >= kTile ? at[1].row : at[0].row) +
-                ((unsigned)(key & 15) * p.row_bytes + min((unsigned)(c % kPerRow) * 16, last)));
+            const unsigned r = (unsigned)(key & 15) * p.row_bytes + min((unsigned)(c % kPerRow) * 16, last);
+            if constexpr (kTile * kPerRow % 64 == 0) {  // 16 keys are whole chunks of a wave
+                const Place& x = at[n / (kTile * kPerRow / 64)];
+                v[n] = read<u32x4>(at_place(p.v, x.byte, x.row), r);
+            } else {
+                const Bytes rows0 = at_place(p.v, at[0].byte, at[0].row), rows1 = at_place(p.v, at[1].byte, at[1].row);
+                v[n] = read<u32x4>(key < kTile ? rows0 : rows1, r);
+            }
         }
     }
     __device__ __forceinline__ Frag key(int x, int u) const { return __builtin_bit_cast(Frag, k[x][u]); }
+    static __device__ __forceinline__ unsigned store_base(unsigned lds, int lane) {
+        return lds + Values<DP>::at(lane / kPerRow, lane % kPerRow);
+    }
     template <typename Keep>
-    __device__ __forceinline__ void store(char* lds, int lane, bool all, const Keep& keep) const {
+    __device__ __forceinline__ void store(unsigned lds, unsigned base, int lane, const Keep& keep) const {
 #pragma unroll
         for (int n = 0; n < kChunks; ++n) {
             const int c = n * 64 + lane, key = c / kPerRow;
-            *reinterpret_cast<u32x4*>(lds + Values<DP>::at(key, c % kPerRow)) = all || keep(key) ? v[n] : u32x4{0, 0, 0, 0};
+            // rows of a power of two: only bits of S change
+            constexpr int kRowsOn = 64 / kPerRow;
+            const unsigned to = 64 % kPerRow ? lds + Values<DP>::at(key, c % kPerRow)
+                                             : (base ^ (Values<DP>::S(n * kRowsOn) << 4)) + n * kRowsOn * Values<DP>::kRowBytes;
+            lds_write(to, keep(key) ? v[n] : u32x4{0, 0, 0, 0});
         }
     }
 };
@@ -205,7 +294,6 @@ struct Bf16 {
 template <int DP>
 struct F32 {
     typedef float Frag;
-    static constexpr int kWaves = 1;
     static constexpr int kSteps = DP / 4;
     static constexpr int kLds = 16;
     f32x4 k[kHalves][DP / 16];
@@ -219,12 +307,12 @@ struct F32 {
         for (int x = 0; x < kHalves; ++x) {
 #pragma unroll
             for (int u = 0; u < DP / 16; ++u)
-                k[x][u] = *reinterpret_cast<const f32x4*>(p.k + at[x].row + (row * p.row_bytes + min(64 * u + 16 * h, last)));
+                k[x][u] = read<f32x4>(at_place(p.k, at[x].byte, at[x].row), row * p.row_bytes + min(64 * u + 16 * h, last));
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
                 for (int d = 0; d < DP / 16; ++d)
-                    v[x][j][d] = *reinterpret_cast<const float*>(p.v + at[x].row + ((4 * h + j) * p.row_bytes + min(64 * d + 4 * row, last + 12)));
+                    v[x][j][d] = read<float>(at_place(p.v, at[x].byte, at[x].row), (4 * h + j) * p.row_bytes + min(64 * d + 4 * row, last + 12));
         }
     }
     __device__ __forceinline__ Frag key(int x, int u) const { return k[x][u / 4][u % 4]; }
@@ -242,374 +330,528 @@ __device__ __forceinline__ float2 taken(const float* p) {
     return make_float2(__builtin_bit_cast(float, (unsigned)v), __builtin_bit_cast(float, (unsigned)(v >> 32)));
 }
 
+// The work of a launch is a row of steps: of all requests, all their key heads and tiles of
+// queries (a unit each), and its keys, 128 a step.  Every workgroup has an equal share of it, which may
+// be the end of a unit, whole units and the beginning of another; requests' lengths are on
+// the device, so shares are formed there, by every workgroup for itself.  A unit that more
+// than one share has a part of is joined from their partial results.
 struct Few {
-    unsigned* tickets;
-    float* partial;  // [units, splits, rows, DP + 2]: outputs, then reference (units of log2) and sum
-    int tiles, splits, each;  // tiles of a key head's queries; workgroups of a unit; their keys
+    unsigned* tickets;  // a unit each
+    float* partial;     // [workers, 2, rows, DP + 2]: outputs, then reference (units of log2) and sum; of a
+                        // unit that began before the share, and of one that goes on behind it
+    int tiles;          // of a key head's queries
+    int workers;        // shares; 0: a workgroup a unit
 };
+constexpr int kMostParts = 64;  // of a unit
 
-template <typename T, template <int> class PAGES, int DP, int NT>
-__global__ __launch_bounds__(kTpb, PAGES<DP>::kWaves) void cache_few_kernel(Args a, Pages p, Few f) {
+// Steps of a unit of request b: those of its last query, one at least.
+__device__ __forceinline__ int steps_of(const Args& a, const Pages& p, int b) {
+    const int keys = p.pages ? keys_of(a, b) : 0;
+    return max(1, (limit_of(a, b, keys, start_of(a, b) + a.len_q - 1) + kStep - 1) / kStep);
+}
+// Inclusive sums over the lanes.
+__device__ __forceinline__ long long scan(long long v, int lane) {
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        const long long y = __shfl_up(v, m);
+        if (lane >= m) v += y;
+    }
+    return v;
+}
+__device__ __forceinline__ long long uniform(long long v, int lane) {
+    const unsigned lo = __builtin_amdgcn_readlane((int)v, lane), hi = __builtin_amdgcn_readlane((int)(v >> 32), lane);
+    return (long long)((unsigned long long)hi << 32 | lo);
+}
+// A share: where in a request's units it begins, and its end.
+struct Share {
+    long long first, last;  // steps
+    long long each;         // of every share
+    long long before;       // steps of the requests before `request`
+    int request, steps;     // steps of a unit of it
+};
+__device__ __forceinline__ void share_of(Share& x, const Args& a, const Pages& p, const Few& f, int worker, int lane) {
+    const long long units = (long long)a.kv_heads * f.tiles;
+    long long total = 0;
+    int most = 1;
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+        const int n = b0 + lane < a.batch ? steps_of(a, p, b0 + lane) : 0;
+        total += uniform(scan(n, lane), 63);
+        most = max(most, n);
+    }
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) most = max(most, __shfl_xor(most, m));
+    most = __builtin_amdgcn_readfirstlane(most);
+    total *= units;
+    const long long even = (total + f.workers - 1) / f.workers;
+    x.each = max(uniform(even, 0), (long long)((most + kMostParts - 2) / (kMostParts - 1)));
+    x.first = worker * x.each;
+    x.last = min(x.first + x.each, total);
+    x.before = 0;
+    x.request = 0;
+    if (x.first >= x.last) return;
+    for (int b0 = 0;; b0 += 64) {
+        const int n = b0 + lane < a.batch ? steps_of(a, p, b0 + lane) : 0;
+        const long long sum = x.before + scan(n, lane) * units;
+        const unsigned long long behind = __ballot(sum > x.first);
+        if (behind) {
+            const int i = __builtin_ctzll(behind);
+            x.steps = __builtin_amdgcn_readlane(n, i);
+            x.request = b0 + i;
+            x.before = uniform(sum, i) - x.steps * units;
+            return;
+        }
+        x.before = uniform(sum, 63);
+    }
+}
+
+// The call.  What only the beginning and the end of a share need is read again there: held over the
+// keys' loop it was some 130 scalar registers too many, which go to lanes of vector registers.
+struct All {  // the kernel's only argument
+    Args a;
+    Pages p;
+    Few f;
+};
+__device__ __forceinline__ All call_again() {
+    auto q = __builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(q));
+    All all;
+    __builtin_memcpy(&all, (const void*)q, sizeof all);
+    return all;
+}
+
+// Workgroups a CU, which is waves a SIMD: as many as their registers allow.
+template <typename T, typename E, int NT>
+constexpr int held_by_a_cu() {
+    if constexpr (std::is_same_v<typename E::Frag, float>) return 1;
+    else return sizeof(T) == 2 && NT == 1 && E::kFourBits ? 3 : 2;
+}
+
+// TERMS: scores have a cap or a bias
+template <typename T, template <int> class PAGES, int DP, int NT, bool TERMS>
+__global__ __launch_bounds__(kTpb, (held_by_a_cu<T, PAGES<DP>, NT>())) void cache_few_kernel(All) {
     using E = PAGES<DP>;
     constexpr bool kWide = std::is_same_v<typename E::Frag, bf16x8>;     // bf16 products
     constexpr int kParts = kWide && sizeof(T) == 4 ? 3 : 1;              // of a query or probability
     constexpr int kRowsEach = kTile * NT;
     constexpr int kRow = DP + 4;  // floats of an output row in LDS
-    constexpr int kShared = E::kLds > kTile * kRow * 4 ? E::kLds : kTile * kRow * 4;
-    __shared__ __attribute__((aligned(16))) char lds[kWaves][kShared];
+    constexpr int kUsed = E::kLds > kTile * kRow * 4 ? E::kLds : kTile * kRow * 4;
+    constexpr int kShared = (kUsed + Values<DP>::kAlign - 1) / Values<DP>::kAlign * Values<DP>::kAlign;
+    __shared__ __attribute__((aligned(Values<DP>::kAlign))) char lds[kWaves][kShared];
     __shared__ float m_lds[kWaves][kRowsEach], l_lds[kWaves][kRowsEach];
-    __shared__ float weight[kRowsEach][kMaxSplits];
+    __shared__ float weight[kRowsEach][kMostParts];
     __shared__ float total[kRowsEach];
     __shared__ int last_one;
 
     const int lane = threadIdx.x & 63, h = lane >> 4, col = lane & 15, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int split = blockIdx.x % f.splits, unit = blockIdx.x / f.splits;
-    const int tile = unit % f.tiles, kv = unit / f.tiles % a.kv_heads, b = unit / f.tiles / a.kv_heads;
-    const int rows = min(kRowsEach, a.len_q * a.group - tile * kRowsEach);
-    const int keys = p.pages ? keys_of(a, b) : 0, start = start_of(a, b);
-    const int most = limit_of(a, b, keys, start + (tile * kRowsEach + rows - 1) / a.group);
-    const int active = max(1, (most + f.each - 1) / f.each);  // workgroups of the unit that have keys
-    if (split >= active) return;
+    Share share;
+    long long units;  // of a request
+    {
+    const auto [a, p, f] = call_again();
+    units = (long long)a.kv_heads * f.tiles;
+    if (f.workers) {
+        share_of(share, a, p, f, blockIdx.x, lane);
+        if (share.first >= share.last) return;
+    } else {
+        share.request = __builtin_amdgcn_readfirstlane((int)(blockIdx.x / units));
+        share.steps = __builtin_amdgcn_readfirstlane(steps_of(a, p, share.request));
+        share.before = 0;
+        share.first = (blockIdx.x - share.request * units) * share.steps;
+        share.last = share.first + share.steps;
+        share.each = 1LL << 62;
+    }
+    }
 
-    int pos[NT], limit[NT], head[NT], least = INT32_MAX;
-    typename E::Frag qf[NT][kParts][E::kSteps];
+    for (long long g = share.first;;) {
+        const All now = call_again();
+        const Args& a = now.a;
+        const Pages& p = now.p;
+        const Few& f = now.f;
+        const int b = share.request;
+        const long long begin = g - share.before;
+        // divisions are vector instructions: what is uniform says so
+        const int unit = __builtin_amdgcn_readfirstlane((int)(begin / share.steps));
+        const int step0 = (int)(begin - (long long)unit * share.steps);
+        const int step1 = (int)min((long long)share.steps, step0 + (share.last - g));
+        const int kv = __builtin_amdgcn_readfirstlane(unit / f.tiles), tile = unit - kv * f.tiles;
+        const int rows = min(kRowsEach, a.len_q * a.group - tile * kRowsEach);
+        const int keys = __builtin_amdgcn_readfirstlane(p.pages ? keys_of(a, b) : 0), start = __builtin_amdgcn_readfirstlane(start_of(a, b));
+        const int most = __builtin_amdgcn_readfirstlane(limit_of(a, b, keys, start + (tile * kRowsEach + rows - 1) / a.group));
+
+        int pos[NT], limit[NT], head[NT], least = INT32_MAX;
+        typename E::Frag qf[NT][kParts][E::kSteps];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const bool in = t * kTile + col < rows;
-        const int row = tile * kRowsEach + (in ? t * kTile + col : 0), i = row / a.group;
-        head[t] = kv * a.group + row - i * a.group;
-        pos[t] = start + i;
-        limit[t] = in ? limit_of(a, b, keys, pos[t]) : 0;
-        if (in) least = min(least, limit[t]);
-        const T* q = (const T*)a.q + b * a.qs[0] + i * a.qs[1] + head[t] * a.qs[2];
-        if constexpr (kWide) {
+        for (int t = 0; t < NT; ++t) {
+            const bool in = t * kTile + col < rows;
+            const int row = tile * kRowsEach + (in ? t * kTile + col : 0), i = row / a.group;
+            head[t] = kv * a.group + row - i * a.group;
+            pos[t] = start + i;
+            limit[t] = in ? limit_of(a, b, keys, pos[t]) : 0;
+            if (in) least = min(least, limit[t]);
+            const T* q = (const T*)a.q + b * a.qs[0] + i * a.qs[1] + head[t] * a.qs[2];
+            if constexpr (kWide) {
 #pragma unroll
-            for (int u = 0; u < E::kSteps; ++u) {
-                const int d0 = E::feature(h, u);
-                if constexpr (kParts == 1) {
-                    qf[t][0][u] = a.vec ? load_frag<bf16, true>((const bf16*)q, d0, a.dim) : load_frag<bf16, false>((const bf16*)q, d0, a.dim);
-                } else {
-                    float x[8];
-                    bf16x8 y[kParts];
+                for (int u = 0; u < E::kSteps; ++u) {
+                    const int d0 = E::feature(h, u);
+                    if constexpr (kParts == 1) {
+                        qf[t][0][u] = a.vec ? load_frag<bf16, true>((const bf16*)q, d0, a.dim) : load_frag<bf16, false>((const bf16*)q, d0, a.dim);
+                    } else {
+                        float x[8];
+                        bf16x8 y[kParts];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) x[j] = d0 + j < a.dim ? (float)q[d0 + j] : 0.0f;
-                    parts_of<kParts>(x, y);
+                        for (int j = 0; j < 8; ++j) x[j] = d0 + j < a.dim ? (float)q[d0 + j] : 0.0f;
+                        parts_of<kParts>(x, y);
 #pragma unroll
-                    for (int n = 0; n < kParts; ++n) qf[t][n][u] = y[n];
+                        for (int n = 0; n < kParts; ++n) qf[t][n][u] = y[n];
+                    }
                 }
-            }
-        } else {
+            } else {
 #pragma unroll
-            for (int u = 0; u < E::kSteps; ++u) qf[t][0][u] = E::feature(h, u) < a.dim ? (float)q[E::feature(h, u)] : 0.0f;
+                for (int u = 0; u < E::kSteps; ++u) qf[t][0][u] = E::feature(h, u) < a.dim ? (float)q[E::feature(h, u)] : 0.0f;
+            }
         }
-    }
 #pragma unroll
-    for (int m = 1; m < kTile; m <<= 1) least = min(least, __shfl_xor(least, m));
-    least = __builtin_amdgcn_readfirstlane(least);
+        for (int m = 1; m < kTile; m <<= 1) least = min(least, __shfl_xor(least, m));
+        least = __builtin_amdgcn_readfirstlane(least);
 
-    const auto bias_of = [&](int rel, int of_head) {
-        const int i = min(max(rel, -a.max_distance), a.max_distance) + a.max_distance;
-        return a.bias[(size_t)min(max(a.bucket[i], 0), a.buckets - 1) * a.heads + of_head] * kLog2e;
-    };
-    float far[NT];  // bias of keys max_distance or more before the query
+        const auto bias_of = [&](int rel, int of_head) {
+            const int i = min(max(rel, -a.max_distance), a.max_distance) + a.max_distance;
+            return a.bias[(size_t)min(max(a.bucket[i], 0), a.buckets - 1) * a.heads + of_head] * kLog2e;
+        };
+        [[maybe_unused]] float far[NT];  // bias of keys max_distance or more before the query
+        if constexpr (TERMS) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) far[t] = a.buckets ? bias_of(-a.max_distance, head[t]) : 0.0f;
-    const bool plain = a.c2 == 0.0f && !a.buckets;
-    const float unit_of = plain ? a.c1 : 1.0f;  // what a score is multiplied with in the exponent
+            for (int t = 0; t < NT; ++t) far[t] = a.buckets ? bias_of(-a.max_distance, head[t]) : 0.0f;
+        }
+        const float unit_of = TERMS ? 1.0f : a.c1;  // what a score is multiplied with in the exponent
 
-    f32x4 o[NT][DP / 16];
-    float m[NT], l[NT];
+        f32x4 o[NT][DP / 16];
+        float m[NT], l[NT];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
+        for (int t = 0; t < NT; ++t) {
 #pragma unroll
-        for (int d = 0; d < DP / 16; ++d) o[t][d] = f32x4{0, 0, 0, 0};
-        m[t] = -INFINITY;
-        l[t] = 0.0f;
-    }
+            for (int d = 0; d < DP / 16; ++d) o[t][d] = f32x4{0, 0, 0, 0};
+            m[t] = -INFINITY;
+            l[t] = 0.0f;
+        }
 
-    // this wave's blocks of the workgroup's keys
-    const int end = min(most, (split + 1) * f.each);
-    E e;
-    Place at[kHalves], next[kHalves];
-    int k0 = split * f.each + wave * kKeys;
-    if (k0 < end) {
-        find(at, p, b, kv, k0);
-        e.load(at, p, lane);
-        find(next, p, b, kv, k0 + kWaves * kKeys);
-    }
-    for (; k0 < end; k0 += kWaves * kKeys) {
-        const bool held = at[0].held && at[1].held, all = held && k0 + kKeys <= keys;
-        const bool held0 = at[0].held, held1 = at[1].held;
-        [[maybe_unused]] char* values = lds[wave];
-        f32x4 s[NT][kHalves];
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int x = 0; x < kHalves; ++x) s[t][x] = f32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int x = 0; x < kHalves; ++x)
-#pragma unroll
-            for (int u = 0; u < E::kSteps; ++u) {
-                const typename E::Frag y = e.key(x, u);
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int n = kParts - 1; n >= 0; --n) s[t][x] = mma16(y, qf[t][n][u], s[t][x]);
-            }
-        const auto keep = [&](int key) { return k0 + key < keys && (key < kTile ? held0 : held1); };
-        [[maybe_unused]] float v[kWide ? 1 : kHalves][4][kWide ? 1 : DP / 16];
+        [[maybe_unused]] const unsigned values = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)lds[wave];
+        unsigned to_values = 0, of_columns = 0;
         if constexpr (kWide) {
-            e.store(values, lane, all, keep);
-        } else {
+            to_values = E::store_base(values, lane);
+            of_columns = values + Values<DP>::column_base(lane);
+        }
+
+        // this wave's blocks of the steps
+        const int end = min(most, step1 * kStep);
+        int k0 = step0 * kStep + wave * kKeys;
+        E e;
+        Place at[kHalves];
+        Blocks32 blocks(p, b, kv, k0 < end ? k0 : 0, lane);
+        if (k0 < end) {
+            blocks.next(at, p, k0, lane);
+            e.load(at, p, lane);
+        }
+        for (; k0 < end; k0 += kStep) {
+            const bool held0 = at[0].held, held1 = at[1].held, all = held0 && held1 && k0 + kKeys <= keys;
+            // (kept from taking a register for every address over the loop)
+            asm volatile("" : "+v"(to_values), "+v"(of_columns));
+            f32x4 s[NT][kHalves];
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int x = 0; x < kHalves; ++x) s[t][x] = f32x4{0, 0, 0, 0};
 #pragma unroll
             for (int x = 0; x < kHalves; ++x)
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                for (int u = 0; u < E::kSteps; ++u) {
+                    const typename E::Frag y = e.key(x, u);
 #pragma unroll
-                    for (int d = 0; d < DP / 16; ++d) v[x][j][d] = all || keep(x * kTile + 4 * h + j) ? e.v[x][j][d] : 0.0f;
-        }
-        // the next block's, while this one's scores become shares
-        at[0] = next[0];
-        at[1] = next[1];
-        if (k0 + kWaves * kKeys < end) {
-            e.load(at, p, lane);
-            find(next, p, b, kv, k0 + 2 * kWaves * kKeys);
-        }
-
+                    for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            if (a.c2 != 0.0f) {
-                float top = 0.0f;
-#pragma unroll
-                for (int x = 0; x < kHalves; ++x)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        s[t][x][j] *= a.c1;
-                        top = fmaxf(top, fabsf(s[t][x][j]));
-                    }
-                if (__all(top < kSeriesEnd)) {
-#pragma unroll
-                    for (int x = 0; x < kHalves; ++x)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) s[t][x][j] = tanh_series(s[t][x][j]) * a.c2;
-                } else {
-#pragma unroll
-                    for (int x = 0; x < kHalves; ++x)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const float y = s[t][x][j], r = __builtin_amdgcn_rcpf(exp2_fast(fabsf(y) * (2.0f * kLog2e)) + 1.0f);
-                            s[t][x][j] = (fabsf(y) < kSeriesEnd ? tanh_series(y) : copysignf(fmaf(-2.0f, r, 1.0f), y)) * a.c2;
-                        }
+                        for (int n = kParts - 1; n >= 0; --n) s[t][x] = mma16(y, qf[t][n][u], s[t][x]);
                 }
-            }
-            if (a.buckets) {
-                const float c = a.c2 != 0.0f ? 1.0f : a.c1;
-                if (__all(k0 + kKeys - 1 - pos[t] <= -a.max_distance)) {
-#pragma unroll
-                    for (int x = 0; x < kHalves; ++x)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) s[t][x][j] = s[t][x][j] * c + far[t];
-                } else {
-#pragma unroll
-                    for (int x = 0; x < kHalves; ++x)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            s[t][x][j] = s[t][x][j] * c + bias_of(k0 + x * kTile + 4 * h + j - pos[t], head[t]);
-                }
-            }
-            if (!held || k0 + kKeys > least) {
+            const auto keep = [&](int key) { return k0 + key < keys && (key < kTile ? held0 : held1); };
+            [[maybe_unused]] float v[kWide ? 1 : kHalves][4][kWide ? 1 : DP / 16];
+            if constexpr (kWide) {
+                if (all) e.store(values, to_values, lane, [](int) { return true; });
+                else e.store(values, to_values, lane, keep);
+            } else {
 #pragma unroll
                 for (int x = 0; x < kHalves; ++x)
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        s[t][x][j] = k0 + x * kTile + 4 * h + j < limit[t] && (x ? held1 : held0) ? s[t][x][j] : -INFINITY;
+#pragma unroll
+                        for (int d = 0; d < DP / 16; ++d) v[x][j][d] = all || keep(x * kTile + 4 * h + j) ? e.v[x][j][d] : 0.0f;
             }
-            float top = -INFINITY;
-#pragma unroll
-            for (int x = 0; x < kHalves; ++x)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) top = fmaxf(top, s[t][x][j]);
-            top = max_column(top) * unit_of;
-            // the reference follows the largest score when that has left it behind
-            if (__any(top > m[t] + kSlack)) {
-                const float to = fmaxf(m[t], top), g = exp2_fast(m[t] - (to == -INFINITY ? 0.0f : to));
-                l[t] *= g;
-#pragma unroll
-                for (int d = 0; d < DP / 16; ++d) o[t][d] *= g;
-                m[t] = to;
+            // the next block's, while this one's scores become shares
+            if (k0 + kStep < end) {
+                blocks.next(at, p, k0 + kStep, lane);
+                e.load(at, p, lane);
             }
-            const float base = m[t] == -INFINITY ? 0.0f : m[t];
-#pragma unroll
-            for (int x = 0; x < kHalves; ++x)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    s[t][x][j] = exp2_fast(fmaf(s[t][x][j], unit_of, -base));
-                    l[t] += s[t][x][j];
-                }
-        }
-        if constexpr (kWide) {
-            bf16x8 shares[NT][kParts];
+
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                float x[8];
+                if constexpr (TERMS) {
+                    if (a.c2 != 0.0f) {
+                        float top = 0.0f;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = s[t][j / 4][j % 4];
-                parts_of<kParts>(x, shares[t]);
+                        for (int x = 0; x < kHalves; ++x)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(s[t][x][j]));
+                        if (__all(top < a.tiny)) {
+#pragma unroll
+                            for (int x = 0; x < kHalves; ++x)
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) s[t][x][j] = cap_series<4>(s[t][x][j], a);
+                        } else if (__all(top < a.small)) {
+#pragma unroll
+                            for (int x = 0; x < kHalves; ++x)
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) s[t][x][j] = cap_series<6>(s[t][x][j], a);
+                        } else {
+#pragma unroll
+                            for (int x = 0; x < kHalves; ++x)
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    const float y = s[t][x][j] * a.c1, r = __builtin_amdgcn_rcpf(exp2_fast(fabsf(y) * (2.0f * kLog2e)) + 1.0f);
+                                    s[t][x][j] = (fabsf(y) < kSeriesEnd ? tanh_series(y) : copysignf(fmaf(-2.0f, r, 1.0f), y)) * a.c2;
+                                }
+                        }
+                    }
+                    if (a.buckets) {
+                        const float c = a.c2 != 0.0f ? 1.0f : a.c1;
+                        if (__all(k0 + kKeys - 1 - pos[t] <= -a.max_distance)) {
+#pragma unroll
+                            for (int x = 0; x < kHalves; ++x)
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) s[t][x][j] = s[t][x][j] * c + far[t];
+                        } else {
+#pragma unroll
+                            for (int x = 0; x < kHalves; ++x)
+#pragma unroll
+                                for (int j = 0; j < 4; ++j)
+                                    s[t][x][j] = s[t][x][j] * c + bias_of(k0 + x * kTile + 4 * h + j - pos[t], head[t]);
+                        }
+                    }
+                }
+                if (!held0 || !held1 || k0 + kKeys > least) {
+#pragma unroll
+                    for (int x = 0; x < kHalves; ++x)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            s[t][x][j] = k0 + x * kTile + 4 * h + j < limit[t] && (x ? held1 : held0) ? s[t][x][j] : -INFINITY;
+                }
+                float top = -INFINITY;
+#pragma unroll
+                for (int x = 0; x < kHalves; ++x)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) top = fmaxf(top, s[t][x][j]);
+                top = max_column(top) * unit_of;
+                // the reference follows the largest score when that has left it behind
+                if (__any(top > m[t] + kSlack)) {
+                    const float to = fmaxf(m[t], top), by = exp2_fast(m[t] - (to == -INFINITY ? 0.0f : to));
+                    l[t] *= by;
+#pragma unroll
+                    for (int d = 0; d < DP / 16; ++d) o[t][d] *= by;
+                    m[t] = to;
+                }
+                const float base = m[t] == -INFINITY ? 0.0f : m[t];
+#pragma unroll
+                for (int x = 0; x < kHalves; ++x)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        s[t][x][j] = exp2_fast(TERMS ? s[t][x][j] - base : fmaf(s[t][x][j], unit_of, -base));
+                        l[t] += s[t][x][j];
+                    }
             }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
+            if constexpr (kWide) {
+                bf16x8 shares[NT][kParts];
 #pragma unroll
-            for (int d = 0; d < DP / 16; ++d) {
-                const bf16x8 y = Values<DP>::columns(values, d, lane);
+                for (int t = 0; t < NT; ++t) {
+                    float x[8];
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
+                    for (int j = 0; j < 8; ++j) x[j] = s[t][j / 4][j % 4];
+                    parts_of<kParts>(x, shares[t]);
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
 #pragma unroll
-                    for (int n = kParts - 1; n >= 0; --n) o[t][d] = mma16(y, shares[t][n], o[t][d]);
-            }
-            // the next values are written over these when they have been read
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-        } else {
+                for (int d = 0; d < DP / 16; ++d) {
+                    const bf16x8 y = Values<DP>::columns(of_columns, d);
 #pragma unroll
-            for (int x = 0; x < kHalves; ++x)
+                    for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int d = 0; d < DP / 16; ++d)
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) o[t][d] = mma16(v[x][j][d], s[t][x][j], o[t][d]);
-        }
-    }
-
-    // the waves of the workgroup, a tile of queries at a time
-    constexpr int kQuads = DP / 4;  // 4 features a thread
-    const size_t step = kRowsEach * (DP + 2);
-    float* to = f.partial + ((size_t)unit * f.splits + split) * step;
-    const auto finish = [&](int r, int d, float4 x, float ref, float sum) {
-        const int n = tile * kRowsEach + r, qi = n / a.group, hd = kv * a.group + n - qi * a.group;
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        T* out = (T*)a.out + b * a.os[0] + qi * a.os[1] + hd * a.os[2];
-        if (a.vec) store4<T, true>(out, d, a.dim, x.x * inv, x.y * inv, x.z * inv, x.w * inv);
-        else store4<T, false>(out, d, a.dim, x.x * inv, x.y * inv, x.z * inv, x.w * inv);
-        if (d == 0)
-            a.lse[((size_t)b * a.heads + hd) * a.len_q + qi] = sum == 0.0f ? -INFINITY : (ref + log2f(sum)) * kLn2;
-    };
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        if (t * kTile >= rows) break;
-        const float sum = sum_column(l[t]);
-        if (t) __syncthreads();
-        float* mine = reinterpret_cast<float*>(lds[wave]) + col * kRow;
-#pragma unroll
-        for (int d = 0; d < DP / 16; ++d) *reinterpret_cast<f32x4*>(mine + 16 * d + 4 * h) = o[t][d];
-        if (h == 0) {
-            m_lds[wave][t * kTile + col] = m[t];
-            l_lds[wave][t * kTile + col] = sum;
-        }
-        __syncthreads();
-        for (int n = threadIdx.x; n < min(kTile, rows - t * kTile) * kQuads; n += kTpb) {
-            const int c = n / kQuads, r = t * kTile + c, d = n % kQuads * 4;
-            float ref = m_lds[0][r];
-#pragma unroll
-            for (int w = 1; w < kWaves; ++w) ref = fmaxf(ref, m_lds[w][r]);
-            float all = 0.0f;
-            float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-            for (int w = 0; w < kWaves; ++w) {
-                const float g = ref == -INFINITY ? 0.0f : exp2_fast(m_lds[w][r] - ref);
-                const float4 y = nnk::ld4(reinterpret_cast<const float*>(lds[w]) + c * kRow + d);
-                all = fmaf(l_lds[w][r], g, all);
-                x.x = fmaf(y.x, g, x.x);
-                x.y = fmaf(y.y, g, x.y);
-                x.z = fmaf(y.z, g, x.z);
-                x.w = fmaf(y.w, g, x.w);
-            }
-            if (active == 1) {
-                finish(r, d, x, ref, all);
+                        for (int n = kParts - 1; n >= 0; --n) o[t][d] = mma16(y, shares[t][n], o[t][d]);
+                }
+                // the next values are written over these when they have been read
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
             } else {
-                float* q = to + r * (DP + 2);
-                hand(q + d, x.x, x.y);
-                hand(q + d + 2, x.z, x.w);
-                if (d == 0) hand(q + DP, ref, all);
+#pragma unroll
+                for (int x = 0; x < kHalves; ++x)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int d = 0; d < DP / 16; ++d)
+#pragma unroll
+                            for (int t = 0; t < NT; ++t) o[t][d] = mma16(v[x][j][d], s[t][x][j], o[t][d]);
             }
         }
-    }
-    if (active == 1) return;
 
-    // the workgroups of the unit
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // handed over
-    __syncthreads();
-    if (threadIdx.x == 0)
-        last_one = __hip_atomic_fetch_add(f.tickets + unit, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
-            (unsigned)(active - 1);
-    __syncthreads();
-    if (!last_one) return;
-    const float* from = f.partial + (size_t)unit * f.splits * step;
-    for (int r = wave; r < rows; r += kWaves) {  // a lane a split: their shares of the row
-        float ms = -INFINITY, ls = 0.0f;
-        if (lane < active) {
-            const float2 y = taken(from + lane * step + r * (DP + 2) + DP);
-            ms = y.x;
-            ls = y.y;
-        }
-        float ref = ms;
+        // The shares that the unit has parts in.
+        const All after = call_again();
+        const auto close = [&](const Args& a, const Pages& p, const Few& f) {
+        const long long unit_at = share.before + (long long)unit * share.steps;
+        const int worker0 = f.workers ? (int)(unit_at / share.each) : 0;
+        const int parts = f.workers ? (int)((unit_at + share.steps - 1) / share.each) - worker0 + 1 : 1;
+        const long long step = kRowsEach * (DP + 2);
+        const auto partial_of = [&](int part) {  // its first part goes on behind its share
+            return f.partial + (2LL * (worker0 + part) + (part == 0)) * step;
+        };
+
+        // the waves of the workgroup, a tile of queries at a time
+        constexpr int kQuads = DP / 4;  // 4 features a thread
+        const auto finish = [&](int r, int d, float4 x, float ref, float sum) {
+            const int n = tile * kRowsEach + r, qi = n / a.group, hd = kv * a.group + n - qi * a.group;
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            T* out = (T*)a.out + b * a.os[0] + qi * a.os[1] + hd * a.os[2];
+            if (a.vec) store4<T, true>(out, d, a.dim, x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+            else store4<T, false>(out, d, a.dim, x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+            if (d == 0)
+                a.lse[((size_t)b * a.heads + hd) * a.len_q + qi] = sum == 0.0f ? -INFINITY : (ref + log2f(sum)) * kLn2;
+        };
 #pragma unroll
-        for (int x = 1; x < 64; x <<= 1) ref = fmaxf(ref, __shfl_xor(ref, x));
-        const float g = ref == -INFINITY ? 0.0f : exp2_fast(ms - ref);
-        weight[r][lane] = g;
-        const float sum = nnk::wave_sum(ls * g);
-        if (lane == 0) {
-            m_lds[0][r] = ref;
-            total[r] = sum;
+        for (int t = 0; t < NT; ++t) {
+            if (t * kTile >= rows) break;
+            const float sum = sum_column(l[t]);
+            if (t) __syncthreads();
+            float* mine = reinterpret_cast<float*>(lds[wave]) + col * kRow;
+#pragma unroll
+            for (int d = 0; d < DP / 16; ++d) *reinterpret_cast<f32x4*>(mine + 16 * d + 4 * h) = o[t][d];
+            if (h == 0) {
+                m_lds[wave][t * kTile + col] = m[t];
+                l_lds[wave][t * kTile + col] = sum;
+            }
+            __syncthreads();
+            for (int n = threadIdx.x; n < min(kTile, rows - t * kTile) * kQuads; n += kTpb) {
+                const int c = n / kQuads, r = t * kTile + c, d = n % kQuads * 4;
+                float ref = m_lds[0][r];
+#pragma unroll
+                for (int w = 1; w < kWaves; ++w) ref = fmaxf(ref, m_lds[w][r]);
+                float all = 0.0f;
+                float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) {
+                    const float by = ref == -INFINITY ? 0.0f : exp2_fast(m_lds[w][r] - ref);
+                    const float4 y = nnk::ld4(reinterpret_cast<const float*>(lds[w]) + c * kRow + d);
+                    all = fmaf(l_lds[w][r], by, all);
+                    x.x = fmaf(y.x, by, x.x);
+                    x.y = fmaf(y.y, by, x.y);
+                    x.z = fmaf(y.z, by, x.z);
+                    x.w = fmaf(y.w, by, x.w);
+                }
+                if (parts == 1) {
+                    finish(r, d, x, ref, all);
+                } else {
+                    float* to = partial_of((int)blockIdx.x - worker0) + r * (DP + 2);
+                    hand(to + d, x.x, x.y);
+                    hand(to + d + 2, x.z, x.w);
+                    if (d == 0) hand(to + DP, ref, all);
+                }
+            }
         }
-    }
-    __syncthreads();
-    for (int n = threadIdx.x; n < rows * kQuads; n += kTpb) {
-        const int r = n / kQuads, d = n % kQuads * 4;
-        const float* q = from + r * (DP + 2) + d;
-        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+
+        if (parts > 1) {  // the workgroups of the unit
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // handed over
+            __syncthreads();
+            unsigned* ticket = f.tickets + (size_t)b * units + unit;
+            if (threadIdx.x == 0)
+                last_one = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(parts - 1);
+            __syncthreads();
+            if (last_one) {
+                for (int r = wave; r < rows; r += kWaves) {  // a lane a part: their shares of the row
+                    float ms = -INFINITY, ls = 0.0f;
+                    if (lane < parts) {
+                        const float2 y = taken(partial_of(lane) + r * (DP + 2) + DP);
+                        ms = y.x;
+                        ls = y.y;
+                    }
+                    float ref = ms;
+#pragma unroll
+                    for (int x = 1; x < 64; x <<= 1) ref = fmaxf(ref, __shfl_xor(ref, x));
+                    const float by = ref == -INFINITY ? 0.0f : exp2_fast(ms - ref);
+                    weight[r][lane] = by;
+                    const float sum = nnk::wave_sum(ls * by);
+                    if (lane == 0) {
+                        m_lds[0][r] = ref;
+                        total[r] = sum;
+                    }
+                }
+                __syncthreads();
+                for (int n = threadIdx.x; n < rows * kQuads; n += kTpb) {
+                    const int r = n / kQuads, d = n % kQuads * 4;
+                    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-        for (int sp = 0; sp < active; ++sp) {
-            const float g = weight[r][sp];
-            const float2 y = taken(q + sp * step), z = taken(q + sp * step + 2);
-            x.x = fmaf(y.x, g, x.x);
-            x.y = fmaf(y.y, g, x.y);
-            x.z = fmaf(z.x, g, x.z);
-            x.w = fmaf(z.y, g, x.w);
+                    for (int part = 0; part < parts; ++part) {
+                        const float by = weight[r][part];
+                        const float* q = partial_of(part) + r * (DP + 2) + d;
+                        const float2 y = taken(q), z = taken(q + 2);
+                        x.x = fmaf(y.x, by, x.x);
+                        x.y = fmaf(y.y, by, x.y);
+                        x.z = fmaf(z.x, by, x.z);
+                        x.w = fmaf(z.y, by, x.w);
+                    }
+                    finish(r, d, x, m_lds[0][r], total[r]);
+                }
+                if (threadIdx.x == 0) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
         }
-        finish(r, d, x, m_lds[0][r], total[r]);
+
+        g += step1 - step0;
+        if (g < share.last && unit + 1 == units && step1 == share.steps) {
+            share.before += units * share.steps;
+            share.request += 1;
+            share.steps = __builtin_amdgcn_readfirstlane(steps_of(a, p, share.request));
+        }
+        };
+        close(after.a, after.p, after.f);
+        if (g >= share.last) return;
+        __syncthreads();  // LDS is read
     }
-    if (threadIdx.x == 0) __hip_atomic_store(f.tickets + unit, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// Tiles of queries, and how the keys are split: enough workgroups to fill the card several
-// times over (requests' lengths differ, and those without keys of theirs end at once), a block
-// a wave at least.
+// Tiles of queries, and workgroups: as many as the card holds at once, kWorkers at most.
+constexpr int kWorkers = 3 * kCus;
 struct Plan {
     long long units;
-    int tiles, rows, splits, each;
+    int tiles, rows, workers;
 };
 Plan plan_of(const NnAttention* a) {
     Plan p;
-    const long long rows = (long long)a->len_q * (a->heads / a->kv_heads);
+    const long long rows = (long long)a->len_q * (a->heads / a->kv_heads), steps = std::max(1, (a->len_k + kStep - 1) / kStep);
     p.rows = rows <= kTile ? kTile : 2 * kTile;
     p.tiles = (int)((rows + p.rows - 1) / p.rows);
     p.units = (long long)a->batch * a->kv_heads * p.tiles;
-    const int step = kWaves * kKeys, steps = std::max(1, (a->len_k + step - 1) / step);
-    const long long want = p.units >= kTicketWords ? 1 : std::min<long long>(kMaxSplits, (2 * kTicketWords + p.units - 1) / p.units);
-    const int n = (int)((steps + want - 1) / want);
-    p.each = n * step;
-    p.splits = (steps + n - 1) / n;
+    p.workers = p.units > kTicketWords || steps == 1 ? 0 : (int)std::min<long long>(kWorkers, p.units * steps);
     return p;
 }
 int padded(int dim) { return (dim + 31) / 32 * 32; }
 
 template <typename T, template <int> class PAGES, int DP>
 void launch(const Args& a, const Pages& p, const Plan& plan, float* ws, hipStream_t s, const char* what) {
-    const Few f = {reinterpret_cast<unsigned*>(ws), ws + kTicketWords, plan.tiles, plan.splits, plan.each};
-    const unsigned blocks = (unsigned)(plan.units * plan.splits);
-    if (plan.rows == kTile) cache_few_kernel<T, PAGES, DP, 1><<<blocks, kTpb, 0, s>>>(a, p, f);
-    else cache_few_kernel<T, PAGES, DP, 2><<<blocks, kTpb, 0, s>>>(a, p, f);
+    const auto with = [&](auto tiles, auto terms) {
+        constexpr int NT = decltype(tiles)::value;
+        const int workers = plan.workers ? std::min(plan.workers, kCus * held_by_a_cu<T, PAGES<DP>, NT>()) : 0;
+        const All all = {a, p, {reinterpret_cast<unsigned*>(ws), ws + kTicketWords, plan.tiles, workers}};
+        cache_few_kernel<T, PAGES, DP, NT, decltype(terms)::value>
+            <<<workers ? (unsigned)workers : (unsigned)plan.units, kTpb, 0, s>>>(all);
+    };
+    const auto by_terms = [&](auto tiles) {
+        if (a.c2 != 0.0f || a.buckets) with(tiles, std::true_type{});
+        else with(tiles, std::false_type{});
+    };
+    if (plan.rows == kTile) by_terms(std::integral_constant<int, 1>{});
+    else by_terms(std::integral_constant<int, 2>{});
     nnk_after_launch(what, s);
 }
 template <typename T, template <int> class PAGES>
@@ -628,11 +870,18 @@ void by_dim(const Args& a, const Pages& p, const Plan& plan, float* ws, hipStrea
 size_t nnk_cache_few_floats(const NnAttention* a) {
     if (!a->batch || !a->len_q) return 0;
     const Plan p = plan_of(a);
-    return p.splits == 1 ? 0 : kTicketWords + (size_t)p.units * p.splits * p.rows * (padded(a->head_dim) + 2);
+    return p.workers ? kTicketWords + 2 * (size_t)p.workers * p.rows * (padded(a->head_dim) + 2) : 0;
+}
+// Every smaller call has fewer units, steps and rows.
+size_t nnk_cache_few_most(const NnAttention* a) {
+    if (!a->batch || !a->len_q || a->len_k <= kStep) return 0;
+    const Plan p = plan_of(a);
+    const long long workers = p.workers ? p.workers : kWorkers;
+    return kTicketWords + 2 * (size_t)workers * p.rows * (padded(a->head_dim) + 2);
 }
 void nnk_cache_few(const Args& a, const Pages& p, const NnAttention* d, float* ws, hipStream_t s, const char* what) {
     const Plan plan = plan_of(d);
-    NNK_REQUIRE(plan.units * plan.splits < (1LL << 32) / kTpb, what, "%s: too many rows", what);
+    NNK_REQUIRE(plan.units < (1LL << 32) / kTpb, what, "%s: too many rows", what);
     if (d->dtype == NN_BF16) {
         if (p.groups) by_dim<bf16, Mxfp4>(a, p, plan, ws, s, what);
         else by_dim<bf16, Bf16>(a, p, plan, ws, s, what);
@@ -640,12 +889,4 @@ void nnk_cache_few(const Args& a, const Pages& p, const NnAttention* d, float* w
         if (p.groups) by_dim<float, Mxfp4>(a, p, plan, ws, s, what);
         else by_dim<float, F32>(a, p, plan, ws, s, what);
     }
-}
-size_t nnk_cache_few_most(const NnAttention* a) {
-    const long long steps = ((long long)a->len_k + kWaves * kKeys - 1) / (kWaves * kKeys);
-    if (steps < 2) return 0;
-    const Plan p = plan_of(a);
-    const long long units = std::min<long long>(kTicketWords - 1, p.units);
-    const long long groups = std::min(units * std::min<long long>(kMaxSplits, steps), units + 2 * kTicketWords - 1);
-    return kTicketWords + (size_t)groups * p.rows * (padded(a->head_dim) + 2);
 }
