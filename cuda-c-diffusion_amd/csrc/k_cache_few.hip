@@ -106,7 +106,7 @@ __device__ __forceinline__ Bytes at_place(const char* pool, unsigned long long b
 }
 template <typename V>
 __device__ __forceinline__ V read(Bytes q, unsigned offset) {
-    return *reinterpret_cast<const __attribute__((address_space(1))) V*>(q + offset);
+    return __builtin_nontemporal_load(reinterpret_cast<const __attribute__((address_space(1))) V*>(q + offset));
 }
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
@@ -294,6 +294,7 @@ struct Bf16 {
 template <int DP>
 struct F32 {
     typedef float Frag;
+    static constexpr bool kFourBits = false;
     static constexpr int kSteps = DP / 4;
     static constexpr int kLds = 16;
     f32x4 k[kHalves][DP / 16];
@@ -340,67 +341,63 @@ struct Few {
     float* partial;     // [workers, 2, rows, DP + 2]: outputs, then reference (units of log2) and sum; of a
                         // unit that began before the share, and of one that goes on behind it
     int tiles;          // of a key head's queries
+    int units;          // of a request: key heads and tiles
     int workers;        // shares; 0: a workgroup a unit
+    int step;           // keys of a step, kStep or, so that all steps are counted in 32 bits, a multiple
 };
 constexpr int kMostParts = 64;  // of a unit
 
 // Steps of a unit of request b: those of its last query, one at least.
-__device__ __forceinline__ int steps_of(const Args& a, const Pages& p, int b) {
+__device__ __forceinline__ int steps_of(const Args& a, const Pages& p, const Few& f, int b) {
     const int keys = p.pages ? keys_of(a, b) : 0;
-    return max(1, (limit_of(a, b, keys, start_of(a, b) + a.len_q - 1) + kStep - 1) / kStep);
+    return max(1, (int)((unsigned)(limit_of(a, b, keys, start_of(a, b) + a.len_q - 1) + f.step - 1) / (unsigned)f.step));
 }
 // Inclusive sums over the lanes.
-__device__ __forceinline__ long long scan(long long v, int lane) {
+__device__ __forceinline__ int scan(int v, int lane) {
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) {
-        const long long y = __shfl_up(v, m);
+        const int y = __shfl_up(v, m);
         if (lane >= m) v += y;
     }
     return v;
 }
-__device__ __forceinline__ long long uniform(long long v, int lane) {
-    const unsigned lo = __builtin_amdgcn_readlane((int)v, lane), hi = __builtin_amdgcn_readlane((int)(v >> 32), lane);
-    return (long long)((unsigned long long)hi << 32 | lo);
-}
 // A share: where in a request's units it begins, and its end.
 struct Share {
-    long long first, last;  // steps
-    long long each;         // of every share
-    long long before;       // steps of the requests before `request`
-    int request, steps;     // steps of a unit of it
+    int first, last;     // steps
+    int each;            // of every share
+    int before;          // steps of the requests before `request`
+    int request, steps;  // steps of a unit of it
 };
 __device__ __forceinline__ void share_of(Share& x, const Args& a, const Pages& p, const Few& f, int worker, int lane) {
-    const long long units = (long long)a.kv_heads * f.tiles;
-    long long total = 0;
-    int most = 1;
-    for (int b0 = 0; b0 < a.batch; b0 += 64) {
-        const int n = b0 + lane < a.batch ? steps_of(a, p, b0 + lane) : 0;
-        total += uniform(scan(n, lane), 63);
-        most = max(most, n);
+    const auto steps_at = [&](int b) { return b < a.batch ? steps_of(a, p, f, b) : 0; };
+    int n = steps_at(lane), sum = scan(n, lane), most = n;
+    int total = __builtin_amdgcn_readlane(sum, 63);
+    for (int b0 = 64; b0 < a.batch; b0 += 64) {
+        const int more = steps_at(b0 + lane);
+        total += __builtin_amdgcn_readlane(scan(more, lane), 63);
+        most = max(most, more);
     }
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) most = max(most, __shfl_xor(most, m));
-    most = __builtin_amdgcn_readfirstlane(most);
-    total *= units;
-    const long long even = (total + f.workers - 1) / f.workers;
-    x.each = max(uniform(even, 0), (long long)((most + kMostParts - 2) / (kMostParts - 1)));
+    const unsigned even = ((unsigned)(total * f.units) + f.workers - 1) / (unsigned)f.workers;
+    x.each = __builtin_amdgcn_readfirstlane(max((int)even, (most + kMostParts - 2) / (kMostParts - 1)));
     x.first = worker * x.each;
-    x.last = min(x.first + x.each, total);
-    x.before = 0;
-    x.request = 0;
+    x.last = min(x.first + x.each, total * f.units);
+    x.before = x.request = 0;
     if (x.first >= x.last) return;
-    for (int b0 = 0;; b0 += 64) {
-        const int n = b0 + lane < a.batch ? steps_of(a, p, b0 + lane) : 0;
-        const long long sum = x.before + scan(n, lane) * units;
-        const unsigned long long behind = __ballot(sum > x.first);
+    for (int b0 = 0;;) {
+        const unsigned long long behind = __ballot((x.before + sum * f.units) > x.first);
         if (behind) {
             const int i = __builtin_ctzll(behind);
             x.steps = __builtin_amdgcn_readlane(n, i);
             x.request = b0 + i;
-            x.before = uniform(sum, i) - x.steps * units;
+            x.before += (__builtin_amdgcn_readlane(sum, i) - x.steps) * f.units;
             return;
         }
-        x.before = uniform(sum, 63);
+        x.before += __builtin_amdgcn_readlane(sum, 63) * f.units;
+        b0 += 64;
+        n = steps_at(b0 + lane);
+        sum = scan(n, lane);
     }
 }
 
@@ -426,8 +423,9 @@ constexpr int held_by_a_cu() {
     else return sizeof(T) == 2 && NT == 1 && E::kFourBits ? 3 : 2;
 }
 
-// TERMS: scores have a cap or a bias
-template <typename T, template <int> class PAGES, int DP, int NT, bool TERMS>
+// TERMS: 0 none, 1 a cap, 2 a bias and maybe a cap (which a register or two more, and their
+// instructions, would cost the others)
+template <typename T, template <int> class PAGES, int DP, int NT, int TERMS>
 __global__ __launch_bounds__(kTpb, (held_by_a_cu<T, PAGES<DP>, NT>())) void cache_few_kernel(All) {
     using E = PAGES<DP>;
     constexpr bool kWide = std::is_same_v<typename E::Frag, bf16x8>;     // bf16 products
@@ -438,40 +436,34 @@ __global__ __launch_bounds__(kTpb, (held_by_a_cu<T, PAGES<DP>, NT>())) void cach
     constexpr int kShared = (kUsed + Values<DP>::kAlign - 1) / Values<DP>::kAlign * Values<DP>::kAlign;
     __shared__ __attribute__((aligned(Values<DP>::kAlign))) char lds[kWaves][kShared];
     __shared__ float m_lds[kWaves][kRowsEach], l_lds[kWaves][kRowsEach];
-    __shared__ float weight[kRowsEach][kMostParts];
-    __shared__ float total[kRowsEach];
     __shared__ int last_one;
 
     const int lane = threadIdx.x & 63, h = lane >> 4, col = lane & 15, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Share share;
-    long long units;  // of a request
     {
-    const auto [a, p, f] = call_again();
-    units = (long long)a.kv_heads * f.tiles;
-    if (f.workers) {
-        share_of(share, a, p, f, blockIdx.x, lane);
-        if (share.first >= share.last) return;
-    } else {
-        share.request = __builtin_amdgcn_readfirstlane((int)(blockIdx.x / units));
-        share.steps = __builtin_amdgcn_readfirstlane(steps_of(a, p, share.request));
-        share.before = 0;
-        share.first = (blockIdx.x - share.request * units) * share.steps;
-        share.last = share.first + share.steps;
-        share.each = 1LL << 62;
-    }
+        const auto [a, p, f] = call_again();
+        if (f.workers) {
+            share_of(share, a, p, f, blockIdx.x, lane);
+            if (share.first >= share.last) return;
+        } else {
+            share.request = __builtin_amdgcn_readfirstlane((int)(blockIdx.x / (unsigned)f.units));
+            share.steps = __builtin_amdgcn_readfirstlane(steps_of(a, p, f, share.request));
+            share.before = 0;
+            share.first = (blockIdx.x - share.request * f.units) * share.steps;
+            share.last = share.first + share.steps;
+            share.each = 0;
+        }
     }
 
-    for (long long g = share.first;;) {
+    for (int g = share.first;;) {
         const All now = call_again();
         const Args& a = now.a;
         const Pages& p = now.p;
         const Few& f = now.f;
-        const int b = share.request;
-        const long long begin = g - share.before;
+        const int b = share.request, begin = g - share.before;
         // divisions are vector instructions: what is uniform says so
-        const int unit = __builtin_amdgcn_readfirstlane((int)(begin / share.steps));
-        const int step0 = (int)(begin - (long long)unit * share.steps);
-        const int step1 = (int)min((long long)share.steps, step0 + (share.last - g));
+        const int unit = __builtin_amdgcn_readfirstlane((int)((unsigned)begin / (unsigned)share.steps));
+        const int step0 = begin - unit * share.steps, step1 = min(share.steps, step0 + (share.last - g));
         const int kv = __builtin_amdgcn_readfirstlane(unit / f.tiles), tile = unit - kv * f.tiles;
         const int rows = min(kRowsEach, a.len_q * a.group - tile * kRowsEach);
         const int keys = __builtin_amdgcn_readfirstlane(p.pages ? keys_of(a, b) : 0), start = __builtin_amdgcn_readfirstlane(start_of(a, b));
@@ -518,9 +510,9 @@ __global__ __launch_bounds__(kTpb, (held_by_a_cu<T, PAGES<DP>, NT>())) void cach
             return a.bias[(size_t)min(max(a.bucket[i], 0), a.buckets - 1) * a.heads + of_head] * kLog2e;
         };
         [[maybe_unused]] float far[NT];  // bias of keys max_distance or more before the query
-        if constexpr (TERMS) {
+        if constexpr (TERMS == 2) {
 #pragma unroll
-            for (int t = 0; t < NT; ++t) far[t] = a.buckets ? bias_of(-a.max_distance, head[t]) : 0.0f;
+            for (int t = 0; t < NT; ++t) far[t] = bias_of(-a.max_distance, head[t]);
         }
         const float unit_of = TERMS ? 1.0f : a.c1;  // what a score is multiplied with in the exponent
 
@@ -542,16 +534,17 @@ __global__ __launch_bounds__(kTpb, (held_by_a_cu<T, PAGES<DP>, NT>())) void cach
         }
 
         // this wave's blocks of the steps
-        const int end = min(most, step1 * kStep);
-        int k0 = step0 * kStep + wave * kKeys;
+        const int end = (int)min((long long)most, (long long)step1 * f.step);
+        int k0 = step0 * f.step + wave * kKeys;
         E e;
         Place at[kHalves];
         Blocks32 blocks(p, b, kv, k0 < end ? k0 : 0, lane);
-        if (k0 < end) {
-            blocks.next(at, p, k0, lane);
+        const auto load = [&](int from) {
+            if (from >= end) return;
+            blocks.next(at, p, from, lane);
             e.load(at, p, lane);
-        }
-        for (; k0 < end; k0 += kStep) {
+        };
+        for (load(k0); k0 < end; k0 += kStep) {
             const bool held0 = at[0].held, held1 = at[1].held, all = held0 && held1 && k0 + kKeys <= keys;
             // (kept from taking a register for every address over the loop)
             asm volatile("" : "+v"(to_values), "+v"(of_columns));
@@ -561,9 +554,9 @@ __global__ __launch_bounds__(kTpb, (held_by_a_cu<T, PAGES<DP>, NT>())) void cach
 #pragma unroll
                 for (int x = 0; x < kHalves; ++x) s[t][x] = f32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int x = 0; x < kHalves; ++x)
+            for (int u = 0; u < E::kSteps; ++u)  // the halves in turn: a product waits for the one before it
 #pragma unroll
-                for (int u = 0; u < E::kSteps; ++u) {
+                for (int x = 0; x < kHalves; ++x) {
                     const typename E::Frag y = e.key(x, u);
 #pragma unroll
                     for (int t = 0; t < NT; ++t)
@@ -575,6 +568,8 @@ __global__ __launch_bounds__(kTpb, (held_by_a_cu<T, PAGES<DP>, NT>())) void cach
             if constexpr (kWide) {
                 if (all) e.store(values, to_values, lane, [](int) { return true; });
                 else e.store(values, to_values, lane, keep);
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
             } else {
 #pragma unroll
                 for (int x = 0; x < kHalves; ++x)
@@ -584,15 +579,12 @@ __global__ __launch_bounds__(kTpb, (held_by_a_cu<T, PAGES<DP>, NT>())) void cach
                         for (int d = 0; d < DP / 16; ++d) v[x][j][d] = all || keep(x * kTile + 4 * h + j) ? e.v[x][j][d] : 0.0f;
             }
             // the next block's, while this one's scores become shares
-            if (k0 + kStep < end) {
-                blocks.next(at, p, k0 + kStep, lane);
-                e.load(at, p, lane);
-            }
+            load(k0 + kStep);
 
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 if constexpr (TERMS) {
-                    if (a.c2 != 0.0f) {
+                    if (TERMS == 1 || a.c2 != 0.0f) {
                         float top = 0.0f;
 #pragma unroll
                         for (int x = 0; x < kHalves; ++x)
@@ -618,7 +610,7 @@ __global__ __launch_bounds__(kTpb, (held_by_a_cu<T, PAGES<DP>, NT>())) void cach
                                 }
                         }
                     }
-                    if (a.buckets) {
+                    if constexpr (TERMS == 2) {
                         const float c = a.c2 != 0.0f ? 1.0f : a.c1;
                         if (__all(k0 + kKeys - 1 - pos[t] <= -a.max_distance)) {
 #pragma unroll
@@ -666,6 +658,14 @@ __global__ __launch_bounds__(kTpb, (held_by_a_cu<T, PAGES<DP>, NT>())) void cach
             }
             if constexpr (kWide) {
                 bf16x8 shares[NT][kParts];
+                struct Columns {
+                    bf16x8 x[2];
+                } columns[2];
+                const auto read_columns = [&](Columns& y, int n) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) y.x[i] = Values<DP>::columns(of_columns, 2 * n + i);
+                };
+                read_columns(columns[0], 0);
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
                     float x[8];
@@ -673,16 +673,14 @@ __global__ __launch_bounds__(kTpb, (held_by_a_cu<T, PAGES<DP>, NT>())) void cach
                     for (int j = 0; j < 8; ++j) x[j] = s[t][j / 4][j % 4];
                     parts_of<kParts>(x, shares[t]);
                 }
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                __builtin_amdgcn_wave_barrier();
+                piped<DP / 32>(columns, read_columns, [&](const Columns& y, int n) {
 #pragma unroll
-                for (int d = 0; d < DP / 16; ++d) {
-                    const bf16x8 y = Values<DP>::columns(of_columns, d);
+                    for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int t = 0; t < NT; ++t)
+                        for (int t = 0; t < NT; ++t)
 #pragma unroll
-                        for (int n = kParts - 1; n >= 0; --n) o[t][d] = mma16(y, shares[t][n], o[t][d]);
-                }
+                            for (int k = kParts - 1; k >= 0; --k) o[t][2 * n + i] = mma16(y.x[i], shares[t][k], o[t][2 * n + i]);
+                });
                 // the next values are written over these when they have been read
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                 __builtin_amdgcn_wave_barrier();
@@ -701,9 +699,12 @@ __global__ __launch_bounds__(kTpb, (held_by_a_cu<T, PAGES<DP>, NT>())) void cach
         // The shares that the unit has parts in.
         const All after = call_again();
         const auto close = [&](const Args& a, const Pages& p, const Few& f) {
-        const long long unit_at = share.before + (long long)unit * share.steps;
-        const int worker0 = f.workers ? (int)(unit_at / share.each) : 0;
-        const int parts = f.workers ? (int)((unit_at + share.steps - 1) / share.each) - worker0 + 1 : 1;
+        const unsigned unit_at = share.before + unit * share.steps;
+        int worker0 = 0, parts = 1;
+        if (f.workers) {
+            worker0 = __builtin_amdgcn_readfirstlane((int)(unit_at / (unsigned)share.each));
+            parts = __builtin_amdgcn_readfirstlane((int)((unit_at + share.steps - 1) / (unsigned)share.each)) - worker0 + 1;
+        }
         const long long step = kRowsEach * (DP + 2);
         const auto partial_of = [&](int part) {  // its first part goes on behind its share
             return f.partial + (2LL * (worker0 + part) + (part == 0)) * step;
@@ -764,54 +765,57 @@ __global__ __launch_bounds__(kTpb, (held_by_a_cu<T, PAGES<DP>, NT>())) void cach
         if (parts > 1) {  // the workgroups of the unit
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // handed over
             __syncthreads();
-            unsigned* ticket = f.tickets + (size_t)b * units + unit;
+            unsigned* ticket = f.tickets + (size_t)b * f.units + unit;
             if (threadIdx.x == 0)
                 last_one = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(parts - 1);
             __syncthreads();
             if (last_one) {
-                for (int r = wave; r < rows; r += kWaves) {  // a lane a part: their shares of the row
-                    float ms = -INFINITY, ls = 0.0f;
-                    if (lane < parts) {
-                        const float2 y = taken(partial_of(lane) + r * (DP + 2) + DP);
-                        ms = y.x;
-                        ls = y.y;
-                    }
-                    float ref = ms;
-#pragma unroll
-                    for (int x = 1; x < 64; x <<= 1) ref = fmaxf(ref, __shfl_xor(ref, x));
-                    const float by = ref == -INFINITY ? 0.0f : exp2_fast(ms - ref);
-                    weight[r][lane] = by;
-                    const float sum = nnk::wave_sum(ls * by);
-                    if (lane == 0) {
-                        m_lds[0][r] = ref;
-                        total[r] = sum;
-                    }
-                }
-                __syncthreads();
+                constexpr int kAtOnce = 8;  // parts whose loads are under way together
                 for (int n = threadIdx.x; n < rows * kQuads; n += kTpb) {
                     const int r = n / kQuads, d = n % kQuads * 4;
+                    float ref = -INFINITY, sum = 0.0f;
                     float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-                    for (int part = 0; part < parts; ++part) {
-                        const float by = weight[r][part];
-                        const float* q = partial_of(part) + r * (DP + 2) + d;
-                        const float2 y = taken(q), z = taken(q + 2);
-                        x.x = fmaf(y.x, by, x.x);
-                        x.y = fmaf(y.y, by, x.y);
-                        x.z = fmaf(z.x, by, x.z);
-                        x.w = fmaf(z.y, by, x.w);
+                    for (int part0 = 0; part0 < parts; part0 += kAtOnce) {
+                        float2 y[kAtOnce], z[kAtOnce], w[kAtOnce];
+#pragma unroll
+                        for (int i = 0; i < kAtOnce; ++i) {
+                            const float* q = partial_of(min(part0 + i, parts - 1)) + r * (DP + 2);
+                            y[i] = taken(q + d);
+                            z[i] = taken(q + d + 2);
+                            w[i] = taken(q + DP);
+                        }
+                        float top = ref;
+#pragma unroll
+                        for (int i = 0; i < kAtOnce; ++i) {
+                            if (part0 + i >= parts) w[i] = make_float2(-INFINITY, 0.0f);
+                            top = fmaxf(top, w[i].x);
+                        }
+                        const float base = top == -INFINITY ? 0.0f : top, old = exp2_fast(ref - base);
+                        sum *= old;
+                        x = make_float4(x.x * old, x.y * old, x.z * old, x.w * old);
+#pragma unroll
+                        for (int i = 0; i < kAtOnce; ++i) {
+                            if (part0 + i >= parts) continue;
+                            const float by = exp2_fast(w[i].x - base);
+                            sum = fmaf(w[i].y, by, sum);
+                            x.x = fmaf(y[i].x, by, x.x);
+                            x.y = fmaf(y[i].y, by, x.y);
+                            x.z = fmaf(z[i].x, by, x.z);
+                            x.w = fmaf(z[i].y, by, x.w);
+                        }
+                        ref = top;
                     }
-                    finish(r, d, x, m_lds[0][r], total[r]);
+                    finish(r, d, x, ref, sum);
                 }
                 if (threadIdx.x == 0) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
         }
 
         g += step1 - step0;
-        if (g < share.last && unit + 1 == units && step1 == share.steps) {
-            share.before += units * share.steps;
+        if (g < share.last && unit + 1 == f.units && step1 == share.steps) {
+            share.before += f.units * share.steps;
             share.request += 1;
-            share.steps = __builtin_amdgcn_readfirstlane(steps_of(a, p, share.request));
+            share.steps = __builtin_amdgcn_readfirstlane(steps_of(a, p, f, share.request));
         }
         };
         close(after.a, after.p, after.f);
@@ -824,7 +828,7 @@ __global__ __launch_bounds__(kTpb, (held_by_a_cu<T, PAGES<DP>, NT>())) void cach
 constexpr int kWorkers = 3 * kCus;
 struct Plan {
     long long units;
-    int tiles, rows, workers;
+    int tiles, rows, workers, step;
 };
 Plan plan_of(const NnAttention* a) {
     Plan p;
@@ -832,6 +836,8 @@ Plan plan_of(const NnAttention* a) {
     p.rows = rows <= kTile ? kTile : 2 * kTile;
     p.tiles = (int)((rows + p.rows - 1) / p.rows);
     p.units = (long long)a->batch * a->kv_heads * p.tiles;
+    p.step = kStep;
+    while (p.step < 1 << 30 && p.units * ((a->len_k + (long long)p.step - 1) / p.step + 1) >= 1LL << 30) p.step *= 2;
     p.workers = p.units > kTicketWords || steps == 1 ? 0 : (int)std::min<long long>(kWorkers, p.units * steps);
     return p;
 }
@@ -842,13 +848,14 @@ void launch(const Args& a, const Pages& p, const Plan& plan, float* ws, hipStrea
     const auto with = [&](auto tiles, auto terms) {
         constexpr int NT = decltype(tiles)::value;
         const int workers = plan.workers ? std::min(plan.workers, kCus * held_by_a_cu<T, PAGES<DP>, NT>()) : 0;
-        const All all = {a, p, {reinterpret_cast<unsigned*>(ws), ws + kTicketWords, plan.tiles, workers}};
+        const All all = {a, p, {reinterpret_cast<unsigned*>(ws), ws + kTicketWords, plan.tiles, a.kv_heads * plan.tiles, workers, plan.step}};
         cache_few_kernel<T, PAGES, DP, NT, decltype(terms)::value>
             <<<workers ? (unsigned)workers : (unsigned)plan.units, kTpb, 0, s>>>(all);
     };
     const auto by_terms = [&](auto tiles) {
-        if (a.c2 != 0.0f || a.buckets) with(tiles, std::true_type{});
-        else with(tiles, std::false_type{});
+        if (a.buckets) with(tiles, std::integral_constant<int, 2>{});
+        else if (a.c2 != 0.0f) with(tiles, std::integral_constant<int, 1>{});
+        else with(tiles, std::integral_constant<int, 0>{});
     };
     if (plan.rows == kTile) by_terms(std::integral_constant<int, 1>{});
     else by_terms(std::integral_constant<int, 2>{});

@@ -166,6 +166,16 @@ def test_long(nn, L, rng, kind, dtype, batch, len_q, len_k):
 
 
 @pytest.mark.parametrize("kind, dtype", KINDS)
+@pytest.mark.parametrize("batch, heads, kv", [(65, 4, 2), (150, 2, 1), (300, 8, 8)])
+def test_many_requests(nn, L, rng, kind, dtype, batch, heads, kv):
+    """Lengths from none to several pages, more requests than a wave has lanes, and (300 x 8) a unit a workgroup."""
+    k_len = rng.integers(0, 400, batch)
+    k_len[rng.integers(0, batch, 5)] = 0
+    c = case(dtype, batch, 1, 400, heads, kv, 32, "causal", k_len=list(k_len), q_start=list(k_len - 1))
+    run(nn, L, rng, c, kind, 64)
+
+
+@pytest.mark.parametrize("kind, dtype", KINDS)
 def test_prompt_chunk_and_steps(nn, L, rng, kind, dtype):
     """A prompt, a chunk and single tokens appended and attended to, as a program serves a request: each agrees with
     the 64-bit attention over what the cache then holds."""
