@@ -4,22 +4,27 @@
 // A key row x of head_dim features:  y = x [rsqrt(mean(x^2) + eps) w],  its pairs turned by
 // their angles;  in 4 bits then, for 32 features at a time, the least exponent e with
 // max|y| <= 7 2^e and the 8 sizes' nearest to |y| 2^-e.  Every row is read once and written
-// once: memory bounds long prompts, latency a decoding step, whose rows are therefore dealt
-// out over workgroups that make one pass each.  A row belongs to the G lanes of a group, 16
-// bytes a lane, so that sums and maxima are cross-lane steps in the group; a pair's other
-// member comes from the group's row in LDS.
+// once: memory bounds long prompts, latency a decoding step.  A row belongs to the G lanes of a
+// group, 16 bytes a lane, so that sums and maxima are cross-lane steps in the group; a pair's
+// other member comes from the group's row in LDS.  A workgroup takes the queries, the keys or the
+// values of some tokens, whose places and sines it has once.  Its groups take heads that lie
+// together and go from token to token, the next two rows on their way (a group a
+// token, 12 KB apart, was two to three times as long: the groups of all workgroups met on a few
+// of the memory's channels).  Few tokens are one a workgroup or less, a row a group.
 //
 // Keys for 4 bits are formed in 64 bits, as a code is a choice: with fp32 sums the order of
 // the additions would decide it for some values in 10^5, and with it half a step of the value.
 #include "cache_common.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 using namespace cache;
 
 constexpr int kTpb = 256;
-constexpr int kAngles = 1024;  // sines and cosines of a workgroup's tokens
+constexpr int kAngles = 512;    // sines and cosines of a workgroup's tokens
+constexpr int kMostTokensEach = 16;
 
 struct Append {
     const void *q, *k, *v;
@@ -30,18 +35,12 @@ struct Append {
     const int *pos, *request, *place;
     const double* freq;
     int tokens, heads, kv_heads, rows, dim, half, axes, per_axis, interleaved, norm;
-    int tokens_each, parts, rows_each;  // tokens of a workgroup; workgroups that share them; rows of a token that it has
+    int tokens_each;       // tokens of a workgroup
+    int q_parts, kv_parts; // workgroups that share their queries, and their keys, and their values
     float eps;
     bool vec;
 };
 
-// The code of |x| = a 2^e, a <= 7: steps of 1/2 below 2, of 1 below 4, of 2 from there.
-template <typename A>
-__device__ __forceinline__ unsigned code_of(A a) {
-    const A step = a < (A)2 ? (A)2 : a < (A)4 ? (A)1 : (A)0.5;
-    const int base = a < (A)2 ? 0 : a < (A)4 ? 2 : 4;
-    return (unsigned)min((int)rint(a * step) + base, 7);
-}
 // floor(log2 |x|), and whether the fraction is past 1.75
 __device__ __forceinline__ int exponent_of(float x, bool& past) {
     const unsigned u = __builtin_bit_cast(unsigned, x);
@@ -53,36 +52,47 @@ __device__ __forceinline__ int exponent_of(double x, bool& past) {
     past = (u & 0xfffffffffffffull) > 0xc000000000000ull;
     return (int)(u >> 52) - 1023;
 }
+// Codes of two values: the conversion rounds to the nearest, half way to even, and ends at 6.
+__device__ __forceinline__ unsigned codes_of(float x, float y, int e) {
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, x, y, __builtin_bit_cast(float, (unsigned)(e + 127) << 23), 0);
+}
+// It takes fp32, to which a 64-bit value may round onto a border that it is beside.  So |x| 2^-e in
+// steps of 2^-20, cut off, and a last bit for what was: the same choice, as borders are whole steps.
+__device__ __forceinline__ float beside(double x, double down) {
+    const double y = fmin(fabs(x) * down, 0x1p23);
+    const unsigned u = (unsigned)y;
+    const float f = (float)(2 * u + ((double)u != y ? 1u : 0u));
+    return x < 0 ? -f : f;
+}
+constexpr int kBeside = -21;  // exponent of its last bit
+__device__ __forceinline__ unsigned codes_of(double x, double y, int e) {
+    const double down = __builtin_bit_cast(double, (unsigned long long)(20 - e + 1023) << 52);
+    return codes_of(beside(x, down), beside(y, down), -kBeside);
+}
 template <typename A>
-struct Limits;
-template <>
-struct Limits<float> {
-    static constexpr int kTop = 128;
-    static __device__ __forceinline__ float power(int e) { return __builtin_bit_cast(float, (unsigned)(e + 127) << 23); }
-};
-template <>
-struct Limits<double> {
-    static constexpr int kTop = 1024;
-    static __device__ __forceinline__ double power(int e) {
-        return __builtin_bit_cast(double, (unsigned long long)(e + 1023) << 52);
-    }
-};
+constexpr int kTop = sizeof(A) == 8 ? 1024 : 128;  // exponent of infinity
 
 template <typename T, int G>
 struct Row {
     static constexpr int CE = 16 / (int)sizeof(T);
     static constexpr int kGroups = kTpb / G;
 
-    template <typename A>
-    static __device__ __forceinline__ void load(A* x, const T* row, int d0, const Append& a) {
-        T e[CE];
-        if (a.vec && d0 < a.dim) {
-            const u32x4 v = *reinterpret_cast<const u32x4*>(row + d0);
-            __builtin_memcpy(e, &v, 16);
+    static __device__ __forceinline__ u32x4 load(const T* row, int d0, const Append& a) {
+        u32x4 v = {0, 0, 0, 0};
+        if (a.vec) {
+            if (d0 < a.dim) v = *reinterpret_cast<const u32x4*>(row + d0);
         } else {
+            T e[CE];
 #pragma unroll
             for (int j = 0; j < CE; ++j) e[j] = d0 + j < a.dim ? row[d0 + j] : (T)0.0f;
+            __builtin_memcpy(&v, e, 16);
         }
+        return v;
+    }
+    template <typename A>
+    static __device__ __forceinline__ void values(A* x, const u32x4& v) {
+        T e[CE];
+        __builtin_memcpy(e, &v, 16);
 #pragma unroll
         for (int j = 0; j < CE; ++j) x[j] = (A)(float)e[j];
     }
@@ -107,20 +117,63 @@ struct Row {
         return v;
     }
     template <typename A>
-    static __device__ __forceinline__ A other_of(A v, int m) { return __shfl_xor(v, m); }
-
-    // Norm and turn of the lane's features d0 ..; `row`: the group's values in LDS
-    template <typename A, typename CS>
-    static __device__ __forceinline__ void turn(A* x, int d0, A* row, const CS* cs, const float* weight, const Append& a) {
-        if (a.norm) {
-            A ss = 0;
+    static __device__ __forceinline__ void normalise(A* x, const float* w, const Append& a) {
+        A ss = 0;
 #pragma unroll
-            for (int j = 0; j < CE; ++j) ss += x[j] * x[j];
-            ss = group_sum(ss) / (A)a.dim + (A)a.eps;
-            const A rstd = sizeof(A) == 8 ? (A)(1.0 / sqrt((double)ss)) : (A)rsqrtf((float)ss);
+        for (int j = 0; j < CE; ++j) ss = fma(x[j], x[j], ss);
+        ss = group_sum(ss) / (A)a.dim + (A)a.eps;
+        const A rstd = sizeof(A) == 8 ? (A)(1.0 / sqrt((double)ss)) : (A)rsqrtf((float)ss);
 #pragma unroll
-            for (int j = 0; j < CE; ++j) x[j] = x[j] * rstd * (A)(weight && d0 + j < a.dim ? weight[d0 + j] : 1.0f);
+        for (int j = 0; j < CE; ++j) x[j] = x[j] * rstd * (A)w[j];
+    }
+    // A turn of pairs that lie whole chunks of a lane apart: cosines and signed sines of the
+    // lane's features, and the lane of their pairs' other members.
+    template <typename A>
+    struct Part {
+        A cos[CE], sin[CE];
+        int other;
+        template <typename CS>
+        __device__ __forceinline__ void set(int d0, const CS* cs, const Append& a) {
+            const int c = d0 / CE, hc = a.half / CE;
+            const bool first = c < hc, turns = c < 2 * hc;
+            other = !turns ? c : first ? c + hc : c - hc;
+#pragma unroll
+            for (int j = 0; j < CE; ++j) {
+                const int p = !turns ? 0 : (first ? c : c - hc) * CE + j;
+                cos[j] = turns ? (A)cs[p].x : (A)1;
+                sin[j] = !turns ? (A)0 : first ? -(A)cs[p].y : (A)cs[p].y;
+            }
         }
+    };
+    // `row`: the group's values in LDS, G * CE of them, in an order without bank conflicts
+    template <typename A>
+    static __device__ __forceinline__ void turn(A* x, int d0, A* row, const Part<A>& t) {
+        constexpr int V = 16 / (int)sizeof(A);  // values of an access
+        typedef A Vec __attribute__((ext_vector_type(V)));
+        const int c = d0 / CE;
+        // the group's lanes are in one wave, whose LDS accesses are in order
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int j = 0; j < CE; j += V) {
+            Vec y;
+#pragma unroll
+            for (int i = 0; i < V; ++i) y[i] = x[j + i];
+            *reinterpret_cast<Vec*>(row + j * G + V * c) = y;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int j = 0; j < CE; j += V) {
+            const Vec y = *reinterpret_cast<const Vec*>(row + j * G + V * t.other);
+#pragma unroll
+            for (int i = 0; i < V; ++i) x[j + i] = fma(x[j + i], t.cos[j + i], y[i] * t.sin[j + i]);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+    // Any other turn.
+    template <typename A, typename CS>
+    static __device__ __forceinline__ void turn(A* x, int d0, A* row, const CS* cs, const Append& a) {
         if (a.interleaved) {
 #pragma unroll
             for (int j = 0; j < CE; j += 2) {
@@ -133,7 +186,6 @@ struct Row {
             return;
         }
         if (!a.half) return;
-        // the group's lanes are in one wave, whose LDS accesses are in order
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int j = 0; j < CE; ++j) row[d0 + j] = x[j];
@@ -163,15 +215,14 @@ struct Row {
         }
         constexpr int kLanes = kGroup / CE < G ? kGroup / CE : G;  // of a scale
 #pragma unroll
-        for (int m = 1; m < kLanes; m <<= 1) most = fmax(most, other_of(most, m));
+        for (int m = 1; m < kLanes; m <<= 1) most = fmax(most, __shfl_xor(most, m));
         bool past;
         int e = exponent_of(most, past);
-        const bool none = e == Limits<A>::kTop;
+        const bool none = e == kTop<A>;
         e = min(max(e - (past ? 1 : 2), -120), 125);
-        const A down = Limits<A>::power(-e);
         unsigned code = 0;
 #pragma unroll
-        for (int j = 0; j < CE; ++j) code |= (code_of(fmin(fabs(x[j]) * down, (A)7)) | (x[j] < 0 ? 8u : 0u)) << (4 * j);
+        for (int j = 0; j < CE; j += 2) code |= codes_of(x[j], x[j + 1], e) << (4 * j);
         if (d0 >= p.groups * kGroup) return;
         char* to = block + slot * p.row_bytes + d0 / 2;
         if constexpr (CE == 8) *reinterpret_cast<unsigned*>(to) = code;
@@ -195,9 +246,9 @@ struct Turns<true> {
 };
 
 // Cosine and sine of each pair of `count` tokens; the angle is formed and reduced in 64 bits.
-// `fine`: so are they.
+// `fine`: so are they.  `rounded`: in fp32 too, if it is not null.
 template <typename CS>
-__device__ __forceinline__ void angles(CS* cs, const Append& a, int token0, int count, bool fine) {
+__device__ __forceinline__ void angles(CS* cs, float2* rounded, const Append& a, int token0, int count, bool fine) {
     for (int i = threadIdx.x; i < count * a.half; i += kTpb) {
         const int t = i / a.half, p = i - t * a.half;
         double turns = (double)a.pos[(size_t)(token0 + t) * a.axes + p / a.per_axis] * a.freq[p] * 0.15915494309189533577;
@@ -207,6 +258,7 @@ __device__ __forceinline__ void angles(CS* cs, const Append& a, int token0, int 
             sincospi(2.0 * turns, &s, &c);
             cs[i].x = c;
             cs[i].y = s;
+            if (rounded) rounded[i] = make_float2((float)c, (float)s);
         } else {
             // to an eighth of a turn either way: fp32 rounds what is left, and the small one of
             // sine and cosine keeps its digits
@@ -215,76 +267,137 @@ __device__ __forceinline__ void angles(CS* cs, const Append& a, int token0, int 
             float s, c;
             sincospif(0.5f * (float)(4.0 * turns - quarters), &s, &c);
             const float x = q & 1 ? s : c, y = q & 1 ? c : s;
-            cs[i].x = (q + 1) & 2 ? -x : x;
-            cs[i].y = q & 2 ? -y : y;
+            const float2 turn = make_float2((q + 1) & 2 ? -x : x, q & 2 ? -y : y);
+            if (rounded) {
+                rounded[i] = turn;
+            } else {
+                cs[i].x = turn.x;
+                cs[i].y = turn.y;
+            }
         }
     }
 }
 
-template <typename T, int G, bool FP4>
-__global__ __launch_bounds__(kTpb) void cache_append_kernel(Append a) {
+enum { kQueries, kKeyRows, kValueRows };
+
+// CHUNKS: pairs lie whole chunks of a lane apart
+template <typename T, int G, bool FP4, bool CHUNKS>
+__global__ __launch_bounds__(kTpb, 4) void cache_append_kernel(Append a) {
     using R = Row<T, G>;
-    using A = typename Turns<FP4>::A;
     using CS = typename Turns<FP4>::CS;
-    constexpr int CE = R::CE;
+    constexpr int CE = R::CE, kGroups = R::kGroups;
     __shared__ __attribute__((aligned(16))) CS cs[kAngles];
-    __shared__ __attribute__((aligned(16))) A lds[R::kGroups][G * CE];
+    __shared__ __attribute__((aligned(16))) float2 cs_q[FP4 ? kAngles : 1];
+    __shared__ __attribute__((aligned(16))) typename Turns<FP4>::A lds[kGroups][G * CE];
+    __shared__ long long blocks[kMostTokensEach];  // a token's page, as its first head's byte, or -1
+    __shared__ int places[kMostTokensEach];
     const int group = threadIdx.x / G, d0 = (threadIdx.x % G) * CE;
-    const int part = blockIdx.x % a.parts, token0 = blockIdx.x / a.parts * a.tokens_each;
-    const int tokens = min(a.tokens_each, a.tokens - token0);
-    const int row0 = part * a.rows_each, each = min(a.rows_each, a.rows - row0);
-    if (each <= 0) return;
-    const int turned = a.heads + a.kv_heads;
-    if (row0 < turned) {
-        angles(cs, a, token0, tokens, row0 + each > a.heads);
-        __syncthreads();
-    }
-    for (int r = group; r < tokens * each; r += R::kGroups) {
-        const int t = r / each, row = row0 + r - t * each, token = token0 + t;
-        const int place = a.place[token];
-        if (place < 0) continue;
-        if (row < a.heads) {
-            float x[CE];
-            R::load(x, (const T*)a.q + token * a.qs[0] + row * a.qs[1], d0, a);
-            R::turn(x, d0, reinterpret_cast<float*>(lds[group]), cs + t * a.half, a.q_weight, a);
-            R::store((T*)a.q_out + token * a.qos[0] + row * a.qos[1], d0, a.dim, a.vec, x);
-            continue;
+    const int parts = a.q_parts + 2 * a.kv_parts, part = blockIdx.x % parts;
+    const int token0 = blockIdx.x / parts * a.tokens_each, tokens = min(a.tokens_each, a.tokens - token0);
+
+    const auto rows_of = [&](auto kind_, int head0, int head1) {
+        constexpr int kind = decltype(kind_)::value;
+        using A = std::conditional_t<kind == kKeyRows, typename Turns<FP4>::A, float>;
+        const int heads = min(head1 - head0, kGroups), strands = heads > 0 ? kGroups / heads : 0;
+        const int strand = heads > 0 ? group / heads : 0, first = group - strand * heads;  // a token's groups, and tokens at a time
+        const T* from = (const T*)(kind == kQueries ? a.q : kind == kKeyRows ? a.k : a.v);
+        const long long by_token = kind == kQueries ? a.qs[0] : kind == kKeyRows ? a.ks[0] : a.vs[0];
+        const long long by_head = kind == kQueries ? a.qs[1] : kind == kKeyRows ? a.ks[1] : a.vs[1];
+        const float* weight = kind == kQueries ? a.q_weight : a.k_weight;
+        float w[CE];
+        if (kind != kValueRows) {
+#pragma unroll
+            for (int j = 0; j < CE; ++j) w[j] = weight && d0 + j < a.dim ? weight[d0 + j] : 1.0f;
         }
-        const int page = a.pages.page_of(a.request ? a.request[token] : token, place), slot = a.pages.slot_of(place);
-        if (page < 0) continue;
-        if (row < turned) {
-            const int head = row - a.heads;
-            char* block = a.pages.k + a.pages.block_at(page, head);
-            A x[CE];
-            R::load(x, (const T*)a.k + token * a.ks[0] + head * a.ks[1], d0, a);
-            R::turn(x, d0, lds[group], cs + t * a.half, a.k_weight, a);
-            if constexpr (FP4) R::pack(block, slot, d0, x, a.pages);
-            else R::store((T*)(block + slot * a.pages.row_bytes), d0, a.dim, true, x);
-        } else {
-            const int head = row - turned;
-            char* block = a.pages.v + a.pages.block_at(page, head);
-            float x[CE];
-            R::load(x, (const T*)a.v + token * a.vs[0] + head * a.vs[1], d0, a);
-            if constexpr (FP4) R::pack(block, slot, d0, x, a.pages);
-            else R::store((T*)(block + slot * a.pages.row_bytes), d0, a.dim, true, x);
+        for (int head = head0 + first; head0 < head1; head += heads) {
+            const bool in = strand < strands && head < head1;
+            const T* next_row = from + (token0 + strand) * by_token + head * by_head;
+            const long long on = strands * by_token;
+            u32x4 next[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+            if (in && strand < tokens) next[0] = R::load(next_row, d0, a);
+            if (in && strand + strands < tokens) next[1] = R::load(next_row + on, d0, a);
+            next_row += 2 * on;
+            if (head == head0 + first) {  // once, the first rows on their way
+                for (int t = threadIdx.x; t < tokens; t += kTpb) {
+                    const int place = a.place[token0 + t];
+                    const int page = place < 0 ? -1 : a.pages.page_of(a.request ? a.request[token0 + t] : token0 + t, place);
+                    places[t] = place;
+                    blocks[t] = page < 0 ? -1 : a.pages.block_at(page, 0);
+                }
+                if (kind != kValueRows) angles(cs, FP4 ? cs_q : nullptr, a, token0, tokens, kind == kKeyRows);
+                __syncthreads();
+            }
+            if (in)
+                for (int t = strand; t < tokens; t += strands) {
+                    const u32x4 v = next[0];
+                    next[0] = next[1];
+                    if (t + 2 * strands < tokens) next[1] = R::load(next_row, d0, a);
+                    next_row += on;
+                    const int place = places[t];
+                    if (place < 0 || (kind != kQueries && blocks[t] < 0)) continue;
+                    A x[CE];
+                    R::values(x, v);
+                    if constexpr (kind != kValueRows) {
+                        if (a.norm) R::normalise(x, w, a);
+                        A* row = reinterpret_cast<A*>(lds[group]);
+                        const auto turn = [&](const auto* table) {
+                            if constexpr (CHUNKS) {
+                                typename R::template Part<A> angle;
+                                angle.set(d0, table, a);
+                                R::turn(x, d0, row, angle);
+                            } else {
+                                R::turn(x, d0, row, table, a);
+                            }
+                        };
+                        if constexpr (FP4 && kind == kQueries) turn(cs_q + t * a.half);
+                        else turn(cs + t * a.half);
+                    }
+                    if constexpr (kind == kQueries) {
+                        R::store((T*)a.q_out + (token0 + t) * a.qos[0] + head * a.qos[1], d0, a.dim, a.vec, x);
+                    } else {
+                        char* block = (kind == kKeyRows ? a.pages.k : a.pages.v) + blocks[t] + (long long)head * a.pages.block_bytes;
+                        const int slot = a.pages.slot_of(place);
+                        if constexpr (FP4) R::pack(block, slot, d0, x, a.pages);
+                        else R::store((T*)(block + slot * a.pages.row_bytes), d0, a.dim, true, x);
+                    }
+                }
+            if (head - first + heads >= head1) break;
         }
+    };
+    using Queries = std::integral_constant<int, kQueries>;
+    using Keys = std::integral_constant<int, kKeyRows>;
+    using Values = std::integral_constant<int, kValueRows>;
+    if (part < a.q_parts) {
+        const int each = (a.heads + a.q_parts - 1) / a.q_parts;
+        rows_of(Queries{}, part * each, min((part + 1) * each, a.heads));
+    } else {
+        const int i = (part - a.q_parts) % a.kv_parts, each = (a.kv_heads + a.kv_parts - 1) / a.kv_parts;
+        if (part < a.q_parts + a.kv_parts) rows_of(Keys{}, i * each, min((i + 1) * each, a.kv_heads));
+        else rows_of(Values{}, i * each, min((i + 1) * each, a.kv_heads));
     }
 }
 
-// Few tokens: one each, their rows shared by workgroups of one pass.  Many: rows for 16 passes
-// of a workgroup's groups, as far as their sines fit.
+// Few tokens: one each, their rows shared by workgroups of one pass.  Many: as many as leave four
+// workgroups of each kind a CU, as far as their sines fit.
 constexpr int kFewTokens = 1024;
 template <typename T, int G>
 void launch(Append& p, hipStream_t s, const char* what) {
-    constexpr int groups = Row<T, G>::kGroups;
-    const int by_rows = std::max(1, 16 * groups / p.rows), by_angles = kAngles / std::max(1, p.half);
-    p.tokens_each = std::max(1, std::min({by_rows, by_angles, p.tokens / kFewTokens}));
-    p.parts = p.tokens < kFewTokens ? (p.rows + groups - 1) / groups : 1;
-    p.rows_each = (p.rows + p.parts - 1) / p.parts;
-    const long long blocks = ((long long)p.tokens + p.tokens_each - 1) / p.tokens_each * p.parts;
+    constexpr int groups = Row<T, G>::kGroups, CE = Row<T, G>::CE;
+    p.tokens_each = std::max(1, std::min({kAngles / std::max(1, p.half), kMostTokensEach, p.tokens / kFewTokens}));
+    const bool few = p.tokens < kFewTokens;
+    p.q_parts = few ? (p.heads + groups - 1) / groups : p.heads > 0;
+    p.kv_parts = few ? (p.kv_heads + groups - 1) / groups : 1;
+    const long long parts = p.q_parts + 2 * p.kv_parts;
+    const long long blocks = ((long long)p.tokens + p.tokens_each - 1) / p.tokens_each * parts;
     NNK_REQUIRE(blocks < (1LL << 32) / kTpb, what, "%s: too many rows", what);  // threads of a launch
-    if (p.pages.groups) cache_append_kernel<T, G, true><<<(unsigned)blocks, kTpb, 0, s>>>(p);
-    else cache_append_kernel<T, G, false><<<(unsigned)blocks, kTpb, 0, s>>>(p);
+    const bool chunks = !p.interleaved && p.half > 0 && p.half % CE == 0;
+    const auto with = [&](auto four_bits, auto whole) {
+        cache_append_kernel<T, G, decltype(four_bits)::value, decltype(whole)::value><<<(unsigned)blocks, kTpb, 0, s>>>(p);
+    };
+    using Yes = std::true_type;
+    using No = std::false_type;
+    if (p.pages.groups) chunks ? with(Yes{}, Yes{}) : with(Yes{}, No{});
+    else chunks ? with(No{}, Yes{}) : with(No{}, No{});
     nnk_after_launch(what, s);
 }
 
