@@ -593,12 +593,11 @@ bool nnk_attention_few(const attn::Args& args, bool half, float* ws, hipStream_t
 // Bias gradient from args.dist_sums.
 void nnk_attention_bias_grad(const attn::Args& args, float* dbias, hipStream_t s, const char* what);
 
-// FN<T, DP, CAP, BIAS, VEC> for the call's type, feature count, score terms and alignment.
-// Rows that are not on 16 bytes are taken element by element, in one size.
-#define NNK_ATTN_DISPATCH(args, bf, FN, ...)                                                              \
+// FN<T, DP, CAP, BIAS, VEC> for values of type T_ and the call's feature count, score terms and
+// alignment.  Rows that are not on 16 bytes are taken element by element, in one size.
+#define NNK_ATTN_DISPATCH_OF(T_, args, FN, ...)                                                           \
     [&]() {                                                                                               \
-        auto by_dim = [&](auto type, auto cap, auto bias) {                                               \
-            using T_ = decltype(type);                                                                    \
+        auto by_dim = [&](auto cap, auto bias) {                                                          \
             constexpr bool C_ = decltype(cap)::value, B_ = decltype(bias)::value;                         \
             if (!(args).vec) return FN<T_, 128, C_, B_, false>(__VA_ARGS__);                              \
             switch (((args).dim + 31) / 32) {                                                             \
@@ -608,11 +607,11 @@ void nnk_attention_bias_grad(const attn::Args& args, float* dbias, hipStream_t s
             default: return FN<T_, 128, C_, B_, true>(__VA_ARGS__);                                       \
             }                                                                                             \
         };                                                                                                \
-        auto by_terms = [&](auto type) {                                                                  \
-            using Yes = std::true_type;                                                                   \
-            using No = std::false_type;                                                                   \
-            if ((args).c2 != 0.0f) return (args).buckets > 0 ? by_dim(type, Yes{}, Yes{}) : by_dim(type, Yes{}, No{}); \
-            return (args).buckets > 0 ? by_dim(type, No{}, Yes{}) : by_dim(type, No{}, No{});             \
-        };                                                                                                \
-        return (bf) ? by_terms(attn::bf16{}) : by_terms(0.0f);                                            \
+        using Yes = std::true_type;                                                                       \
+        using No = std::false_type;                                                                       \
+        if ((args).c2 != 0.0f) return (args).buckets > 0 ? by_dim(Yes{}, Yes{}) : by_dim(Yes{}, No{});    \
+        return (args).buckets > 0 ? by_dim(No{}, Yes{}) : by_dim(No{}, No{});                             \
     }()
+// For both types.
+#define NNK_ATTN_DISPATCH(args, bf, FN, ...)                                                              \
+    ((bf) ? NNK_ATTN_DISPATCH_OF(attn::bf16, args, FN, __VA_ARGS__) : NNK_ATTN_DISPATCH_OF(float, args, FN, __VA_ARGS__))

@@ -10,7 +10,7 @@ using cache::Pages;
 // Floats of a workspace: enough for the call and for each one of a smaller batch or of fewer
 // queries or keys, which may be divided into more parts.
 size_t most_floats(const NnAttention* a) {
-    return a->batch && a->len_q ? nnk_cache_few_most(a) : 0;
+    return nnk_cache_few_most(a);
 }
 
 bool fits(Pages& p, const NnAttention* a, const NnCache* c, bool pools, const char* what) {
@@ -53,13 +53,17 @@ void launch_cache_attention_forward(void* out, float* lse, const void* q, const 
     const long long n[3] = {a->batch, a->len_q, a->heads};
     NNK_REQUIRE(nnk_rows_apart(3, a->out_stride, n, a->head_dim), what, "%s: rows of out overlap (strides %lld, %lld, %lld)",
         what, a->out_stride[0], a->out_stride[1], a->out_stride[2]);
-    NNK_REQUIRE(!nnk_cache_few_floats(a) || workspace, what, "%s: null workspace", what);
+    const bool few = nnk_cache_is_few(a, p.groups > 0);
+    NNK_REQUIRE(!few || !nnk_cache_few_floats(a) || workspace, what, "%s: null workspace", what);
     NNK_REQUIRE(nnk::aligned16(workspace), what, "%s: workspace is not aligned to 16 bytes", what);
     args.q = q;
     args.out = out;
     args.lse = lse;
     args.vec = by_16(a) && nnk::aligned16(q) && nnk::aligned16(out);
-    nnk_cache_few(args, p, a, workspace, s, what);
+    if (few) return nnk_cache_few(args, p, a, workspace, s, what);
+    args.q_rows = ((long long)a->len_q + kRows - 1) / kRows * a->heads * a->batch < kSplitBelow ? kRows / 2 : kRows;
+    if (p.groups) nnk_cache_forward_mxfp4(args, p, s, what);
+    else nnk_cache_forward_plain(args, p, a->dtype == NN_BF16, s, what);
 }
 
 }  // extern "C"

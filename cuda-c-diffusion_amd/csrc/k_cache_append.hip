@@ -24,7 +24,7 @@ using namespace cache;
 
 constexpr int kTpb = 256;
 constexpr int kAngles = 512;    // sines and cosines of a workgroup's tokens
-constexpr int kMostTokensEach = 16;
+constexpr int kMostTokensEach = 16;  // lanes of a wave at most
 
 struct Append {
     const void *q, *k, *v;
@@ -318,7 +318,7 @@ __global__ __launch_bounds__(kTpb, 4) void cache_append_kernel(Append a) {
             if (in && strand + strands < tokens) next[1] = R::load(next_row + on, d0, a);
             next_row += 2 * on;
             if (head == head0 + first) {  // once, the first rows on their way
-                for (int t = threadIdx.x; t < tokens; t += kTpb) {
+                if (const int t = (int)threadIdx.x - (kTpb - 64); t >= 0 && t < tokens) {  // a wave without the first sines
                     const int place = a.place[token0 + t];
                     const int page = place < 0 ? -1 : a.pages.page_of(a.request ? a.request[token0 + t] : token0 + t, place);
                     places[t] = place;

@@ -346,6 +346,8 @@ struct Few {
     int step;           // keys of a step, kStep or, so that all steps are counted in 32 bits, a multiple
 };
 constexpr int kMostParts = 64;  // of a unit
+// A line of memory for each ticket: on one line, those of 32 units were 2 us of a step over 4 caches of 4096.
+constexpr int kTicketEvery = 32, kTicketRoom = kTicketWords * kTicketEvery;
 
 // Steps of a unit of request b: those of its last query, one at least.
 __device__ __forceinline__ int steps_of(const Args& a, const Pages& p, const Few& f, int b) {
@@ -380,7 +382,10 @@ __device__ __forceinline__ void share_of(Share& x, const Args& a, const Pages& p
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) most = max(most, __shfl_xor(most, m));
     const unsigned even = ((unsigned)(total * f.units) + f.workers - 1) / (unsigned)f.workers;
-    x.each = __builtin_amdgcn_readfirstlane(max((int)even, (most + kMostParts - 2) / (kMostParts - 1)));
+    // A part more is a sixteenth of a step's time more for the workgroup that joins a unit's: of e steps
+    // a share, e + most / 16 e is least at this.
+    const int least = max((int)ceilf(sqrtf(0.0625f * (float)most)), (most + kMostParts - 2) / (kMostParts - 1));
+    x.each = __builtin_amdgcn_readfirstlane(max((int)even, least));
     x.first = worker * x.each;
     x.last = min(x.first + x.each, total * f.units);
     x.before = x.request = 0;
@@ -420,7 +425,8 @@ __device__ __forceinline__ All call_again() {
 template <typename T, typename E, int NT>
 constexpr int held_by_a_cu() {
     if constexpr (std::is_same_v<typename E::Frag, float>) return 1;
-    else return sizeof(T) == 2 && NT == 1 && E::kFourBits ? 3 : 2;
+    else if constexpr (sizeof(T) == 4) return NT == 2 ? 1 : 2;
+    else return NT == 1 && E::kFourBits ? 3 : 2;
 }
 
 // TERMS: 0 none, 1 a cap, 2 a bias and maybe a cap (which a register or two more, and their
@@ -765,7 +771,7 @@ __global__ __launch_bounds__(kTpb, (held_by_a_cu<T, PAGES<DP>, NT>())) void cach
         if (parts > 1) {  // the workgroups of the unit
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // handed over
             __syncthreads();
-            unsigned* ticket = f.tickets + (size_t)b * f.units + unit;
+            unsigned* ticket = f.tickets + ((size_t)b * f.units + unit) * kTicketEvery;
             if (threadIdx.x == 0)
                 last_one = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(parts - 1);
             __syncthreads();
@@ -848,7 +854,7 @@ void launch(const Args& a, const Pages& p, const Plan& plan, float* ws, hipStrea
     const auto with = [&](auto tiles, auto terms) {
         constexpr int NT = decltype(tiles)::value;
         const int workers = plan.workers ? std::min(plan.workers, kCus * held_by_a_cu<T, PAGES<DP>, NT>()) : 0;
-        const All all = {a, p, {reinterpret_cast<unsigned*>(ws), ws + kTicketWords, plan.tiles, a.kv_heads * plan.tiles, workers, plan.step}};
+        const All all = {a, p, {reinterpret_cast<unsigned*>(ws), ws + kTicketRoom, plan.tiles, a.kv_heads * plan.tiles, workers, plan.step}};
         cache_few_kernel<T, PAGES, DP, NT, decltype(terms)::value>
             <<<workers ? (unsigned)workers : (unsigned)plan.units, kTpb, 0, s>>>(all);
     };
@@ -873,18 +879,36 @@ void by_dim(const Args& a, const Pages& p, const Plan& plan, float* ws, hipStrea
 
 }  // namespace
 
+// Which form is quicker, by the work of each in workgroups of the other one times keys: that one has
+// 128 queries of a head a workgroup, two of them a CU, with fewer gains less than it has less to do, and
+// nothing below about one of 64 queries a CU; this one has units of 32 rows, whose keys it shares
+// out evenly, and takes some 4 us for that if they are more than a step.  A unit's keys cost it,
+// against a workgroup of the other, a third (4 bits, bf16) or 1.25 times as much (plain pages).
+// Measured, bf16, heads of 128, this form and the other in us: 512 queries, 32 heads (8 of keys), 8192 keys
+// 4 bits 113 / 164, plain 268 / 177; 2048 queries 431 / 307, 1127 / 326; 8 requests of 32 queries, 16
+// heads (4), 2048 keys 28 / 45, 47 / 49, of 128 queries 38 / 48, 100 / 52; 4 of 300 queries over 300 keys,
+// 8 heads of 64, 19 / 12.  fp32 queries over 4 bits come here always: the products of three bf16 parts
+// are quicker than the other form's fp32 ones (512 queries over 8192 keys 221 / 684).
+bool nnk_cache_is_few(const NnAttention* a, bool four_bits) {
+    const bool half = a->dtype == NN_BF16;
+    if (four_bits && !half) return true;
+    const double rows = (double)a->len_q * (a->heads / a->kv_heads), units = std::ceil(rows / 32) * a->kv_heads * a->batch;
+    const double groups = std::ceil(a->len_q / 128.0) * a->heads * a->batch;
+    const double own = units * a->len_k * (four_bits ? 0.35 : 1.25) + (a->len_k > kStep ? 55e3 : 0.0);
+    return own <= std::max(0.66 * groups + 200.0, 273.0) * a->len_k;
+}
 // Floats that one call takes, its tickets among them.
 size_t nnk_cache_few_floats(const NnAttention* a) {
     if (!a->batch || !a->len_q) return 0;
     const Plan p = plan_of(a);
-    return p.workers ? kTicketWords + 2 * (size_t)p.workers * p.rows * (padded(a->head_dim) + 2) : 0;
+    return p.workers ? kTicketRoom + 2 * (size_t)p.workers * p.rows * (padded(a->head_dim) + 2) : 0;
 }
 // Every smaller call has fewer units, steps and rows.
 size_t nnk_cache_few_most(const NnAttention* a) {
     if (!a->batch || !a->len_q || a->len_k <= kStep) return 0;
     const Plan p = plan_of(a);
     const long long workers = p.workers ? p.workers : kWorkers;
-    return kTicketWords + 2 * (size_t)workers * p.rows * (padded(a->head_dim) + 2);
+    return kTicketRoom + 2 * (size_t)workers * p.rows * (padded(a->head_dim) + 2);
 }
 void nnk_cache_few(const Args& a, const Pages& p, const NnAttention* d, float* ws, hipStream_t s, const char* what) {
     const Plan plan = plan_of(d);

@@ -1,7 +1,8 @@
 // k_cache_read.hip -- rows of the cache as tensors.
 //
-// A thread takes 8 features of a row: 4 bytes and a scale of 4-bit pages, or the values
-// themselves.  Memory bounds it: every byte is read and written once.
+// A thread takes 8 features of a row at a time: 4 bytes and a scale of 4-bit pages, or the values
+// themselves, four rows under way together.  A workgroup has some tokens, whose pages it looks up
+// once.  Memory bounds it: every byte is read and written once.
 #include "cache_common.h"
 
 #include <algorithm>
@@ -11,68 +12,97 @@ using namespace cache;
 
 constexpr int kTpb = 256;
 constexpr int kFeatures = 8;  // of a thread
+constexpr int kMostTokensEach = 64;
+constexpr int kAtOnce = 4;
 
 struct Read {
     void *k, *v;
     Pages pages;
     long long ks[2], vs[2];
     const int *request, *place;
-    int tokens, kv_heads, dim, chunks;
+    int tokens, kv_heads, dim, chunks, tokens_each;
     nnk::FastDiv by_chunks, by_heads;
-    unsigned total;
     bool vec;
 };
 
 template <typename T, bool FP4>
 __global__ __launch_bounds__(kTpb) void cache_read_kernel(Read a) {
-    const unsigned n = blockIdx.x * kTpb + threadIdx.x;
-    if (n >= a.total) return;
-    unsigned row, chunk, t, side;
-    a.by_chunks.divmod(n, row, chunk);
-    a.by_heads.divmod(row, t, side);  // side: keys' heads, then values'
-    const int place = a.place[t], d0 = (int)chunk * kFeatures;
-    if (place < 0) return;
-    const bool values = side >= (unsigned)a.kv_heads;
-    const int head = (int)side - (values ? a.kv_heads : 0);
-    const int page = a.pages.page_of(a.request ? a.request[t] : (int)t, place), slot = a.pages.slot_of(place);
-    T x[kFeatures];
-#pragma unroll
-    for (int j = 0; j < kFeatures; ++j) x[j] = (T)0.0f;
-    if (page >= 0) {
-        const char* block = (values ? a.pages.v : a.pages.k) + a.pages.block_at(page, head);
-        const char* from = block + slot * a.pages.row_bytes;
-        if constexpr (FP4) {
-            const unsigned code = *reinterpret_cast<const unsigned*>(from + d0 / 2);
-            const float scale = scale_of(*reinterpret_cast<const unsigned char*>(block + a.pages.scales + slot * a.pages.groups + d0 / kGroup));
-            typedef T T2 __attribute__((ext_vector_type(2)));
-            T2 y[4];
-            values8(code, scale, y);
-#pragma unroll
-            for (int j = 0; j < kFeatures; ++j) x[j] = y[j / 2][j % 2];
-        } else {
-#pragma unroll
-            for (int j = 0; j < kFeatures * (int)sizeof(T); j += 16)  // rows are padded to 16 bytes
-                if (d0 * (int)sizeof(T) + j < a.pages.row_bytes)
-                    __builtin_memcpy(reinterpret_cast<char*>(x) + j, __builtin_assume_aligned(from + d0 * sizeof(T) + j, 16), 16);
-        }
+    __shared__ long long blocks[kMostTokensEach];  // a token's page, as its first head's byte, or -1
+    __shared__ int places[kMostTokensEach];
+    const int token0 = blockIdx.x * a.tokens_each, tokens = min(a.tokens_each, a.tokens - token0);
+    for (int t = threadIdx.x; t < tokens; t += kTpb) {
+        const int place = a.place[token0 + t];
+        const int page = place < 0 ? -1 : a.pages.page_of(a.request ? a.request[token0 + t] : token0 + t, place);
+        places[t] = place;
+        blocks[t] = page < 0 ? -1 : a.pages.block_at(page, 0);
     }
-    T* to = (T*)(values ? a.v : a.k) + t * (values ? a.vs[0] : a.ks[0]) + head * (values ? a.vs[1] : a.ks[1]);
-    constexpr int CE = 16 / (int)sizeof(T);
+    __syncthreads();
+    typedef T Chunk __attribute__((ext_vector_type(kFeatures)));
+    const unsigned total = (unsigned)tokens * 2 * a.kv_heads * a.chunks;
+    for (unsigned n0 = threadIdx.x; n0 < total; n0 += kAtOnce * kTpb) {
+        Chunk x[kAtOnce];
+        unsigned code[kAtOnce], scale[kAtOnce];
+        T* to[kAtOnce];
+        int from[kAtOnce];  // first feature, or -1: nothing to write
 #pragma unroll
-    for (int j = 0; j < kFeatures; j += CE) {
-        if (a.vec) {
-            if (d0 + j < a.dim) __builtin_memcpy(__builtin_assume_aligned(to + d0 + j, 16), x + j, 16);
-        } else {
+        for (int i = 0; i < kAtOnce; ++i) {
+            const unsigned n = n0 + i * kTpb;
+            unsigned row, chunk, t, side;
+            a.by_chunks.divmod(min(n, total - 1), row, chunk);
+            a.by_heads.divmod(row, t, side);  // side: keys' heads, then values'
+            const int place = places[t], d0 = (int)chunk * kFeatures;
+            const bool values = side >= (unsigned)a.kv_heads;
+            const int head = (int)side - (values ? a.kv_heads : 0);
+            from[i] = n < total && place >= 0 ? d0 : -1;
+            to[i] = (T*)(values ? a.v : a.k) + (token0 + t) * (values ? a.vs[0] : a.ks[0]) + head * (values ? a.vs[1] : a.ks[1]);
+            x[i] = Chunk{};
+            code[i] = 0;
+            scale[i] = 127;
+            if (from[i] < 0 || blocks[t] < 0) continue;
+            const char* block = (values ? a.pages.v : a.pages.k) + blocks[t] + (long long)head * a.pages.block_bytes;
+            const int slot = a.pages.slot_of(place);
+            const char* p = block + slot * a.pages.row_bytes;
+            if constexpr (FP4) {
+                code[i] = *reinterpret_cast<const unsigned*>(p + d0 / 2);
+                scale[i] = *reinterpret_cast<const unsigned char*>(block + a.pages.scales + slot * a.pages.groups + d0 / kGroup);
+            } else {
 #pragma unroll
-            for (int i = j; i < j + CE; ++i)
-                if (d0 + i < a.dim) to[d0 + i] = x[i];
+                for (int j = 0; j < (int)sizeof(Chunk); j += 16)  // rows are padded to 16 bytes
+                    if (d0 * (int)sizeof(T) + j < a.pages.row_bytes)
+                        __builtin_memcpy(reinterpret_cast<char*>(&x[i]) + j, __builtin_assume_aligned(p + d0 * sizeof(T) + j, 16), 16);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            if (from[i] < 0) continue;
+            if constexpr (FP4) {
+                typedef T T2 __attribute__((ext_vector_type(2)));
+                T2 y[4];
+                values8(code[i], scale_of(scale[i]), y);
+                __builtin_memcpy(&x[i], y, sizeof y);
+            }
+            constexpr int CE = 16 / (int)sizeof(T);
+#pragma unroll
+            for (int j = 0; j < kFeatures; j += CE) {
+                if (a.vec) {
+                    if (from[i] + j < a.dim) {
+                        u32x4 y;
+                        __builtin_memcpy(&y, reinterpret_cast<const char*>(&x[i]) + j * sizeof(T), 16);
+                        __builtin_nontemporal_store(y, reinterpret_cast<u32x4*>(to[i] + from[i] + j));
+                    }
+                } else {
+#pragma unroll
+                    for (int k = j; k < j + CE; ++k)
+                        if (from[i] + k < a.dim) to[i][from[i] + k] = x[i][k];
+                }
+            }
         }
     }
 }
 
 template <typename T>
 void launch(const Read& p, hipStream_t s, const char* what) {
-    const unsigned blocks = (p.total + kTpb - 1) / kTpb;
+    const unsigned blocks = (unsigned)((p.tokens + (long long)p.tokens_each - 1) / p.tokens_each);
     if (p.pages.groups) cache_read_kernel<T, true><<<blocks, kTpb, 0, s>>>(p);
     else cache_read_kernel<T, false><<<blocks, kTpb, 0, s>>>(p);
     nnk_after_launch(what, s);
@@ -95,8 +125,10 @@ extern "C" void launch_cache_read(void* k, void* v, const NnCacheRead* a, const 
     NNK_REQUIRE(nnk_rows_apart(2, a->v_stride, n, a->head_dim), what, "%s: rows of v overlap (strides %lld, %lld)", what,
         a->v_stride[0], a->v_stride[1]);
     p.chunks = (a->head_dim + kFeatures - 1) / kFeatures;
-    const long long total = 2LL * a->tokens * a->kv_heads * p.chunks;
-    NNK_REQUIRE(total <= (1LL << 31) - kTpb, what, "%s: too many rows", what);  // of the divisions and the launch
+    // Tokens of a workgroup: for two passes of its threads, as few as still make four workgroups a CU.
+    const int rows = 2 * a->kv_heads * p.chunks;
+    p.tokens_each = std::max(1, std::min({kMostTokensEach, 2 * kAtOnce * kTpb / rows, a->tokens / 1024}));
+    NNK_REQUIRE((long long)a->tokens / p.tokens_each < (1LL << 32) / kTpb - 1, what, "%s: too many rows", what);  // of a launch
     const long long e = a->dtype == NN_BF16 ? 8 : 4;
     p.vec = a->head_dim % e == 0 && nnk::aligned16(k) && nnk::aligned16(v);
     for (int i = 0; i < 2; ++i) {
@@ -111,7 +143,6 @@ extern "C" void launch_cache_read(void* k, void* v, const NnCacheRead* a, const 
     p.tokens = a->tokens;
     p.kv_heads = a->kv_heads;
     p.dim = a->head_dim;
-    p.total = (unsigned)total;
     p.by_chunks = nnk::FastDiv((uint32_t)p.chunks);
     p.by_heads = nnk::FastDiv((uint32_t)(2 * a->kv_heads));
     if (a->dtype == NN_BF16) launch<bf16>(p, s, what);
