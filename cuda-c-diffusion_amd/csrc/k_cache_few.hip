@@ -68,11 +68,9 @@ struct Blocks32 {
         entry[0] = table[min(key >> p.shift, last)];
         entry[1] = p.shift > 4 ? entry[0] : table[min((key + kTile) >> p.shift, last)];
     }
-    __device__ __forceinline__ Blocks32(const Pages& p, int b, int kv, int k0, int lane)
-        : table(p.table + (size_t)b * p.table_pages), block((unsigned long long)kv * (unsigned)p.block_bytes), n(0) {
-        look(p, k0, lane);
-    }
-    // The next block, which begins at k0.
+    __device__ __forceinline__ Blocks32(const Pages& p, int b, int kv)
+        : table(p.table + (size_t)b * p.table_pages), block((unsigned long long)kv * (unsigned)p.block_bytes), entry{0, 0}, n(64) {}
+    // The next block, which begins at k0: there is one, and so there are pages in the table.
     __device__ __forceinline__ void next(Place (&at)[kHalves], const Pages& p, int k0, int lane) {
         if (n == 64) {
             look(p, k0, lane);
@@ -544,7 +542,7 @@ __global__ __launch_bounds__(kTpb, (held_by_a_cu<T, PAGES<DP>, NT>())) void cach
         int k0 = step0 * f.step + wave * kKeys;
         E e;
         Place at[kHalves];
-        Blocks32 blocks(p, b, kv, k0 < end ? k0 : 0, lane);
+        Blocks32 blocks(p, b, kv);
         const auto load = [&](int from) {
             if (from >= end) return;
             blocks.next(at, p, from, lane);

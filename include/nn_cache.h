@@ -65,7 +65,8 @@ size_t nnhip_cache_page_bytes(const NnCache* c, int dtype, int kv_heads, int hea
  * way to the even code: off by half a step at most, as 7 still rounds to 6.  (From
  * 7 * 2^125 on, sizes end at 6 * 2^125.)  If any of the 32 is infinite or NaN all are NaN.
  *
- * place[t] < 0: row t is no token (a padded batch), and is neither read nor written.  A
+ * place[t] < 0: row t is no token (a padded batch): what it holds has no effect, and nothing is
+ * written for it.  A
  * request that is none, or a place past the table, is an entry that is no page: q_out is
  * written, key and value are dropped.  No two rows of a call may have the same slot;
  * which of them it then holds, and whether whole, is not defined. */

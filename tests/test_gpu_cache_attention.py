@@ -259,3 +259,115 @@ def test_two_streams(nn, L, rng, kind):
         assert L.nnhip_stream_synchronize(stream) == 0
         call.compare()
         L.nnhip_stream_destroy(stream)
+
+
+@pytest.mark.parametrize("kind, dtype", KINDS)
+@pytest.mark.parametrize("table_pages, pages", [(0, 0), (0, 3), (2, 0)])
+@pytest.mark.parametrize("len_q", [1, 200])
+def test_empty_tables_and_pools(nn, L, kind, dtype, table_pages, pages, len_q):
+    """No entries, or no pages, and no pointers where there is nothing: every query sees nothing."""
+    heads, kv, dim = 2, 1, 32
+    table = ints(L, np.zeros(max(1, 2 * table_pages)))
+    pool = {n: L.alloc(max(1, pages) * 16 * 512) for n in ("k", "v")}
+    cache = nn.NnCache(kind=nn.NN_CACHE_MXFP4 if kind == "mxfp4" else nn.NN_CACHE_PLAIN, page_tokens=16, pages=pages,
+                       requests=2, table_pages=table_pages, table=table.p if table_pages else None,
+                       k=pool["k"].p if pages else None, v=pool["v"].p if pages else None)
+    q = Tensor(L, (2, len_q, heads, dim), dtype, values=np.ones((2, len_q, heads, dim)))
+    out, lse = Tensor(L, (2, len_q, heads, dim), dtype, fill=7.0), L.alloc(2 * heads * len_q)
+    a = nn.NnAttention(dtype=nn.NN_BF16 if dtype == "bf16" else nn.NN_F32, batch=2, len_q=len_q, len_k=16 * table_pages,
+                       heads=heads, kv_heads=kv, head_dim=dim, scale=1.0, mask=nn.NN_MASK_NONE, q_stride=q.strides[:3],
+                       out_stride=out.strides[:3])
+    assert L.nnhip_cache_attention_workspace(a, cache) == 0
+    L.launch_cache_attention_forward(out.p, lse.p, q.p, a, cache, None, None)
+    L.sync()
+    assert not out.result().any() and np.isneginf(lse.download(2 * heads * len_q)).all()
+
+
+@pytest.mark.parametrize("batch, heads, kv, len_k", [(300, 8, 8, 9000), (64, 16, 8, 16384)])
+def test_requests_that_share_pages(nn, L, rng, batch, heads, kv, len_k):
+    """All requests read the same pages with the same queries, in a workgroup's long row of keys (9000) and
+    in long shares of them (16384), both of more blocks than are looked up at once."""
+    dim, page = 32, 64
+    cache = Cache(nn, L, rng, "mxfp4", "bf16", kv, dim, page, [-(-len_k // page)])
+    cache.fill(rng, [len_k])
+    one = Call(nn, L, rng, case("bf16", 1, 1, len_k, heads, kv, dim, "causal"), "mxfp4", page, cache=cache)
+    one.launch()
+    L.sync()
+    one.compare()
+    ref, mag = one.expected()
+    table = ints(L, np.repeat(cache.table, batch, 0))
+    shared = nn.NnCache(kind=nn.NN_CACHE_MXFP4, page_tokens=page, pages=cache.pages, requests=batch,
+                        table_pages=cache.table.shape[1], table=table.p, k=cache.dev["k"].p, v=cache.dev["v"].p)
+    q = Tensor(L, (batch, 1, heads, dim), "bf16", values=np.repeat(one.q.values(), batch, 0))
+    out, lse = Tensor(L, (batch, 1, heads, dim), "bf16"), L.alloc(batch * heads)
+    a = nn.NnAttention(dtype=nn.NN_BF16, batch=batch, len_q=1, len_k=len_k, heads=heads, kv_heads=kv, head_dim=dim,
+                       scale=dim**-0.5, mask=nn.NN_MASK_CAUSAL, q_stride=q.strides[:3], out_stride=out.strides[:3])
+    ws = L.to_device(np.zeros(max(1, L.nnhip_cache_attention_workspace(a, shared)), np.float32))
+    L.launch_cache_attention_forward(out.p, lse.p, q.p, a, shared, ws.p, None)
+    L.sync()
+    # Against the formulas and not against the one request's results: there the keys are divided otherwise, so
+    # shares are rounded relative to another reference, each by up to 2^-8 of itself on either side.
+    check("out", out.result(), np.repeat(ref["out"], batch, 0), np.repeat(mag["out"], batch, 0), "bf16")
+    got = lse.download(shape=(batch, heads, 1)).astype(np.float64)
+    check("lse", got, np.repeat(ref["lse"], batch, 0), np.repeat(mag["lse"], batch, 0), "f32")
+
+
+@pytest.mark.parametrize("len_q", [1, 300])
+def test_pools_past_32_bits(nn, L, rng, len_q):
+    """Pages whose offsets need more than 32 bits, read by both forms."""
+    heads, kv, dim, tokens, length = 8, 8, 128, 4096, 8192 + 700
+    size = tokens * 68 * kv
+    pages = (1 << 32) // size + 3
+    pool = {n: L.alloc(pages * size // 4) for n in ("k", "v")}
+    order = [pages - 1, 0, pages - 2]
+    table = ints(L, [order])
+    far = nn.NnCache(kind=nn.NN_CACHE_MXFP4, page_tokens=tokens, pages=pages, requests=1, table_pages=3, table=table.p,
+                     k=pool["k"].p, v=pool["v"].p)
+    cache = Cache(nn, L, rng, "mxfp4", "bf16", kv, dim, tokens, [3])
+    cache.fill(rng, [length])
+    for n in pool:  # the same pages, far apart
+        for i, at in enumerate(order):
+            raw = np.ascontiguousarray(cache.bytes[n][cache.table[0, i]]).ravel().view(np.float32)
+            assert L.dll.nnhip_memcpy_htod(pool[n].ptr + at * size, raw.ctypes.data, raw.nbytes) == 0
+    c = case("bf16", 1, len_q, length, heads, kv, dim, "causal")
+    call = Call(nn, L, rng, c, "mxfp4", tokens, cache=cache)
+    call.launch()
+    L.sync()
+    near = call.results()
+    call.cache.args = far
+    call.out.dev.fill_bytes(0xFF)
+    call.launch()
+    L.sync()
+    got = call.results()
+    assert np.array_equal(got["out"], near["out"]) and np.array_equal(got["lse"], near["lse"])
+    if len_q == 1:
+        call.compare()
+
+
+@pytest.mark.parametrize("kind, dtype", KINDS)
+def test_append_attend_and_read(nn, L, rng, kind, dtype):
+    """What is read out of the cache is what attention over it used: attention over tensors of it agrees."""
+    heads, kv, dim, tokens = 4, 2, 64, 150
+    cache = Cache(nn, L, rng, kind, dtype, kv, dim, 32, [5])
+    a = Append(nn, L, rng, cache, np.zeros(tokens, int), np.arange(tokens), heads, dim)
+    a.launch()
+    c = case(dtype, 1, tokens, tokens, heads, kv, dim, "causal")
+    rows = {n: Tensor(L, (tokens, kv, dim), dtype) for n in ("k", "v")}
+    L.launch_cache_read(rows["k"].p, rows["v"].p, nn.NnCacheRead(
+        dtype=cache.nn_dtype(), tokens=tokens, kv_heads=kv, head_dim=dim, k_stride=rows["k"].strides[:2],
+        v_stride=rows["v"].strides[:2], request=a.keep[2].p, place=a.keep[3].p), cache.args, None)
+    out = {n: Tensor(L, (1, tokens, heads, dim), dtype) for n in ("paged", "plain")}
+    lse = {n: L.alloc(heads * tokens) for n in out}
+    q = a.t["q_out"]
+    args = nn.NnAttention(dtype=cache.nn_dtype(), batch=1, len_q=tokens, len_k=tokens, heads=heads, kv_heads=kv, head_dim=dim,
+                          scale=c["scale"], mask=nn.NN_MASK_CAUSAL, q_stride=(0, heads * dim, dim),
+                          k_stride=(0, kv * dim, dim), v_stride=(0, kv * dim, dim), out_stride=(tokens * heads * dim, heads * dim, dim))
+    ws = L.to_device(np.zeros(max(1, L.nnhip_cache_attention_workspace(args, cache.args),
+                                  L.nnhip_attention_forward_workspace(args)), np.float32))
+    L.launch_cache_attention_forward(out["paged"].p, lse["paged"].p, q.p, args, cache.args, ws.p, None)
+    L.launch_attention_forward(out["plain"].p, lse["plain"].p, q.p, rows["k"].p, rows["v"].p, args, ws.p, None)
+    L.sync()
+    ref, mag = attention(c, q.result()[None], rows["k"].result()[None], rows["v"].result()[None])
+    for n in out:
+        check(n, out[n].result(), ref["out"], mag["out"], dtype)
+        check(n, lse[n].download(shape=(1, heads, tokens)).astype(np.float64), ref["lse"], mag["lse"], "f32")
