@@ -23,7 +23,7 @@ namespace {
 using namespace cache;
 
 constexpr int kTpb = 256;
-constexpr int kAngles = 512;    // sines and cosines of a workgroup's tokens
+constexpr int kTableBytes = 16384;  // sines and cosines of a workgroup's tokens
 constexpr int kMostTokensEach = 16;  // lanes of a wave at most
 
 struct Append {
@@ -126,28 +126,23 @@ struct Row {
 #pragma unroll
         for (int j = 0; j < CE; ++j) x[j] = x[j] * rstd * (A)w[j];
     }
-    // A turn of pairs that lie whole chunks of a lane apart: cosines and signed sines of the
-    // lane's features, and the lane of their pairs' other members.
+    // A turn of pairs that lie whole chunks of a lane apart: out = x cos + other sin, with the sine's
+    // sign in it.  The table has a token's cosines by feature, then its sines, both in an order
+    // of 16-byte accesses without bank conflicts.
+    static constexpr int kFeatures = G * CE;
     template <typename A>
-    struct Part {
-        A cos[CE], sin[CE];
-        int other;
-        template <typename CS>
-        __device__ __forceinline__ void set(int d0, const CS* cs, const Append& a) {
-            const int c = d0 / CE, hc = a.half / CE;
-            const bool first = c < hc, turns = c < 2 * hc;
-            other = !turns ? c : first ? c + hc : c - hc;
-#pragma unroll
-            for (int j = 0; j < CE; ++j) {
-                const int p = !turns ? 0 : (first ? c : c - hc) * CE + j;
-                cos[j] = turns ? (A)cs[p].x : (A)1;
-                sin[j] = !turns ? (A)0 : first ? -(A)cs[p].y : (A)cs[p].y;
-            }
-        }
-    };
-    // `row`: the group's values in LDS, G * CE of them, in an order without bank conflicts
+    static __device__ __forceinline__ int place(int d) {
+        constexpr int V = 16 / (int)sizeof(A);
+        return d % CE / V * (G * V) + d / CE * V + d % V;
+    }
+    // The lane of the other members.
+    static __device__ __forceinline__ int other_lane(int d0, const Append& a) {
+        const int c = d0 / CE, hc = a.half / CE;
+        return c >= 2 * hc ? c : c < hc ? c + hc : c - hc;
+    }
+    // `row`: the group's values in LDS, kFeatures of them
     template <typename A>
-    static __device__ __forceinline__ void turn(A* x, int d0, A* row, const Part<A>& t) {
+    static __device__ __forceinline__ void turn(A* x, int d0, int other, A* row, const A* table) {
         constexpr int V = 16 / (int)sizeof(A);  // values of an access
         typedef A Vec __attribute__((ext_vector_type(V)));
         const int c = d0 / CE;
@@ -164,9 +159,11 @@ struct Row {
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int j = 0; j < CE; j += V) {
-            const Vec y = *reinterpret_cast<const Vec*>(row + j * G + V * t.other);
+            const Vec y = *reinterpret_cast<const Vec*>(row + j * G + V * other);
+            const Vec cos = *reinterpret_cast<const Vec*>(table + j * G + V * c);
+            const Vec sin = *reinterpret_cast<const Vec*>(table + kFeatures + j * G + V * c);
 #pragma unroll
-            for (int i = 0; i < V; ++i) x[j + i] = fma(x[j + i], t.cos[j + i], y[i] * t.sin[j + i]);
+            for (int i = 0; i < V; ++i) x[j + i] = fma(x[j + i], cos[i], y[i] * sin[i]);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -232,48 +229,49 @@ struct Row {
     }
 };
 
-template <bool WIDE>
-struct Turns;
-template <>
-struct Turns<false> {
-    typedef float A;
-    typedef float2 CS;
+// Cosine and sine of an angle in turns, formed in 64 bits.  fp32: reduced there to an eighth of a
+// turn either way, so that what is left is rounded and the small one of the two keeps its digits.
+__device__ __forceinline__ void cos_sin(double turns, double& c, double& s) {
+    turns -= rint(turns);
+    sincospi(2.0 * turns, &s, &c);
+}
+__device__ __forceinline__ void cos_sin(double turns, float& c, float& s) {
+    turns -= rint(turns);
+    const double quarters = rint(4.0 * turns);
+    const int q = (int)quarters;
+    float u, v;
+    sincospif(0.5f * (float)(4.0 * turns - quarters), &u, &v);
+    const float x = q & 1 ? u : v, y = q & 1 ? v : u;
+    c = (q + 1) & 2 ? -x : x;
+    s = q & 2 ? -y : y;
+}
+template <typename A>
+struct Pair {
+    A x, y;  // cosine, sine
 };
-template <>
-struct Turns<true> {
-    typedef double A;
-    typedef double2 CS;
-};
-
-// Cosine and sine of each pair of `count` tokens; the angle is formed and reduced in 64 bits.
-// `fine`: so are they.  `rounded`: in fp32 too, if it is not null.
-template <typename CS>
-__device__ __forceinline__ void angles(CS* cs, float2* rounded, const Append& a, int token0, int count, bool fine) {
-    for (int i = threadIdx.x; i < count * a.half; i += kTpb) {
-        const int t = i / a.half, p = i - t * a.half;
-        double turns = (double)a.pos[(size_t)(token0 + t) * a.axes + p / a.per_axis] * a.freq[p] * 0.15915494309189533577;
-        turns -= rint(turns);
-        if (sizeof(CS) == 16 && fine) {
-            double s, c;
-            sincospi(2.0 * turns, &s, &c);
-            cs[i].x = c;
-            cs[i].y = s;
-            if (rounded) rounded[i] = make_float2((float)c, (float)s);
-        } else {
-            // to an eighth of a turn either way: fp32 rounds what is left, and the small one of
-            // sine and cosine keeps its digits
-            const double quarters = rint(4.0 * turns);
-            const int q = (int)quarters;
-            float s, c;
-            sincospif(0.5f * (float)(4.0 * turns - quarters), &s, &c);
-            const float x = q & 1 ? s : c, y = q & 1 ? c : s;
-            const float2 turn = make_float2((q + 1) & 2 ? -x : x, q & 2 ? -y : y);
-            if (rounded) {
-                rounded[i] = turn;
-            } else {
-                cs[i].x = turn.x;
-                cs[i].y = turn.y;
+// Of each pair of `count` tokens into the table, for one turn or the other.
+template <typename R, typename A, bool CHUNKS>
+__device__ __forceinline__ void angles(A* table, const Append& a, int token0, int count) {
+    const int each = CHUNKS ? R::kFeatures - a.half : a.half;  // with the features that are not turned
+    for (int i = threadIdx.x; i < count * each; i += kTpb) {
+        const int t = i / each, p = i - t * each;
+        A c = 1, s = 0;
+        if (p < a.half) {
+            const double angle = (double)a.pos[(size_t)(token0 + t) * a.axes + p / a.per_axis] * a.freq[p];
+            cos_sin(angle * 0.15915494309189533577, c, s);
+        }
+        if constexpr (CHUNKS) {
+            A* mine = table + t * 2 * R::kFeatures;
+            const int second = R::template place<A>(p + a.half);
+            mine[second] = c;
+            mine[R::kFeatures + second] = s;
+            if (p < a.half) {
+                const int first = R::template place<A>(p);
+                mine[first] = c;
+                mine[R::kFeatures + first] = -s;
             }
+        } else {
+            reinterpret_cast<Pair<A>*>(table)[t * a.half + p] = {c, s};
         }
     }
 }
@@ -284,11 +282,10 @@ enum { kQueries, kKeyRows, kValueRows };
 template <typename T, int G, bool FP4, bool CHUNKS>
 __global__ __launch_bounds__(kTpb, 4) void cache_append_kernel(Append a) {
     using R = Row<T, G>;
-    using CS = typename Turns<FP4>::CS;
+    using KeyType = std::conditional_t<FP4, double, float>;
     constexpr int CE = R::CE, kGroups = R::kGroups;
-    __shared__ __attribute__((aligned(16))) CS cs[kAngles];
-    __shared__ __attribute__((aligned(16))) float2 cs_q[FP4 ? kAngles : 1];
-    __shared__ __attribute__((aligned(16))) typename Turns<FP4>::A lds[kGroups][G * CE];
+    __shared__ __attribute__((aligned(16))) char tables[kTableBytes];
+    __shared__ __attribute__((aligned(16))) KeyType lds[kGroups][R::kFeatures];
     __shared__ long long blocks[kMostTokensEach];  // a token's page, as its first head's byte, or -1
     __shared__ int places[kMostTokensEach];
     const int group = threadIdx.x / G, d0 = (threadIdx.x % G) * CE;
@@ -297,7 +294,9 @@ __global__ __launch_bounds__(kTpb, 4) void cache_append_kernel(Append a) {
 
     const auto rows_of = [&](auto kind_, int head0, int head1) {
         constexpr int kind = decltype(kind_)::value;
-        using A = std::conditional_t<kind == kKeyRows, typename Turns<FP4>::A, float>;
+        using A = std::conditional_t<kind == kKeyRows, KeyType, float>;
+        A* table = reinterpret_cast<A*>(tables);
+        const int other = R::other_lane(d0, a);
         const int heads = min(head1 - head0, kGroups), strands = heads > 0 ? kGroups / heads : 0;
         const int strand = heads > 0 ? group / heads : 0, first = group - strand * heads;  // a token's groups, and tokens at a time
         const T* from = (const T*)(kind == kQueries ? a.q : kind == kKeyRows ? a.k : a.v);
@@ -324,7 +323,7 @@ __global__ __launch_bounds__(kTpb, 4) void cache_append_kernel(Append a) {
                     places[t] = place;
                     blocks[t] = page < 0 ? -1 : a.pages.block_at(page, 0);
                 }
-                if (kind != kValueRows) angles(cs, FP4 ? cs_q : nullptr, a, token0, tokens, kind == kKeyRows);
+                if (kind != kValueRows) angles<R, A, CHUNKS>(table, a, token0, tokens);
                 __syncthreads();
             }
             if (in)
@@ -340,17 +339,8 @@ __global__ __launch_bounds__(kTpb, 4) void cache_append_kernel(Append a) {
                     if constexpr (kind != kValueRows) {
                         if (a.norm) R::normalise(x, w, a);
                         A* row = reinterpret_cast<A*>(lds[group]);
-                        const auto turn = [&](const auto* table) {
-                            if constexpr (CHUNKS) {
-                                typename R::template Part<A> angle;
-                                angle.set(d0, table, a);
-                                R::turn(x, d0, row, angle);
-                            } else {
-                                R::turn(x, d0, row, table, a);
-                            }
-                        };
-                        if constexpr (FP4 && kind == kQueries) turn(cs_q + t * a.half);
-                        else turn(cs + t * a.half);
+                        if constexpr (CHUNKS) R::turn(x, d0, other, row, table + t * 2 * R::kFeatures);
+                        else R::turn(x, d0, row, reinterpret_cast<const Pair<A>*>(table) + t * a.half, a);
                     }
                     if constexpr (kind == kQueries) {
                         R::store((T*)a.q_out + (token0 + t) * a.qos[0] + head * a.qos[1], d0, a.dim, a.vec, x);
@@ -383,14 +373,15 @@ constexpr int kFewTokens = 1024;
 template <typename T, int G>
 void launch(Append& p, hipStream_t s, const char* what) {
     constexpr int groups = Row<T, G>::kGroups, CE = Row<T, G>::CE;
-    p.tokens_each = std::max(1, std::min({kAngles / std::max(1, p.half), kMostTokensEach, p.tokens / kFewTokens}));
+    const bool chunks = !p.interleaved && p.half > 0 && p.half % CE == 0;
+    const int table = (p.pages.groups ? 16 : 8) * (chunks ? G * CE : std::max(1, p.half));  // bytes of a token
+    p.tokens_each = std::max(1, std::min({kTableBytes / table, kMostTokensEach, p.tokens / 512}));
     const bool few = p.tokens < kFewTokens;
     p.q_parts = few ? (p.heads + groups - 1) / groups : p.heads > 0;
     p.kv_parts = few ? (p.kv_heads + groups - 1) / groups : 1;
     const long long parts = p.q_parts + 2 * p.kv_parts;
     const long long blocks = ((long long)p.tokens + p.tokens_each - 1) / p.tokens_each * parts;
     NNK_REQUIRE(blocks < (1LL << 32) / kTpb, what, "%s: too many rows", what);  // threads of a launch
-    const bool chunks = !p.interleaved && p.half > 0 && p.half % CE == 0;
     const auto with = [&](auto four_bits, auto whole) {
         cache_append_kernel<T, G, decltype(four_bits)::value, decltype(whole)::value><<<(unsigned)blocks, kTpb, 0, s>>>(p);
     };
