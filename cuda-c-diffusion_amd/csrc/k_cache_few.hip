@@ -14,6 +14,12 @@
 // bf16, which holds them exactly, two an instruction, their scale included.  Values pass through
 // LDS, where the transposing read turns them (bf16), or are read a feature a lane (fp32 pages).
 // fp32 queries and probabilities meet 4-bit pages as three bf16 parts each, 24 bits of them.
+//
+// Measured: 16 requests of 8192 to 32768 keys, 32 heads of 128 (8 of keys), scores under a cap: bf16
+// pages 209 us, 6.4 TB/s (reads alone reach 7.1); 4 bits 73 us, 4.9 TB/s of a third of the bytes, of which
+// the loop reads at 5.6 and some 8 us are lengths, table, first loads and the join.  48 requests of
+// five queries over 4096 keys, 16 heads (4), 4 bits 37 us; one of 777 keys, 8 heads of 64, 7.8 us; three of
+// seven fp32 queries over 5001 keys, 12 heads of 96 (4), 4 bits 27 us.
 #include "attn_common.h"
 #include "cache_common.h"
 
