@@ -7,12 +7,6 @@ namespace {
 using namespace attn;
 using cache::Pages;
 
-// Floats of a workspace: enough for the call and for each one of a smaller batch or of fewer
-// queries or keys, which may be divided into more parts.
-size_t most_floats(const NnAttention* a) {
-    return nnk_cache_few_most(a);
-}
-
 bool fits(Pages& p, const NnAttention* a, const NnCache* c, bool pools, const char* what) {
     NNK_REQUIRE_RET(a, false, what, "%s: null description", what);
     if (!nnk_cache_take(p, c, a->dtype, a->kv_heads, a->head_dim, pools, what)) return false;
@@ -38,7 +32,7 @@ extern "C" {
 size_t nnhip_cache_attention_workspace(const NnAttention* a, const NnCache* c) {
     const char* what = "nnhip_cache_attention_workspace";
     Pages p;
-    return fits(p, a, c, false, what) ? most_floats(a) : 0;
+    return fits(p, a, c, false, what) ? nnk_cache_few_floats(a) : 0;
 }
 
 void launch_cache_attention_forward(void* out, float* lse, const void* q, const NnAttention* a, const NnCache* c,
@@ -54,7 +48,7 @@ void launch_cache_attention_forward(void* out, float* lse, const void* q, const 
     NNK_REQUIRE(nnk_rows_apart(3, a->out_stride, n, a->head_dim), what, "%s: rows of out overlap (strides %lld, %lld, %lld)",
         what, a->out_stride[0], a->out_stride[1], a->out_stride[2]);
     const bool few = nnk_cache_is_few(a, p.groups > 0);
-    NNK_REQUIRE(!few || !nnk_cache_few_floats(a) || workspace, what, "%s: null workspace", what);
+    NNK_REQUIRE(!few || !nnk_cache_few_parted(a) || workspace, what, "%s: null workspace", what);
     NNK_REQUIRE(nnk::aligned16(workspace), what, "%s: workspace is not aligned to 16 bytes", what);
     args.q = q;
     args.out = out;

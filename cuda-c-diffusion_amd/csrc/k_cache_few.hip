@@ -335,18 +335,18 @@ __device__ __forceinline__ float2 taken(const float* p) {
     return make_float2(__builtin_bit_cast(float, (unsigned)v), __builtin_bit_cast(float, (unsigned)(v >> 32)));
 }
 
-// The work of a launch is a row of steps: of all requests, all their key heads and tiles of
-// queries (a unit each), and its keys, 128 a step.  Every workgroup has an equal share of it, which may
-// be the end of a unit, whole units and the beginning of another; requests' lengths are on
-// the device, so shares are formed there, by every workgroup for itself.  A unit that more
-// than one share has a part of is joined from their partial results.
+// The work of a launch are units, a request's key heads and tiles of queries, of as many steps of
+// 128 keys as the request has.  A unit is divided into parts of about as many steps as every other's, a
+// workgroup each, so many that they fill the card; requests' lengths are on the device, so this is
+// done there, by every workgroup for itself.  Parts of a unit are joined from their partial results.
+// (Equal shares of the steps in a row, that ended and began within units, had two ends of parts to a
+// workgroup where units are short, some 10 us each: 48 requests of five queries over 4096 keys 37 us.)
 struct Few {
     unsigned* tickets;  // a unit each
-    float* partial;     // [workers, 2, rows, DP + 2]: outputs, then reference (units of log2) and sum; of a
-                        // unit that began before the share, and of one that goes on behind it
+    float* partial;     // [workers, rows, DP + 2]: outputs, then reference (units of log2) and sum
     int tiles;          // of a key head's queries
     int units;          // of a request: key heads and tiles
-    int workers;        // shares; 0: a workgroup a unit
+    int workers;        // parts at most; 0: a workgroup a unit
     int step;           // keys of a step, kStep or, so that all steps are counted in 32 bits, a multiple
 };
 constexpr int kMostParts = 64;  // of a unit
@@ -367,47 +367,58 @@ __device__ __forceinline__ int scan(int v, int lane) {
     }
     return v;
 }
-// A share: where in a request's units it begins, and its end.
-struct Share {
-    int first, last;     // steps
-    int each;            // of every share
-    int before;          // steps of the requests before `request`
-    int request, steps;  // steps of a unit of it
+struct Part {
+    int request, unit;  // of the request's
+    int steps;          // of the unit
+    int part, parts;    // of the unit's
+    int first;          // workgroup of the unit's first part
 };
-__device__ __forceinline__ void share_of(Share& x, const Args& a, const Pages& p, const Few& f, int worker, int lane) {
+// The part of workgroup `worker`; false if there is none.
+__device__ __forceinline__ bool part_of(Part& x, const Args& a, const Pages& p, const Few& f, int worker, int lane) {
     const auto steps_at = [&](int b) { return b < a.batch ? steps_of(a, p, f, b) : 0; };
-    int n = steps_at(lane), sum = scan(n, lane), most = n;
-    int total = __builtin_amdgcn_readlane(sum, 63);
+    const auto sum_of = [&](int v) { return __builtin_amdgcn_readlane(scan(v, lane), 63); };
+    int n = steps_at(lane), most = n, total = sum_of(n);
     for (int b0 = 64; b0 < a.batch; b0 += 64) {
         const int more = steps_at(b0 + lane);
-        total += __builtin_amdgcn_readlane(scan(more, lane), 63);
+        total += sum_of(more);
         most = max(most, more);
     }
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) most = max(most, __shfl_xor(most, m));
-    const unsigned even = ((unsigned)(total * f.units) + f.workers - 1) / (unsigned)f.workers;
     // A part more is a sixteenth of a step's time more for the workgroup that joins a unit's: of e steps
-    // a share, e + most / 16 e is least at this.
-    const int least = max((int)ceilf(sqrtf(0.0625f * (float)most)), (most + kMostParts - 2) / (kMostParts - 1));
-    x.each = __builtin_amdgcn_readfirstlane(max((int)even, least));
-    x.first = worker * x.each;
-    x.last = min(x.first + x.each, total * f.units);
-    x.before = x.request = 0;
-    if (x.first >= x.last) return;
-    for (int b0 = 0;;) {
-        const unsigned long long behind = __ballot((x.before + sum * f.units) > x.first);
+    // a part, e + most / 16 e is least at this.
+    const int least = max((int)ceilf(sqrtf(0.0625f * (float)most)), (most + kMostParts - 1) / kMostParts);
+    // The fewest steps a part of which there are no more than workgroups: between what an even row of them
+    // would be and what is enough if every unit has a part that is not full.
+    const unsigned all = (unsigned)(total * f.units), units = (unsigned)(a.batch * f.units);
+    const auto up = [](unsigned x, unsigned y) { return (int)((x + y - 1) / y); };
+    int low = max(up(all, f.workers), least), each = max(up(all, f.workers - units), low);
+    if (a.batch <= 64) {
+        while (low < each) {
+            const int mid = (low + each) / 2;
+            if (sum_of(up(n, mid)) * f.units <= f.workers) each = mid;
+            else low = mid + 1;
+        }
+    }
+    int before = 0;  // parts of the requests so far
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+        if (b0) n = steps_at(b0 + lane);
+        const int parts = up(n, each), sum = before + scan(parts, lane) * f.units;
+        const unsigned long long behind = __ballot(sum > worker);
         if (behind) {
             const int i = __builtin_ctzll(behind);
-            x.steps = __builtin_amdgcn_readlane(n, i);
             x.request = b0 + i;
-            x.before += (__builtin_amdgcn_readlane(sum, i) - x.steps) * f.units;
-            return;
+            x.steps = __builtin_amdgcn_readlane(n, i);
+            x.parts = __builtin_amdgcn_readlane(parts, i);
+            const int from = __builtin_amdgcn_readlane(sum, i) - x.parts * f.units;
+            x.unit = __builtin_amdgcn_readfirstlane((int)((unsigned)(worker - from) / (unsigned)x.parts));
+            x.first = from + x.unit * x.parts;
+            x.part = worker - x.first;
+            return true;
         }
-        x.before += __builtin_amdgcn_readlane(sum, 63) * f.units;
-        b0 += 64;
-        n = steps_at(b0 + lane);
-        sum = scan(n, lane);
+        before = __builtin_amdgcn_readlane(sum, 63);
     }
+    return false;
 }
 
 // The call.  What only the beginning and the end of a share need is read again there: held over the
@@ -449,32 +460,32 @@ __global__ __launch_bounds__(kTpb, (held_by_a_cu<T, PAGES<DP>, NT>())) void cach
     __shared__ int last_one;
 
     const int lane = threadIdx.x & 63, h = lane >> 4, col = lane & 15, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    Share share;
+    Part part;
     {
         const auto [a, p, f] = call_again();
         if (f.workers) {
-            share_of(share, a, p, f, blockIdx.x, lane);
-            if (share.first >= share.last) return;
+            if (!part_of(part, a, p, f, blockIdx.x, lane)) return;
         } else {
-            share.request = __builtin_amdgcn_readfirstlane((int)(blockIdx.x / (unsigned)f.units));
-            share.steps = __builtin_amdgcn_readfirstlane(steps_of(a, p, f, share.request));
-            share.before = 0;
-            share.first = (blockIdx.x - share.request * f.units) * share.steps;
-            share.last = share.first + share.steps;
-            share.each = 0;
+            part.request = __builtin_amdgcn_readfirstlane((int)(blockIdx.x / (unsigned)f.units));
+            part.unit = blockIdx.x - part.request * f.units;
+            part.steps = __builtin_amdgcn_readfirstlane(steps_of(a, p, f, part.request));
+            part.part = part.first = 0;
+            part.parts = 1;
         }
     }
 
-    for (int g = share.first;;) {
+    {
         const All now = call_again();
         const Args& a = now.a;
         const Pages& p = now.p;
         const Few& f = now.f;
-        const int b = share.request, begin = g - share.before;
+        const int b = part.request;
         // divisions are vector instructions: what is uniform says so
-        const int unit = __builtin_amdgcn_readfirstlane((int)((unsigned)begin / (unsigned)share.steps));
-        const int step0 = begin - unit * share.steps, step1 = min(share.steps, step0 + (share.last - g));
-        const int kv = __builtin_amdgcn_readfirstlane(unit / f.tiles), tile = unit - kv * f.tiles;
+        const int kv = __builtin_amdgcn_readfirstlane((int)((unsigned)part.unit / (unsigned)f.tiles)), tile = part.unit - kv * f.tiles;
+        const auto step_at = [&](int i) {  // where a part begins
+            return __builtin_amdgcn_readfirstlane((int)((unsigned long long)(unsigned)part.steps * (unsigned)i / (unsigned)part.parts));
+        };
+        const int step0 = step_at(part.part), step1 = step_at(part.part + 1);
         const int rows = min(kRowsEach, a.len_q * a.group - tile * kRowsEach);
         const int keys = __builtin_amdgcn_readfirstlane(p.pages ? keys_of(a, b) : 0), start = __builtin_amdgcn_readfirstlane(start_of(a, b));
         const int most = __builtin_amdgcn_readfirstlane(limit_of(a, b, keys, start + (tile * kRowsEach + rows - 1) / a.group));
@@ -706,19 +717,11 @@ __global__ __launch_bounds__(kTpb, (held_by_a_cu<T, PAGES<DP>, NT>())) void cach
             }
         }
 
-        // The shares that the unit has parts in.
         const All after = call_again();
         const auto close = [&](const Args& a, const Pages& p, const Few& f) {
-        const unsigned unit_at = share.before + unit * share.steps;
-        int worker0 = 0, parts = 1;
-        if (f.workers) {
-            worker0 = __builtin_amdgcn_readfirstlane((int)(unit_at / (unsigned)share.each));
-            parts = __builtin_amdgcn_readfirstlane((int)((unit_at + share.steps - 1) / (unsigned)share.each)) - worker0 + 1;
-        }
+        const int parts = part.parts;
         const long long step = kRowsEach * (DP + 2);
-        const auto partial_of = [&](int part) {  // its first part goes on behind its share
-            return f.partial + (2LL * (worker0 + part) + (part == 0)) * step;
-        };
+        const auto partial_of = [&](int i) { return f.partial + (part.first + i) * step; };
 
         // the waves of the workgroup, a tile of queries at a time
         constexpr int kQuads = DP / 4;  // 4 features a thread
@@ -764,7 +767,7 @@ __global__ __launch_bounds__(kTpb, (held_by_a_cu<T, PAGES<DP>, NT>())) void cach
                 if (parts == 1) {
                     finish(r, d, x, ref, all);
                 } else {
-                    float* to = partial_of((int)blockIdx.x - worker0) + r * (DP + 2);
+                    float* to = partial_of(part.part) + r * (DP + 2);
                     hand(to + d, x.x, x.y);
                     hand(to + d + 2, x.z, x.w);
                     if (d == 0) hand(to + DP, ref, all);
@@ -775,7 +778,7 @@ __global__ __launch_bounds__(kTpb, (held_by_a_cu<T, PAGES<DP>, NT>())) void cach
         if (parts > 1) {  // the workgroups of the unit
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // handed over
             __syncthreads();
-            unsigned* ticket = f.tickets + ((size_t)b * f.units + unit) * kTicketEvery;
+            unsigned* ticket = f.tickets + ((size_t)b * f.units + part.unit) * kTicketEvery;
             if (threadIdx.x == 0)
                 last_one = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(parts - 1);
             __syncthreads();
@@ -820,36 +823,36 @@ __global__ __launch_bounds__(kTpb, (held_by_a_cu<T, PAGES<DP>, NT>())) void cach
                 if (threadIdx.x == 0) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
         }
-
-        g += step1 - step0;
-        if (g < share.last && unit + 1 == f.units && step1 == share.steps) {
-            share.before += f.units * share.steps;
-            share.request += 1;
-            share.steps = __builtin_amdgcn_readfirstlane(steps_of(a, p, f, share.request));
-        }
         };
         close(after.a, after.p, after.f);
-        if (g >= share.last) return;
-        __syncthreads();  // LDS is read
     }
 }
 
-// Tiles of queries, and workgroups: as many as the card holds at once, kWorkers at most.
-constexpr int kWorkers = 3 * kCus;
+// Tiles of queries, and parts at most.
+constexpr int kHeld = 3;  // workgroups a CU at most
 struct Plan {
-    long long units;
-    int tiles, rows, workers, step;
+    long long units, steps;
+    int tiles, rows, step;
+    bool parted;
 };
 Plan plan_of(const NnAttention* a) {
     Plan p;
-    const long long rows = (long long)a->len_q * (a->heads / a->kv_heads), steps = std::max(1, (a->len_k + kStep - 1) / kStep);
+    const long long rows = (long long)a->len_q * (a->heads / a->kv_heads);
+    p.steps = std::max(1, (a->len_k + kStep - 1) / kStep);
     p.rows = rows <= kTile ? kTile : 2 * kTile;
     p.tiles = (int)((rows + p.rows - 1) / p.rows);
     p.units = (long long)a->batch * a->kv_heads * p.tiles;
     p.step = kStep;
     while (p.step < 1 << 30 && p.units * ((a->len_k + (long long)p.step - 1) / p.step + 1) >= 1LL << 30) p.step *= 2;
-    p.workers = p.units > kTicketWords || steps == 1 ? 0 : (int)std::min<long long>(kWorkers, p.units * steps);
+    p.parted = p.units <= kTicketWords && p.steps > 1;
     return p;
+}
+// Parts at most: as many as the card holds at once, `held` a CU, or where there are units for more
+// than half of those, several times as many, which even out as they end; twice the units at least.
+long long workers_of(const Plan& p, int held, bool most) {
+    const long long at_once = (long long)kCus * held;
+    const long long n = !most && 2 * p.units <= at_once ? at_once : std::max(4 * at_once, 2 * p.units);
+    return std::min(n, p.units * p.steps);
 }
 int padded(int dim) { return (dim + 31) / 32 * 32; }
 
@@ -857,7 +860,7 @@ template <typename T, template <int> class PAGES, int DP>
 void launch(const Args& a, const Pages& p, const Plan& plan, float* ws, hipStream_t s, const char* what) {
     const auto with = [&](auto tiles, auto terms) {
         constexpr int NT = decltype(tiles)::value;
-        const int workers = plan.workers ? std::min(plan.workers, kCus * held_by_a_cu<T, PAGES<DP>, NT>()) : 0;
+        const int workers = plan.parted ? (int)workers_of(plan, held_by_a_cu<T, PAGES<DP>, NT>(), false) : 0;
         const All all = {a, p, {reinterpret_cast<unsigned*>(ws), ws + kTicketRoom, plan.tiles, a.kv_heads * plan.tiles, workers, plan.step}};
         cache_few_kernel<T, PAGES, DP, NT, decltype(terms)::value>
             <<<workers ? (unsigned)workers : (unsigned)plan.units, kTpb, 0, s>>>(all);
@@ -901,19 +904,15 @@ bool nnk_cache_is_few(const NnAttention* a, bool four_bits) {
     const double own = units * a->len_k * (four_bits ? 0.35 : 1.25) + (a->len_k > kStep ? 55e3 : 0.0);
     return own <= std::max(0.66 * groups + 200.0, 273.0) * a->len_k;
 }
-// Floats that one call takes, its tickets among them.
+// Floats of a call's workspace: enough for its tickets and parts, and for every smaller call's, which
+// has fewer units, steps and rows (and 2048 of them at most in parts).
 size_t nnk_cache_few_floats(const NnAttention* a) {
-    if (!a->batch || !a->len_q) return 0;
-    const Plan p = plan_of(a);
-    return p.workers ? kTicketRoom + 2 * (size_t)p.workers * p.rows * (padded(a->head_dim) + 2) : 0;
-}
-// Every smaller call has fewer units, steps and rows.
-size_t nnk_cache_few_most(const NnAttention* a) {
     if (!a->batch || !a->len_q || a->len_k <= kStep) return 0;
-    const Plan p = plan_of(a);
-    const long long workers = p.workers ? p.workers : kWorkers;
-    return kTicketRoom + 2 * (size_t)workers * p.rows * (padded(a->head_dim) + 2);
+    Plan p = plan_of(a);
+    p.units = std::min<long long>(p.units, kTicketWords);
+    return kTicketRoom + (size_t)workers_of(p, kHeld, true) * p.rows * (padded(a->head_dim) + 2);
 }
+bool nnk_cache_few_parted(const NnAttention* a) { return a->batch && a->len_q && plan_of(a).parted; }
 void nnk_cache_few(const Args& a, const Pages& p, const NnAttention* d, float* ws, hipStream_t s, const char* what) {
     const Plan plan = plan_of(d);
     NNK_REQUIRE(plan.units < (1LL << 32) / kTpb, what, "%s: too many rows", what);
