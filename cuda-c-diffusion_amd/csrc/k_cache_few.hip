@@ -347,6 +347,7 @@ struct Few {
     int tiles;          // of a key head's queries
     int units;          // of a request: key heads and tiles
     int workers;        // parts at most; 0: a workgroup a unit
+    int at_once;        // workgroups that the card holds
     int step;           // keys of a step, kStep or, so that all steps are counted in 32 bits, a multiple
 };
 constexpr int kMostParts = 64;  // of a unit
@@ -358,7 +359,15 @@ __device__ __forceinline__ int steps_of(const Args& a, const Pages& p, const Few
     const int keys = p.pages ? keys_of(a, b) : 0;
     return max(1, (int)((unsigned)(limit_of(a, b, keys, start_of(a, b) + a.len_q - 1) + f.step - 1) / (unsigned)f.step));
 }
-// Inclusive sums over the lanes.
+// Sum over the wave; and inclusive sums over the lanes.
+__device__ __forceinline__ int sum_of(int v) {
+    v += __builtin_amdgcn_mov_dpp(v, nnk::kDppQuadXor1, 0xf, 0xf, true);
+    v += __builtin_amdgcn_mov_dpp(v, nnk::kDppQuadXor2, 0xf, 0xf, true);
+    v += __builtin_amdgcn_mov_dpp(v, nnk::kDppRowHalfMirror, 0xf, 0xf, true);
+    v += __builtin_amdgcn_mov_dpp(v, nnk::kDppRowMirror, 0xf, 0xf, true);
+    return __builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16) + __builtin_amdgcn_readlane(v, 32) +
+        __builtin_amdgcn_readlane(v, 48);
+}
 __device__ __forceinline__ int scan(int v, int lane) {
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) {
@@ -376,7 +385,6 @@ struct Part {
 // The part of workgroup `worker`; false if there is none.
 __device__ __forceinline__ bool part_of(Part& x, const Args& a, const Pages& p, const Few& f, int worker, int lane) {
     const auto steps_at = [&](int b) { return b < a.batch ? steps_of(a, p, f, b) : 0; };
-    const auto sum_of = [&](int v) { return __builtin_amdgcn_readlane(scan(v, lane), 63); };
     int n = steps_at(lane), most = n, total = sum_of(n);
     for (int b0 = 64; b0 < a.batch; b0 += 64) {
         const int more = steps_at(b0 + lane);
@@ -392,11 +400,15 @@ __device__ __forceinline__ bool part_of(Part& x, const Args& a, const Pages& p, 
     // would be and what is enough if every unit has a part that is not full.
     const unsigned all = (unsigned)(total * f.units), units = (unsigned)(a.batch * f.units);
     const auto up = [](unsigned x, unsigned y) { return (int)((x + y - 1) / y); };
-    int low = max(up(all, f.workers), least), each = max(up(all, f.workers - units), low);
+    // As many as there are places, or twice that where there are units for more than half of them.
+    // (Three times as many wherever parts are long, to even out as they end: 68 us became 82.)
+    const int places = 2 * (int)units <= f.at_once ? f.at_once : 2 * f.at_once;
+    const int target = max(min(places, f.workers), (int)units + 1);
+    int low = max(up(all, target), least), each = max(up(all, target - units), low);
     if (a.batch <= 64) {
         while (low < each) {
             const int mid = (low + each) / 2;
-            if (sum_of(up(n, mid)) * f.units <= f.workers) each = mid;
+            if (sum_of(up(n, mid)) * f.units <= target) each = mid;
             else low = mid + 1;
         }
     }
@@ -792,17 +804,16 @@ __global__ __launch_bounds__(kTpb, (held_by_a_cu<T, PAGES<DP>, NT>())) void cach
                         float2 y[kAtOnce], z[kAtOnce], w[kAtOnce];
 #pragma unroll
                         for (int i = 0; i < kAtOnce; ++i) {
-                            const float* q = partial_of(min(part0 + i, parts - 1)) + r * (DP + 2);
+                            w[i] = make_float2(-INFINITY, 0.0f);
+                            if (part0 + i >= parts) continue;
+                            const float* q = partial_of(part0 + i) + r * (DP + 2);
                             y[i] = taken(q + d);
                             z[i] = taken(q + d + 2);
                             w[i] = taken(q + DP);
                         }
                         float top = ref;
 #pragma unroll
-                        for (int i = 0; i < kAtOnce; ++i) {
-                            if (part0 + i >= parts) w[i] = make_float2(-INFINITY, 0.0f);
-                            top = fmaxf(top, w[i].x);
-                        }
+                        for (int i = 0; i < kAtOnce; ++i) top = fmaxf(top, w[i].x);
                         const float base = top == -INFINITY ? 0.0f : top, old = exp2_fast(ref - base);
                         sum *= old;
                         x = make_float4(x.x * old, x.y * old, x.z * old, x.w * old);
@@ -847,21 +858,17 @@ Plan plan_of(const NnAttention* a) {
     p.parted = p.units <= kTicketWords && p.steps > 1;
     return p;
 }
-// Parts at most: as many as the card holds at once, `held` a CU, or where there are units for more
-// than half of those, several times as many, which even out as they end; twice the units at least.
-long long workers_of(const Plan& p, int held, bool most) {
-    const long long at_once = (long long)kCus * held;
-    const long long n = !most && 2 * p.units <= at_once ? at_once : std::max(4 * at_once, 2 * p.units);
-    return std::min(n, p.units * p.steps);
-}
+// Parts at most, where the card holds `held` workgroups a CU; twice the units at least.
+long long workers_of(const Plan& p, int held) { return std::min(std::max(2LL * kCus * held, 2 * p.units), p.units * p.steps); }
 int padded(int dim) { return (dim + 31) / 32 * 32; }
 
 template <typename T, template <int> class PAGES, int DP>
 void launch(const Args& a, const Pages& p, const Plan& plan, float* ws, hipStream_t s, const char* what) {
     const auto with = [&](auto tiles, auto terms) {
         constexpr int NT = decltype(tiles)::value;
-        const int workers = plan.parted ? (int)workers_of(plan, held_by_a_cu<T, PAGES<DP>, NT>(), false) : 0;
-        const All all = {a, p, {reinterpret_cast<unsigned*>(ws), ws + kTicketRoom, plan.tiles, a.kv_heads * plan.tiles, workers, plan.step}};
+        constexpr int held = held_by_a_cu<T, PAGES<DP>, NT>();
+        const int workers = plan.parted && plan.units < 2 * kCus * held ? (int)workers_of(plan, held) : 0;
+        const All all = {a, p, {reinterpret_cast<unsigned*>(ws), ws + kTicketRoom, plan.tiles, a.kv_heads * plan.tiles, workers, kCus * held, plan.step}};
         cache_few_kernel<T, PAGES, DP, NT, decltype(terms)::value>
             <<<workers ? (unsigned)workers : (unsigned)plan.units, kTpb, 0, s>>>(all);
     };
@@ -910,7 +917,7 @@ size_t nnk_cache_few_floats(const NnAttention* a) {
     if (!a->batch || !a->len_q || a->len_k <= kStep) return 0;
     Plan p = plan_of(a);
     p.units = std::min<long long>(p.units, kTicketWords);
-    return kTicketRoom + (size_t)workers_of(p, kHeld, true) * p.rows * (padded(a->head_dim) + 2);
+    return kTicketRoom + (size_t)workers_of(p, kHeld) * p.rows * (padded(a->head_dim) + 2);
 }
 bool nnk_cache_few_parted(const NnAttention* a) { return a->batch && a->len_q && plan_of(a).parted; }
 void nnk_cache_few(const Args& a, const Pages& p, const NnAttention* d, float* ws, hipStream_t s, const char* what) {
