@@ -16,10 +16,10 @@
 // fp32 queries and probabilities meet 4-bit pages as three bf16 parts each, 24 bits of them.
 //
 // Measured: 16 requests of 8192 to 32768 keys, 32 heads of 128 (8 of keys), scores under a cap: bf16
-// pages 209 us, 6.4 TB/s (reads alone reach 7.1); 4 bits 73 us, 4.9 TB/s of a third of the bytes, of which
-// the loop reads at 5.6 and some 8 us are lengths, table, first loads and the join.  48 requests of
-// five queries over 4096 keys, 16 heads (4), 4 bits 37 us; one of 777 keys, 8 heads of 64, 7.8 us; three of
-// seven fp32 queries over 5001 keys, 12 heads of 96 (4), 4 bits 27 us.
+// pages 218 us, 6.2 TB/s (reads alone reach 7.1); 4 bits 68 us, 5.3 TB/s of a third of the bytes, some
+// 14 us of it lengths, table, first loads and the joins (11 of those with no join between workgroups).
+// 48 requests of five queries over 4096 keys, 16 heads (4), 4 bits 29 us, 17 of them such ends; one of 777
+// keys, 8 heads of 64, 7.9 us; three of seven fp32 queries over 5001 keys, 12 heads of 96 (4), 4 bits 24 us.
 #include "attn_common.h"
 #include "cache_common.h"
 
@@ -339,8 +339,9 @@ __device__ __forceinline__ float2 taken(const float* p) {
 // 128 keys as the request has.  A unit is divided into parts of about as many steps as every other's, a
 // workgroup each, so many that they fill the card; requests' lengths are on the device, so this is
 // done there, by every workgroup for itself.  Parts of a unit are joined from their partial results.
-// (Equal shares of the steps in a row, that ended and began within units, had two ends of parts to a
-// workgroup where units are short, some 10 us each: 48 requests of five queries over 4096 keys 37 us.)
+// (Equal shares of the steps in a row, that ended and began within units, fill the card more evenly,
+// 16 long requests in bf16 209 us where parts are 218, but a workgroup then has two ends of parts,
+// some 10 us each: the same in 4 bits 73 us for 68, 48 requests of five queries over 4096 keys 37 for 29.)
 struct Few {
     unsigned* tickets;  // a unit each
     float* partial;     // [workers, rows, DP + 2]: outputs, then reference (units of log2) and sum
@@ -401,7 +402,8 @@ __device__ __forceinline__ bool part_of(Part& x, const Args& a, const Pages& p, 
     const unsigned all = (unsigned)(total * f.units), units = (unsigned)(a.batch * f.units);
     const auto up = [](unsigned x, unsigned y) { return (int)((x + y - 1) / y); };
     // As many as there are places, or twice that where there are units for more than half of them.
-    // (Three times as many wherever parts are long, to even out as they end: 68 us became 82.)
+    // (Twice as many always: 16 long requests 218 -> 213 us in bf16, but 68 -> 77 in 4 bits, and the 48 of
+    // five queries 29 -> 42; three times as many where parts are long 68 -> 82.)
     const int places = 2 * (int)units <= f.at_once ? f.at_once : 2 * f.at_once;
     const int target = max(min(places, f.workers), (int)units + 1);
     int low = max(up(all, target), least), each = max(up(all, target - units), low);
@@ -433,7 +435,7 @@ __device__ __forceinline__ bool part_of(Part& x, const Args& a, const Pages& p, 
     return false;
 }
 
-// The call.  What only the beginning and the end of a share need is read again there: held over the
+// The call.  What only the beginning and the end of a part need is read again there: held over the
 // keys' loop it was some 130 scalar registers too many, which go to lanes of vector registers.
 struct All {  // the kernel's only argument
     Args a;
