@@ -88,7 +88,28 @@ size_t backward_most(const NnAttention* a) {
         by4(stat_floats(a)) + (a->buckets ? (size_t)tables * (2 * a->max_distance + 1) : 0);
 }
 
-bool sizes_fit(const NnAttention* a, bool backward, const char* what) {
+// Whether the rows of a tensor that the call writes lie apart; false after recording an error.
+bool rows_apart(const long long* stride, int batch, int len, int heads, int dim, const char* name, const char* what) {
+    const long long n[3] = {batch, len, heads};
+    NNK_REQUIRE_RET(nnk_rows_apart(3, stride, n, dim), false, what, "%s: rows of %s overlap (strides %lld, %lld, %lld)", what,
+        name, stride[0], stride[1], stride[2]);
+    return true;
+}
+
+// Whether rows of 16-byte chunks can be read and written: strides here, pointers by the
+// callers.  The offsets of 64 rows have to fit in 32 bits.
+bool strides_by_16(const NnAttention* a) {
+    const long long e = a->dtype == NN_BF16 ? 8 : 4, far = (1LL << 32) / (16 / e) / 64 - 128;
+    bool ok = a->head_dim % e == 0;
+    for (int i = 0; i < 3; ++i)
+        for (const long long* s : {a->q_stride, a->k_stride, a->v_stride, a->out_stride})
+            ok = ok && s[i] % e == 0 && (i != 1 || (s[i] >= 0 && s[i] <= far));
+    return ok;
+}
+
+}  // namespace
+
+bool nnk_attention_sizes_fit(const NnAttention* a, bool backward, const char* what) {
     NNK_REQUIRE_RET(a, false, what, "%s: null description", what);
     NNK_REQUIRE_RET(a->dtype == NN_F32 || a->dtype == NN_BF16, false, what, "%s: unknown dtype %d", what, a->dtype);
     NNK_REQUIRE_RET(a->batch >= 0 && a->len_q >= 0 && a->len_k >= 0 && a->len_q <= kMaxLen && a->len_k <= kMaxLen,
@@ -113,29 +134,8 @@ bool sizes_fit(const NnAttention* a, bool backward, const char* what) {
     return true;
 }
 
-// Whether the rows of a tensor that the call writes lie apart; false after recording an error.
-bool rows_apart(const long long* stride, int batch, int len, int heads, int dim, const char* name, const char* what) {
-    const long long n[3] = {batch, len, heads};
-    NNK_REQUIRE_RET(nnk_rows_apart(3, stride, n, dim), false, what, "%s: rows of %s overlap (strides %lld, %lld, %lld)", what,
-        name, stride[0], stride[1], stride[2]);
-    return true;
-}
-
-// Whether rows of 16-byte chunks can be read and written: strides here, pointers by the
-// callers.  The offsets of 64 rows have to fit in 32 bits.
-bool strides_by_16(const NnAttention* a) {
-    const long long e = a->dtype == NN_BF16 ? 8 : 4, far = (1LL << 32) / (16 / e) / 64 - 128;
-    bool ok = a->head_dim % e == 0;
-    for (int i = 0; i < 3; ++i)
-        for (const long long* s : {a->q_stride, a->k_stride, a->v_stride, a->out_stride})
-            ok = ok && s[i] % e == 0 && (i != 1 || (s[i] >= 0 && s[i] <= far));
-    return ok;
-}
-
-}  // namespace
-
 bool nnk_attention_take(Args& p, const NnAttention* a, bool backward, const char* what) {
-    if (!sizes_fit(a, backward, what)) return false;
+    if (!nnk_attention_sizes_fit(a, backward, what)) return false;
     NNK_REQUIRE_RET(a->scale > 0.0f && a->scale < INFINITY, false, what, "%s: scale=%g is not positive", what, a->scale);
     NNK_REQUIRE_RET(a->softcap >= 0.0f && a->softcap < INFINITY, false, what, "%s: softcap=%g is negative", what,
         a->softcap);
@@ -206,7 +206,7 @@ bool nnk_attention_take(Args& p, const NnAttention* a, bool backward, const char
 extern "C" {
 
 size_t nnhip_attention_forward_workspace(const NnAttention* a) {
-    if (!sizes_fit(a, false, "nnhip_attention_forward_workspace")) return 0;
+    if (!nnk_attention_sizes_fit(a, false, "nnhip_attention_forward_workspace")) return 0;
     return forward_most(a);
 }
 
@@ -238,7 +238,7 @@ void launch_attention_forward(void* out, float* lse, const void* q, const void* 
 }
 
 size_t nnhip_attention_backward_workspace(const NnAttention* a) {
-    if (!sizes_fit(a, true, "nnhip_attention_backward_workspace")) return 0;
+    if (!nnk_attention_sizes_fit(a, true, "nnhip_attention_backward_workspace")) return 0;
     return backward_most(a);
 }
 

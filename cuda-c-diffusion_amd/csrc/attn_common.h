@@ -572,7 +572,8 @@ inline bool raise_lds(const void* fn, size_t bytes, std::atomic<unsigned long lo
 
 }  // namespace attn
 
-// Fills `p` for the call's description; false after recording an error.
+// Whether a call's sizes can be had; fills `p` for the call's description.  False after recording an error.
+bool nnk_attention_sizes_fit(const NnAttention* a, bool backward, const char* what);
 bool nnk_attention_take(attn::Args& p, const NnAttention* a, bool backward, const char* what);
 // Documents of each block of 64 into `ws`, for args.key_docs and query_docs (no documents:
 // nothing).

@@ -32,7 +32,7 @@ extern "C" {
 size_t nnhip_cache_attention_workspace(const NnAttention* a, const NnCache* c) {
     const char* what = "nnhip_cache_attention_workspace";
     Pages p;
-    return fits(p, a, c, false, what) ? nnk_cache_few_floats(a) : 0;
+    return fits(p, a, c, false, what) && nnk_attention_sizes_fit(a, false, what) ? nnk_cache_few_floats(a) : 0;
 }
 
 void launch_cache_attention_forward(void* out, float* lse, const void* q, const NnAttention* a, const NnCache* c,

@@ -181,6 +181,32 @@ def test_attention_refusals(nn, more, text):
     assert L.last_error()[0] == 0
 
 
+BAD_SIZES = [
+    (dict(dtype=7), "unknown dtype 7"),
+    (dict(batch=-1), "bad shape"),
+    (dict(batch=3), "batch=3 of a cache of 2 requests"),
+    (dict(len_q=-2), "bad shape"),
+    (dict(len_q=1 << 30), "bad shape"),
+    (dict(len_k=-1), "bad shape"),
+    (dict(len_k=1 << 20), "does not fit"),
+    (dict(heads=3, kv_heads=2), "not a multiple of kv_heads"),
+    (dict(heads=0), "not a multiple of kv_heads"),
+    (dict(heads=-2), "not a multiple of kv_heads"),
+    (dict(head_dim=0), "head_dim=0"),
+    (dict(doc_q=DUMMY, doc_k=DUMMY), "documents"),
+]
+
+
+@pytest.mark.parametrize("more, text", BAD_SIZES, ids=[f"{n}-{t}" for n, (_, t) in enumerate(BAD_SIZES)])
+def test_workspace_refusals(nn, more, text):
+    """What the launch refuses by its sizes has no workspace either."""
+    L = nn.lib()
+    L.last_error()
+    with pytest.raises(nn.NnHipError, match=f"nnhip_cache_attention_workspace: error 1: .*{text}"):
+        L.nnhip_cache_attention_workspace(_attn(nn, **dict(dict(len_k=1000), **more)), _cache(nn, table_pages=64))
+    assert L.last_error()[0] == 0
+
+
 def test_null_pointers(nn):
     L = nn.lib()
     L.last_error()
