@@ -207,6 +207,20 @@ def test_workspace_refusals(nn, more, text):
     assert L.last_error()[0] == 0
 
 
+@pytest.mark.parametrize("kind", ["NN_CACHE_PLAIN", "NN_CACHE_MXFP4"])
+@pytest.mark.parametrize("heads, kv", [(8, 8), (32, 1), (8, 1)])
+def test_launches_past_32_bits(nn, kind, heads, kv):
+    """Single queries of more requests than a launch has threads for, by either form: units or heads of 256."""
+    L = nn.lib()
+    L.last_error()
+    batch = 1 << 24 if kv == 1 else 1 << 22
+    a = _attn(nn, dtype=nn.NN_BF16, batch=batch, len_q=1, heads=heads, kv_heads=kv, out_stride=(8 * heads, 8 * heads, 8))
+    c = _cache(nn, kind=getattr(nn, kind), requests=batch)
+    with pytest.raises(nn.NnHipError, match="launch_cache_attention_forward: error 1: .*too many rows"):
+        L.launch_cache_attention_forward(DUMMY, DUMMY, DUMMY, a, c, DUMMY, None)
+    assert L.last_error()[0] == 0
+
+
 def test_null_pointers(nn):
     L = nn.lib()
     L.last_error()
