@@ -343,7 +343,7 @@ __device__ __forceinline__ float2 taken(const float* p) {
 // 16 long requests in bf16 209 us where parts are 218, but a workgroup then has two ends of parts,
 // some 10 us each: the same in 4 bits 73 us for 68, 48 requests of five queries over 4096 keys 37 for 29.)
 struct Few {
-    unsigned* tickets;  // a unit each
+    unsigned* tickets;  // a unit each, by ticket_of
     float* partial;     // [workers, rows, DP + 2]: outputs, then reference (units of log2) and sum
     int tiles;          // of a key head's queries
     int units;          // of a request: key heads and tiles
@@ -352,8 +352,11 @@ struct Few {
     int step;           // keys of a step, kStep or, so that all steps are counted in 32 bits, a multiple
 };
 constexpr int kMostParts = 64;  // of a unit
-// A line of memory for each ticket: on one line, those of 32 units were 2 us of a step over 4 caches of 4096.
-constexpr int kTicketEvery = 32, kTicketRoom = kTicketWords * kTicketEvery;
+// Tickets are in the words where launch_attention_forward has its own, so that a workspace serves both,
+// in an order that keeps successive units' on lines of their own: on one line, those of 32 units were
+// 2 us of a step over 4 caches of 4096.
+constexpr int kTicketLine = 32, kTicketLines = kTicketWords / kTicketLine;
+__device__ __forceinline__ int ticket_of(int unit) { return unit % kTicketLines * kTicketLine + unit / kTicketLines; }
 
 // Steps of a unit of request b: those of its last query, one at least.
 __device__ __forceinline__ int steps_of(const Args& a, const Pages& p, const Few& f, int b) {
@@ -792,7 +795,7 @@ __global__ __launch_bounds__(kTpb, (held_by_a_cu<T, PAGES<DP>, NT>())) void cach
         if (parts > 1) {  // the workgroups of the unit
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // handed over
             __syncthreads();
-            unsigned* ticket = f.tickets + ((size_t)b * f.units + part.unit) * kTicketEvery;
+            unsigned* ticket = f.tickets + ticket_of(b * f.units + part.unit);  // fewer than kTicketWords: they are in parts
             if (threadIdx.x == 0)
                 last_one = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(parts - 1);
             __syncthreads();
@@ -870,7 +873,7 @@ void launch(const Args& a, const Pages& p, const Plan& plan, float* ws, hipStrea
         constexpr int NT = decltype(tiles)::value;
         constexpr int held = held_by_a_cu<T, PAGES<DP>, NT>();
         const int workers = plan.parted && plan.units < 2 * kCus * held ? (int)workers_of(plan, held) : 0;
-        const All all = {a, p, {reinterpret_cast<unsigned*>(ws), ws + kTicketRoom, plan.tiles, a.kv_heads * plan.tiles, workers, kCus * held, plan.step}};
+        const All all = {a, p, {reinterpret_cast<unsigned*>(ws), ws + kTicketWords, plan.tiles, a.kv_heads * plan.tiles, workers, kCus * held, plan.step}};
         cache_few_kernel<T, PAGES, DP, NT, decltype(terms)::value>
             <<<workers ? (unsigned)workers : (unsigned)plan.units, kTpb, 0, s>>>(all);
     };
@@ -919,7 +922,7 @@ size_t nnk_cache_few_floats(const NnAttention* a) {
     if (!a->batch || !a->len_q || a->len_k <= kStep) return 0;
     Plan p = plan_of(a);
     p.units = std::min<long long>(p.units, kTicketWords);
-    return kTicketRoom + (size_t)workers_of(p, kHeld) * p.rows * (padded(a->head_dim) + 2);
+    return kTicketWords + (size_t)workers_of(p, kHeld) * p.rows * (padded(a->head_dim) + 2);
 }
 bool nnk_cache_few_parted(const NnAttention* a) { return a->batch && a->len_q && plan_of(a).parted; }
 void nnk_cache_few(const Args& a, const Pages& p, const NnAttention* d, float* ws, hipStream_t s, const char* what) {

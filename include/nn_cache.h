@@ -117,8 +117,10 @@ void launch_cache_read(void* k, void* v, const NnCacheRead* a, const NnCache* c,
  * `workspace`: nnhip_cache_attention_workspace floats (NULL if that is 0), zero-filled
  * before its first use; every launch leaves it fit for the next, also of another shape
  * that it is large enough for, and its size serves every call of a smaller batch or of
- * fewer queries or keys too.  Launches that may run concurrently need separate
- * workspaces. */
+ * fewer queries or keys too.  launch_attention_forward leaves a workspace as fit, and
+ * takes one that this call has left, so one of the larger size serves both; what
+ * anything else has written to is to be filled with zeros again.  Launches that may run
+ * concurrently need separate workspaces. */
 size_t nnhip_cache_attention_workspace(const NnAttention* a, const NnCache* c);
 void launch_cache_attention_forward(void* out, float* lse, const void* q,
     const NnAttention* a, const NnCache* c, float* workspace, hipStream_t s);
