@@ -65,7 +65,7 @@ bool nnk_cache_take(cache::Pages& p, const NnCache* c, int dtype, int kv_heads, 
 namespace attn {
 struct Args;
 }
-bool nnk_cache_is_few(const NnAttention* a, bool four_bits);
+extern "C" int nnk_cache_is_few(const NnAttention* a, int four_bits);
 size_t nnk_cache_few_floats(const NnAttention* a);
 bool nnk_cache_few_parted(const NnAttention* a);
 void nnk_cache_few(const attn::Args& a, const cache::Pages& p, const NnAttention* d, float* ws, hipStream_t s, const char* what);

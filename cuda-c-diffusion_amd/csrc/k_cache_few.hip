@@ -898,23 +898,41 @@ void by_dim(const Args& a, const Pages& p, const Plan& plan, float* ws, hipStrea
 
 }  // namespace
 
-// Which form is quicker, by the work of each in workgroups of the other one times keys: that one has
-// 128 queries of a head a workgroup, two of them a CU, with fewer gains less than it has less to do, and
-// nothing below about one of 64 queries a CU; this one has units of 32 rows, whose keys it shares
-// out evenly, and takes some 4 us for that if they are more than a step.  A unit's keys cost it,
-// against a workgroup of the other, a third (4 bits, bf16) or 1.25 times as much (plain pages).
-// Measured, bf16, heads of 128, this form and the other in us: 512 queries, 32 heads (8 of keys), 8192 keys
-// 4 bits 113 / 164, plain 268 / 177; 2048 queries 431 / 307, 1127 / 326; 8 requests of 32 queries, 16
-// heads (4), 2048 keys 28 / 45, 47 / 49, of 128 queries 38 / 48, 100 / 52; 4 of 300 queries over 300 keys,
-// 8 heads of 64, 19 / 12.  fp32 queries over 4 bits come here always: the products of three bf16 parts
-// are quicker than the other form's fp32 ones (512 queries over 8192 keys 221 / 684).
-bool nnk_cache_is_few(const NnAttention* a, bool four_bits) {
+// Which form is quicker, by the work of each.  This one has units of one tile of 16 rows or two, whose
+// keys it shares out evenly; what a unit costs a key depends on what it reads (plain pages) or converts and
+// multiplies, and its parts' ends some hundred keys more.  The other one has workgroups of 128 queries of a
+// head, whatever they fill of them, and takes as long as kFill of them (of 64) where CUs are left over.  It
+// reads a key head once for each of its heads; in fp32 its tiles leave one workgroup a CU.  In units of a
+// workgroup and key:
+struct Costs {
+    double tile, two_tiles, ends;  // of a unit: a key with a tile or two; its ends, in keys
+    double start;                  // of a call whose keys are more than a step
+    double group, more;            // of the other form's
+};
+constexpr double kFill = 273.0;
+constexpr Costs kPlainBf16 = {0.75, 1.0, 0.0, 60e3, 0.75, 50.0}, kPlainF32 = {0.6, 0.95, 200.0, 0.0, 1.8, 0.0},
+                kFourBits = {0.45, 0.55, 560.0, 60e3, 1.4, 220.0};
+// Measured, this form and the other in us (heads with those of keys, features in brackets; uneven: a quarter of
+// the keys to all).  One token: 32 requests of 4096 keys, 32 heads (32, 128), bf16 317 / 351, uneven 278 / 272, fp32 849 /
+// 2302, uneven 571 / 1472; 64 of 32768 bf16 5000 / 5551, fp32 11520 / 36165; 48 of 32768 uneven, 8 heads (8, 128), bf16
+// 642 / 847, fp32 1958 / 4286, 4 bits 197 / 602; 64 of 300 uneven, 32 heads (32, 64), 31 / 28, 66 / 167, 20 / 27.
+// Several: 64 requests of 16 over 1024 keys, 8 heads (8, 128), 64 / 45, 122 / 305, 39 / 34; of 32 over 300 keys 47 / 20,
+// 83 / 106, 38 / 16; 16 of 64 over 1024, 16 heads (4, 128), 73 / 30, 178 / 99, 48 / 28; 2 of 256 over 8192 130 / 174,
+// 550 / 683, 68 / 161.  Prompts: 512 tokens over 8192 keys, 32 heads (8, 128), 235 / 175, 1021 / 684, 125 / 161; 2048 over 16384,
+// 16 heads (4, 128), 881 / 443, 3953 / 2555, 369 / 402; 4 of 300 over 300, 8 heads (8, 64), 24 / 11, 33 / 22, 19 / 12.  Over 489
+// shapes, 300 of them drawn and 150 of these left out of the choice of the costs, the form taken is slower than the
+// other by 0.9 % in the mean (bf16 1.2, fp32 0.7, 4 bits 0.9), and by up to 36 % (31 uneven requests of 85 fp32 queries).
+// fp32 queries over 4 bits come here always: the products of three bf16 parts are quicker than the other form's fp32
+// ones (512 queries over 8192 keys 221 / 684).
+extern "C" int nnk_cache_is_few(const NnAttention* a, int four_bits) {
     const bool half = a->dtype == NN_BF16;
     if (four_bits && !half) return true;
-    const double rows = (double)a->len_q * (a->heads / a->kv_heads), units = std::ceil(rows / 32) * a->kv_heads * a->batch;
-    const double groups = std::ceil(a->len_q / 128.0) * a->heads * a->batch;
-    const double own = units * a->len_k * (four_bits ? 0.35 : 1.25) + (a->len_k > kStep ? 55e3 : 0.0);
-    return own <= std::max(0.66 * groups + 200.0, 273.0) * a->len_k;
+    const Costs& c = four_bits ? kFourBits : half ? kPlainBf16 : kPlainF32;
+    const Plan p = plan_of(a);
+    const double len = a->len_k, units = (double)p.units, groups = std::ceil(a->len_q / 128.0) * a->heads * a->batch;
+    const bool parts = p.steps > 1 && p.units < 4 * kCus;
+    const double own = units * (len * (p.rows == kTile ? c.tile : c.two_tiles) + (parts ? c.ends : 0.0)) + (p.steps > 1 ? c.start : 0.0);
+    return own <= std::max(c.group * groups + c.more, kFill) * len;
 }
 // Floats of a call's workspace: enough for its tickets and parts, and for every smaller call's, which
 // has fewer units, steps and rows (and 2048 of them at most in parts).
