@@ -139,10 +139,10 @@ struct Row {
         constexpr int V = 16 / (int)sizeof(A);
         return d % CE / V * (G * V) + d / CE * V + d % V;
     }
-    // The lane of the other members.
+    // The lane of the other members, or -1: this one's features are not turned.
     static __device__ __forceinline__ int other_lane(int d0, const Append& a) {
         const int c = d0 / CE, hc = a.half / CE;
-        return c >= 2 * hc ? c : c < hc ? c + hc : c - hc;
+        return c >= 2 * hc ? -1 : c < hc ? c + hc : c - hc;
     }
     // `row`: the group's values in LDS, kFeatures of them
     template <typename A>
@@ -150,6 +150,9 @@ struct Row {
         constexpr int V = 16 / (int)sizeof(A);  // values of an access
         typedef A Vec __attribute__((ext_vector_type(V)));
         const int c = d0 / CE;
+        // What is not turned meets its cosine, 1, times its sine, -0, and so stays as it is, infinities and
+        // the signs of zeros too.
+        const A* others = other >= 0 ? row + V * other : table + V * c;
         // the group's lanes are in one wave, whose LDS accesses are in order
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -163,7 +166,7 @@ struct Row {
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int j = 0; j < CE; j += V) {
-            const Vec y = *reinterpret_cast<const Vec*>(row + j * G + V * other);
+            const Vec y = *reinterpret_cast<const Vec*>(others + j * G);
             const Vec cos = *reinterpret_cast<const Vec*>(table + j * G + V * c);
             const Vec sin = *reinterpret_cast<const Vec*>(table + kFeatures + j * G + V * c);
 #pragma unroll
@@ -259,7 +262,7 @@ __device__ __forceinline__ void angles(A* table, const Append& a, int token0, in
     const int each = CHUNKS ? R::kFeatures - a.half : a.half;  // with the features that are not turned
     for (int i = threadIdx.x; i < count * each; i += kTpb) {
         const int t = i / each, p = i - t * each;
-        A c = 1, s = 0;
+        A c = 1, s = (A)-0.0;
         if (p < a.half) {
             const double angle = (double)a.pos[(size_t)(token0 + t) * a.axes + p / a.per_axis] * a.freq[p];
             cos_sin(angle * 0.15915494309189533577, c, s);
