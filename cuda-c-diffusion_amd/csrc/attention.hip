@@ -109,7 +109,7 @@ bool strides_by_16(const NnAttention* a) {
 
 }  // namespace
 
-bool nnk_attention_sizes_fit(const NnAttention* a, bool backward, const char* what) {
+bool nnk_attention_sizes_fit(const NnAttention* a, bool backward, const char* what, bool (*few)(const NnAttention*)) {
     NNK_REQUIRE_RET(a, false, what, "%s: null description", what);
     NNK_REQUIRE_RET(a->dtype == NN_F32 || a->dtype == NN_BF16, false, what, "%s: unknown dtype %d", what, a->dtype);
     NNK_REQUIRE_RET(a->batch >= 0 && a->len_q >= 0 && a->len_k >= 0 && a->len_q <= kMaxLen && a->len_k <= kMaxLen,
@@ -126,7 +126,7 @@ bool nnk_attention_sizes_fit(const NnAttention* a, bool backward, const char* wh
     bool fits = rows * a->batch <= kMostRows / a->heads && (long long)a->buckets * a->heads <= kMostRows;
     // workgroups of tiles of queries, of keys, and of documents (of 64 threads)
     const auto launched = [&](long long n) { return n * a->batch <= kMostGroups / a->heads; };
-    fits = fits && ((!backward && nnk_attention_is_few(a)) || launched(up(a->len_q, kRows)));
+    fits = fits && ((!backward && few(a)) || launched(up(a->len_q, kRows)));
     fits = fits && (!backward || launched(up(a->len_k, kRows)));
     fits = fits && (!a->doc_q || up(std::max(a->len_q, a->len_k), kBlock) * a->batch <= kMostGroups * (kTpb / 64));
     NNK_REQUIRE_RET(fits, false, what, "%s: too many rows (batch=%d heads=%d len_q=%d len_k=%d)", what, a->batch, a->heads,
@@ -134,8 +134,8 @@ bool nnk_attention_sizes_fit(const NnAttention* a, bool backward, const char* wh
     return true;
 }
 
-bool nnk_attention_take(Args& p, const NnAttention* a, bool backward, const char* what) {
-    if (!nnk_attention_sizes_fit(a, backward, what)) return false;
+bool nnk_attention_take(Args& p, const NnAttention* a, bool backward, const char* what, bool (*few)(const NnAttention*)) {
+    if (!nnk_attention_sizes_fit(a, backward, what, few)) return false;
     NNK_REQUIRE_RET(a->scale > 0.0f && a->scale < INFINITY, false, what, "%s: scale=%g is not positive", what, a->scale);
     NNK_REQUIRE_RET(a->softcap >= 0.0f && a->softcap < INFINITY, false, what, "%s: softcap=%g is negative", what,
         a->softcap);

@@ -572,9 +572,14 @@ inline bool raise_lds(const void* fn, size_t bytes, std::atomic<unsigned long lo
 
 }  // namespace attn
 
+// The form of attention over tensors for few queries: when it is taken.
+bool nnk_attention_is_few(const NnAttention* a);
 // Whether a call's sizes can be had; fills `p` for the call's description.  False after recording an error.
-bool nnk_attention_sizes_fit(const NnAttention* a, bool backward, const char* what);
-bool nnk_attention_take(attn::Args& p, const NnAttention* a, bool backward, const char* what);
+// few(a): whether a form takes the call whose launch is not of tiles of queries of a head.
+bool nnk_attention_sizes_fit(const NnAttention* a, bool backward, const char* what,
+    bool (*few)(const NnAttention*) = nnk_attention_is_few);
+bool nnk_attention_take(attn::Args& p, const NnAttention* a, bool backward, const char* what,
+    bool (*few)(const NnAttention*) = nnk_attention_is_few);
 // Documents of each block of 64 into `ws`, for args.key_docs and query_docs (no documents:
 // nothing).
 void nnk_attention_docs(attn::Args& args, float* ws, hipStream_t s, const char* what);
@@ -585,9 +590,8 @@ const int* nnk_attention_order(const attn::Args& args, bool keys, int own, float
 bool nnk_attention_forward(const attn::Args& args, bool half, hipStream_t s, const char* what);
 bool nnk_attention_backward_q(const attn::Args& args, bool half, hipStream_t s, const char* what);
 bool nnk_attention_backward_kv(const attn::Args& args, bool half, hipStream_t s, const char* what);
-// The form for few queries; when it is taken; the floats that it needs after the tickets, and
-// a bound on them for every smaller batch and shorter lengths.
-bool nnk_attention_is_few(const NnAttention* a);
+// The form for few queries: the floats that it needs after the tickets, and a bound on them for
+// every smaller batch and shorter lengths.
 size_t nnk_attention_few_floats(const NnAttention* a);
 size_t nnk_attention_few_most(const NnAttention* a);
 bool nnk_attention_few(const attn::Args& args, bool half, float* ws, hipStream_t s, const char* what);

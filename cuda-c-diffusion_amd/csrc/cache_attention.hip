@@ -7,13 +7,21 @@ namespace {
 using namespace attn;
 using cache::Pages;
 
-bool fits(Pages& p, const NnAttention* a, const NnCache* c, bool pools, const char* what) {
+bool few_plain(const NnAttention* a) { return nnk_cache_is_few(a, false); }
+bool few_four_bits(const NnAttention* a) { return nnk_cache_is_few(a, true); }
+
+// Whether a call can be had; with `args`, what its kernels take.
+bool fits(Args* args, Pages& p, const NnAttention* a, const NnCache* c, const char* what) {
     NNK_REQUIRE_RET(a, false, what, "%s: null description", what);
-    if (!nnk_cache_take(p, c, a->dtype, a->kv_heads, a->head_dim, pools, what)) return false;
+    if (!nnk_cache_take(p, c, a->dtype, a->kv_heads, a->head_dim, args != nullptr, what)) return false;
     NNK_REQUIRE_RET(!a->doc_q && !a->doc_k, false, what, "%s: documents", what);
     NNK_REQUIRE_RET(a->batch <= c->requests, false, what, "%s: batch=%d of a cache of %d requests", what, a->batch, c->requests);
     NNK_REQUIRE_RET(a->len_k <= (long long)c->table_pages * c->page_tokens, false, what,
         "%s: len_k=%d does not fit in %d pages of %d tokens", what, a->len_k, c->table_pages, c->page_tokens);
+    const auto few = p.groups ? few_four_bits : few_plain;
+    if (!(args ? nnk_attention_take(*args, a, false, what, few) : nnk_attention_sizes_fit(a, false, what, few))) return false;
+    NNK_REQUIRE_RET(!few(a) || nnk_cache_few_fits(a), false, what, "%s: too many rows (batch=%d heads=%d len_q=%d)", what,
+        a->batch, a->heads, a->len_q);
     return true;
 }
 
@@ -32,7 +40,7 @@ extern "C" {
 size_t nnhip_cache_attention_workspace(const NnAttention* a, const NnCache* c) {
     const char* what = "nnhip_cache_attention_workspace";
     Pages p;
-    return fits(p, a, c, false, what) && nnk_attention_sizes_fit(a, false, what) ? nnk_cache_few_floats(a) : 0;
+    return fits(nullptr, p, a, c, what) ? nnk_cache_few_floats(a) : 0;
 }
 
 void launch_cache_attention_forward(void* out, float* lse, const void* q, const NnAttention* a, const NnCache* c,
@@ -40,8 +48,7 @@ void launch_cache_attention_forward(void* out, float* lse, const void* q, const 
     const char* what = "launch_cache_attention_forward";
     Pages p;
     Args args;
-    if (!fits(p, a, c, true, what)) return;
-    if (!nnk_attention_take(args, a, false, what)) return;
+    if (!fits(&args, p, a, c, what)) return;
     if (!a->batch || !a->len_q) return;
     NNK_REQUIRE(out && lse && q, what, "%s: null pointer", what);
     const long long n[3] = {a->batch, a->len_q, a->heads};

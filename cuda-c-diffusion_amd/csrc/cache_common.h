@@ -60,15 +60,18 @@ __device__ __forceinline__ void values8(unsigned code, float scale, f32x2 (&v)[4
 // Fills `p` from the description; false after recording an error.  `pools`: whether the
 // pointers are looked at.
 bool nnk_cache_take(cache::Pages& p, const NnCache* c, int dtype, int kv_heads, int head_dim, bool pools, const char* what);
-// Attention of few queries: one launch; when it is taken; the floats of its workspace, which are enough
-// for every smaller batch and fewer queries or keys, and whether a call needs it.
+// Attention of few queries: one launch; when it is taken; whether a launch has that many workgroups; the
+// floats of its workspace, which are enough for every smaller batch and fewer queries or keys, and whether a
+// call needs it.
 namespace attn {
 struct Args;
 }
 extern "C" int nnk_cache_is_few(const NnAttention* a, int four_bits);
+bool nnk_cache_few_fits(const NnAttention* a);
 size_t nnk_cache_few_floats(const NnAttention* a);
 bool nnk_cache_few_parted(const NnAttention* a);
-void nnk_cache_few(const attn::Args& a, const cache::Pages& p, const NnAttention* d, float* ws, hipStream_t s, const char* what);
+void nnk_cache_few(const attn::Args& a, const cache::Pages& p, const NnAttention* d, float* ws, hipStream_t s,
+    const char* what);
 // Of many queries; over pages of 4 bits for bf16 alone.
 bool nnk_cache_forward_plain(const attn::Args& a, const cache::Pages& p, bool half, hipStream_t s, const char* what);
 bool nnk_cache_forward_mxfp4(const attn::Args& a, const cache::Pages& p, hipStream_t s, const char* what);

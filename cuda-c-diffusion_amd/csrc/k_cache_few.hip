@@ -934,6 +934,7 @@ extern "C" int nnk_cache_is_few(const NnAttention* a, int four_bits) {
     const double own = units * (len * (p.rows == kTile ? c.tile : c.two_tiles) + (parts ? c.ends : 0.0)) + (p.steps > 1 ? c.start : 0.0);
     return own <= std::max(c.group * groups + c.more, kFill) * len;
 }
+bool nnk_cache_few_fits(const NnAttention* a) { return plan_of(a).units < (1LL << 32) / kTpb; }  // threads of a launch
 // Floats of a call's workspace: enough for its tickets and parts, and for every smaller call's, which
 // has fewer units, steps and rows (and 2048 of them at most in parts).
 size_t nnk_cache_few_floats(const NnAttention* a) {
@@ -945,7 +946,6 @@ size_t nnk_cache_few_floats(const NnAttention* a) {
 bool nnk_cache_few_parted(const NnAttention* a) { return a->batch && a->len_q && plan_of(a).parted; }
 void nnk_cache_few(const Args& a, const Pages& p, const NnAttention* d, float* ws, hipStream_t s, const char* what) {
     const Plan plan = plan_of(d);
-    NNK_REQUIRE(plan.units < (1LL << 32) / kTpb, what, "%s: too many rows", what);
     if (d->dtype == NN_BF16) {
         if (p.groups) by_dim<bf16, Mxfp4>(a, p, plan, ws, s, what);
         else by_dim<bf16, Bf16>(a, p, plan, ws, s, what);

@@ -3,7 +3,11 @@ from __future__ import annotations
 
 import ctypes
 
+import numpy as np
 import pytest
+
+from cache_ref import Cache, Tensor, ints
+from attention_ref import check
 
 
 def is_few(nn, dtype, kind, batch, len_q, len_k, heads, kv_heads, head_dim):
@@ -47,3 +51,59 @@ def test_the_quicker_form_is_taken(nn, case):
 
 def test_fp32_queries_over_four_bits(nn):
     assert is_few(nn, "f32", "mxfp4", 1, 2048, 16384, 16, 4, 128)
+
+
+DUMMY, FAR = 16, 1 << 40  # never dereferenced
+# more (request, head) pairs than a launch has workgroups, fewer units: 128 heads of one key head are four of these
+MANY, HEADS = 131100, 128
+
+
+def _cache(nn, kind, requests, table_pages):
+    return nn.NnCache(kind=nn.NN_CACHE_MXFP4 if kind == "mxfp4" else nn.NN_CACHE_PLAIN, page_tokens=16, pages=1,
+                      requests=requests, table_pages=table_pages, table=DUMMY, k=DUMMY, v=FAR)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("kind", ["plain", "mxfp4"])
+def test_sizes_are_those_of_the_form_taken(nn, dtype, kind):
+    """What a launch of the form for few queries has room for is not refused for the other form's workgroups."""
+    L = nn.lib()
+    L.last_error()
+    t = nn.NN_BF16 if dtype == "bf16" else nn.NN_F32
+    a = nn.NnAttention(dtype=t, batch=MANY, len_q=1, len_k=200, heads=HEADS, kv_heads=1, head_dim=8)
+    assert is_few(nn, dtype, kind, MANY, 1, 200, HEADS, 1, 8)
+    assert L.nnhip_cache_attention_workspace(a, _cache(nn, kind, MANY, 13)) > 0
+    a.batch = 1 << 22  # units past a launch
+    with pytest.raises(nn.NnHipError, match="nnhip_cache_attention_workspace: error 1: .*too many rows"):
+        L.nnhip_cache_attention_workspace(a, _cache(nn, kind, a.batch, 13))
+    assert L.last_error()[0] == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["plain", "mxfp4"])
+def test_more_heads_than_a_launch_has_workgroups(nn, L, rng, kind):
+    """Every request has the same page and the same queries (strides of 0), and a result of its own."""
+    from test_gpu_attention import case
+    from test_gpu_cache_attention import Call
+
+    dim, len_k = 8, 13
+    cache = Cache(nn, L, rng, kind, "bf16", 1, dim, 16, [1])
+    cache.fill(rng, [len_k])
+    one = Call(nn, L, rng, case("bf16", 1, 1, len_k, HEADS, 1, dim), kind, 16, cache=cache)
+    one.launch()
+    L.sync()
+    one.compare()
+    ref, mag = one.expected()
+    table = ints(L, np.repeat(cache.table, MANY, 0))
+    many = nn.NnCache(kind=cache.args.kind, page_tokens=16, pages=cache.pages, requests=MANY, table_pages=1, table=table.p,
+                      k=cache.dev["k"].p, v=cache.dev["v"].p)
+    out, lse = Tensor(L, (MANY, 1, HEADS, dim), "bf16"), L.alloc(MANY * HEADS)
+    a = nn.NnAttention(dtype=nn.NN_BF16, batch=MANY, len_q=1, len_k=len_k, heads=HEADS, kv_heads=1, head_dim=dim,
+                       scale=dim**-0.5, mask=nn.NN_MASK_NONE, q_stride=(0, 0, dim), out_stride=out.strides[:3])
+    assert L.nnhip_cache_attention_workspace(a, many) == 0
+    L.launch_cache_attention_forward(out.p, lse.p, one.q.p, a, many, None, None)
+    L.sync()
+    got, sums = out.result(), lse.download(shape=(MANY, HEADS, 1))
+    assert (got == got[:1]).all() and (sums == sums[:1]).all()
+    check("out", got[:1], ref["out"], mag["out"], "bf16")
+    check("lse", sums[:1].astype(np.float64), ref["lse"], mag["lse"], "f32")
