@@ -357,15 +357,16 @@ __global__ __launch_bounds__(kTpb, sizeof(T) == 2 && VEC ? 2 : 1) void attn_fwd_
         const float2 y = parts[strip * 32 + (lane & 31)];
         const float unit = CAP || BIAS ? 1.0f : a.c1, top = fmaxf(m, y.x), base = top == -INFINITY ? 0.0f : top;
         const float f = exp2_fast((m - base) * unit), g = exp2_fast((y.x - base) * unit);
+        // half of each: both may be near the type's end where the reference is fixed
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) o[d][r] = o[d][r] * f + to[(d * 16 + r) * 64] * g;
+            for (int r = 0; r < 16; ++r) o[d][r] = o[d][r] * (0.5f * f) + to[(d * 16 + r) * 64] * (0.5f * g);
         l = l * f + y.y * g;
         m = top;
     }
     if (!in) return;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float inv = l == 0.0f ? 0.0f : (SPLIT > 1 ? 2.0f : 1.0f) / l;
     T* out = (T*)a.out + b * a.os[0] + (long long)row * a.os[1] + head * a.os[2];
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
