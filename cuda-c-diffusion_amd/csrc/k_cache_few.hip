@@ -904,14 +904,17 @@ void by_dim(const Args& a, const Pages& p, const Plan& plan, float* ws, hipStrea
 // head, whatever they fill of them, and takes as long as kFill of them (of 64) where CUs are left over.  It
 // reads a key head once for each of its heads; in fp32 its tiles leave one workgroup a CU.  In units of a
 // workgroup and key:
+struct Unit {
+    double key, ends;  // a key, and the ends of its parts
+    double start;      // of a call of more keys than a step
+};
 struct Costs {
-    double tile, two_tiles, ends;  // of a unit: a key with a tile or two; its ends, in keys
-    double start;                  // of a call whose keys are more than a step
-    double group, more;            // of the other form's
+    Unit one, two;       // tiles a unit
+    double group, more;  // of the other form's
 };
 constexpr double kFill = 273.0;
-constexpr Costs kPlainBf16 = {0.75, 1.0, 0.0, 60e3, 0.75, 50.0}, kPlainF32 = {0.6, 0.95, 200.0, 0.0, 1.8, 0.0},
-                kFourBits = {0.45, 0.55, 560.0, 60e3, 1.4, 220.0};
+constexpr Costs kPlainBf16 = {{0.72, 0.0, 33e3}, {0.92, 250.0, 88e3}, 0.75, 0.0}, kPlainF32 = {{0.6, 100.0, 0.0}, {1.0, 100.0, 40e3}, 2.0, 0.0},
+                kFourBits = {{0.45, 400.0, 10e3}, {0.5, 550.0, 100e3}, 1.3, 210.0};
 // Measured, this form and the other in us (heads with those of keys, features in brackets; uneven: a quarter of
 // the keys to all).  One token: 32 requests of 4096 keys, 32 heads (32, 128), bf16 317 / 351, uneven 278 / 272, fp32 849 /
 // 2302, uneven 571 / 1472; 64 of 32768 bf16 5000 / 5551, fp32 11520 / 36165; 48 of 32768 uneven, 8 heads (8, 128), bf16
@@ -919,9 +922,10 @@ constexpr Costs kPlainBf16 = {0.75, 1.0, 0.0, 60e3, 0.75, 50.0}, kPlainF32 = {0.
 // Several: 64 requests of 16 over 1024 keys, 8 heads (8, 128), 64 / 45, 122 / 305, 39 / 34; of 32 over 300 keys 47 / 20,
 // 83 / 106, 38 / 16; 16 of 64 over 1024, 16 heads (4, 128), 73 / 30, 178 / 99, 48 / 28; 2 of 256 over 8192 130 / 174,
 // 550 / 683, 68 / 161.  Prompts: 512 tokens over 8192 keys, 32 heads (8, 128), 235 / 175, 1021 / 684, 125 / 161; 2048 over 16384,
-// 16 heads (4, 128), 881 / 443, 3953 / 2555, 369 / 402; 4 of 300 over 300, 8 heads (8, 64), 24 / 11, 33 / 22, 19 / 12.  Over 489
-// shapes, 300 of them drawn and 150 of these left out of the choice of the costs, the form taken is slower than the
-// other by 0.9 % in the mean (bf16 1.2, fp32 0.7, 4 bits 0.9), and by up to 36 % (31 uneven requests of 85 fp32 queries).
+// 16 heads (4, 128), 881 / 443, 3953 / 2555, 369 / 402; 4 of 300 over 300, 8 heads (8, 64), 24 / 11, 33 / 22, 19 / 12.  Short
+// caches, one request, 8 heads (2, 128): one token of 200 keys 10.0 / 11.2, 13.7 / 28.5, 8.7 / 11.2, six tokens 13.6 / 11.9,
+// 23.8 / 28.9, 12.3 / 11.2.  Over 150 drawn shapes that had no part in the choice of the costs, the form taken is slower than
+// the other by 0.6 % in the mean, and by up to 57 % (209 requests of 35 fp32 queries over 124 keys, 4 heads, 128 / 82).
 // fp32 queries over 4 bits come here always: the products of three bf16 parts are quicker than the other form's fp32
 // ones (512 queries over 8192 keys 221 / 684).
 extern "C" int nnk_cache_is_few(const NnAttention* a, int four_bits) {
@@ -930,8 +934,9 @@ extern "C" int nnk_cache_is_few(const NnAttention* a, int four_bits) {
     const Costs& c = four_bits ? kFourBits : half ? kPlainBf16 : kPlainF32;
     const Plan p = plan_of(a);
     const double len = a->len_k, units = (double)p.units, groups = std::ceil(a->len_q / 128.0) * a->heads * a->batch;
+    const Unit& u = p.rows == kTile ? c.one : c.two;
     const bool parts = p.steps > 1 && p.units < 4 * kCus;
-    const double own = units * (len * (p.rows == kTile ? c.tile : c.two_tiles) + (parts ? c.ends : 0.0)) + (p.steps > 1 ? c.start : 0.0);
+    const double own = units * (len * u.key + (parts ? u.ends : 0.0)) + (p.steps > 1 ? u.start : 0.0);
     return own <= std::max(c.group * groups + c.more, kFill) * len;
 }
 bool nnk_cache_few_fits(const NnAttention* a) { return plan_of(a).units < (1LL << 32) / kTpb; }  // threads of a launch

@@ -27,6 +27,10 @@ MEASURED = [
     ("f32", "plain", 16, 1, 4096, 32, 32, 128, 460, 1156), ("f32", "plain", 64, 1, 32768, 32, 32, 128, 11520, 36165),
     ("f32", "plain", 256, 1, 512, 16, 16, 64, 173, 491), ("f32", "plain", 2000, 1, 128, 12, 12, 64, 442, 1122),
     ("f32", "plain", 64, 1, 64, 16, 16, 128, 40, 58), ("bf16", "mxfp4", 48, 1, 32768, 8, 8, 128, 197, 602),
+    # few keys
+    ("bf16", "plain", 1, 1, 200, 8, 2, 128, 10.0, 11.2), ("bf16", "plain", 1, 6, 200, 8, 2, 128, 13.6, 11.9),
+    ("f32", "plain", 1, 1, 130, 8, 2, 128, 13.6, 23.3), ("f32", "plain", 4, 6, 280, 8, 2, 128, 24.9, 34.8),
+    ("bf16", "mxfp4", 4, 1, 200, 32, 8, 128, 9.6, 11.5), ("bf16", "mxfp4", 4, 6, 130, 32, 8, 128, 13.4, 10.4),
     # one token, shared key heads
     ("bf16", "plain", 32, 1, 4096, 32, 8, 128, 70, 187), ("f32", "plain", 64, 1, 4096, 64, 32, 128, 1066, 5765),
     ("bf16", "mxfp4", 64, 1, 2048, 32, 16, 128, 47, 165),
