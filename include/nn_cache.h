@@ -87,8 +87,8 @@ void launch_cache_append(void* q_out, const void* q, const void* k, const void* 
  * Read
  * ------------------------------------------------------------------------
  * k[t], v[t] = the key and value of token place[t] of request request[t] (NULL: t), as
- * the values that they stand for: exact, but that bf16 turns 4-bit values below 2^-126
- * to those that it has.  Rows with place[t] < 0 are left as they are. */
+ * the values that they stand for: exact in both types, and infinite from 2^128 on (scales
+ * of 253 and 254, which no append writes).  Rows with place[t] < 0 are left as they are. */
 typedef struct {
     int dtype;              /* NnDtype of k and v, and of plain pages */
     int tokens;
