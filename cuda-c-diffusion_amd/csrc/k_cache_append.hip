@@ -38,7 +38,7 @@ struct Append {
     const float *q_weight, *k_weight;
     const int *pos, *request, *place;
     const double* freq;
-    int tokens, heads, kv_heads, rows, dim, half, axes, per_axis, interleaved, norm;
+    int tokens, heads, kv_heads, dim, half, axes, per_axis, interleaved, norm;
     int tokens_each;       // tokens of a workgroup
     int q_parts, kv_parts; // workgroups that share their queries, and their keys, and their values
     float eps;
@@ -446,7 +446,6 @@ extern "C" void launch_cache_append(void* q_out, const void* q, const void* k, c
     p.tokens = o.tokens;
     p.heads = o.heads;
     p.kv_heads = o.kv_heads;
-    p.rows = o.heads + 2 * o.kv_heads;
     p.dim = o.head_dim;
     p.half = o.rot_dim / 2;
     p.axes = o.axes;
