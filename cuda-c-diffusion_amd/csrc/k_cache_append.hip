@@ -15,9 +15,9 @@
 // Keys for 4 bits are formed in 64 bits, as a code is a choice: with fp32 sums the order of
 // the additions would decide it for some values in 10^5, and with it half a step of the value.
 //
-// Measured: 8192 tokens, 32 + 8 + 8 heads of 128, bf16 into 4 bits 43 us (4.0 TB/s; vector instructions
-// about half of the SIMDs' cycles); 2355 rows, 39 of them no tokens, 16 + 16 + 16 heads of 72, fp32 into
-// plain pages 23 us (2.8 TB/s); four tokens 6.2 us.
+// Measured: 8192 tokens, 32 + 8 + 8 heads of 128, bf16 into 4 bits 44 us (3.9 TB/s; vector instructions
+// half of the SIMDs' cycles); 2355 rows, 39 of them no tokens, 16 + 16 + 16 heads of 72, fp32 into
+// plain pages 23 us (2.8 TB/s); four tokens 6.7 us.
 #include "cache_common.h"
 
 #include <algorithm>

@@ -13,10 +13,13 @@
 // A key goes from memory to the registers of the lanes that multiply it; 4-bit features become
 // bf16, which holds them exactly, two an instruction, their scale included.  Values pass through
 // LDS, where the transposing read turns them (bf16), or are read a feature a lane (fp32 pages).
-// fp32 queries and probabilities meet 4-bit pages as three bf16 parts each, 24 bits of them.
+// fp32 queries and probabilities meet 4-bit pages as three bf16 parts each, 24 bits of them.  With bf16
+// tensors a probability is one bf16 value in its product with the values, off by up to 2^-8 of itself and
+// independently of the others (its sum is fp32 and of what it was before): outputs are then 2.1e-3 to 2.4e-3 of their
+// norm off, where their own rounding alone is 1.7e-3.  A second part would double those products.
 //
 // Measured: 16 requests of 8192 to 32768 keys, 32 heads of 128 (8 of keys), scores under a cap: bf16
-// pages 218 us, 6.2 TB/s (reads alone reach 7.1); 4 bits 68 us, 5.3 TB/s of a third of the bytes, some
+// pages 218 us, 6.2 TB/s (reads alone reach 7.1); 4 bits 68 us, 5.3 TB/s of about a quarter of the bytes, some
 // 14 us of it lengths, table, first loads and the joins (11 of those with no join between workgroups).
 // 48 requests of five queries over 4096 keys, 16 heads (4), 4 bits 29 us, 17 of them such ends; one of 777
 // keys, 8 heads of 64, 7.9 us; three of seven fp32 queries over 5001 keys, 12 heads of 96 (4), 4 bits 24 us.

@@ -107,8 +107,9 @@ void launch_cache_read(void* k, void* v, const NnCacheRead* a, const NnCache* c,
  * is row b of the table, key j its token j.  All of NnAttention's terms and masks but
  * documents (a request is one), with these differences: k_stride and v_stride are not
  * used; len_k, which has to fit in the table, bounds k_len; keys of entries that are no
- * page are not seen.  What seen pages hold up to k_len should be finite; slots behind
- * k_len may hold anything.
+ * page are not seen.  What seen pages hold up to k_len should be finite (and values below
+ * 2^119 / len_k in size: fp32 sums have shares of up to 2^8); slots behind k_len may hold
+ * anything.
  *
  * With bf16 tensors queries, probabilities and plain pages are bf16 and 4-bit values,
  * which bf16 holds exactly, meet them there; with fp32 tensors all products are of fp32
