@@ -850,8 +850,8 @@ __global__ __launch_bounds__(kTpb, (held_by_a_cu<T, PAGES<DP>, NT>())) void cach
 // Tiles of queries, and parts at most.
 constexpr int kHeld = 3;  // workgroups a CU at most
 struct Plan {
-    long long units, steps;
-    int tiles, rows, step;
+    long long units, steps, tiles;
+    int rows, step;
     bool parted;
 };
 Plan plan_of(const NnAttention* a) {
@@ -859,7 +859,7 @@ Plan plan_of(const NnAttention* a) {
     const long long rows = (long long)a->len_q * (a->heads / a->kv_heads);
     p.steps = std::max(1, (a->len_k + kStep - 1) / kStep);
     p.rows = rows <= kTile ? kTile : 2 * kTile;
-    p.tiles = (int)((rows + p.rows - 1) / p.rows);
+    p.tiles = (rows + p.rows - 1) / p.rows;
     p.units = (long long)a->batch * a->kv_heads * p.tiles;
     p.step = kStep;
     while (p.step < 1 << 30 && p.units * ((a->len_k + (long long)p.step - 1) / p.step + 1) >= 1LL << 30) p.step *= 2;
@@ -876,7 +876,7 @@ void launch(const Args& a, const Pages& p, const Plan& plan, float* ws, hipStrea
         constexpr int NT = decltype(tiles)::value;
         constexpr int held = held_by_a_cu<T, PAGES<DP>, NT>();
         const int workers = plan.parted && plan.units < 2 * kCus * held ? (int)workers_of(plan, held) : 0;
-        const All all = {a, p, {reinterpret_cast<unsigned*>(ws), ws + kTicketWords, plan.tiles, a.kv_heads * plan.tiles, workers, kCus * held, plan.step}};
+        const All all = {a, p, {reinterpret_cast<unsigned*>(ws), ws + kTicketWords, (int)plan.tiles, (int)(a.kv_heads * plan.tiles), workers, kCus * held, plan.step}};
         cache_few_kernel<T, PAGES, DP, NT, decltype(terms)::value>
             <<<workers ? (unsigned)workers : (unsigned)plan.units, kTpb, 0, s>>>(all);
     };

@@ -83,6 +83,24 @@ def test_sizes_are_those_of_the_form_taken(nn, dtype, kind):
     assert L.last_error()[0] == 0
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("kind", ["plain", "mxfp4"])
+@pytest.mark.parametrize("len_q", [1 << 17, (1 << 17) + 32, (1 << 18) - 128])
+def test_tiles_past_32_bits(nn, dtype, kind, len_q):
+    """2^20 heads of one key head: 2^32 tiles of queries and more, which are too many, not the few that 32 bits hold of them."""
+    L = nn.lib()
+    L.last_error()
+    t = nn.NN_BF16 if dtype == "bf16" else nn.NN_F32
+    a = nn.NnAttention(dtype=t, batch=1, len_q=len_q, len_k=200, heads=1 << 20, kv_heads=1, head_dim=8, scale=1.0,
+                       q_stride=(0, 0, 8), out_stride=(0, 8 << 20, 8))
+    c = _cache(nn, kind, 1, 13)
+    with pytest.raises(nn.NnHipError, match="nnhip_cache_attention_workspace: error 1: .*too many rows"):
+        L.nnhip_cache_attention_workspace(a, c)
+    with pytest.raises(nn.NnHipError, match="launch_cache_attention_forward: error 1: .*too many rows"):
+        L.launch_cache_attention_forward(DUMMY, DUMMY, DUMMY, a, c, DUMMY, None)
+    assert L.last_error()[0] == 0
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["plain", "mxfp4"])
 def test_more_heads_than_a_launch_has_workgroups(nn, L, rng, kind):
